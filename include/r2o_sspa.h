@@ -467,6 +467,108 @@ int r2o_qkv_norm_rope(const uint16_t* q, const uint16_t* k, const uint16_t* v, u
                       const uint16_t* sin, const int64_t* cos_strides, const int64_t* sin_strides,
                       int64_t apply_hadamard, void* stream);
 
+/* ------------------------------------- prompt attention and accumulated weights ---- */
+
+/* Row i of a request with q query rows and n keys (query_lengths / key_lengths [batch], NULL for all rows; a
+ * length is clamped to its tensor) stands at position p = n - q + i and sees key j where j <= p and, with a window
+ * (window > 0), p - j < window or j < sinks.  Tensors hold bf16 (dtype 0) or fp16 (1) rows of 128 unit-strided
+ * channels, 16-byte aligned, with element strides (batch, head, row), each a multiple of 8; hq is a multiple of
+ * hkv, query head h reads KV head h / (hq / hkv).  lse, lse_in: fp32 [batch, hq, queries], contiguous. */
+typedef struct r2o_prompt_params {
+    const uint16_t* query;    /* [batch, hq, queries, 128] */
+    const uint16_t* key;      /* [batch, hkv, keys, 128] */
+    const uint16_t* value;    /* as key; attention only */
+    uint16_t* out;            /* as query; attention only */
+    float* lse;               /* attention only */
+    int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3];
+    const int32_t* query_lengths;
+    const int32_t* key_lengths;
+    int64_t batch, hq, hkv, queries, keys, dtype, window, sinks;
+    float sm_scale;           /* positive and finite */
+    const float* lse_in;      /* weights only */
+    float* weights;           /* weights only: fp32 [batch, hkv, keys], contiguous */
+    float* scratch;           /* weights with splits > 1: [splits, batch, hkv, keys] */
+    int64_t scratch_floats, splits;
+} r2o_prompt_params;
+
+/* out = softmax(sm_scale q k^T) v over the keys that each row sees, and lse = log of the sum of exponentials.
+ * Every row is written: one that sees no key, or lies behind its request's length, is 0 with lse -inf. */
+int r2o_prompt_attention(const r2o_prompt_params* p, void* stream);
+
+/* weights[b, h, j] = sum over KV head h's query heads and the rows that see key j of
+ * exp(sm_scale q . k_j - lse_in); 0 behind a request's length.  Rows with lse_in -inf give nothing.  The rows are
+ * shared out over `splits` workgroups a key tile, whose sums are joined in a fixed order. */
+int r2o_attention_weights(const r2o_prompt_params* p, void* stream);
+
+/* ------------------------------------------------------------------- paged KV cache ---- */
+
+#define R2O_PAGED_MAX_BATCH 1024
+#define R2O_PAGED_MAX_WORKERS 4096
+
+/* Slot j of request b is slot j % page_size of page page_table[b][j / page_size], for every KV head; lengths[b]
+ * slots are filled (clamped to max_pages * page_size).  Slots of a page id outside [0, pages) are not seen and not
+ * written.  K and V rows as above with element strides (page, head, slot); weight_pages (may be NULL): fp32 with
+ * element strides (page, head), slots unit-strided. */
+typedef struct r2o_paged_cache {
+    uint16_t* key_pages;      /* [pages, hkv, page_size, 128] */
+    uint16_t* value_pages;
+    float* weight_pages;      /* [pages, hkv, page_size] */
+    const int32_t* page_table; /* [batch, max_pages], rows table_stride apart */
+    const int32_t* lengths;   /* [batch] */
+    int64_t key_strides[3], value_strides[3], weight_strides[2];
+    int64_t table_stride, pages, max_pages, page_size, batch, hkv, dtype;
+} r2o_paged_cache;
+
+/* Row i of request b (i < counts[b], or all `rows` when counts is NULL) goes to slot lengths[b] - counts[b] + i:
+ * lengths already count the rows.  Weights (fp32 [batch, hkv, rows], element strides (batch, head)) go along, or
+ * zeros where the cache keeps weights and none are given. */
+typedef struct r2o_paged_extend_params {
+    r2o_paged_cache cache;
+    const uint16_t* key;      /* [batch, hkv, rows, 128], element strides (batch, head, row) */
+    const uint16_t* value;
+    const float* weights;
+    const int32_t* counts;
+    int64_t key_strides[3], value_strides[3], weights_strides[2];
+    int64_t rows;
+} r2o_paged_extend_params;
+int r2o_paged_extend(const r2o_paged_extend_params* p, void* stream);
+
+/* Attention of one token per request, hq / hkv <= 16 heads a KV head, over the filled slots: with a window the
+ * last `window` and the first `sinks` ones.  append_key / append_value (both or neither): the rows of slot lengths[b]
+ * - 1, which are attended and written into their page.  Where the cache keeps weights, the weight of each slot seen
+ * grows by the sum of its probabilities over the KV head's query heads; the appended slot's is set to it.  A request
+ * without a slot to see gets 0 and lse -inf.  Two launches; no atomics, so equal calls give equal bits. */
+typedef struct r2o_paged_attention_params {
+    r2o_paged_cache cache;
+    const uint16_t* query;    /* [batch, hq, 128], element strides (batch, head) */
+    const uint16_t* append_key;   /* [batch, hkv, 128] */
+    const uint16_t* append_value;
+    int64_t query_strides[2], append_strides[4]; /* append: key's (batch, head), value's (batch, head) */
+    int64_t hq, window, sinks;
+    float sm_scale;
+    uint16_t* out;            /* [batch, hq, 128], contiguous */
+    float* lse;               /* [batch, hq] */
+    float* partial_out;       /* [partial_states, 128] */
+    float* partial_ml;        /* [partial_states, 2] */
+    float* logits;            /* where the cache keeps weights */
+    int64_t partial_states;   /* at least (workers + batch * hkv) * (hq / hkv) */
+    int64_t logits_floats;    /* at least batch * hq * (max_pages * page_size rounded up to 32) */
+    int64_t workers;          /* workgroups that share the slots */
+} r2o_paged_attention_params;
+int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream);
+
+/* Of each (request, KV head) of `source` that holds more than `keep` slots, the first `sinks`, the last `recent` and
+ * those of largest weight stay (ties to the lower slot, NaN above all), in order; they are copied, with their
+ * weights where the target keeps them, into slots 0.. of `target`, whose pages must not be the source's.
+ * target_lengths[b] = min(lengths[b], keep), kept [batch, hkv, keep] = the source slots in order, then -1. */
+typedef struct r2o_paged_evict_params {
+    r2o_paged_cache source, target;
+    int64_t keep, sinks, recent;
+    int32_t* kept;
+    int32_t* target_lengths;
+} r2o_paged_evict_params;
+int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream);
+
 /* Library identification: returns the gfx target the code objects were built for. */
 const char* r2o_build_target(void);
 

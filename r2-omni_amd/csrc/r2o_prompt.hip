@@ -1,0 +1,424 @@
+// Attention of a prompt's rows for gfx950, and the attention weight that each key received.
+//
+// Row i of a request with q rows and n keys stands at position p = n - q + i.  It sees key j where j <= p and,
+// with a window of W, p - j < W or j < sinks.  prompt_attention_kernel:
+//     out_i = sum_j softmax_j(c q_i . k_j) v_j,     lse_i = log sum_j exp(c q_i . k_j)
+// in one pass over the keys with the running maximum and sum of the softmax.  attention_weights_kernel:
+//     w_j = sum over a KV head's query heads and rows of exp(c q_i . k_j - lse_i)
+// which needs lse alone, so keys are the outer loop and nothing of size rows x keys is stored.
+//
+// Both keep the products' operands in the layouts of v_mfma_f32_32x32x16: A holds row m = lane % 32, k = 8
+// (lane / 32) + 0..7; B column n = lane % 32, the same k; C column n = lane % 32 and rows 8 (i / 4) + 4 (lane /
+// 32) + i % 4 in register i.
+#include <algorithm>
+#include <initializer_list>
+
+#include "r2o_common.hpp"
+
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+constexpr int kRows = 128;      // query rows of a workgroup: 4 waves of 32
+constexpr int kTile = 64;       // keys of a tile
+constexpr int kTileBytes = kTile * 256;
+constexpr int kNoWindow = 1 << 30;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The running maximum is raised only when a tile exceeds it by more than this (log2 units): p stays below 2^8
+// and most tiles skip the rescaling of 64 accumulators.  Maximum, sum and accumulators refer to one value, so
+// the quotient is exact.
+constexpr float kSlack = 8.f;
+
+template <int RF>
+__device__ __forceinline__ f16v mfma32(r2o_u4 a, r2o_u4 b, f16v c) {
+    if constexpr (RF == 0)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(r2o_bf16x8, a), __builtin_bit_cast(r2o_bf16x8, b),
+                                                       c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(r2o_half8, a), __builtin_bit_cast(r2o_half8, b), c,
+                                                      0, 0, 0);
+}
+
+template <int RF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    return RF == 0 ? r2o_pack_bf2(lo, hi) : r2o_pack_h2(lo, hi);
+}
+
+__device__ __forceinline__ void load_lds16(const void* gsrc, unsigned char* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gsrc,
+                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// One wave's 16 rows of a 64-row tile into LDS, rows from `row0` on clamped to `last`: a row is 16 chunks of 16
+// bytes, chunk c of row r at place c ^ swizzle(r).  The hardware writes lane l at 16 l, so the swizzle is made by
+// which chunk a lane reads.  SWZ 0: r & 7, for reads of one chunk by 32 rows; 1: 2 (r & 3), for transposing reads
+// of two chunks by 4 rows.
+template <int SWZ>
+__device__ __forceinline__ void stage_rows(const uint16_t* base, int64_t stride, int row0, int last, unsigned char* lds,
+                                           int wave, int lane) {
+    const int r4 = lane >> 4, place = lane & 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 16 * wave + 4 * i + r4;
+        const int c = place ^ (SWZ == 0 ? (r & 7) : 2 * (r & 3));
+        load_lds16(base + (int64_t)min(row0 + r, last) * stride + 8 * c, lds + (16 * wave + 4 * i) * 256);
+    }
+}
+
+// 32 rows of a staged tile (SWZ 0) as the A operand of step t (channels 16 t ..).
+__device__ __forceinline__ r2o_u4 read_rows(const unsigned char* tile, int block, int t, int lane) {
+    const int r = lane & 31, c = 2 * t + (lane >> 5);
+    return *reinterpret_cast<const r2o_u4*>(tile + (32 * block + r) * 256 + 16 * (c ^ (r & 7)));
+}
+
+// 16 keys from 16 kb on, transposed, as the A operand of channels 32 db ..: lane half h holds keys 4 h + 0..3 and
+// 8 + 4 h + 0..3, the order in which the products' C registers hold the probabilities.
+__device__ __forceinline__ r2o_u4 read_values(const unsigned char* tile, int kb, int db, int lane) {
+    const int i = lane & 15, r = i >> 2;
+    const int c = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    const unsigned char* p = tile + (16 * kb + 4 * (lane >> 5) + r) * 256 + 16 * (c ^ (2 * r)) + 8 * (i & 1);
+    typedef __attribute__((address_space(3))) s4v lds4;
+    const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+    const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * 256));
+    const r2o_u2 a = __builtin_bit_cast(r2o_u2, lo), b = __builtin_bit_cast(r2o_u2, hi);
+    return r2o_u4{a[0], a[1], b[0], b[1]};
+}
+
+struct Lengths {
+    int q, n, off;  // rows, keys, position of row 0
+};
+
+__device__ __forceinline__ Lengths request_lengths(const r2o_prompt_params& a, int b) {
+    Lengths s;
+    s.q = a.query_lengths ? min(max(r2o_ldg(a.query_lengths + b), 0), (int)a.queries) : (int)a.queries;
+    s.n = a.key_lengths ? min(max(r2o_ldg(a.key_lengths + b), 0), (int)a.keys) : (int)a.keys;
+    s.off = s.n - s.q;
+    return s;
+}
+
+__device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
+    return j <= p && (j > p - window || j < sinks);
+}
+
+// Infinite or NaN.
+template <int RF>
+__device__ __forceinline__ bool not_finite(uint32_t bits16) {
+    constexpr uint32_t e = RF == 0 ? 0x7f80u : 0x7c00u;
+    return (bits16 & e) == e;
+}
+
+// In a tile that some row of the workgroup sees in part, a masked key's probability is 0, but 0 times an infinite
+// or NaN value is NaN.  A thread takes a quarter of a V row, turns such elements to zero in LDS and reports the row;
+// returns this wave's rows (16 wave ..) that had any.
+template <int RF>
+__device__ __forceinline__ uint32_t zero_not_finite(unsigned char* tile, int wave, int lane) {
+    r2o_u4* src = reinterpret_cast<r2o_u4*>(tile + (16 * wave + (lane >> 2)) * 256 + 64 * (lane & 3));
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r2o_u4 x = src[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool lo = not_finite<RF>(x[k]), hi = not_finite<RF>(x[k] >> 16);
+            any |= lo | hi;
+            x[k] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        }
+        if (any) src[i] = x;
+    }
+    uint64_t b = __ballot(any);
+    b |= b >> 1;
+    b |= b >> 2;
+    uint32_t rows = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rows |= (uint32_t)((b >> (4 * r)) & 1) << r;
+    return rows;
+}
+
+// ------------------------------------------------------------------------------ prompt attention
+template <int RF>
+__global__ __launch_bounds__(256, 2) void prompt_attention_kernel(r2o_prompt_params a) {
+    __shared__ __align__(16) unsigned char k_lds[2][kTileBytes];
+    __shared__ __align__(16) unsigned char v_lds[2][kTileBytes];
+    __shared__ uint32_t bad_lds[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int h = blockIdx.y, b = blockIdx.z, kvh = h / (int)(a.hq / a.hkv);
+    const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kRows;  // the longest rows first
+    const Lengths s = request_lengths(a, b);
+    const int window = a.window ? (int)min(a.window, (int64_t)kNoWindow) : kNoWindow, sinks = a.window ? (int)a.sinks : 0;
+    const uint16_t* kbase = a.key + b * a.k_strides[0] + kvh * a.k_strides[1];
+    const uint16_t* vbase = a.value + b * a.v_strides[0] + kvh * a.v_strides[1];
+
+    const int row = row0 + 32 * wave + col;  // this lane's query row
+    r2o_u4 q[8];
+    {
+        const uint16_t* src = a.query + b * a.q_strides[0] + h * a.q_strides[1] +
+                              (int64_t)min(row, (int)a.queries - 1) * a.q_strides[2] + 8 * half;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) q[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
+    }
+
+    // key tiles that any row of the workgroup sees: sink tiles, then the window's
+    const int top = min(s.n - 1, s.off + min(row0 + kRows, s.q) - 1);  // last position of the workgroup's rows
+    const int first = max(0, s.off + row0 - window + 1) / kTile;
+    const int end = row0 < s.q && top >= 0 ? top / kTile + 1 : 0;
+    const int sink_tiles = end ? min((sinks + kTile - 1) / kTile, min(first, end)) : 0;
+    const int tiles = sink_tiles + max(0, end - first);
+    const int last = max(s.n - 1, 0);
+
+    const float c2 = a.sm_scale * kLog2e;
+    float m = -INFINITY, l = 0.f;
+    f16v acc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = f16v{};
+
+    auto tile_key = [&](int it) { return (it < sink_tiles ? it : first + it - sink_tiles) * kTile; };
+    auto stage = [&](int it) {
+        const int kt = tile_key(it);
+        stage_rows<0>(kbase, a.k_strides[2], kt, last, k_lds[it & 1], wave, lane);
+        stage_rows<1>(vbase, a.v_strides[2], kt, last, v_lds[it & 1], wave, lane);
+    };
+    const int pmin = s.off + row0 + 32 * wave, pmax = pmin + 31, p = pmin + col;
+    if (tiles > 0) stage(0);
+    for (int it = 0; it < tiles; ++it) {
+        const int kt = tile_key(it);
+        __syncthreads();  // the tile is there, and every wave is done with the one before
+        const int wg_min = s.off + row0;
+        uint64_t bad = 0;
+        if (!(kt + kTile - 1 <= wg_min && (kt > wg_min + kRows - 1 - window || kt + kTile <= sinks))) {
+            const uint32_t rows = zero_not_finite<RF>(v_lds[it & 1], wave, lane);
+            if (lane == 0) bad_lds[it & 1][wave] = rows;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 4; ++w) bad |= (uint64_t)__builtin_amdgcn_readfirstlane(bad_lds[it & 1][w]) << (16 * w);
+        }
+        if (it + 1 < tiles) stage(it + 1);
+        if (kt > pmax || (kt + kTile - 1 <= pmin - window && kt >= sinks)) continue;  // nothing for this wave
+        const unsigned char *kl = k_lds[it & 1], *vl = v_lds[it & 1];
+        f16v sc[2] = {f16v{}, f16v{}};
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) sc[kb] = mfma32<RF>(read_rows(kl, kb, t, lane), q[t], sc[kb]);
+        if (!(kt + kTile - 1 <= pmin && (kt > pmax - window || kt + kTile <= sinks))) {
+            const int pv = min(p, s.n - 1);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = kt + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
+                    sc[kb][i] = sees(pv, j, window, sinks) ? sc[kb][i] : -INFINITY;
+                }
+        }
+        float tmax = sc[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[kb][i]);
+        {
+            float x, y;
+            r2o_row_swap<32>(tmax, x, y);
+            tmax = fmaxf(x, y) * c2;  // -inf stays (c2 > 0)
+        }
+        if (__any(tmax > m + kSlack)) {
+            // of the rows that exceed it alone: a row's result does not depend on its neighbours
+            const float m_new = tmax > m + kSlack ? tmax : m;
+            const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] *= alpha;
+            m = m_new;
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        r2o_u4 pk[4];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i], c2, -mm));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i + 1], c2, -mm));
+                l += e0 + e1;
+                pk[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<RF>(e0, e1);
+            }
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] = mfma32<RF>(read_values(vl, kb, db, lane), pk[kb], acc[db]);
+        while (bad) {  // what was taken out, for the rows that see it
+            const int j = kt + __builtin_ctzll(bad);
+            bad &= bad - 1;
+            if (!sees(min(p, s.n - 1), j, window, sinks)) continue;
+            const uint16_t* src = vbase + (int64_t)j * a.v_strides[2] + 4 * half;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t x = r2o_ldg(src + 32 * db + 8 * (i >> 2) + (i & 3));
+                    if (not_finite<RF>(x)) acc[db][i] += RF == 0 ? r2o_bf16_to_f32(x) : r2o_f16_to_f32(x);
+                }
+        }
+    }
+
+    {
+        float x, y;
+        r2o_row_swap<32>(l, x, y);
+        l = x + y;
+    }
+    if (row >= (int)a.queries) return;
+    const bool live = row < s.q && m != -INFINITY;
+    const float inv = live ? 1.f / l : 0.f;
+    uint16_t* dst = a.out + b * a.o_strides[0] + h * a.o_strides[1] + (int64_t)row * a.o_strides[2];
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            r2o_u2 w;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                w[k] = live ? pack2<RF>(acc[db][4 * g + 2 * k] * inv, acc[db][4 * g + 2 * k + 1] * inv) : 0u;
+            *reinterpret_cast<r2o_u2*>(dst + 32 * db + 8 * g + 4 * half) = w;
+        }
+    if (half == 0)
+        a.lse[((int64_t)b * a.hq + h) * a.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+// ----------------------------------------------------------------------------- attention weights
+constexpr int kWeightKeys = 128;  // keys of a workgroup: 4 waves of 32, whose rows stay in registers
+
+// grid: (key tiles, splits, batch * hkv).  A split takes a share of the (query head, 64-row tile) pairs that see
+// the key tile; its sums go to `dst` ([splits, batch, hkv, keys]; the result itself where there is one split).
+template <int RF>
+__global__ __launch_bounds__(256, 2) void attention_weights_kernel(r2o_prompt_params a, float* dst) {
+    __shared__ __align__(16) unsigned char q_lds[2][kTileBytes];
+    __shared__ __align__(16) float lse_lds[2][kTile];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int kvh = (int)(blockIdx.z % a.hkv), b = (int)(blockIdx.z / a.hkv), group = (int)(a.hq / a.hkv);
+    const Lengths s = request_lengths(a, b);
+    const int window = a.window ? (int)min(a.window, (int64_t)kNoWindow) : kNoWindow, sinks = a.window ? (int)a.sinks : 0;
+    const int key0 = blockIdx.x * kWeightKeys, kw = key0 + 32 * wave, j = kw + col;
+
+    // rows that see any of the tile's keys: p >= key0, and without a sink among them p < last key + window
+    const int last_key = min(key0 + kWeightKeys, s.n) - 1;
+    const int row_lo = max(0, key0 - s.off);
+    const int row_hi = key0 < sinks ? s.q : min((int64_t)s.q, (int64_t)last_key + window - s.off);
+    const int first = row_lo / kTile, per_head = key0 < s.n ? max(0, (row_hi + kTile - 1) / kTile - first) : 0;
+    const int64_t pairs = (int64_t)per_head * group;
+    const int begin = (int)(pairs * blockIdx.y / gridDim.y), end = (int)(pairs * (blockIdx.y + 1) / gridDim.y);
+
+    float sum = 0.f, lost = 0.f;  // of up to hq / hkv * queries terms: what each addition loses is kept
+    if (begin < end) {
+        const float c2 = a.sm_scale * kLog2e;
+        r2o_u4 k[8];
+        const uint16_t* src = a.key + b * a.k_strides[0] + kvh * a.k_strides[1] + (int64_t)min(j, s.n - 1) * a.k_strides[2] + 8 * half;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) k[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
+        auto stage = [&](int it, int buf) {
+            const int h = kvh * group + it / per_head, r0 = (first + it % per_head) * kTile;
+            stage_rows<0>(a.query + b * a.q_strides[0] + h * a.q_strides[1], a.q_strides[2], r0, s.q - 1,
+                          q_lds[buf], wave, lane);
+            if (threadIdx.x < kTile) {
+                const int r = r0 + threadIdx.x;
+                float x = INFINITY;  // rows behind the request, and those that saw no key, give exp2(-inf)
+                if (r < s.q) x = r2o_ldg(a.lse_in + ((int64_t)b * a.hq + h) * a.queries + r) * kLog2e;
+                lse_lds[buf][threadIdx.x] = x == -INFINITY ? INFINITY : x;
+            }
+        };
+        stage(begin, 0);
+        for (int it = begin; it < end; ++it) {
+            const int buf = (it - begin) & 1;
+            __syncthreads();
+            if (it + 1 < end) stage(it + 1, buf ^ 1);
+            const int p0 = s.off + (first + it % per_head) * kTile;
+            if (p0 + kTile - 1 < kw || (kw + 31 <= p0 - window && kw >= sinks)) continue;
+            const bool full = p0 >= kw + 31 && (kw > p0 + kTile - 1 - window || kw + 32 <= sinks);
+            float part = 0.f;
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                f16v sc = f16v{};
+#pragma unroll
+                for (int t = 0; t < 8; ++t) sc = mfma32<RF>(read_rows(q_lds[buf], rb, t, lane), k[t], sc);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const r2o_f4 x = *reinterpret_cast<const r2o_f4*>(&lse_lds[buf][32 * rb + 8 * g + 4 * half]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * g + i], c2, -x[i]));
+                        if (full) part += e;
+                        else part += sees(p0 + 32 * rb + 8 * g + 4 * half + i, j, window, sinks) ? e : 0.f;
+                    }
+                }
+            }
+            const float add = part - lost, next = sum + add;
+            lost = (next - sum) - add;
+            sum = next;
+        }
+        float x, y;
+        r2o_row_swap<32>(sum, x, y);
+        sum = x + y;
+    }
+    if (half == 0 && j < (int)a.keys)
+        dst[((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * a.keys + j] = j < s.n ? sum : 0.f;
+}
+
+__global__ __launch_bounds__(256) void weights_join_kernel(const float* src, float* dst, int64_t n, int splits) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float sum = 0.f;
+    for (int k = 0; k < splits; ++k) sum += r2o_ldg(src + k * n + i);
+    dst[i] = sum;
+}
+
+bool strides_ok(const int64_t* st) { return st[0] >= 0 && st[1] >= 0 && st[2] >= 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0; }
+
+bool aligned(std::initializer_list<const void*> ps, uintptr_t n) {
+    for (const void* p : ps)
+        if (!p || reinterpret_cast<uintptr_t>(p) % n) return false;
+    return true;
+}
+
+bool shapes_ok(const r2o_prompt_params* p) {
+    constexpr int64_t kMost = 1 << 29;
+    return p && (p->dtype == 0 || p->dtype == 1) && p->batch >= 1 && p->hkv >= 1 && p->hq >= p->hkv && p->hq % p->hkv == 0 &&
+           p->batch * p->hkv <= 65535 && p->batch <= 65535 && p->hq <= 65535 && p->queries >= 1 && p->queries <= kMost &&
+           p->keys >= 1 && p->keys <= kMost && p->window >= 0 && p->sinks >= 0 && p->sinks <= kMost && p->sm_scale > 0.f &&
+           p->sm_scale < INFINITY && aligned({p->query, p->key}, 16) && strides_ok(p->q_strides) && strides_ok(p->k_strides) &&
+           reinterpret_cast<uintptr_t>(p->query_lengths) % 4 == 0 && reinterpret_cast<uintptr_t>(p->key_lengths) % 4 == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int r2o_prompt_attention(const r2o_prompt_params* p, void* stream) {
+    if (!shapes_ok(p) || !aligned({p->value, p->out}, 16) || !aligned({p->lse}, 4) || !strides_ok(p->v_strides) ||
+        !strides_ok(p->o_strides))
+        return R2O_EINVAL;
+    const dim3 grid((unsigned)((p->queries + kRows - 1) / kRows), (unsigned)p->hq, (unsigned)p->batch);
+    const hipStream_t st = (hipStream_t)stream;
+    if (p->dtype == 0) hipLaunchKernelGGL(prompt_attention_kernel<0>, grid, dim3(256), 0, st, *p);
+    else hipLaunchKernelGGL(prompt_attention_kernel<1>, grid, dim3(256), 0, st, *p);
+    R2O_CHECK_LAUNCH();
+    return R2O_OK;
+}
+
+int r2o_attention_weights(const r2o_prompt_params* p, void* stream) {
+    if (!shapes_ok(p) || !aligned({p->lse_in, p->weights}, 4) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
+    const int64_t n = p->batch * p->hkv * p->keys;
+    if (p->splits > 1 && (!aligned({p->scratch}, 4) || p->scratch_floats < p->splits * n)) return R2O_EINVAL;
+    if ((n + 255) / 256 > 0x7fffffff) return R2O_EINVAL;
+    const dim3 grid((unsigned)((p->keys + kWeightKeys - 1) / kWeightKeys), (unsigned)p->splits, (unsigned)(p->batch * p->hkv));
+    const hipStream_t st = (hipStream_t)stream;
+    float* dst = p->splits > 1 ? p->scratch : p->weights;
+    if (p->dtype == 0) hipLaunchKernelGGL(attention_weights_kernel<0>, grid, dim3(256), 0, st, *p, dst);
+    else hipLaunchKernelGGL(attention_weights_kernel<1>, grid, dim3(256), 0, st, *p, dst);
+    R2O_CHECK_LAUNCH();
+    if (p->splits > 1) {
+        hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p->scratch, p->weights, n,
+                           (int)p->splits);
+        R2O_CHECK_LAUNCH();
+    }
+    return R2O_OK;
+}
+
+}  // extern "C"

@@ -29,6 +29,7 @@ from .cache import (
     precision_cache_active_storage_breakdown,
     precision_cache_storage_breakdown,
 )
+from .paged import PagedCache, paged_attention, paged_evict, paged_extend
 from .policy import (
     LayerCompressionPlan,
     PageAssignment,
@@ -39,6 +40,7 @@ from .policy import (
     plan_from_pages,
     project_token_bits_to_pages,
 )
+from .prompt import attention_weights, prompt_attention
 from .reference import normalized_fwht, triton_mixed_reference
 from .rope import FusedQwen3Rotary, FusedRotary, qwen3_qk_norm_rope, qwen_qk_mrope
 from .splitk import (

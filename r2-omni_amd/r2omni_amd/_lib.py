@@ -135,6 +135,48 @@ class CacheBuild(ctypes.Structure):  # r2o_cache_build_params
     ]
 
 
+class PromptParams(ctypes.Structure):  # r2o_prompt_params
+    _fields_ = [
+        ("query", c_vp), ("key", c_vp), ("value", c_vp), ("out", c_vp), ("lse", c_vp),
+        ("q_strides", c_i64 * 3), ("k_strides", c_i64 * 3), ("v_strides", c_i64 * 3), ("o_strides", c_i64 * 3),
+        ("query_lengths", c_vp), ("key_lengths", c_vp), ("batch", c_i64), ("hq", c_i64), ("hkv", c_i64),
+        ("queries", c_i64), ("keys", c_i64), ("dtype", c_i64), ("window", c_i64), ("sinks", c_i64),
+        ("sm_scale", ctypes.c_float), ("lse_in", c_vp), ("weights", c_vp), ("scratch", c_vp), ("scratch_floats", c_i64),
+        ("splits", c_i64),
+    ]
+
+
+class PagedCacheParams(ctypes.Structure):  # r2o_paged_cache
+    _fields_ = [
+        ("key_pages", c_vp), ("value_pages", c_vp), ("weight_pages", c_vp), ("page_table", c_vp), ("lengths", c_vp),
+        ("key_strides", c_i64 * 3), ("value_strides", c_i64 * 3), ("weight_strides", c_i64 * 2), ("table_stride", c_i64),
+        ("pages", c_i64), ("max_pages", c_i64), ("page_size", c_i64), ("batch", c_i64), ("hkv", c_i64), ("dtype", c_i64),
+    ]
+
+
+class PagedExtend(ctypes.Structure):  # r2o_paged_extend_params
+    _fields_ = [
+        ("cache", PagedCacheParams), ("key", c_vp), ("value", c_vp), ("weights", c_vp), ("counts", c_vp),
+        ("key_strides", c_i64 * 3), ("value_strides", c_i64 * 3), ("weights_strides", c_i64 * 2), ("rows", c_i64),
+    ]
+
+
+class PagedAttention(ctypes.Structure):  # r2o_paged_attention_params
+    _fields_ = [
+        ("cache", PagedCacheParams), ("query", c_vp), ("append_key", c_vp), ("append_value", c_vp),
+        ("query_strides", c_i64 * 2), ("append_strides", c_i64 * 4), ("hq", c_i64), ("window", c_i64), ("sinks", c_i64),
+        ("sm_scale", ctypes.c_float), ("out", c_vp), ("lse", c_vp), ("partial_out", c_vp), ("partial_ml", c_vp),
+        ("logits", c_vp), ("partial_states", c_i64), ("logits_floats", c_i64), ("workers", c_i64),
+    ]
+
+
+class PagedEvict(ctypes.Structure):  # r2o_paged_evict_params
+    _fields_ = [
+        ("source", PagedCacheParams), ("target", PagedCacheParams), ("keep", c_i64), ("sinks", c_i64), ("recent", c_i64),
+        ("kept", c_vp), ("target_lengths", c_vp),
+    ]
+
+
 _SIGNATURES = {
     "r2o_plan_work_items": (ctypes.POINTER(PlanRun), c_i64, ctypes.POINTER(PlanConfig), c_vp, c_i64, c_i64, c_i64,
                             c_vp, c_i64, c_vp, c_i64, ctypes.POINTER(c_i64)),
@@ -156,6 +198,11 @@ _SIGNATURES = {
     "r2o_cache_page_words": (c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64),
     "r2o_cache_build": (ctypes.POINTER(CacheBuild), c_vp),
     "r2o_ring_flush": (ctypes.POINTER(RingFlush), c_vp),
+    "r2o_prompt_attention": (ctypes.POINTER(PromptParams), c_vp),
+    "r2o_attention_weights": (ctypes.POINTER(PromptParams), c_vp),
+    "r2o_paged_extend": (ctypes.POINTER(PagedExtend), c_vp),
+    "r2o_paged_attention": (ctypes.POINTER(PagedAttention), c_vp),
+    "r2o_paged_evict": (ctypes.POINTER(PagedEvict), c_vp),
     "r2o_fwht128": (c_vp, c_vp, c_i64, c_i64, c_vp),
     "r2o_qk_mrope": (c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp,
                      c_i64, c_i64, c_i64, c_vp),
@@ -222,6 +269,28 @@ def check(rc: int, name: str) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
+
+
+def launch(name: str, params: ctypes.Structure, device: torch.device) -> None:
+    """Call an entry point that takes (params, stream), on the device's current stream, with the device current for
+    the launches."""
+    stream = stream_of(device)
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(getattr(load(), name)(ctypes.byref(params), stream), name)
+    else:
+        with torch.cuda.device(device):
+            check(getattr(load(), name)(ctypes.byref(params), stream), name)
+
+
+_NUM_CUS: dict[int, int] = {}
+
+
+def num_cus(device: torch.device) -> int:
+    """Compute units of a GPU (looked up once for each)."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index not in _NUM_CUS:
+        _NUM_CUS[index] = int(torch.cuda.get_device_properties(index).multi_processor_count)
+    return _NUM_CUS[index]
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

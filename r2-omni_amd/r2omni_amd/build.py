@@ -21,7 +21,7 @@ CSRC = os.path.join(ROOT_DIR, "csrc")
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libr2o_sspa.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ("r2o_decode.hip", "r2o_pack.hip", "r2o_rope.hip", "r2o_plan.cpp")  # r2o_plan.cpp: host code only
+SOURCES = ("r2o_decode.hip", "r2o_pack.hip", "r2o_rope.hip", "r2o_prompt.hip", "r2o_paged.hip", "r2o_plan.cpp")  # r2o_plan.cpp: host code only
 # bench.py's streaming-read probe, a library of its own (not part of the decode C-ABI)
 BENCH_LIB_PATH = os.path.join(PKG_DIR, "libr2o_bench.so")
 BENCH_SOURCES = ("bench_read.hip",)
