@@ -469,11 +469,13 @@ int r2o_qkv_norm_rope(const uint16_t* q, const uint16_t* k, const uint16_t* v, u
 
 /* ------------------------------------- prompt attention and accumulated weights ---- */
 
+#define R2O_MAX_ROW_STRIDE (1 << 24) /* elements from one row of a prompt to the next */
+
 /* Row i of a request with q query rows and n keys (query_lengths / key_lengths [batch], NULL for all rows; a
  * length is clamped to its tensor) stands at position p = n - q + i and sees key j where j <= p and, with a window
  * (window > 0), p - j < window or j < sinks.  Tensors hold bf16 (dtype 0) or fp16 (1) rows of 128 unit-strided
- * channels, 16-byte aligned, with element strides (batch, head, row), each a multiple of 8; hq is a multiple of
- * hkv, query head h reads KV head h / (hq / hkv).  lse, lse_in: fp32 [batch, hq, queries], contiguous. */
+ * channels, 16-byte aligned, with element strides (batch, head, row), each a multiple of 8, the rows' at most
+ * 2^24; hq is a multiple of hkv, query head h reads KV head h / (hq / hkv).  lse, lse_in: fp32 [batch, hq, queries], contiguous. */
 typedef struct r2o_prompt_params {
     const uint16_t* query;    /* [batch, hq, queries, 128] */
     const uint16_t* key;      /* [batch, hkv, keys, 128] */
@@ -504,10 +506,11 @@ int r2o_attention_weights(const r2o_prompt_params* p, void* stream);
 
 #define R2O_PAGED_MAX_BATCH 1024
 #define R2O_PAGED_MAX_WORKERS 4096
+#define R2O_PAGED_MAX_SLOT_STRIDE (1 << 24) /* elements from one slot's row to the next */
 
 /* Slot j of request b is slot j % page_size of page page_table[b][j / page_size], for every KV head; lengths[b]
  * slots are filled (clamped to max_pages * page_size).  Slots of a page id outside [0, pages) are not seen and not
- * written.  K and V rows as above with element strides (page, head, slot); weight_pages (may be NULL): fp32 with
+ * written.  K and V rows as above with element strides (page, head, slot) below 2^31, the slots' at most 2^24; weight_pages (may be NULL): fp32 with
  * element strides (page, head), slots unit-strided. */
 typedef struct r2o_paged_cache {
     uint16_t* key_pages;      /* [pages, hkv, page_size, 128] */

@@ -11,14 +11,18 @@
 
 namespace {
 
-typedef short s4v __attribute__((ext_vector_type(4)));
-
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Filled slots of a request, within what its page table can hold.
 __device__ __forceinline__ int filled(const r2o_paged_cache& c, int b) {
     return min(max(r2o_ldg(c.lengths + b), 0), (int)(c.max_pages * c.page_size));
+}
+
+// A word at an address that the whole wave shares and that nothing writes meanwhile, through the scalar cache: it
+// waits for no vector load and no vector load waits for it.
+__device__ __forceinline__ int load_uniform(const int32_t* p) {
+    return *(const __attribute__((address_space(4))) int32_t*)p;
 }
 
 __device__ __forceinline__ int shift_of(const r2o_paged_cache& c) { return 31 - __builtin_clz((int)c.page_size); }
@@ -53,9 +57,33 @@ __global__ __launch_bounds__(256) void paged_extend_kernel(r2o_paged_extend_para
 // ------------------------------------------------------------------------------------- attention
 constexpr int kWaves = 4;
 constexpr int kSlots = 32;                 // slots of a wave's tile
-constexpr int kVBytes = kSlots * 256;
 constexpr int kMinTiles = 4;               // tiles a workgroup takes at least: one a wave
+constexpr int kNoWindow = 1 << 30;
 constexpr float kSlack = 8.f;
+
+// r2o_paged_attention_params in the kernels' widths (the host has checked that they fit): fewer scalar registers.
+struct AttentionArgs {
+    uint16_t *key, *value;
+    float* weight;
+    const int32_t *table, *lengths;
+    const uint16_t *query, *new_key, *new_value;
+    uint16_t* out;
+    float *lse, *partial_out, *partial_ml, *logits;
+    int k_page, k_head, k_slot, v_page, v_head, v_slot, w_page, w_head, table_stride;
+    int q_batch, q_head, nk_batch, nk_head, nv_batch, nv_head;
+    int pages, last_page, shift, batch, hkv, group, window, sinks, workers;
+    float c2;  // scale, in log2 units
+};
+
+// A kernel's arguments where the hardware put them.  Each place that asks anew loads what it uses again, instead of
+// holding 60 words in scalar registers from the first use to the last, which spills.
+typedef const __attribute__((address_space(4))) AttentionArgs Args;
+
+__device__ __forceinline__ Args& kernel_args() {
+    auto p = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
 
 template <int RF>
 __device__ __forceinline__ r2o_f4 mfma16(r2o_u4 a, r2o_u4 b, r2o_f4 c) {
@@ -74,51 +102,80 @@ struct Tiles {
     __device__ __forceinline__ bool sees(int j, int sinks) const { return j < n && (j >= lo || j < sinks); }
 };
 
-__device__ __forceinline__ Tiles request_tiles(const r2o_paged_attention_params& p, int b) {
+__device__ __forceinline__ Tiles tiles_of(Args& a, int length) {
     Tiles t;
-    t.n = filled(p.cache, b);
-    t.lo = p.window ? max(0, t.n - (int)min(p.window, (int64_t)1 << 30)) : 0;
+    t.n = min(max(length, 0), (a.last_page + 1) << a.shift);
+    t.lo = max(0, t.n - a.window);
     t.first = t.lo / kSlots;
-    t.sink_tiles = p.window ? min(((int)p.sinks + kSlots - 1) / kSlots, t.first) : 0;
+    t.sink_tiles = min((a.sinks + kSlots - 1) / kSlots, t.first);
     t.count = t.sink_tiles + (t.n + kSlots - 1) / kSlots - t.first;
     return t;
 }
 
-// Sum over the batch of the requests' tiles (one head's), by the whole wave.
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, R2O_WAVE);
-    return x;
-}
-
-// How the tiles of all (request, head) pairs, in order, are shared: worker i takes [i total / workers, (i + 1)
-// total / workers).  The partial state of worker i for pair q lies in slot i + q: along the list of (worker,
-// pair) one of the two grows by one at a time, so the slots differ.
+// The tiles of all (request, head) pairs, in order, shared evenly: worker i takes `each` tiles from begin(i) on, the
+// first `more` workers one more.  The partial state of worker i for pair q lies in slot i + q: along the list of
+// (worker, pair) one of the two grows by one at a time, so the slots differ.
 struct Share {
-    int64_t total;
-    int workers;
-    __device__ __forceinline__ int64_t begin(int i) const { return total * i / workers; }
-    // the worker that takes tile u
-    __device__ __forceinline__ int worker(int64_t u) const {
-        int64_t i = u * workers / total;
-        while (begin((int)i) > u) --i;
-        while (begin((int)i + 1) <= u) ++i;
-        return (int)i;
+    int total, workers, each, more;
+    __device__ __forceinline__ int begin(int i) const { return i * each + min(i, more); }
+    __device__ __forceinline__ int worker(int u) const {  // the one that takes tile u
+        const int wide = more * (each + 1);
+        return u < wide ? (int)((uint32_t)u / (uint32_t)(each + 1)) : more + (int)((uint32_t)(u - wide) / (uint32_t)each);
     }
 };
 
-__device__ __forceinline__ Share make_share(const r2o_paged_attention_params& p) {
-    const int lane = threadIdx.x & 63;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < (int)p.cache.batch; b0 += 64) {
-        const int b = b0 + lane;
-        total += wave_sum(b < (int)p.cache.batch ? request_tiles(p, b).count : 0);
+// The wave goes through the batch 64 requests at a time: this lane's request's tiles, and the sum of those up to it.
+struct Lane {
+    int count, upto;
+};
+
+__device__ __forceinline__ Lane lane_tiles(Args& a, int b0) {
+    const int lane = threadIdx.x & 63, b = b0 + lane;
+    Lane x;
+    x.count = b < a.batch ? tiles_of(a, r2o_ldg(a.lengths + b)).count : 0;
+    x.upto = x.count;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(x.upto, m, R2O_WAVE);
+        if (lane >= m) x.upto += y;
     }
-    total *= p.cache.hkv;
+    return x;
+}
+
+__device__ __forceinline__ Share make_share(Args& a) {
+    int total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) total += __builtin_amdgcn_readlane(lane_tiles(a, b0).upto, 63);
     Share s;
-    s.total = total;
-    s.workers = (int)max((int64_t)1, min(p.workers, (total + kMinTiles - 1) / kMinTiles));
+    s.total = total * a.hkv;
+    s.workers = max(1, min(a.workers, (s.total + kMinTiles - 1) / kMinTiles));
+    s.each = (int)((uint32_t)s.total / (uint32_t)s.workers);
+    s.more = s.total - s.each * s.workers;
     return s;
+}
+
+// The request that holds tile u, and the tiles before it.
+__device__ __forceinline__ int request_of(Args& a, int u, int& before) {
+    before = 0;
+    for (int b0 = 0;; b0 += 64) {
+        const Lane x = lane_tiles(a, b0);
+        const int all = __builtin_amdgcn_readlane(x.upto, 63) * a.hkv;
+        if (u < before + all) {
+            const int at = __builtin_ctzll(__ballot(before + x.upto * a.hkv > u));
+            before += __builtin_amdgcn_readlane(x.upto - x.count, at) * a.hkv;
+            return b0 + at;
+        }
+        before += all;
+    }
+}
+
+// The tiles of the requests before b.
+__device__ __forceinline__ int tiles_before(Args& a, int b) {
+    int before = 0;
+    for (int b0 = 0; b0 <= b; b0 += 64) {
+        const Lane x = lane_tiles(a, b0);
+        before += b - b0 < 64 ? __builtin_amdgcn_readlane(x.upto - x.count, b - b0) : __builtin_amdgcn_readlane(x.upto, 63);
+    }
+    return before * a.hkv;
 }
 
 __device__ __forceinline__ void load_lds16(const void* gsrc, unsigned char* lds) {
@@ -126,170 +183,241 @@ __device__ __forceinline__ void load_lds16(const void* gsrc, unsigned char* lds)
                                      (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-// One workgroup: its share of the tiles, 4 waves taking a pair's tiles in turn.  Per tile of 32 slots a wave loads
-// K rows into registers as the A operand of S^T = K Q^T (16 slots x 16 heads a product), V rows into LDS by
-// asynchronous loads, from which transposing reads give the A operand of O^T = V^T P^T; P^T's operand is the C
-// registers of S^T as they are, the slots of a product being summed in that order on both sides.
-template <int RF>
-__global__ __launch_bounds__(256, 2) void paged_partial_kernel(r2o_paged_attention_params p) {
-    __shared__ __align__(16) unsigned char lds[kWaves][2][kVBytes];
-    __shared__ float ml_lds[kWaves][2][16];
-    const r2o_paged_cache& c = p.cache;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
-    const int group = (int)(p.hq / c.hkv), hkv = (int)c.hkv, shift = shift_of(c);
-    const Share share = make_share(p);
-    const int worker = blockIdx.x;
-    if (worker >= share.workers || share.total == 0) return;
-    int64_t u = share.begin(worker);
-    const int64_t u_end = share.begin(worker + 1);
-    const float c2 = p.sm_scale * kLog2e;
-    const int sinks = (int)p.sinks;
+constexpr int vmcnt_imm(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4) | (0xF << 8); }
 
-    // the request of tile u
-    int b = 0;
-    int64_t base = 0;
-    Tiles t = request_tiles(p, 0);
-    while (u >= base + (int64_t)t.count * hkv) {
-        base += (int64_t)t.count * hkv;
-        t = request_tiles(p, ++b);
+// The pages of a tile's two halves; -1 for one outside the pool.
+__device__ __forceinline__ void tile_pages(Args& a, const int32_t* table, int j0, int (&page)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int id = load_uniform(table + min((j0 + 16 * k) >> a.shift, a.last_page));
+        page[k] = (uint32_t)id < (uint32_t)a.pages ? id : -1;
+    }
+}
+
+// One tile of a (request, head): its page ids and the place of its slots in LDS.  A wave's stage holds 32 K rows, then
+// 32 V rows, each row 16 chunks of 16 bytes: K row r's chunk c at place c ^ (r & 7), for reads of one chunk by 16 rows;
+// V row r's at c ^ 2 (r & 3), for transposing reads of two chunks by four rows.
+constexpr int kStage = 2 * kSlots * 256;
+
+struct Head {
+    const uint16_t *k, *v;   // the head's rows in the pools
+    int k_page, v_page;      // strides, elements
+    int k_slot, v_slot;
+    int shift;
+    int k_lane[2], v_lane;   // byte offsets of this lane's row and chunk among four rows (K: among four even, four odd)
+};
+
+// Asynchronous loads of one tile into a stage: 16 of 1 KB, four rows each.
+__device__ __forceinline__ void load_tile(const Head& x, int j0, const int (&page)[2], unsigned char* stage) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const int at = (j0 + 16 * m) & ((1 << x.shift) - 1), id = max(page[m], 0);
+        const unsigned char* k = reinterpret_cast<const unsigned char*>(x.k + (int64_t)id * x.k_page + (int64_t)at * x.k_slot);
+        const unsigned char* v = reinterpret_cast<const unsigned char*>(x.v + (int64_t)id * x.v_page + (int64_t)at * x.v_slot);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            load_lds16(k + (int64_t)(8 * i) * x.k_slot + x.k_lane[i & 1], stage + 4096 * m + 1024 * i);
+            load_lds16(v + (int64_t)(8 * i) * x.v_slot + x.v_lane, stage + 8192 + 4096 * m + 1024 * i);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)p;
+}
+
+// A stage's K rows l16 and 16 + l16 as A operands: chunks 4 x + g, at `row` + (16 (4 x + g) ^ the row's swizzle).  In
+// assembly, with its wait: before a load from LDS that the compiler makes it waits for every asynchronous load into
+// LDS, the next tile's among them.
+__device__ __forceinline__ void read_keys(uint32_t row, uint32_t chunk, r2o_u4 (&k)[2][4]) {
+    const uint32_t a = row + chunk, b = row + (chunk ^ 64);
+    asm volatile(
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %8 offset:128\n\tds_read_b128 %3, %9 offset:128\n\t"
+        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %8 offset:4224\n\t"
+        "ds_read_b128 %7, %9 offset:4224\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]), "=&v"(k[1][1]), "=&v"(k[1][2]), "=&v"(k[1][3])
+        : "v"(a), "v"(b)
+        : "memory");
+}
+
+// V rows 4 g + 0..3 and 16 more, transposed, as the A operands of channels 64 d + 16 x ..
+__device__ __forceinline__ void read_values(uint32_t row, uint32_t chunk, int d, r2o_u4 (&v)[4]) {
+    const uint32_t a = row + chunk + 128 * d, b = row + (chunk ^ 32) + 128 * d, c = row + (chunk ^ 64) + 128 * d,
+                   e = row + (chunk ^ 96) + 128 * d;
+    r2o_u2 lo[4], hi[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %3, %11\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:4096\n\tds_read_b64_tr_b16 %5, %9 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %6, %10 offset:4096\n\tds_read_b64_tr_b16 %7, %11 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+        : "v"(a), "v"(b), "v"(c), "v"(e)
+        : "memory");
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = r2o_u4{lo[x][0], lo[x][1], hi[x][0], hi[x][1]};
+}
+
+// One workgroup: its share of the tiles, 4 waves taking a pair's tiles in turn, each with its own softmax state and
+// two LDS stages: the next tile's loads go out before this one's products, its page ids one tile earlier still.
+// S^T = K Q^T (16 slots x 16 heads a product), O^T += V^T P^T; P^T's operand is the C registers of S^T as they are: the
+// slots of a product are summed in that order on both sides.
+template <int RF, bool WEIGHTS>
+__global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
+    __shared__ __align__(16) unsigned char lds[kWaves][2][kStage];
+    __shared__ float ml_lds[kWaves][2][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+    const int worker = blockIdx.x;
+    int u, u_end, base, b;
+    {
+        Args& a = kernel_args();
+        const Share share = make_share(a);
+        if (worker >= share.workers || share.total == 0) return;
+        u = share.begin(worker);
+        u_end = share.begin(worker + 1);
+        b = request_of(a, u, base);
     }
     while (u < u_end) {
-        while (u >= base + (int64_t)t.count * hkv) {
-            base += (int64_t)t.count * hkv;
-            t = request_tiles(p, ++b);
+        Args& a = kernel_args();
+        Tiles t = tiles_of(a, load_uniform(a.lengths + b));
+        while (u >= base + t.count * a.hkv) {
+            base += t.count * a.hkv;
+            t = tiles_of(a, load_uniform(a.lengths + ++b));
         }
-        const int h = (int)((u - base) / t.count);
-        const int64_t pair_base = base + (int64_t)h * t.count;
-        const int t0 = (int)(u - pair_base), t1 = (int)min((int64_t)t.count, u_end - pair_base);
+        const int h = (int)((uint32_t)(u - base) / (uint32_t)t.count), pair_base = base + h * t.count;
+        const int t0 = u - pair_base, t1 = min(t.count, u_end - pair_base), group = a.group, sinks = min(a.sinks, t.n);
+        const int new_slot = a.new_key ? t.n - 1 : -1;
+        const float c2 = a.c2;
 
         r2o_u4 q[4];
         {
-            const uint16_t* src = p.query + b * p.query_strides[0] + (int64_t)(h * group + min(l16, group - 1)) * p.query_strides[1] + 8 * g;
+            const uint16_t* src = a.query + (int64_t)b * a.q_batch + (int64_t)(h * group + min(l16, group - 1)) * a.q_head + 8 * g;
 #pragma unroll
             for (int k = 0; k < 4; ++k) q[k] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 32 * k));
         }
-        const uint16_t* kpool = c.key_pages + h * c.key_strides[1];
-        const uint16_t* vpool = c.value_pages + h * c.value_strides[1];
-        const uint16_t* new_k = p.append_key + b * p.append_strides[0] + h * p.append_strides[1];
-        const uint16_t* new_v = p.append_value + b * p.append_strides[2] + h * p.append_strides[3];
-        const int new_slot = p.append_key ? t.n - 1 : -1;
-        const int32_t* table = c.page_table + b * c.table_stride;
-        const int last_page = (int)c.max_pages - 1, in_page = (1 << shift) - 1;
-        const int kp = (int)c.key_strides[0], ks = (int)c.key_strides[2], vp0 = (int)c.value_strides[0], vs = (int)c.value_strides[2];
-
-        auto pages_at = [&](int j0, int (&page)[2]) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int id = r2o_ldg(table + min((j0 + 16 * k) >> shift, last_page));
-                page[k] = __builtin_amdgcn_readfirstlane((uint32_t)id < (uint32_t)c.pages ? id : -1);
-            }
-        };
-        auto load = [&](int j0, const int (&page)[2], r2o_u4 (&k)[2][4], unsigned char* vl) {
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int j = j0 + 16 * m + l16;
-                const uint16_t* src = kpool + (int64_t)max(page[m], 0) * kp + (int64_t)(j & in_page) * ks;
-                if (j == new_slot) src = new_k;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) k[m][x] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 32 * x + 8 * g));
-            }
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {  // 4 rows at a time; chunk cc of row r lies at cc ^ 2 (r & 3)
-                const int j = j0 + 4 * x + g, cc = l16 ^ (2 * g);
-                const uint16_t* src = vpool + (int64_t)max(page[x >> 2], 0) * vp0 + (int64_t)(j & in_page) * vs;
-                if (j == new_slot) src = new_v;
-                load_lds16(src + 8 * cc, vl + 1024 * x);
-            }
-        };
+        Head head;
+        head.k = a.key + (int64_t)h * a.k_head;
+        head.v = a.value + (int64_t)h * a.v_head;
+        head.k_page = a.k_page;
+        head.v_page = a.v_page;
+        head.k_slot = a.k_slot;
+        head.v_slot = a.v_slot;
+        head.shift = a.shift;
+        head.k_lane[0] = 2 * g * a.k_slot + 16 * (l16 ^ g);
+        head.k_lane[1] = 2 * g * a.k_slot + 16 * (l16 ^ (g + 4));
+        head.v_lane = 2 * g * a.v_slot + 16 * (l16 ^ (2 * g));
+        const int32_t* table = a.table + (int64_t)b * a.table_stride;
+        float* logits = WEIGHTS ? a.logits + (int64_t)pair_base * group * kSlots : nullptr;
 
         float m = -INFINITY, l = 0.f;
         r2o_f4 acc[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = r2o_f4{};
-        for (int it = t0 + wave; it < t1; it += kWaves) {
-            unsigned char* vl = lds[wave][0];
+        int page[2] = {}, next[2] = {}, after[2] = {};
+        int it = t0 + wave;
+        if (it < t1) {
+            tile_pages(a, table, t.slot(it), page);
+            load_tile(head, t.slot(it), page, lds[wave][0]);
+            if (it + kWaves < t1) tile_pages(a, table, t.slot(it + kWaves), next);
+        }
+        for (int buf = 0; it < t1; it += kWaves, buf ^= 1) {
+            unsigned char *stage = lds[wave][buf], *other = lds[wave][buf ^ 1];
             const int j0 = t.slot(it);
-            int page[2];
-            pages_at(j0, page);
-            r2o_u4 k[2][4];
-            load(j0, page, k, vl);
-            r2o_f4 s[2] = {r2o_f4{}, r2o_f4{}};
-#pragma unroll
-            for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) s[mm] = mfma16<RF>(k[mm][x], q[x], s[mm]);
-            __builtin_amdgcn_s_waitcnt(0);
+            if (it + kWaves < t1) {
+                load_tile(head, t.slot(it + kWaves), next, other);
+                if (it + 2 * kWaves < t1) tile_pages(a, table, t.slot(it + 2 * kWaves), after);
+            } else {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            }
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(16));  // all but the next tile's have landed
             __builtin_amdgcn_wave_barrier();
-            const bool full = page[0] >= 0 && page[1] >= 0 && j0 + kSlots <= t.n && (j0 >= t.lo || j0 + kSlots <= sinks);
-            if (!full) {
-                // rows that are not seen: their logits leave, and their V bits, which may be anything, become zero
-#pragma unroll
-                for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (page[mm] < 0 || !t.sees(j0 + 16 * mm + 4 * g + i, sinks)) s[mm][i] = -INFINITY;
+            unsigned char* vl = stage + 8192;
+            const bool has_new = (uint32_t)(new_slot - j0) < (uint32_t)kSlots;
+            const bool part = (page[0] | page[1]) < 0 || j0 + kSlots > t.n || (j0 < t.lo && j0 + kSlots > sinks);
+            const int lo0 = page[0] < 0 ? 0x7fffffff : t.lo, lo1 = page[1] < 0 ? 0x7fffffff : t.lo;
+            const int sink0 = page[0] < 0 ? 0 : sinks, sink1 = page[1] < 0 ? 0 : sinks;
+            auto sees = [&](int j, int lo, int sink) { return ((j >= lo) & (j < t.n)) | (j < sink); };
+            if (has_new) {  // the appended rows, into the stage and into their page
+                Args& e = kernel_args();
+                const int r = new_slot - j0, page_new = r < 16 ? page[0] : page[1];
+                const int64_t at = new_slot & ((1 << e.shift) - 1);
+                const uint16_t* ks = e.new_key + (int64_t)b * e.nk_batch + (int64_t)h * e.nk_head;
+                const uint16_t* vs = e.new_value + (int64_t)b * e.nv_batch + (int64_t)h * e.nv_head;
+                uint16_t* kd = e.key + (int64_t)h * e.k_head + (int64_t)page_new * e.k_page + at * e.k_slot;
+                uint16_t* vd = e.value + (int64_t)h * e.v_head + (int64_t)page_new * e.v_page + at * e.v_slot;
+                if (lane < 32) {
+                    const r2o_u4 x = r2o_ldg(reinterpret_cast<const r2o_u4*>(lane < 16 ? ks : vs) + l16);
+                    *reinterpret_cast<r2o_u4*>(stage + (lane < 16 ? 0 : 8192) + 256 * r + 16 * (l16 ^ (lane < 16 ? r & 7 : 2 * (r & 3)))) = x;
+                    if (page_new >= 0) r2o_store8<true>((lane < 16 ? kd : vd) + 8 * l16, x);
+                }
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            }
+            if (part) {  // V bits of slots that are not seen may be anything: zero
                 const int r = lane >> 1;
-                if ((r < 16 ? page[0] : page[1]) < 0 || !t.sees(j0 + r, sinks))
+                if (!sees(j0 + r, r < 16 ? lo0 : lo1, r < 16 ? sink0 : sink1))
 #pragma unroll
                     for (int i = 0; i < 8; ++i) reinterpret_cast<r2o_u4*>(vl)[16 * r + 8 * (lane & 1) + i] = r2o_u4{};
-                __builtin_amdgcn_s_waitcnt(0);
-                __builtin_amdgcn_wave_barrier();
             }
-            if (new_slot >= j0 && new_slot < j0 + kSlots && lane < 32) {  // the appended rows into their page
-                const int page_new = new_slot - j0 < 16 ? page[0] : page[1], at = new_slot & in_page;
-                if (page_new >= 0) {
-                    const uint16_t* src = lane < 16 ? new_k : new_v;
-                    uint16_t* dst = lane < 16 ? c.key_pages + h * c.key_strides[1] + (int64_t)page_new * kp + (int64_t)at * ks
-                                              : c.value_pages + h * c.value_strides[1] + (int64_t)page_new * vp0 + (int64_t)at * vs;
-                    r2o_store8<true>(dst + 8 * l16, r2o_ldg(reinterpret_cast<const r2o_u4*>(src) + l16));
+            __builtin_amdgcn_wave_barrier();  // LDS operations of a wave stay in order
+            r2o_f4 s[2] = {r2o_f4{}, r2o_f4{}};
+            {
+                r2o_u4 k[2][4];
+                read_keys(lds_address(stage) + 256 * l16, (16 * g) ^ (16 * (l16 & 7)), k);
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) s[y] = mfma16<RF>(k[y][x], q[x], s[y]);
+            }
+            if (part) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + 4 * g + i;
+                    s[0][i] = sees(j, lo0, sink0) ? s[0][i] : -INFINITY;
+                    s[1][i] = sees(j + 16, lo1, sink1) ? s[1][i] : -INFINITY;
                 }
             }
-            if (c.weight_pages && l16 < group) {
-                float* dst = p.logits + ((pair_base + it) * group + l16) * kSlots;
+            if (WEIGHTS && l16 < group) {
+                float* dst = logits + ((int64_t)it * group + l16) * kSlots + 4 * g;
 #pragma unroll
-                for (int mm = 0; mm < 2; ++mm) *reinterpret_cast<r2o_f4*>(dst + 16 * mm + 4 * g) = s[mm] * c2;
+                for (int y = 0; y < 2; ++y) *reinterpret_cast<R2O_GLOBAL r2o_f4*>((R2O_GLOBAL float*)(dst + 16 * y)) = s[y] * c2;
             }
-            float tmax = s[0][0];
+            float tmax = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-            for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, s[mm][i]);
+            for (int i = 1; i < 4; ++i) tmax = fmaxf(tmax, fmaxf(s[0][i], s[1][i]));
             float x, y;
             r2o_row_swap<16>(tmax, x, y);
             tmax = fmaxf(x, y);
             r2o_row_swap<32>(tmax, x, y);
             tmax = fmaxf(x, y) * c2;
-            if (__any(tmax > m + kSlack)) {
-                const float m_new = fmaxf(m, tmax);
-                const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+            if (__any(tmax > m + kSlack)) {  // of the heads that exceed it alone
+                const float m_new = tmax > m + kSlack ? tmax : m;
+                const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
                 l *= alpha;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) acc[i] *= alpha;
                 m = m_new;
             }
-            const float mm_ = m == -INFINITY ? 0.f : m;
+            const float ms = m == -INFINITY ? 0.f : m;
             r2o_u4 pk;
 #pragma unroll
-            for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mm][i], c2, -mm_));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mm][i + 1], c2, -mm_));
-                    l += e0 + e1;
-                    pk[2 * mm + (i >> 1)] = pack2<RF>(e0, e1);
-                }
-            typedef __attribute__((address_space(3))) s4v lds4;
-            const int r = l16 >> 2;
-            const unsigned char* vp = vl + (4 * g + r) * 256 + 8 * (l16 & 1);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                const int cc = (2 * d + ((l16 & 3) >> 1)) ^ (2 * r);
-                const r2o_u2 lo = __builtin_bit_cast(r2o_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vp + 16 * cc)));
-                const r2o_u2 hi = __builtin_bit_cast(r2o_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vp + 16 * 256 + 16 * cc)));
-                acc[d] = mfma16<RF>(r2o_u4{lo[0], lo[1], hi[0], hi[1]}, pk, acc[d]);
+            for (int i = 0; i < 8; i += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], c2, -ms));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][(i & 3) + 1], c2, -ms));
+                l += e0 + e1;
+                pk[i >> 1] = pack2<RF>(e0, e1);
             }
-            __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                r2o_u4 v[4];
+                const int r = l16 >> 2;
+                read_values(lds_address(vl) + 1024 * g + 256 * r + 8 * (l16 & 1), (16 * ((l16 & 3) >> 1)) ^ (32 * r), d, v);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[4 * d + x] = mfma16<RF>(v[x], pk, acc[4 * d + x]);
+            }
             __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                page[y] = next[y];
+                next[y] = after[y];
+            }
         }
         {
             float x, y;
@@ -307,25 +435,26 @@ __global__ __launch_bounds__(256, 2) void paged_partial_kernel(r2o_paged_attenti
             ml_lds[wave][1][l16] = l;
         }
         __syncthreads();
-        const int64_t slot = (int64_t)worker + (int64_t)b * hkv + h;
-        for (int e = threadIdx.x; e < group * 32; e += 256) {
-            const int head = e >> 5, d4 = e & 31;
+        Args& e = kernel_args();
+        const int64_t state = ((int64_t)worker + b * e.hkv + h) * group;
+        for (int i = threadIdx.x; i < group * 32; i += 256) {
+            const int qh = i >> 5, d4 = i & 31;
             float mx = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml_lds[w][0][head]);
+            for (int x = 0; x < kWaves; ++x) mx = fmaxf(mx, ml_lds[x][0][qh]);
             const float ms = mx == -INFINITY ? 0.f : mx;
             float lt = 0.f;
             r2o_f4 o{};
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ml_lds[w][0][head] - ms);
-                lt += f * ml_lds[w][1][head];
-                o += f * *reinterpret_cast<const r2o_f4*>(reinterpret_cast<const float*>(lds[w][0]) + head * 128 + 4 * d4);
+            for (int x = 0; x < kWaves; ++x) {
+                const float f = __builtin_amdgcn_exp2f(ml_lds[x][0][qh] - ms);
+                lt += f * ml_lds[x][1][qh];
+                o += f * *reinterpret_cast<const r2o_f4*>(reinterpret_cast<const float*>(lds[x][0]) + qh * 128 + 4 * d4);
             }
-            *reinterpret_cast<r2o_f4*>(p.partial_out + (slot * group + head) * 128 + 4 * d4) = o;
+            *reinterpret_cast<r2o_f4*>(e.partial_out + (state + qh) * 128 + 4 * d4) = o;
             if (d4 == 0) {
-                p.partial_ml[(slot * group + head) * 2] = mx;
-                p.partial_ml[(slot * group + head) * 2 + 1] = lt;
+                e.partial_ml[(state + qh) * 2] = mx;
+                e.partial_ml[(state + qh) * 2 + 1] = lt;
             }
         }
         __syncthreads();
@@ -338,109 +467,105 @@ struct Ml {
     float m, l;
 };
 
+__device__ __forceinline__ void join_states(float& m, float& l, float m2, float l2) {
+    const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
+    l = l * __builtin_amdgcn_exp2f(m - ms) + l2 * __builtin_amdgcn_exp2f(m2 - ms);
+    m = mn;
+}
+
 __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count, int group, int head) {
     const int lane = threadIdx.x & 63;
     float m = -INFINITY, l = 0.f;
     for (int i = lane; i < count; i += 64) {
         const float* s = ml + ((slot0 + i) * group + head) * 2;
-        const float m2 = r2o_ldg(s), l2 = r2o_ldg(s + 1);
-        const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
-        l = l * __builtin_amdgcn_exp2f(m - ms) + l2 * __builtin_amdgcn_exp2f(m2 - ms);
-        m = mn;
+        join_states(m, l, r2o_ldg(s), r2o_ldg(s + 1));
     }
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const float m2 = __shfl_xor(m, x, R2O_WAVE), l2 = __shfl_xor(l, x, R2O_WAVE);
-        const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
-        l = l * __builtin_amdgcn_exp2f(m - ms) + l2 * __builtin_amdgcn_exp2f(m2 - ms);
-        m = mn;
-    }
+    for (int x = 1; x < 64; x <<= 1) join_states(m, l, __shfl_xor(m, x, R2O_WAVE), __shfl_xor(l, x, R2O_WAVE));
     return {m, l};
 }
 
 // Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: the
 // share of one worker again, whose slots' weights grow by their probabilities.
 template <int RF>
-__global__ __launch_bounds__(256) void paged_join_kernel(r2o_paged_attention_params p) {
+__global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
+    Args& a = kernel_args();
     __shared__ float red[8][128];
     __shared__ float lse2[16];
-    const r2o_paged_cache& c = p.cache;
-    const int group = (int)(p.hq / c.hkv), hkv = (int)c.hkv, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Share share = make_share(p);
-    const int heads = (int)(c.batch * p.hq);
+    const int group = a.group, hkv = a.hkv, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hq = group * hkv;
+    const Share share = make_share(a);
+    const int heads = a.batch * hq;
     if ((int)blockIdx.x < heads) {
-        const int b = blockIdx.x / (int)p.hq, hq = blockIdx.x % (int)p.hq, h = hq / group, head = hq % group;
-        int64_t base = 0;
-        for (int i = 0; i < b; ++i) base += (int64_t)request_tiles(p, i).count * hkv;
-        const Tiles t = request_tiles(p, b);
-        const int64_t u = base + (int64_t)h * t.count;
-        float* lse = p.lse + (int64_t)b * p.hq + hq;
-        uint16_t* dst = p.out + ((int64_t)b * p.hq + hq) * 128;
+        const int b = blockIdx.x / hq, qh = blockIdx.x % hq, h = qh / group, head = qh % group;
+        const int base = tiles_before(a, b);
+        const Tiles t = tiles_of(a, load_uniform(a.lengths + b));
+        float* lse = a.lse + blockIdx.x;
+        uint16_t* dst = a.out + (int64_t)blockIdx.x * 128;
         if (t.count == 0) {
             if (threadIdx.x < 64) reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = 0;
             if (threadIdx.x == 0) *lse = -INFINITY;
             return;
         }
-        const int w0 = share.worker(u), w1 = share.worker(u + t.count - 1), count = w1 - w0 + 1;
-        const int64_t slot0 = (int64_t)w0 + (int64_t)b * hkv + h;
-        const Ml ml = join_ml(p.partial_ml, slot0, count, group, head);
+        const int u = base + h * t.count, w0 = share.worker(u), count = share.worker(u + t.count - 1) - w0 + 1;
+        const int64_t slot0 = (int64_t)w0 + b * hkv + h;
+        const Ml ml = join_ml(a.partial_ml, slot0, count, group, head);
         const bool live = ml.m != -INFINITY;
         const float ms = live ? ml.m : 0.f;
         const int row = threadIdx.x >> 5, d4 = threadIdx.x & 31;
         r2o_f4 o{};
         for (int i = row; i < count; i += 8) {
             const int64_t at = (slot0 + i) * group + head;
-            const float f = __builtin_amdgcn_exp2f(r2o_ldg(p.partial_ml + at * 2) - ms);
-            o += f * r2o_ldg(reinterpret_cast<const r2o_f4*>(p.partial_out + at * 128) + d4);
+            const float f = __builtin_amdgcn_exp2f(r2o_ldg(a.partial_ml + at * 2) - ms);
+            o += f * r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4);
         }
         *reinterpret_cast<r2o_f4*>(&red[row][4 * d4]) = o;
         __syncthreads();
         if (threadIdx.x < 64) {
             const float inv = live ? 1.f / ml.l : 0.f;
-            float a = 0.f, e = 0.f;
+            float x = 0.f, y = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                a += red[i][2 * threadIdx.x];
-                e += red[i][2 * threadIdx.x + 1];
+                x += red[i][2 * threadIdx.x];
+                y += red[i][2 * threadIdx.x + 1];
             }
-            reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = live ? pack2<RF>(a * inv, e * inv) : 0u;
+            reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = live ? pack2<RF>(x * inv, y * inv) : 0u;
             if (threadIdx.x == 0) *lse = live ? (ml.m + __builtin_amdgcn_logf(ml.l)) * kLn2 : -INFINITY;
         }
         return;
     }
     // weights
-    const int worker = blockIdx.x - heads, shift = shift_of(c);
+    const int worker = blockIdx.x - heads;
     if (worker >= share.workers || share.total == 0) return;
-    int64_t u = share.begin(worker);
-    const int64_t u_end = share.begin(worker + 1);
-    int b = 0;
-    int64_t base = 0;
-    Tiles t = request_tiles(p, 0);
+    int u = share.begin(worker);
+    const int u_end = share.begin(worker + 1);
+    int base;
+    int b = request_of(a, u, base);
+    Tiles t = tiles_of(a, load_uniform(a.lengths + b));
     while (u < u_end) {
-        while (u >= base + (int64_t)t.count * hkv) {
-            base += (int64_t)t.count * hkv;
-            t = request_tiles(p, ++b);
+        while (u >= base + t.count * hkv) {
+            base += t.count * hkv;
+            t = tiles_of(a, load_uniform(a.lengths + ++b));
         }
-        const int h = (int)((u - base) / t.count);
-        const int64_t pair_base = base + (int64_t)h * t.count;
-        const int64_t stop = min(pair_base + t.count, u_end);
-        const int w0 = share.worker(pair_base), w1 = share.worker(pair_base + t.count - 1);
+        const int h = (int)((uint32_t)(u - base) / (uint32_t)t.count), pair_base = base + h * t.count;
+        const int stop = min(pair_base + t.count, u_end);
+        const int w0 = share.worker(pair_base), count = share.worker(pair_base + t.count - 1) - w0 + 1;
         for (int head = wave; head < group; head += 4) {
-            const Ml ml = join_ml(p.partial_ml, (int64_t)w0 + (int64_t)b * hkv + h, w1 - w0 + 1, group, head);
+            const Ml ml = join_ml(a.partial_ml, (int64_t)w0 + b * hkv + h, count, group, head);
             if (lane == 0) lse2[head] = ml.m == -INFINITY ? INFINITY : ml.m + __builtin_amdgcn_logf(ml.l);
         }
         __syncthreads();
-        for (int64_t e = u * kSlots + threadIdx.x; e < stop * kSlots; e += 256) {
-            const int64_t tile = e / kSlots;
-            const int r = (int)(e % kSlots), j = t.slot((int)(tile - pair_base)) + r;
-            if (!t.sees(j, (int)p.sinks)) continue;
-            const int page = page_of(c, b, j, shift);
-            if (page < 0) continue;
+        const int32_t* table = a.table + (int64_t)b * a.table_stride;
+        const int r = threadIdx.x % kSlots;
+        for (int tile = u + threadIdx.x / kSlots; tile < stop; tile += 256 / kSlots) {
+            const int j = t.slot(tile - pair_base) + r;
+            if (!t.sees(j, a.sinks)) continue;
+            const int page = r2o_ldg(table + (j >> a.shift));
+            if ((uint32_t)page >= (uint32_t)a.pages) continue;
             float sum = 0.f;
             for (int head = 0; head < group; ++head)
-                sum += __builtin_amdgcn_exp2f(r2o_ldg(p.logits + (tile * group + head) * kSlots + r) - lse2[head]);
-            float* w = c.weight_pages + page * c.weight_strides[0] + h * c.weight_strides[1] + (j & ((1 << shift) - 1));
-            *w = p.append_key && j == t.n - 1 ? sum : *w + sum;
+                sum += __builtin_amdgcn_exp2f(r2o_ldg(a.logits + ((int64_t)tile * group + head) * kSlots + r) - lse2[head]);
+            float* w = a.weight + (int64_t)page * a.w_page + (int64_t)h * a.w_head + (j & ((1 << a.shift) - 1));
+            *w = a.new_key && j == t.n - 1 ? sum : *w + sum;
         }
         __syncthreads();
         u = stop;
@@ -562,10 +687,14 @@ bool rows_ok(const int64_t* st, int n) {  // the kernels hold strides in 32 bits
     return true;
 }
 
+// One slot's rows lie within 32-bit offsets of the next ones'.
+bool slots_ok(const r2o_paged_cache& c) { return c.key_strides[2] <= R2O_PAGED_MAX_SLOT_STRIDE && c.value_strides[2] <= R2O_PAGED_MAX_SLOT_STRIDE; }
+
 bool cache_ok(const r2o_paged_cache& c) {
-    return (c.dtype == 0 || c.dtype == 1) && aligned(c.key_pages, 16) && aligned(c.value_pages, 16) && aligned(c.page_table, 4) &&
+    return slots_ok(c) && (c.dtype == 0 || c.dtype == 1) && aligned(c.key_pages, 16) && aligned(c.value_pages, 16) && aligned(c.page_table, 4) &&
            aligned(c.lengths, 4) && reinterpret_cast<uintptr_t>(c.weight_pages) % 4 == 0 && rows_ok(c.key_strides, 3) &&
-           rows_ok(c.value_strides, 3) && c.weight_strides[0] >= 0 && c.weight_strides[1] >= 0 && c.table_stride >= c.max_pages &&
+           rows_ok(c.value_strides, 3) && c.weight_strides[0] >= 0 && c.weight_strides[0] <= 0x7fffffff && c.weight_strides[1] >= 0 &&
+           c.weight_strides[1] <= 0x7fffffff && c.table_stride >= c.max_pages && c.table_stride <= 0x7fffffff &&
            c.pages >= 1 && c.pages <= 0x7fffffff && c.max_pages >= 1 && c.batch >= 1 && c.batch <= R2O_PAGED_MAX_BATCH &&
            c.hkv >= 1 && c.hkv <= 1024 &&
            (c.page_size == 16 || c.page_size == 32 || c.page_size == 64 || c.page_size == 128) && c.max_pages <= (1 << 29) / c.page_size;
@@ -601,20 +730,60 @@ int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream) {
         return R2O_EINVAL;
     // every slot that the page tables can hold has room for its logits, whatever the lengths on the device say
     const int64_t tiles = (c.max_pages * c.page_size + kSlots - 1) / kSlots;
+    if (pairs * tiles > 0x7fffffff - R2O_PAGED_MAX_WORKERS) return R2O_EINVAL;
     if (c.weight_pages && (!aligned(p->logits, 16) || p->logits_floats < pairs * tiles * kSlots * group)) return R2O_EINVAL;
+    AttentionArgs a{};
+    a.key = c.key_pages;
+    a.value = c.value_pages;
+    a.weight = c.weight_pages;
+    a.table = c.page_table;
+    a.lengths = c.lengths;
+    a.query = p->query;
+    a.new_key = p->append_key;
+    a.new_value = p->append_value;
+    a.out = p->out;
+    a.lse = p->lse;
+    a.partial_out = p->partial_out;
+    a.partial_ml = p->partial_ml;
+    a.logits = p->logits;
+    a.k_page = (int)c.key_strides[0];
+    a.k_head = (int)c.key_strides[1];
+    a.k_slot = (int)c.key_strides[2];
+    a.v_page = (int)c.value_strides[0];
+    a.v_head = (int)c.value_strides[1];
+    a.v_slot = (int)c.value_strides[2];
+    a.w_page = (int)c.weight_strides[0];
+    a.w_head = (int)c.weight_strides[1];
+    a.table_stride = (int)c.table_stride;
+    a.q_batch = (int)p->query_strides[0];
+    a.q_head = (int)p->query_strides[1];
+    a.nk_batch = (int)p->append_strides[0];
+    a.nk_head = (int)p->append_strides[1];
+    a.nv_batch = (int)p->append_strides[2];
+    a.nv_head = (int)p->append_strides[3];
+    a.pages = (int)c.pages;
+    a.last_page = (int)c.max_pages - 1;
+    a.shift = 31 - __builtin_clz((unsigned)c.page_size);
+    a.batch = (int)c.batch;
+    a.hkv = (int)c.hkv;
+    a.group = (int)group;
+    a.window = p->window ? (int)std::min<int64_t>(p->window, kNoWindow) : kNoWindow;
+    a.sinks = p->window ? (int)p->sinks : 0;
+    a.workers = (int)p->workers;
+    a.c2 = p->sm_scale * kLog2e;
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)p->workers), join((unsigned)(c.batch * p->hq + (c.weight_pages ? p->workers : 0)));
-    if (c.dtype == 0) {
-        hipLaunchKernelGGL(paged_partial_kernel<0>, grid, dim3(256), 0, st, *p);
-        R2O_CHECK_LAUNCH();
-        hipLaunchKernelGGL(paged_join_kernel<0>, join, dim3(256), 0, st, *p);
-    } else {
-        hipLaunchKernelGGL(paged_partial_kernel<1>, grid, dim3(256), 0, st, *p);
-        R2O_CHECK_LAUNCH();
-        hipLaunchKernelGGL(paged_join_kernel<1>, join, dim3(256), 0, st, *p);
-    }
-    R2O_CHECK_LAUNCH();
-    return R2O_OK;
+    auto launch = [&](auto partial, auto join_kernel) {
+        hipLaunchKernelGGL(partial, grid, dim3(256), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return R2O_ELAUNCH;
+        hipLaunchKernelGGL(join_kernel, join, dim3(256), 0, st, a);
+        return hipGetLastError() == hipSuccess ? R2O_OK : R2O_ELAUNCH;
+    };
+    if (c.dtype == 0)
+        return c.weight_pages ? launch(paged_partial_kernel<0, true>, paged_join_kernel<0>)
+                              : launch(paged_partial_kernel<0, false>, paged_join_kernel<0>);
+    return c.weight_pages ? launch(paged_partial_kernel<1, true>, paged_join_kernel<1>)
+                          : launch(paged_partial_kernel<1, false>, paged_join_kernel<1>);
 }
 
 int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream) {

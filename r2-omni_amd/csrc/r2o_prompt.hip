@@ -46,25 +46,25 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return RF == 0 ? r2o_pack_bf2(lo, hi) : r2o_pack_h2(lo, hi);
 }
 
-__device__ __forceinline__ void load_lds16(const void* gsrc, unsigned char* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gsrc,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-}
-
-// One wave's 16 rows of a 64-row tile into LDS, rows from `row0` on clamped to `last`: a row is 16 chunks of 16
-// bytes, chunk c of row r at place c ^ swizzle(r).  The hardware writes lane l at 16 l, so the swizzle is made by
-// which chunk a lane reads.  SWZ 0: r & 7, for reads of one chunk by 32 rows; 1: 2 (r & 3), for transposing reads
-// of two chunks by 4 rows.
+// One wave's 16 rows of a 64-row tile, from `row0` on clamped to `last`, into registers, and from there into LDS: a row is
+// 16 chunks of 16 bytes, chunk c of row r at place c ^ swizzle(r); lane l writes at 16 l, so the swizzle is made by which
+// chunk it reads.  SWZ 0: r & 7, for reads of one chunk by 32 rows; 1: 2 (r & 3), for transposing reads of two chunks
+// by 4 rows.
 template <int SWZ>
-__device__ __forceinline__ void stage_rows(const uint16_t* base, int64_t stride, int row0, int last, unsigned char* lds,
-                                           int wave, int lane) {
+__device__ __forceinline__ void load_rows(const uint16_t* base, int stride, int row0, int last, r2o_u4 (&x)[4], int wave, int lane) {
     const int r4 = lane >> 4, place = lane & 15;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int r = 16 * wave + 4 * i + r4;
-        const int c = place ^ (SWZ == 0 ? (r & 7) : 2 * (r & 3));
-        load_lds16(base + (int64_t)min(row0 + r, last) * stride + 8 * c, lds + (16 * wave + 4 * i) * 256);
+        const int r0 = min(row0 + 16 * wave + 4 * i, last);
+        const int c = place ^ (SWZ == 0 ? (4 * i + r4) & 7 : 2 * r4);
+        const uint32_t at = (uint32_t)(2 * min(r4, last - r0) * stride + 16 * c);
+        x[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(reinterpret_cast<const unsigned char*>(base + (int64_t)r0 * stride) + at));
     }
+}
+
+__device__ __forceinline__ void store_rows(unsigned char* lds, const r2o_u4 (&x)[4], int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<r2o_u4*>(lds + (16 * wave + 4 * i) * 256 + 16 * lane) = x[i];
 }
 
 // 32 rows of a staged tile (SWZ 0) as the A operand of step t (channels 16 t ..).
@@ -86,20 +86,14 @@ __device__ __forceinline__ r2o_u4 read_values(const unsigned char* tile, int kb,
     return r2o_u4{a[0], a[1], b[0], b[1]};
 }
 
-struct Lengths {
-    int q, n, off;  // rows, keys, position of row 0
-};
-
-__device__ __forceinline__ Lengths request_lengths(const r2o_prompt_params& a, int b) {
-    Lengths s;
-    s.q = a.query_lengths ? min(max(r2o_ldg(a.query_lengths + b), 0), (int)a.queries) : (int)a.queries;
-    s.n = a.key_lengths ? min(max(r2o_ldg(a.key_lengths + b), 0), (int)a.keys) : (int)a.keys;
-    s.off = s.n - s.q;
-    return s;
-}
-
 __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
     return j <= p && (j > p - window || j < sinks);
+}
+
+// The same for key j = first + c by two comparisons, with `back` = p - first and `sink` = min(sinks, p + 1) - 1 - first
+// formed once: 0 <= p - j < window, or j at most the last sink.
+__device__ __forceinline__ bool sees_from(int back, int sink, int c, uint32_t window) {
+    return ((uint32_t)(back - c) < window) | (sink >= c);
 }
 
 // Infinite or NaN.
@@ -110,54 +104,81 @@ __device__ __forceinline__ bool not_finite(uint32_t bits16) {
 }
 
 // In a tile that some row of the workgroup sees in part, a masked key's probability is 0, but 0 times an infinite
-// or NaN value is NaN.  A thread takes a quarter of a V row, turns such elements to zero in LDS and reports the row;
-// returns this wave's rows (16 wave ..) that had any.
+// or NaN value is NaN: such elements become zero before they reach LDS; true if there was one.
 template <int RF>
-__device__ __forceinline__ uint32_t zero_not_finite(unsigned char* tile, int wave, int lane) {
-    r2o_u4* src = reinterpret_cast<r2o_u4*>(tile + (16 * wave + (lane >> 2)) * 256 + 64 * (lane & 3));
-    bool any = false;
+__device__ __forceinline__ bool zero_not_finite(r2o_u4 (&x)[4]) {
+    constexpr uint32_t e = RF == 0 ? 0x7f807f80u : 0x7c007c00u, one = RF == 0 ? 0x00800080u : 0x04000400u;
+    uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r2o_u4 x = src[i];
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const bool lo = not_finite<RF>(x[k]), hi = not_finite<RF>(x[k] >> 16);
-            any |= lo | hi;
-            x[k] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+            const uint32_t bad = ((x[i][k] & e) + one) & 0x80008000u;  // a full exponent carries into the sign's place
+            any |= bad;
+            x[i][k] &= ~((bad >> 15) * 0xffffu);
         }
-        if (any) src[i] = x;
-    }
-    uint64_t b = __ballot(any);
-    b |= b >> 1;
-    b |= b >> 2;
-    uint32_t rows = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) rows |= (uint32_t)((b >> (4 * r)) & 1) << r;
-    return rows;
+    return any != 0;
+}
+
+// The kernels' arguments in their widths (the host has checked that they fit), read where the hardware put them: each
+// place that asks anew loads what it uses again, instead of holding them all in scalar registers.
+struct PromptArgs {
+    const uint16_t *query, *key, *value;
+    uint16_t* out;
+    float* lse;
+    const int32_t *query_lengths, *key_lengths;
+    const float* lse_in;
+    float* weights;
+    int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head, o_batch, o_head;
+    int q_row, k_row, v_row, o_row, hq, hkv, group, queries, keys, window, sinks;
+    float c2;  // scale, in log2 units
+};
+
+typedef const __attribute__((address_space(4))) PromptArgs Args;
+
+__device__ __forceinline__ Args& kernel_args() {
+    auto p = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+
+struct Lengths {
+    int q, n, off;  // rows, keys, position of row 0
+};
+
+__device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
+    Lengths s;
+    s.q = a.query_lengths ? min(max(r2o_ldg(a.query_lengths + b), 0), a.queries) : a.queries;
+    s.n = a.key_lengths ? min(max(r2o_ldg(a.key_lengths + b), 0), a.keys) : a.keys;
+    s.q = __builtin_amdgcn_readfirstlane(s.q);
+    s.n = __builtin_amdgcn_readfirstlane(s.n);
+    s.off = s.n - s.q;
+    return s;
 }
 
 // ------------------------------------------------------------------------------ prompt attention
 template <int RF>
-__global__ __launch_bounds__(256, 2) void prompt_attention_kernel(r2o_prompt_params a) {
-    __shared__ __align__(16) unsigned char k_lds[2][kTileBytes];
-    __shared__ __align__(16) unsigned char v_lds[2][kTileBytes];
-    __shared__ uint32_t bad_lds[2][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-    const int h = blockIdx.y, b = blockIdx.z, kvh = h / (int)(a.hq / a.hkv);
+__global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
+    __shared__ __align__(16) unsigned char k_lds[2][kTileBytes], v_lds[2][kTileBytes];
+    __shared__ int any_bad;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int h = blockIdx.y, b = blockIdx.z;
     const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kRows;  // the longest rows first
+    Args& a = kernel_args();
     const Lengths s = request_lengths(a, b);
-    const int window = a.window ? (int)min(a.window, (int64_t)kNoWindow) : kNoWindow, sinks = a.window ? (int)a.sinks : 0;
-    const uint16_t* kbase = a.key + b * a.k_strides[0] + kvh * a.k_strides[1];
-    const uint16_t* vbase = a.value + b * a.v_strides[0] + kvh * a.v_strides[1];
+    const int window = a.window, sinks = a.sinks, kvh = h / a.group;
+    const uint16_t* kbase = a.key + b * a.k_batch + kvh * a.k_head;
+    const uint16_t* vbase = a.value + b * a.v_batch + kvh * a.v_head;
+    const int k_row = a.k_row, v_row = a.v_row;
 
     const int row = row0 + 32 * wave + col;  // this lane's query row
     r2o_u4 q[8];
     {
-        const uint16_t* src = a.query + b * a.q_strides[0] + h * a.q_strides[1] +
-                              (int64_t)min(row, (int)a.queries - 1) * a.q_strides[2] + 8 * half;
+        const uint16_t* src = a.query + b * a.q_batch + h * a.q_head + (int64_t)min(row, a.queries - 1) * a.q_row + 8 * half;
 #pragma unroll
         for (int t = 0; t < 8; ++t) q[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
     }
+    if (threadIdx.x == 0) any_bad = 0;
 
     // key tiles that any row of the workgroup sees: sink tiles, then the window's
     const int top = min(s.n - 1, s.off + min(row0 + kRows, s.q) - 1);  // last position of the workgroup's rows
@@ -167,55 +188,46 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(r2o_prompt_par
     const int tiles = sink_tiles + max(0, end - first);
     const int last = max(s.n - 1, 0);
 
-    const float c2 = a.sm_scale * kLog2e;
+    const float c2 = a.c2;
     float m = -INFINITY, l = 0.f;
     f16v acc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = f16v{};
 
     auto tile_key = [&](int it) { return (it < sink_tiles ? it : first + it - sink_tiles) * kTile; };
-    auto stage = [&](int it) {
+    const int wg_min = s.off + row0, pmin = wg_min + 32 * wave, pmax = pmin + 31, p = pmin + col, pv = min(p, s.n - 1);
+    auto seen_in_part = [&](int kt) { return !(kt + kTile - 1 <= wg_min && (kt > wg_min + kRows - 1 - window || kt + kTile <= sinks)); };
+    // The next tile is on its way into registers while this one is computed on: loads straight into LDS would save the
+    // registers, but the compiler waits for all of them before the transposing reads.
+    r2o_u4 kx[4], vx[4];
+    auto load = [&](int it) {
         const int kt = tile_key(it);
-        stage_rows<0>(kbase, a.k_strides[2], kt, last, k_lds[it & 1], wave, lane);
-        stage_rows<1>(vbase, a.v_strides[2], kt, last, v_lds[it & 1], wave, lane);
+        load_rows<0>(kbase, k_row, kt, last, kx, wave, lane);
+        load_rows<1>(vbase, v_row, kt, last, vx, wave, lane);
     };
-    const int pmin = s.off + row0 + 32 * wave, pmax = pmin + 31, p = pmin + col;
-    if (tiles > 0) stage(0);
-    for (int it = 0; it < tiles; ++it) {
-        const int kt = tile_key(it);
-        __syncthreads();  // the tile is there, and every wave is done with the one before
-        const int wg_min = s.off + row0;
-        uint64_t bad = 0;
-        if (!(kt + kTile - 1 <= wg_min && (kt > wg_min + kRows - 1 - window || kt + kTile <= sinks))) {
-            const uint32_t rows = zero_not_finite<RF>(v_lds[it & 1], wave, lane);
-            if (lane == 0) bad_lds[it & 1][wave] = rows;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 4; ++w) bad |= (uint64_t)__builtin_amdgcn_readfirstlane(bad_lds[it & 1][w]) << (16 * w);
-        }
-        if (it + 1 < tiles) stage(it + 1);
-        if (kt > pmax || (kt + kTile - 1 <= pmin - window && kt >= sinks)) continue;  // nothing for this wave
-        const unsigned char *kl = k_lds[it & 1], *vl = v_lds[it & 1];
+    auto store = [&](int it) {
+        if (seen_in_part(tile_key(it)) && zero_not_finite<RF>(vx)) any_bad = 1;
+        store_rows(k_lds[it & 1], kx, wave, lane);
+        store_rows(v_lds[it & 1], vx, wave, lane);
+    };
+    auto compute = [&](int kt, const unsigned char* kl, const unsigned char* vl) __attribute__((always_inline)) {
+        if (kt > pmax || (kt + kTile - 1 <= pmin - window && kt >= sinks)) return;  // nothing for this wave
         f16v sc[2] = {f16v{}, f16v{}};
 #pragma unroll
         for (int t = 0; t < 8; ++t)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) sc[kb] = mfma32<RF>(read_rows(kl, kb, t, lane), q[t], sc[kb]);
         if (!(kt + kTile - 1 <= pmin && (kt > pmax - window || kt + kTile <= sinks))) {
-            const int pv = min(p, s.n - 1);
+            const int from = kt + 4 * half, back = pv - from, sink = min(sinks, pv + 1) - 1 - from;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = kt + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
-                    sc[kb][i] = sees(pv, j, window, sinks) ? sc[kb][i] : -INFINITY;
-                }
+                for (int i = 0; i < 16; ++i)
+                    sc[kb][i] = sees_from(back, sink, 32 * kb + 8 * (i >> 2) + (i & 3), window) ? sc[kb][i] : -INFINITY;
         }
-        float tmax = sc[0][0];
+        float tmax = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[kb][i]);
+        for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, fmaxf(sc[0][i], sc[1][i]));
         {
             float x, y;
             r2o_row_swap<32>(tmax, x, y);
@@ -245,18 +257,34 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(r2o_prompt_par
         for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
             for (int db = 0; db < 4; ++db) acc[db] = mfma32<RF>(read_values(vl, kb, db, lane), pk[kb], acc[db]);
-        while (bad) {  // what was taken out, for the rows that see it
-            const int j = kt + __builtin_ctzll(bad);
-            bad &= bad - 1;
-            if (!sees(min(p, s.n - 1), j, window, sinks)) continue;
-            const uint16_t* src = vbase + (int64_t)j * a.v_strides[2] + 4 * half;
+    };
+    __syncthreads();
+    if (tiles > 0) {
+        load(0);
+        store(0);
+    }
+    for (int it = 0; it < tiles; ++it) {
+        __syncthreads();  // the tile is there, and every wave is done with the one before
+        if (it + 1 < tiles) load(it + 1);
+        compute(tile_key(it), k_lds[it & 1], v_lds[it & 1]);
+        if (it + 1 < tiles) store(it + 1);
+    }
+    __syncthreads();
+    if (any_bad) {  // what was taken out, for the rows that see it
+        for (int it = 0; it < tiles; ++it) {
+            const int kt = tile_key(it);
+            if (!seen_in_part(kt)) continue;
+            for (int j = kt; j < min(kt + kTile, s.n); ++j) {
+                if (!sees(pv, j, window, sinks)) continue;
+                const uint16_t* src = vbase + (int64_t)j * v_row + 4 * half;
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
+                for (int db = 0; db < 4; ++db)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t x = r2o_ldg(src + 32 * db + 8 * (i >> 2) + (i & 3));
-                    if (not_finite<RF>(x)) acc[db][i] += RF == 0 ? r2o_bf16_to_f32(x) : r2o_f16_to_f32(x);
-                }
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t x = r2o_ldg(src + 32 * db + 8 * (i >> 2) + (i & 3));
+                        if (not_finite<RF>(x)) acc[db][i] += RF == 0 ? r2o_bf16_to_f32(x) : r2o_f16_to_f32(x);
+                    }
+            }
         }
     }
 
@@ -265,10 +293,11 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(r2o_prompt_par
         r2o_row_swap<32>(l, x, y);
         l = x + y;
     }
-    if (row >= (int)a.queries) return;
+    Args& e = kernel_args();
+    if (row >= e.queries) return;
     const bool live = row < s.q && m != -INFINITY;
     const float inv = live ? 1.f / l : 0.f;
-    uint16_t* dst = a.out + b * a.o_strides[0] + h * a.o_strides[1] + (int64_t)row * a.o_strides[2];
+    uint16_t* dst = e.out + b * e.o_batch + h * e.o_head + (int64_t)row * e.o_row;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -277,25 +306,25 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(r2o_prompt_par
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 w[k] = live ? pack2<RF>(acc[db][4 * g + 2 * k] * inv, acc[db][4 * g + 2 * k + 1] * inv) : 0u;
-            *reinterpret_cast<r2o_u2*>(dst + 32 * db + 8 * g + 4 * half) = w;
+            *reinterpret_cast<R2O_GLOBAL r2o_u2*>((R2O_GLOBAL uint16_t*)(dst + 32 * db + 8 * g + 4 * half)) = w;
         }
-    if (half == 0)
-        a.lse[((int64_t)b * a.hq + h) * a.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    if (half == 0) e.lse[((int64_t)b * e.hq + h) * e.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
 // ----------------------------------------------------------------------------- attention weights
 constexpr int kWeightKeys = 128;  // keys of a workgroup: 4 waves of 32, whose rows stay in registers
 
 // grid: (key tiles, splits, batch * hkv).  A split takes a share of the (query head, 64-row tile) pairs that see
-// the key tile; its sums go to `dst` ([splits, batch, hkv, keys]; the result itself where there is one split).
+// the key tile; its sums go to `weights` ([splits, batch, hkv, keys]; the result itself where there is one split).
 template <int RF>
-__global__ __launch_bounds__(256, 2) void attention_weights_kernel(r2o_prompt_params a, float* dst) {
+__global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     __shared__ __align__(16) unsigned char q_lds[2][kTileBytes];
     __shared__ __align__(16) float lse_lds[2][kTile];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-    const int kvh = (int)(blockIdx.z % a.hkv), b = (int)(blockIdx.z / a.hkv), group = (int)(a.hq / a.hkv);
+    Args& a = kernel_args();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int kvh = (int)blockIdx.z % a.hkv, b = (int)blockIdx.z / a.hkv, group = a.group;
     const Lengths s = request_lengths(a, b);
-    const int window = a.window ? (int)min(a.window, (int64_t)kNoWindow) : kNoWindow, sinks = a.window ? (int)a.sinks : 0;
+    const int window = a.window, sinks = a.sinks;
     const int key0 = blockIdx.x * kWeightKeys, kw = key0 + 32 * wave, j = kw + col;
 
     // rows that see any of the tile's keys: p >= key0, and without a sink among them p < last key + window
@@ -308,39 +337,37 @@ __global__ __launch_bounds__(256, 2) void attention_weights_kernel(r2o_prompt_pa
 
     float sum = 0.f, lost = 0.f;  // of up to hq / hkv * queries terms: what each addition loses is kept
     if (begin < end) {
-        const float c2 = a.sm_scale * kLog2e;
+        const float c2 = a.c2;
         r2o_u4 k[8];
-        const uint16_t* src = a.key + b * a.k_strides[0] + kvh * a.k_strides[1] + (int64_t)min(j, s.n - 1) * a.k_strides[2] + 8 * half;
+        const uint16_t* src = a.key + b * a.k_batch + kvh * a.k_head + (int64_t)min(j, s.n - 1) * a.k_row + 8 * half;
 #pragma unroll
         for (int t = 0; t < 8; ++t) k[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
-        auto stage = [&](int it, int buf) {
-            const int h = kvh * group + it / per_head, r0 = (first + it % per_head) * kTile;
-            stage_rows<0>(a.query + b * a.q_strides[0] + h * a.q_strides[1], a.q_strides[2], r0, s.q - 1,
-                          q_lds[buf], wave, lane);
-            if (threadIdx.x < kTile) {
-                const int r = r0 + threadIdx.x;
-                float x = INFINITY;  // rows behind the request, and those that saw no key, give exp2(-inf)
-                if (r < s.q) x = r2o_ldg(a.lse_in + ((int64_t)b * a.hq + h) * a.queries + r) * kLog2e;
-                lse_lds[buf][threadIdx.x] = x == -INFINITY ? INFINITY : x;
-            }
+        r2o_u4 qx[4];
+        float lse_next = 0.f;
+        auto tile_row = [&](int it) { return (first + it % per_head) * kTile; };
+        auto load = [&](int it) {
+            const int h = kvh * group + it / per_head, r0 = tile_row(it);
+            lse_next = r2o_ldg(a.lse_in + ((int64_t)b * a.hq + h) * a.queries + min(r0 + ((int)threadIdx.x & (kTile - 1)), s.q - 1));
+            load_rows<0>(a.query + b * a.q_batch + h * a.q_head, a.q_row, r0, s.q - 1, qx, wave, lane);
         };
-        stage(begin, 0);
-        for (int it = begin; it < end; ++it) {
-            const int buf = (it - begin) & 1;
-            __syncthreads();
-            if (it + 1 < end) stage(it + 1, buf ^ 1);
+        auto store = [&](int it, int buf) {  // rows behind the request, and those that saw no key, give exp2(-inf)
+            store_rows(q_lds[buf], qx, wave, lane);
+            const bool none = tile_row(it) + (int)threadIdx.x >= s.q || lse_next == -INFINITY;
+            if (threadIdx.x < kTile) lse_lds[buf][threadIdx.x] = none ? INFINITY : lse_next * kLog2e;
+        };
+        auto tile = [&](int it, const unsigned char* ql, const float* lse) __attribute__((always_inline)) {
             const int p0 = s.off + (first + it % per_head) * kTile;
-            if (p0 + kTile - 1 < kw || (kw + 31 <= p0 - window && kw >= sinks)) continue;
+            if (p0 + kTile - 1 < kw || (kw + 31 <= p0 - window && kw >= sinks)) return;
             const bool full = p0 >= kw + 31 && (kw > p0 + kTile - 1 - window || kw + 32 <= sinks);
             float part = 0.f;
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) {
                 f16v sc = f16v{};
 #pragma unroll
-                for (int t = 0; t < 8; ++t) sc = mfma32<RF>(read_rows(q_lds[buf], rb, t, lane), k[t], sc);
+                for (int t = 0; t < 8; ++t) sc = mfma32<RF>(read_rows(ql, rb, t, lane), k[t], sc);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const r2o_f4 x = *reinterpret_cast<const r2o_f4*>(&lse_lds[buf][32 * rb + 8 * g + 4 * half]);
+                    const r2o_f4 x = *reinterpret_cast<const r2o_f4*>(&lse[32 * rb + 8 * g + 4 * half]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * g + i], c2, -x[i]));
@@ -352,13 +379,21 @@ __global__ __launch_bounds__(256, 2) void attention_weights_kernel(r2o_prompt_pa
             const float add = part - lost, next = sum + add;
             lost = (next - sum) - add;
             sum = next;
+        };
+        load(begin);
+        store(begin, 0);
+        for (int it = begin, buf = 0; it < end; ++it, buf ^= 1) {
+            __syncthreads();
+            if (it + 1 < end) load(it + 1);
+            tile(it, q_lds[buf], lse_lds[buf]);
+            if (it + 1 < end) store(it + 1, buf ^ 1);
         }
         float x, y;
         r2o_row_swap<32>(sum, x, y);
         sum = x + y;
     }
-    if (half == 0 && j < (int)a.keys)
-        dst[((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * a.keys + j] = j < s.n ? sum : 0.f;
+    if (half == 0 && j < a.keys)
+        a.weights[((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * a.keys + j] = j < s.n ? sum : 0.f;
 }
 
 __global__ __launch_bounds__(256) void weights_join_kernel(const float* src, float* dst, int64_t n, int splits) {
@@ -369,7 +404,10 @@ __global__ __launch_bounds__(256) void weights_join_kernel(const float* src, flo
     dst[i] = sum;
 }
 
-bool strides_ok(const int64_t* st) { return st[0] >= 0 && st[1] >= 0 && st[2] >= 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0; }
+// Rows lie within 32-bit offsets of the next ones'.
+bool strides_ok(const int64_t* st) {
+    return st[0] >= 0 && st[1] >= 0 && st[2] >= 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0 && st[2] <= R2O_MAX_ROW_STRIDE;
+}
 
 bool aligned(std::initializer_list<const void*> ps, uintptr_t n) {
     for (const void* p : ps)
@@ -386,6 +424,39 @@ bool shapes_ok(const r2o_prompt_params* p) {
            reinterpret_cast<uintptr_t>(p->query_lengths) % 4 == 0 && reinterpret_cast<uintptr_t>(p->key_lengths) % 4 == 0;
 }
 
+PromptArgs kernel_arguments(const r2o_prompt_params* p) {
+    PromptArgs a{};
+    a.query = p->query;
+    a.key = p->key;
+    a.value = p->value;
+    a.out = p->out;
+    a.lse = p->lse;
+    a.query_lengths = p->query_lengths;
+    a.key_lengths = p->key_lengths;
+    a.lse_in = p->lse_in;
+    a.q_batch = p->q_strides[0];
+    a.q_head = p->q_strides[1];
+    a.q_row = (int)p->q_strides[2];
+    a.k_batch = p->k_strides[0];
+    a.k_head = p->k_strides[1];
+    a.k_row = (int)p->k_strides[2];
+    a.v_batch = p->v_strides[0];
+    a.v_head = p->v_strides[1];
+    a.v_row = (int)p->v_strides[2];
+    a.o_batch = p->o_strides[0];
+    a.o_head = p->o_strides[1];
+    a.o_row = (int)p->o_strides[2];
+    a.hq = (int)p->hq;
+    a.hkv = (int)p->hkv;
+    a.group = (int)(p->hq / p->hkv);
+    a.queries = (int)p->queries;
+    a.keys = (int)p->keys;
+    a.window = p->window ? (int)std::min<int64_t>(p->window, kNoWindow) : kNoWindow;
+    a.sinks = p->window ? (int)p->sinks : 0;
+    a.c2 = p->sm_scale * kLog2e;
+    return a;
+}
+
 }  // namespace
 
 extern "C" {
@@ -396,8 +467,9 @@ int r2o_prompt_attention(const r2o_prompt_params* p, void* stream) {
         return R2O_EINVAL;
     const dim3 grid((unsigned)((p->queries + kRows - 1) / kRows), (unsigned)p->hq, (unsigned)p->batch);
     const hipStream_t st = (hipStream_t)stream;
-    if (p->dtype == 0) hipLaunchKernelGGL(prompt_attention_kernel<0>, grid, dim3(256), 0, st, *p);
-    else hipLaunchKernelGGL(prompt_attention_kernel<1>, grid, dim3(256), 0, st, *p);
+    const PromptArgs a = kernel_arguments(p);
+    if (p->dtype == 0) hipLaunchKernelGGL(prompt_attention_kernel<0>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(prompt_attention_kernel<1>, grid, dim3(256), 0, st, a);
     R2O_CHECK_LAUNCH();
     return R2O_OK;
 }
@@ -409,9 +481,10 @@ int r2o_attention_weights(const r2o_prompt_params* p, void* stream) {
     if ((n + 255) / 256 > 0x7fffffff) return R2O_EINVAL;
     const dim3 grid((unsigned)((p->keys + kWeightKeys - 1) / kWeightKeys), (unsigned)p->splits, (unsigned)(p->batch * p->hkv));
     const hipStream_t st = (hipStream_t)stream;
-    float* dst = p->splits > 1 ? p->scratch : p->weights;
-    if (p->dtype == 0) hipLaunchKernelGGL(attention_weights_kernel<0>, grid, dim3(256), 0, st, *p, dst);
-    else hipLaunchKernelGGL(attention_weights_kernel<1>, grid, dim3(256), 0, st, *p, dst);
+    PromptArgs a = kernel_arguments(p);
+    a.weights = p->splits > 1 ? p->scratch : p->weights;
+    if (p->dtype == 0) hipLaunchKernelGGL(attention_weights_kernel<0>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(attention_weights_kernel<1>, grid, dim3(256), 0, st, a);
     R2O_CHECK_LAUNCH();
     if (p->splits > 1) {
         hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p->scratch, p->weights, n,

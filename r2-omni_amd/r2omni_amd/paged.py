@@ -28,7 +28,7 @@ MAX_BATCH = 1024
 
 def _pool_ok(t: torch.Tensor) -> bool:
     """Rows in place, every slot its own memory."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    return (t.stride(2) <= 1 << 24 and t.stride(-1) == 1 and t.data_ptr() % 16 == 0
             and all(0 < st < 1 << 31 and st % 8 == 0 for st, n in zip(t.stride()[:-1], t.shape) if n > 1))
 
 
@@ -64,10 +64,11 @@ class PagedCache:
             raise ValueError("page_table must be int32 [B,max_pages] with unit-strided rows")
         if n.dtype != torch.int32 or tuple(n.shape) != (table.shape[0],) or not n.is_contiguous():
             raise ValueError("lengths must be contiguous int32 [B]")
-        if table.shape[0] > MAX_BATCH or table.shape[1] * k.shape[2] > 1 << 29 or k.shape[0] >= 1 << 31 or k.shape[1] > 1024:
+        if table.shape[0] > MAX_BATCH or table.shape[1] * k.shape[2] > 1 << 29 or k.shape[0] >= 1 << 31 or k.shape[1] > 1024 \
+                or table.stride(0) >= 1 << 31:
             raise ValueError("paged cache takes at most 1024 requests, 1024 heads and 2^29 slots a request")
         if w is not None and (w.shape != k.shape[:3] or w.dtype != torch.float32 or w.device != k.device
-                              or any(st <= 0 for st, size in zip(w.stride(), w.shape) if size > 1) or w.stride(2) != 1):
+                              or any(not 0 < st < 1 << 31 for st, size in zip(w.stride(), w.shape) if size > 1) or w.stride(2) != 1):
             raise ValueError("weight_pages must be fp32 [pages,Hkv,page_size] on the cache's device with unit-strided slots")
         _lib.require_device(k, "paged cache")
         object.__setattr__(self, "_c", _lib.PagedCacheParams(
@@ -149,6 +150,8 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
         raise ValueError("paged attention query must match the cache's dtype and device")
     if torch.is_grad_enabled() and query.requires_grad:
         raise RuntimeError("paged attention has no backward pass: call it under torch.no_grad()")
+    if batch * hkv * (-(-cache.capacity // 32)) > (1 << 31) - 4097:
+        raise ValueError("paged attention takes at most 2^36 slots over all requests and heads")
     w, s = _window(window, sinks)
     scale = _scale(sm_scale)
     dev = query.device

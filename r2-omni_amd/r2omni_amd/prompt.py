@@ -25,7 +25,8 @@ _MOST_ROWS = 1 << 29
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself if the kernels can read its rows in place (unit channel stride, 16-byte aligned rows),
     otherwise a contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(st % 8 == 0 for st, n in zip(t.stride()[:-1], t.shape) if n > 1):
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[-2] == 1 or t.stride(-2) <= 1 << 24) \
+            and all(st % 8 == 0 for st, n in zip(t.stride()[:-1], t.shape) if n > 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
