@@ -489,17 +489,20 @@ typedef struct r2o_prompt_params {
     float sm_scale;           /* positive and finite */
     const float* lse_in;      /* weights only */
     float* weights;           /* weights only: fp32 [batch, hkv, keys], contiguous */
-    float* scratch;           /* weights with splits > 1: [splits, batch, hkv, keys] */
-    int64_t scratch_floats, splits;
+    float* scratch;           /* splits > 1: 130 floats a (split, request, query head, row), 16-byte aligned, or for
+                                 weights one a (split, request, KV head, key) */
+    int64_t scratch_floats;
+    int64_t splits;           /* workgroups that share the keys of one row tile, or the rows of one key tile */
 } r2o_prompt_params;
 
 /* out = softmax(sm_scale q k^T) v over the keys that each row sees, and lse = log of the sum of exponentials.
- * Every row is written: one that sees no key, or lies behind its request's length, is 0 with lse -inf. */
+ * Every row is written: one that sees no key, or lies behind its request's length, is 0 with lse -inf.  The states of
+ * the splits are joined in order: equal calls give equal bits. */
 int r2o_prompt_attention(const r2o_prompt_params* p, void* stream);
 
 /* weights[b, h, j] = sum over KV head h's query heads and the rows that see key j of
- * exp(sm_scale q . k_j - lse_in); 0 behind a request's length.  Rows with lse_in -inf give nothing.  The rows are
- * shared out over `splits` workgroups a key tile, whose sums are joined in a fixed order. */
+ * exp(sm_scale q . k_j - lse_in); 0 behind a request's length.  Rows with lse_in -inf give nothing.  The sums of
+ * the splits are joined in order. */
 int r2o_attention_weights(const r2o_prompt_params* p, void* stream);
 
 /* ------------------------------------------------------------------- paged KV cache ---- */

@@ -561,9 +561,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
             if (!t.sees(j, a.sinks)) continue;
             const int page = r2o_ldg(table + (j >> a.shift));
             if ((uint32_t)page >= (uint32_t)a.pages) continue;
+            const float* x = a.logits + (int64_t)tile * group * kSlots + r;
             float sum = 0.f;
-            for (int head = 0; head < group; ++head)
-                sum += __builtin_amdgcn_exp2f(r2o_ldg(a.logits + ((int64_t)tile * group + head) * kSlots + r) - lse2[head]);
+            for (int h0 = 0; h0 < group; h0 += 8) {  // eight loads in flight
+                float s[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] = r2o_ldg(x + min(h0 + i, group - 1) * kSlots);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += h0 + i < group ? __builtin_amdgcn_exp2f(s[i] - lse2[min(h0 + i, group - 1)]) : 0.f;
+            }
             float* w = a.weight + (int64_t)page * a.w_page + (int64_t)h * a.w_head + (j & ((1 << a.shift) - 1));
             *w = a.new_key && j == t.n - 1 ? sum : *w + sum;
         }
@@ -573,87 +579,167 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
 }
 
 // ------------------------------------------------------------------------------------------ evict
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / 64;
 
-// A total order of fp32 weights as integers: NaN above everything, -0 equal to 0.
+// Slots in the order in which they stay, as integers: protected ones, then weights (NaN first, -0 equal to 0), then
+// those of no page; 0 behind the filled ones.
+constexpr uint32_t kProtected = 0xffffffffu, kNaN = 0xfffffffeu, kNoPage = 1u;
+
 __device__ __forceinline__ uint32_t order_key(float w) {
-    if (w != w) return 0xffffffffu;
-    const uint32_t u = __float_as_uint(w + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(w + 0.f), k = (u & 0x80000000u) ? ~u : u | 0x80000000u;  // -inf: 0x007fffff, inf: 0xff800000
+    return w != w ? kNaN : k;
 }
 
-// One workgroup a (request, head): the weight that the last kept slot has is found digit by digit (8 bits a pass,
-// counts in LDS), then the kept slots are written in order: those above it, and of the equal ones the first.
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, R2O_WAVE);
+    return x;
+}
+
+// Sum over the workgroup's waves of a wave-uniform count; `slot` alternates, so that one barrier does.
+__device__ __forceinline__ int block_sum(int x, int (*counts)[kSelectWaves], int& slot, int wave) {
+    if ((threadIdx.x & 63) == 0) counts[slot][wave] = x;
+    __syncthreads();
+    const int4* c = reinterpret_cast<const int4*>(counts[slot]);
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < kSelectWaves / 4; ++i) {
+        const int4 y = c[i];
+        sum += y.x + y.y + y.z + y.w;
+    }
+    slot ^= 1;
+    return __builtin_amdgcn_readfirstlane(sum);
+}
+
+// One workgroup a (request, head).  A wave holds a run of neighbouring slots, E keys a lane in registers (the ones
+// behind 64 E are read again when they are needed).  The key of the last slot that stays is found bit by bit: the
+// largest T that at least `keep` keys reach, each step one comparison a key and one barrier, ending early when exactly
+// `keep` reach it.  Then every wave knows how many slots before its own stay, and writes its own in order: those above
+// T, and of the equal ones the first.  Bound by those steps' latency; no atomics.
+template <int E>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_evict_params p) {
-    __shared__ int hist[256];
-    __shared__ int scan[kSelectThreads / 64][2];
-    __shared__ int found[2];
+    __shared__ __align__(16) int counts[2][kSelectWaves];
+    __shared__ int before[kSelectWaves][2];
     const r2o_paged_cache& c = p.source;
-    const int h = blockIdx.x % (int)c.hkv, b = blockIdx.x / (int)c.hkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = filled(c, b), keep = (int)p.keep, shift = shift_of(c), mask = (1 << shift) - 1;
+    const int h = blockIdx.x % (int)c.hkv, b = blockIdx.x / (int)c.hkv, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = filled(c, b), keep = (int)p.keep;
     int32_t* kept = p.kept + (int64_t)blockIdx.x * keep;
     if (h == 0 && tid == 0) p.target_lengths[b] = min(n, keep);
     if (n <= keep) {
         for (int i = tid; i < keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
         return;
     }
-    const int lo = (int)p.sinks, hi = n - (int)p.recent;  // what may go
-    auto key_at = [&](int j) {
-        const int page = page_of(c, b, j, shift);
-        return page < 0 ? 0u : order_key(r2o_ldg(c.weight_pages + page * c.weight_strides[0] + h * c.weight_strides[1] + (j & mask)));
+    const int per_wave = max(E, (n + kSelectThreads - 1) / kSelectThreads), first = wave * per_wave * 64 + lane;
+    const int shift = shift_of(c), mask = (1 << shift) - 1, lo = (int)p.sinks, hi = n - (int)p.recent;  // [lo, hi) may go
+    const int32_t* table = c.page_table + b * c.table_stride;
+    const float* weights = c.weight_pages + h * c.weight_strides[1];
+    const int pages = (int)c.pages, w_page = (int)c.weight_strides[0];
+    auto page_at = [&](int j) { return r2o_ldg(table + (min(j, n - 1) >> shift)); };
+    auto weight_at = [&](int j, int page) {
+        const int id = (uint32_t)page < (uint32_t)pages ? page : 0;
+        return r2o_ldg(weights + (int64_t)id * w_page + (min(j, n - 1) & mask));
     };
-    int need = keep - (int)p.sinks - (int)p.recent;  // of [lo, hi)
-    uint32_t prefix = 0;
-    for (int d = 24; d >= 0; d -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = lo + tid; j < hi; j += kSelectThreads) {
-            const uint32_t k = key_at(j);
-            if (d == 24 || (k >> (d + 8)) == (prefix >> (d + 8))) atomicAdd(&hist[(k >> d) & 255], 1);
+    auto key_of = [&](int j, int page, float w) {
+        uint32_t k = (uint32_t)page < (uint32_t)pages ? order_key(w) : kNoPage;
+        k = j < lo || j >= hi ? kProtected : k;
+        return j < n ? k : 0u;
+    };
+    auto key_at = [&](int j) {
+        const int page = page_at(j);
+        return key_of(j, page, weight_at(j, page));
+    };
+    // the wave's page ids, at most 4 E of them, lie in its lanes; then all weights are in flight together
+    constexpr int kPageRegs = (4 * E + 63) / 64;
+    const int page0 = (first - lane) >> shift, last = (n - 1) >> shift;
+    int ids[kPageRegs];
+#pragma unroll
+    for (int i = 0; i < kPageRegs; ++i) ids[i] = r2o_ldg(table + min(page0 + 64 * i + lane, last));
+    auto page_in = [&](int j, int i) {  // of slot j, in row i
+        const int at = (j >> shift) - page0;
+        int id = __shfl(ids[0], at & 63, R2O_WAVE);
+#pragma unroll
+        for (int x = 1; x < kPageRegs; ++x) {
+            if (4 * i < 64 * x) break;  // 16 slots a page: row i is in register 4 i / 64, with larger pages in one before
+            const int y = __shfl(ids[x], at & 63, R2O_WAVE);
+            id = (at >> 6) == x ? y : id;
         }
-        __syncthreads();
-        if (tid == 0) {  // the digit with which the count from above first reaches `need`
-            int above = 0, x = 255;
-            while (x > 0 && above + hist[x] < need) above += hist[x--];
-            found[0] = x;
-            found[1] = need - above;
-        }
-        __syncthreads();
-        prefix |= (uint32_t)found[0] << d;
-        need = found[1];
-        __syncthreads();
+        return id;
+    };
+    uint32_t keys[E];
+    int from = first;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        asm volatile("" : "+v"(from));  // each place forms its slots anew: kept, they would spill
+        const int j = min(from + 64 * i, n - 1);
+        keys[i] = __float_as_uint(weight_at(j, page_in(j, i)));
+        __builtin_amdgcn_sched_barrier(0);  // row after row: what all of them need at once would spill
     }
-    // `need` of those equal to prefix stay
-    int at = 0, equal = 0;  // kept and equal ones before this chunk
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + tid;
-        const bool inside = j >= lo && j < hi;
-        const uint32_t k = inside ? key_at(j) : 0u;
-        const bool eq = inside && k == prefix, sure = j < n && (!inside || k > prefix);
-        const uint64_t eq_mask = __ballot(eq), sure_mask = __ballot(sure);
-        if (lane == 0) {
-            scan[wave][0] = __popcll(eq_mask);
-            scan[wave][1] = __popcll(sure_mask);
-        }
-        __syncthreads();
-        int eq_before = equal, sure_before = 0, eq_all = 0, sure_all = 0;
-        for (int w = 0; w < kSelectThreads / 64; ++w) {
-            if (w < wave) {
-                eq_before += scan[w][0];
-                sure_before += scan[w][1];
-            }
-            eq_all += scan[w][0];
-            sure_all += scan[w][1];
-        }
-        const uint64_t below = ((uint64_t)1 << lane) - 1;
-        eq_before += __popcll(eq_mask & below);
-        sure_before += __popcll(sure_mask & below);
-        const int eq_kept_before = min(eq_before, need) - min(equal, need);
-        if (sure || (eq && eq_before < need)) kept[at + sure_before + eq_kept_before] = j;
-        at += sure_all + min(equal + eq_all, need) - min(equal, need);
-        equal += eq_all;
-        __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        asm volatile("" : "+v"(from));
+        const int j = from + 64 * i;
+        keys[i] = key_of(j, page_in(min(j, n - 1), i), __uint_as_float(keys[i]));
+        asm volatile("" : "+v"(keys[i]));  // one key whole before the next
     }
+
+    int slot = 0, reach = n;  // keys >= t
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0 && reach > keep; --bit) {
+        const uint32_t trial = t | (1u << bit);
+        int x = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x += keys[i] >= trial ? 1 : 0;
+#pragma unroll 8
+        for (int i = E; i < per_wave; ++i) x += key_at(first + 64 * i) >= trial ? 1 : 0;
+        x = block_sum(wave_sum(x), counts, slot, wave);
+        if (x >= keep) {
+            t = trial;
+            reach = x;
+        }
+    }
+    t = (uint32_t)__builtin_amdgcn_readfirstlane((int)t);
+    if (reach == keep) --t;  // all that reach it stay, as those above t - 1
+    const uint32_t equal = reach == keep ? 0u : t;  // no key at all, or the key whose first slots fill up
+    int sures = 0, equals = 0;
+    auto count = [&](uint32_t k) {
+        sures += k > t ? 1 : 0;
+        equals += k == equal ? 1 : 0;
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < E; ++i) count(keys[i]);
+    for (int i = E; i < per_wave; ++i) count(key_at(first + 64 * i));
+    sures = wave_sum(sures);
+    equals = wave_sum(equals);
+    if (lane == 0) {
+        before[wave][0] = sures;
+        before[wave][1] = equals;
+    }
+    __syncthreads();
+    int sure_at = 0, equal_at = 0, sure_all = 0;
+    for (int x = 0; x < kSelectWaves; ++x) {
+        sure_all += before[x][0];
+        if (x < wave) {
+            sure_at += before[x][0];
+            equal_at += before[x][1];
+        }
+    }
+    const int still = keep - sure_all;  // of the equal ones; 0 where just `keep` reached
+    uint32_t above = t, same = equal;  // values of their own: the comparisons above are made again, not kept
+    asm volatile("" : "+s"(above), "+s"(same), "+v"(from));
+    auto write = [&](int j, uint32_t k) {
+        const bool sure = k > above, eq = k == same;
+        const uint64_t s = __ballot(sure), e = __ballot(eq), below = ((uint64_t)1 << lane) - 1;
+        const int e_at = equal_at + __popcll(e & below);
+        if (sure || (eq && e_at < still)) kept[sure_at + __popcll(s & below) + min(e_at, still)] = j;
+        sure_at += __popcll(s);
+        equal_at += __popcll(e);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < E; ++i) write(from + 64 * i, keys[i]);
+    for (int i = E; i < per_wave; ++i) write(from + 64 * i, key_at(from + 64 * i));
 }
 
 // 16 lanes move one kept slot's K and V row and its weight.
@@ -794,7 +880,11 @@ int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream) {
         !aligned(p->kept, 4) || !aligned(p->target_lengths, 4) || p->target_lengths == c.lengths)
         return R2O_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(c.batch * c.hkv)), dim3(kSelectThreads), 0, st, *p);
+    const dim3 rows((unsigned)(c.batch * c.hkv)), threads(kSelectThreads);
+    const int64_t most = c.max_pages * c.page_size;  // slots that a lane holds: those of the longest request there can be
+    if (most <= 8 * kSelectThreads) hipLaunchKernelGGL(paged_select_kernel<8>, rows, threads, 0, st, *p);
+    else if (most <= 32 * kSelectThreads) hipLaunchKernelGGL(paged_select_kernel<32>, rows, threads, 0, st, *p);
+    else hipLaunchKernelGGL(paged_select_kernel<128>, rows, threads, 0, st, *p);
     R2O_CHECK_LAUNCH();
     hipLaunchKernelGGL(paged_compact_kernel, dim3((unsigned)((p->keep + 15) / 16), (unsigned)c.hkv, (unsigned)c.batch), dim3(256), 0,
                        st, *p);

@@ -128,7 +128,7 @@ struct PromptArgs {
     float* lse;
     const int32_t *query_lengths, *key_lengths;
     const float* lse_in;
-    float* weights;
+    float *weights, *partial_out, *partial_ml;
     int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head, o_batch, o_head;
     int q_row, k_row, v_row, o_row, hq, hkv, group, queries, keys, window, sinks;
     float c2;  // scale, in log2 units
@@ -157,35 +157,45 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
 }
 
 // ------------------------------------------------------------------------------ prompt attention
+// The rows of a KV head's query heads are one list, packed row r = (row r / group, head r % group): a workgroup's 128
+// stand at 128 / group neighbouring positions, so its last tiles are masked in part for few of them, and a chunk of few
+// rows fills it.  grid: (row tiles, splits, batch * hkv); with splits each takes a share of the key tiles and leaves
+// (maximum, sum, products) in scratch for prompt_join_kernel.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     __shared__ __align__(16) unsigned char k_lds[2][kTileBytes], v_lds[2][kTileBytes];
     __shared__ int any_bad;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-    const int h = blockIdx.y, b = blockIdx.z;
-    const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kRows;  // the longest rows first
     Args& a = kernel_args();
+    const int kvh = (int)blockIdx.z % a.hkv, b = (int)blockIdx.z / a.hkv, group = a.group, rows = a.queries * group;
+    const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kRows;  // the longest rows first
     const Lengths s = request_lengths(a, b);
-    const int window = a.window, sinks = a.sinks, kvh = h / a.group;
+    const int window = a.window, sinks = a.sinks;
     const uint16_t* kbase = a.key + b * a.k_batch + kvh * a.k_head;
     const uint16_t* vbase = a.value + b * a.v_batch + kvh * a.v_head;
     const int k_row = a.k_row, v_row = a.v_row;
 
-    const int row = row0 + 32 * wave + col;  // this lane's query row
+    const int packed = row0 + 32 * wave + col, row = min(packed, rows - 1) / group, head = min(packed, rows - 1) - row * group;
     r2o_u4 q[8];
     {
-        const uint16_t* src = a.query + b * a.q_batch + h * a.q_head + (int64_t)min(row, a.queries - 1) * a.q_row + 8 * half;
+        const uint16_t* src = a.query + b * a.q_batch + (kvh * group + head) * a.q_head + (int64_t)row * a.q_row + 8 * half;
 #pragma unroll
         for (int t = 0; t < 8; ++t) q[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
     }
     if (threadIdx.x == 0) any_bad = 0;
 
+    // positions of the workgroup's rows and of this wave's
+    const int wg_first = row0 / group, wg_last = min(row0 + kRows - 1, rows - 1) / group;
+    const int wg_min = s.off + wg_first, wg_max = s.off + wg_last;
+    const int w0 = min(row0 + 32 * wave, rows - 1), pmin = s.off + w0 / group, pmax = s.off + min(w0 + 31, rows - 1) / group;
+    const int p = s.off + row, pv = min(p, s.n - 1);
     // key tiles that any row of the workgroup sees: sink tiles, then the window's
-    const int top = min(s.n - 1, s.off + min(row0 + kRows, s.q) - 1);  // last position of the workgroup's rows
-    const int first = max(0, s.off + row0 - window + 1) / kTile;
-    const int end = row0 < s.q && top >= 0 ? top / kTile + 1 : 0;
+    const int top = min(s.n - 1, wg_max);
+    const int first = max(0, wg_min - window + 1) / kTile;
+    const int end = wg_first < s.q && top >= 0 ? top / kTile + 1 : 0;
     const int sink_tiles = end ? min((sinks + kTile - 1) / kTile, min(first, end)) : 0;
-    const int tiles = sink_tiles + max(0, end - first);
+    const int all = sink_tiles + max(0, end - first);
+    const int begin = (int)((int64_t)all * blockIdx.y / gridDim.y), tiles = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
     const int last = max(s.n - 1, 0);
 
     const float c2 = a.c2;
@@ -195,8 +205,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     for (int i = 0; i < 4; ++i) acc[i] = f16v{};
 
     auto tile_key = [&](int it) { return (it < sink_tiles ? it : first + it - sink_tiles) * kTile; };
-    const int wg_min = s.off + row0, pmin = wg_min + 32 * wave, pmax = pmin + 31, p = pmin + col, pv = min(p, s.n - 1);
-    auto seen_in_part = [&](int kt) { return !(kt + kTile - 1 <= wg_min && (kt > wg_min + kRows - 1 - window || kt + kTile <= sinks)); };
+    auto seen_in_part = [&](int kt) { return !(kt + kTile - 1 <= wg_min && (kt > wg_max - window || kt + kTile <= sinks)); };
     // The next tile is on its way into registers while this one is computed on: loads straight into LDS would save the
     // registers, but the compiler waits for all of them before the transposing reads.
     r2o_u4 kx[4], vx[4];
@@ -259,11 +268,11 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
             for (int db = 0; db < 4; ++db) acc[db] = mfma32<RF>(read_values(vl, kb, db, lane), pk[kb], acc[db]);
     };
     __syncthreads();
-    if (tiles > 0) {
-        load(0);
-        store(0);
+    if (begin < tiles) {
+        load(begin);
+        store(begin);
     }
-    for (int it = 0; it < tiles; ++it) {
+    for (int it = begin; it < tiles; ++it) {
         __syncthreads();  // the tile is there, and every wave is done with the one before
         if (it + 1 < tiles) load(it + 1);
         compute(tile_key(it), k_lds[it & 1], v_lds[it & 1]);
@@ -271,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     }
     __syncthreads();
     if (any_bad) {  // what was taken out, for the rows that see it
-        for (int it = 0; it < tiles; ++it) {
+        for (int it = begin; it < tiles; ++it) {
             const int kt = tile_key(it);
             if (!seen_in_part(kt)) continue;
             for (int j = kt; j < min(kt + kTile, s.n); ++j) {
@@ -293,11 +302,25 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
         r2o_row_swap<32>(l, x, y);
         l = x + y;
     }
+    if (packed >= rows) return;
     Args& e = kernel_args();
-    if (row >= e.queries) return;
+    if (gridDim.y > 1) {
+        const int64_t at = ((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * rows + packed;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<R2O_GLOBAL r2o_f4*>((R2O_GLOBAL float*)(e.partial_out + at * 128 + 32 * db + 8 * g + 4 * half)) =
+                    r2o_f4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+        if (half == 0) {
+            e.partial_ml[2 * at] = row < s.q ? m : -INFINITY;
+            e.partial_ml[2 * at + 1] = l;
+        }
+        return;
+    }
     const bool live = row < s.q && m != -INFINITY;
     const float inv = live ? 1.f / l : 0.f;
-    uint16_t* dst = e.out + b * e.o_batch + h * e.o_head + (int64_t)row * e.o_row;
+    uint16_t* dst = e.out + b * e.o_batch + (kvh * group + head) * e.o_head + (int64_t)row * e.o_row;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -308,7 +331,37 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
                 w[k] = live ? pack2<RF>(acc[db][4 * g + 2 * k] * inv, acc[db][4 * g + 2 * k + 1] * inv) : 0u;
             *reinterpret_cast<R2O_GLOBAL r2o_u2*>((R2O_GLOBAL uint16_t*)(dst + 32 * db + 8 * g + 4 * half)) = w;
         }
-    if (half == 0) e.lse[((int64_t)b * e.hq + h) * e.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    if (half == 0)
+        e.lse[((int64_t)b * e.hq + kvh * group + head) * e.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+// 32 lanes a packed row: its splits' states, joined in order.
+template <int RF>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits) {
+    Args& a = kernel_args();
+    const int kvh = (int)blockIdx.y % a.hkv, b = (int)blockIdx.y / a.hkv, group = a.group, rows = a.queries * group;
+    const int packed = blockIdx.x * 8 + (threadIdx.x >> 5), d4 = threadIdx.x & 31;
+    if (packed >= rows) return;
+    const int row = packed / group, head = packed - row * group;
+    float m = -INFINITY, l = 0.f;
+    r2o_f4 o{};
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) {
+        const int64_t at = ((int64_t)i * gridDim.y + blockIdx.y) * rows + packed;
+        const float m2 = r2o_ldg(a.partial_ml + 2 * at), l2 = r2o_ldg(a.partial_ml + 2 * at + 1);
+        const r2o_f4 o2 = r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4);
+        const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f(m - ms), f2 = __builtin_amdgcn_exp2f(m2 - ms);
+        l = l * f + l2 * f2;
+        o = m2 == -INFINITY ? o : o * f + o2 * f2;
+        m = mn;
+    }
+    const bool live = m != -INFINITY;
+    const float inv = live ? 1.f / l : 0.f;
+    r2o_u2 w{};
+    if (live) w = r2o_u2{pack2<RF>(o[0] * inv, o[1] * inv), pack2<RF>(o[2] * inv, o[3] * inv)};
+    *reinterpret_cast<R2O_GLOBAL r2o_u2*>((R2O_GLOBAL uint16_t*)(a.out + b * a.o_batch + (kvh * group + head) * a.o_head + (int64_t)row * a.o_row + 4 * d4)) = w;
+    if (d4 == 0) a.lse[((int64_t)b * a.hq + kvh * group + head) * a.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
 // ----------------------------------------------------------------------------- attention weights
@@ -465,12 +518,23 @@ int r2o_prompt_attention(const r2o_prompt_params* p, void* stream) {
     if (!shapes_ok(p) || !aligned({p->value, p->out}, 16) || !aligned({p->lse}, 4) || !strides_ok(p->v_strides) ||
         !strides_ok(p->o_strides))
         return R2O_EINVAL;
-    const dim3 grid((unsigned)((p->queries + kRows - 1) / kRows), (unsigned)p->hq, (unsigned)p->batch);
+    const int64_t rows = p->queries * (p->hq / p->hkv), pairs = p->batch * p->hkv;
+    if (rows > (1 << 30) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
+    if (p->splits > 1 && (!aligned({p->scratch}, 16) || p->scratch_floats < p->splits * pairs * rows * 130)) return R2O_EINVAL;
+    const dim3 grid((unsigned)((rows + kRows - 1) / kRows), (unsigned)p->splits, (unsigned)pairs);
+    const dim3 join((unsigned)((rows + 7) / 8), (unsigned)pairs);
     const hipStream_t st = (hipStream_t)stream;
-    const PromptArgs a = kernel_arguments(p);
+    PromptArgs a = kernel_arguments(p);
+    a.partial_out = p->scratch;
+    a.partial_ml = p->scratch + p->splits * pairs * rows * 128;
     if (p->dtype == 0) hipLaunchKernelGGL(prompt_attention_kernel<0>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(prompt_attention_kernel<1>, grid, dim3(256), 0, st, a);
     R2O_CHECK_LAUNCH();
+    if (p->splits > 1) {
+        if (p->dtype == 0) hipLaunchKernelGGL(prompt_join_kernel<0>, join, dim3(256), 0, st, a, (int)p->splits);
+        else hipLaunchKernelGGL(prompt_join_kernel<1>, join, dim3(256), 0, st, a, (int)p->splits);
+        R2O_CHECK_LAUNCH();
+    }
     return R2O_OK;
 }
 

@@ -67,7 +67,8 @@ def _check_rows(query: torch.Tensor, key: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} requires equal batch sizes and positive head and row counts")
     if query.shape[1] % key.shape[1]:
         raise ValueError("GQA requires Hq divisible by Hkv")
-    if max(query.shape[2], key.shape[2]) > _MOST_ROWS or query.shape[0] * query.shape[1] > 65535:
+    if max(query.shape[2], key.shape[2]) > _MOST_ROWS or query.shape[0] * query.shape[1] > 65535 \
+            or query.shape[1] // key.shape[1] * query.shape[2] > 1 << 30:
         raise ValueError(f"{what} takes at most 2^29 rows and 65535 (request, query head) pairs")
     if query.device != key.device or query.dtype != key.dtype:
         raise ValueError("Q/K device and dtype must match")
@@ -83,6 +84,14 @@ def _params(query, key, window, sinks, query_lengths, key_lengths, sm_scale) -> 
         query_lengths=_lib.ptr(query_lengths), key_lengths=_lib.ptr(key_lengths), batch=query.shape[0], hq=query.shape[1],
         hkv=key.shape[1], queries=query.shape[2], keys=key.shape[2], dtype=_lib.dtype_code(query.dtype), window=w, sinks=s,
         sm_scale=_scale(sm_scale))
+
+
+def attention_splits(batch: int, hq: int, hkv: int, queries: int, keys: int, window, num_cus: int) -> int:
+    """Workgroups that share the keys of one 128-row tile: enough for two a compute unit, each with at least four
+    tiles of 64 keys."""
+    row_tiles = -(-(hq // hkv) * queries // 128) * batch * hkv
+    seen = keys if window is None else min(keys, int(window) + queries + 128)
+    return max(1, min(-(-2 * num_cus // row_tiles), -(-seen // 256)))
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, window: int | None = None,
@@ -122,6 +131,11 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != query.device \
                 or not lse.is_contiguous():
             raise ValueError("prompt attention lse output must be contiguous fp32 [B,Hq,Sq] on Q's device")
+    p.splits = attention_splits(batch, hq, key.shape[1], rows, key.shape[2], window, _lib.num_cus(query.device))
+    scratch = None
+    if p.splits > 1:
+        scratch = torch.empty(130 * p.splits * batch * hq * rows, dtype=torch.float32, device=query.device)
+        p.scratch, p.scratch_floats = scratch.data_ptr(), scratch.numel()
     p.value, p.v_strides = value.data_ptr(), _strides(value, 3)
     p.out, p.o_strides, p.lse = out.data_ptr(), _strides(out, 3), lse.data_ptr()
     _lib.launch("r2o_prompt_attention", p, query.device)

@@ -94,7 +94,9 @@ def test_c_abi_refuses(what):
 def test_c_abi_refuses_outputs_and_scratch():
     lib = _lib.load()
     for kw in (dict(out=None), dict(out=0x4008), dict(lse=None), dict(value=None),
-               dict(v_strides=(ctypes.c_int64 * 3)(1, 128, 128))):
+               dict(v_strides=(ctypes.c_int64 * 3)(1, 128, 128)), dict(splits=0), dict(splits=2),
+               dict(splits=2, scratch=0x9000, scratch_floats=2 * 4 * 16 * 130 - 1), dict(splits=2, scratch=0x9008, scratch_floats=1 << 20),
+               dict(q_strides=(ctypes.c_int64 * 3)(8, 8, (1 << 24) + 8))):
         assert lib.r2o_prompt_attention(ctypes.byref(_params(**kw)), None) == 1, kw
     for kw in (dict(lse_in=None), dict(weights=None), dict(splits=0), dict(splits=2), dict(splits=65536),
                dict(splits=2, scratch=0x9000, scratch_floats=2 * 2 * 16 - 1)):
