@@ -5,6 +5,8 @@
 // arguments and ~45 metadata views took ~80 us next to 9 us of kernels: 92 -> 68 us (4k tokens), 99 -> 75
 // (64k, 38 us of kernels).
 //
+// A call on a paged cache or a prompt's rows took 16 to 20 us in Python, more than a decode step's kernels.
+//
 // The decode entry takes the forms that a model's step uses and returns None for every other (strided or
 // misaligned rows, other types, a full ring, a folded rotation, any error): those keep the Python path and
 // its checks and messages.  It keeps nothing from a call.  The library's functions come as addresses, so
@@ -14,9 +16,11 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <vector>
 
@@ -357,10 +361,373 @@ PyObject* cache_build(PyObject*, PyObject* args) {
     return Py_BuildValue("(iNN)", rc, tensors, fields);
 }
 
+// ------------------------------------------------------------------------- prompt and paged calls
+// Each takes the forms that a model's layer uses, allocates its results and scratch and launches; None for every other
+// (strides or alignments that need a copy, other types, an operand that a check refuses, another device than the
+// current one): those keep the Python path and its checks and messages.
+int current_device() {
+    int d = -1;
+    return hipGetDevice(&d) == hipSuccess ? d : -1;
+}
+
+int64_t compute_units(int device) {
+    static int known[64] = {};
+    if (device < 0 || device >= 64) return 0;
+    if (!known[device]) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) return 0;
+        known[device] = n;
+    }
+    return known[device];
+}
+
+bool needs_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// Strides of the axes before the channels: multiples of 8 elements, the rows' within 32-bit offsets; 0 for an axis of one.
+bool row_strides(const at::Tensor& t, int64_t n, int64_t* out, bool own_memory = false) {
+    if (t.stride(-1) != 1 || !aligned16(t)) return false;
+    for (int64_t i = 0; i < n; ++i) {
+        out[i] = t.size(i) > 1 ? t.stride(i) : 0;
+        if (out[i] % 8 || out[i] < 0 || (own_memory && t.size(i) > 1 && out[i] == 0)) return false;
+    }
+    return true;
+}
+
+// None, or a contiguous int32 tensor [batch] on the device.
+bool lengths_arg(PyObject* o, int64_t batch, int64_t device, const int32_t*& out) {
+    out = nullptr;
+    if (o == Py_None) return true;
+    const at::Tensor* t = exact_tensor(o);
+    if (!t || !on_device(*t, device) || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != batch || !t->is_contiguous())
+        return false;
+    out = static_cast<const int32_t*>(t->data_ptr());
+    return true;
+}
+
+// window and sinks as Python ints (window None: 0), the scale as a float (None: 1 / sqrt(128)).
+bool mask_args(PyObject* window_o, PyObject* sinks_o, PyObject* scale_o, int64_t& window, int64_t& sinks, float& scale) {
+    window = 0;
+    if (window_o != Py_None && (!plain_int(window_o, window) || window < 1)) return false;
+    if (!plain_int(sinks_o, sinks) || sinks < 0 || sinks > (1 << 29)) return false;
+    if (scale_o == Py_None) {
+        scale = 0.08838834764831845f;
+        return true;
+    }
+    if (!PyFloat_CheckExact(scale_o)) return false;
+    const double x = PyFloat_AS_DOUBLE(scale_o);
+    scale = (float)x;
+    return x > 0.0 && scale > 0.f && scale < INFINITY;
+}
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Workgroups that share the keys of one 128-row tile: enough for two a compute unit, each with at least four tiles of
+// 64 keys.
+int64_t attention_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries, int64_t keys, int64_t window, int64_t cus) {
+    const int64_t tiles = div_up(hq / hkv * queries, 128) * batch * hkv;
+    const int64_t seen = window ? std::min(keys, std::min(window, keys) + queries + 128) : keys;
+    return std::max<int64_t>(1, std::min(div_up(2 * cus, tiles), div_up(seen, 256)));
+}
+
+// Workgroups that share the query rows of one key tile: enough for four a compute unit, at most one for each (query
+// head, 64-row tile) pair.
+int64_t weight_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries, int64_t keys, int64_t cus) {
+    const int64_t tiles = div_up(keys, 128) * batch * hkv, pairs = hq / hkv * div_up(queries, 64);
+    return std::max<int64_t>(1, std::min(pairs, div_up(4 * cus, tiles)));
+}
+
+// Workgroups that share the slots of a call: one a compute unit (their LDS fills it), fewer when the page tables hold
+// fewer than four tiles of 32 slots for each.
+int64_t paged_workers(int64_t batch, int64_t hkv, int64_t capacity, int64_t cus) {
+    return std::max<int64_t>(1, std::min(cus, batch * hkv * div_up(capacity, 128)));
+}
+
+// The fields that attention and weights share; false for what the Python path has to look at.
+bool prompt_operands(const at::Tensor* q, const at::Tensor* k, PyObject* const* masks, r2o_prompt_params& p, int64_t& device) {
+    if (!q || !k || q->dim() != 4 || k->dim() != 4 || q->size(3) != R2O_HEAD_DIM || k->size(3) != R2O_HEAD_DIM) return false;
+    device = current_device();
+    if (!on_device(*q, device) || !on_device(*k, device) || row_code(*q) < 0 || q->scalar_type() != k->scalar_type() ||
+        needs_grad(*q) || needs_grad(*k))
+        return false;
+    constexpr int64_t kMost = 1 << 29;
+    p.batch = q->size(0);
+    p.hq = q->size(1);
+    p.hkv = k->size(1);
+    p.queries = q->size(2);
+    p.keys = k->size(2);
+    p.dtype = row_code(*q);
+    if (k->size(0) != p.batch || p.batch < 1 || p.hkv < 1 || p.hq < 1 || p.hq % p.hkv || p.queries < 1 || p.keys < 1 ||
+        p.queries > kMost || p.keys > kMost || p.batch * p.hq > 65535 || p.hq / p.hkv * p.queries > 2 * kMost)
+        return false;
+    if (!row_strides(*q, 3, p.q_strides) || !row_strides(*k, 3, p.k_strides) || p.q_strides[2] > R2O_MAX_ROW_STRIDE ||
+        p.k_strides[2] > R2O_MAX_ROW_STRIDE)
+        return false;
+    p.query = static_cast<const uint16_t*>(q->data_ptr());
+    p.key = static_cast<const uint16_t*>(k->data_ptr());
+    return mask_args(masks[0], masks[1], masks[4], p.window, p.sinks, p.sm_scale) &&
+           lengths_arg(masks[2], p.batch, device, p.query_lengths) && lengths_arg(masks[3], p.batch, device, p.key_lengths);
+}
+
+template <class Params>
+int launch_on(PyObject* fn, const Params& p, int64_t device) {
+    auto* f = reinterpret_cast<int (*)(const Params*, void*)>(PyLong_AsVoidPtr(fn));
+    void* stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
+    WithoutGil released;
+    return f(&p, stream);
+}
+
+// (status, tensors ...)
+PyObject* status_and(int rc, const std::vector<at::Tensor>& ts) {
+    PyObject* tuple = PyTuple_New(1 + (Py_ssize_t)ts.size());
+    if (!tuple) return nullptr;
+    PyTuple_SET_ITEM(tuple, 0, PyLong_FromLong(rc));
+    for (size_t i = 0; i < ts.size(); ++i) {
+        PyObject* o = wrap(ts[i]);
+        if (!o) {
+            Py_DECREF(tuple);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(tuple, 1 + (Py_ssize_t)i, o);
+    }
+    return tuple;
+}
+
+// prompt(function, query, key, value, window, sinks, query_lengths, key_lengths, scale): (status, out, lse) or None
+PyObject* prompt_call(PyObject* const* args) {
+    r2o_prompt_params p{};
+    int64_t device;
+    const at::Tensor *q = exact_tensor(args[1]), *k = exact_tensor(args[2]), *v = exact_tensor(args[3]);
+    if (!prompt_operands(q, k, args + 4, p, device) || !v || v->sizes() != k->sizes() || !on_device(*v, device) ||
+        v->scalar_type() != k->scalar_type() || needs_grad(*v) || !row_strides(*v, 3, p.v_strides) || p.v_strides[2] > R2O_MAX_ROW_STRIDE)
+        Py_RETURN_NONE;
+    at::Tensor out = at::empty_like(*q);
+    if (!row_strides(out, 3, p.o_strides, true) || p.o_strides[2] > R2O_MAX_ROW_STRIDE) Py_RETURN_NONE;
+    const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
+    at::Tensor lse = at::empty({p.batch, p.hq, p.queries}, f32), scratch;
+    p.splits = attention_splits(p.batch, p.hq, p.hkv, p.queries, p.keys, p.window, compute_units((int)device));
+    if (p.splits > 1) {
+        p.scratch_floats = 130 * p.splits * p.batch * p.hq * p.queries;
+        scratch = at::empty({p.scratch_floats}, f32);
+        p.scratch = scratch.data_ptr<float>();
+    }
+    p.value = static_cast<const uint16_t*>(v->data_ptr());
+    p.out = static_cast<uint16_t*>(out.data_ptr());
+    p.lse = lse.data_ptr<float>();
+    return status_and(launch_on(args[0], p, device), {out, lse});
+}
+
+// weights(function, query, key, lse, window, sinks, query_lengths, key_lengths, scale): (status, weights) or None
+PyObject* weights_call(PyObject* const* args) {
+    r2o_prompt_params p{};
+    int64_t device;
+    const at::Tensor *q = exact_tensor(args[1]), *k = exact_tensor(args[2]), *lse = exact_tensor(args[3]);
+    if (!prompt_operands(q, k, args + 4, p, device) || !lse || !on_device(*lse, device) || lse->scalar_type() != at::kFloat ||
+        lse->dim() != 3 || lse->size(0) != p.batch || lse->size(1) != p.hq || lse->size(2) != p.queries || !lse->is_contiguous())
+        Py_RETURN_NONE;
+    const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
+    at::Tensor out = at::empty({p.batch, p.hkv, p.keys}, f32), scratch;
+    p.splits = weight_splits(p.batch, p.hq, p.hkv, p.queries, p.keys, compute_units((int)device));
+    if (p.splits > 1) {
+        p.scratch_floats = p.splits * out.numel();
+        scratch = at::empty({p.scratch_floats}, f32);
+        p.scratch = scratch.data_ptr<float>();
+    }
+    p.lse_in = lse->data_ptr<float>();
+    p.weights = out.data_ptr<float>();
+    return status_and(launch_on(args[0], p, device), {out});
+}
+
+// paged_cache(key pages, value pages, page table, lengths, weight pages or None): the r2o_paged_cache as bytes, or None
+PyObject* paged_cache_call(PyObject* const* args) {
+    const at::Tensor *k = exact_tensor(args[0]), *v = exact_tensor(args[1]), *table = exact_tensor(args[2]), *n = exact_tensor(args[3]);
+    const at::Tensor* w = args[4] == Py_None ? nullptr : exact_tensor(args[4]);
+    if (!k || !v || !table || !n || (args[4] != Py_None && !w) || k->dim() != 4 || k->device().type() != at::kCUDA) Py_RETURN_NONE;
+    const int64_t device = k->device().index();
+    r2o_paged_cache c{};
+    c.pages = k->size(0);
+    c.hkv = k->size(1);
+    c.page_size = k->size(2);
+    c.dtype = row_code(*k);
+    for (const at::Tensor* t : {k, v, table, n})
+        if (!on_device(*t, device)) Py_RETURN_NONE;
+    if (c.dtype < 0 || k->size(3) != R2O_HEAD_DIM || c.pages < 1 || c.pages > 0x7fffffff || c.hkv < 1 || c.hkv > 1024 ||
+        v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() ||
+        (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128))
+        Py_RETURN_NONE;
+    if (!row_strides(*k, 3, c.key_strides, true) || !row_strides(*v, 3, c.value_strides, true)) Py_RETURN_NONE;
+    for (int i = 0; i < 3; ++i)
+        if (std::max(c.key_strides[i], c.value_strides[i]) > (i == 2 ? R2O_PAGED_MAX_SLOT_STRIDE : 0x7fffffff)) Py_RETURN_NONE;
+    if (table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) < 1 || table->size(1) < 1 ||
+        (table->size(1) > 1 && table->stride(1) != 1) || n->scalar_type() != at::kInt || n->dim() != 1 || n->size(0) != table->size(0) ||
+        !n->is_contiguous())
+        Py_RETURN_NONE;
+    c.batch = table->size(0);
+    c.max_pages = table->size(1);
+    c.table_stride = std::max(table->stride(0), c.max_pages);
+    if (c.batch > R2O_PAGED_MAX_BATCH || c.max_pages * c.page_size > (1 << 29) || c.table_stride > 0x7fffffff) Py_RETURN_NONE;
+    if (w) {
+        if (!on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != c.pages || w->size(1) != c.hkv ||
+            w->size(2) != c.page_size || w->stride(2) != 1)
+            Py_RETURN_NONE;
+        for (int i = 0; i < 2; ++i) {
+            c.weight_strides[i] = w->size(i) > 1 ? w->stride(i) : 0;
+            if (w->size(i) > 1 && (c.weight_strides[i] < 1 || c.weight_strides[i] > 0x7fffffff)) Py_RETURN_NONE;
+        }
+        c.weight_pages = w->data_ptr<float>();
+    }
+    c.key_pages = static_cast<uint16_t*>(k->data_ptr());
+    c.value_pages = static_cast<uint16_t*>(v->data_ptr());
+    c.page_table = table->data_ptr<int32_t>();
+    c.lengths = n->data_ptr<int32_t>();
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&c), sizeof(c));
+}
+
+// The cache's fields, if its tensors lie on the current device.
+bool cache_arg(PyObject* bytes, PyObject* keys, r2o_paged_cache& c, int64_t& device) {
+    const at::Tensor* k = exact_tensor(keys);
+    device = current_device();
+    if (!PyBytes_CheckExact(bytes) || PyBytes_GET_SIZE(bytes) != (Py_ssize_t)sizeof(c) || !k || !on_device(*k, device)) return false;
+    std::memcpy(&c, PyBytes_AS_STRING(bytes), sizeof(c));
+    return true;
+}
+
+bool cache_rows(const at::Tensor* t, const r2o_paged_cache& c, int64_t device) {
+    return t && on_device(*t, device) && row_code(*t) == c.dtype;
+}
+
+// paged_extend(function, cache, key pages, key, value, counts, weights): (status,) or None
+PyObject* paged_extend_call(PyObject* const* args) {
+    r2o_paged_extend_params p{};
+    int64_t device;
+    const at::Tensor *k = exact_tensor(args[3]), *v = exact_tensor(args[4]);
+    if (!cache_arg(args[1], args[2], p.cache, device) || !cache_rows(k, p.cache, device) || !cache_rows(v, p.cache, device) ||
+        k->dim() != 4 || k->size(0) != p.cache.batch || k->size(1) != p.cache.hkv || k->size(3) != R2O_HEAD_DIM || v->sizes() != k->sizes())
+        Py_RETURN_NONE;
+    p.rows = k->size(2);
+    if (p.rows < 1 || p.rows > p.cache.max_pages * p.cache.page_size || !row_strides(*k, 3, p.key_strides) ||
+        !row_strides(*v, 3, p.value_strides) || p.key_strides[2] > R2O_MAX_ROW_STRIDE || p.value_strides[2] > R2O_MAX_ROW_STRIDE ||
+        !lengths_arg(args[5], p.cache.batch, device, p.counts))
+        Py_RETURN_NONE;
+    if (args[6] != Py_None) {
+        const at::Tensor* w = exact_tensor(args[6]);
+        if (!w || !p.cache.weight_pages || !on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 ||
+            w->size(0) != k->size(0) || w->size(1) != k->size(1) || w->size(2) != k->size(2) || !w->is_contiguous())
+            Py_RETURN_NONE;
+        p.weights = w->data_ptr<float>();
+        p.weights_strides[0] = w->stride(0);
+        p.weights_strides[1] = w->stride(1);
+    }
+    p.key = static_cast<const uint16_t*>(k->data_ptr());
+    p.value = static_cast<const uint16_t*>(v->data_ptr());
+    return status_and(launch_on(args[0], p, device), {});
+}
+
+// paged_attention(function, cache, key pages, query, append or None, window, sinks, scale): (status, out, lse) or None
+PyObject* paged_attention_call(PyObject* const* args) {
+    r2o_paged_attention_params p{};
+    r2o_paged_cache& c = p.cache;
+    int64_t device;
+    const at::Tensor* q = exact_tensor(args[3]);
+    if (!cache_arg(args[1], args[2], c, device) || !cache_rows(q, c, device) || needs_grad(*q) ||
+        !(q->dim() == 3 || (q->dim() == 4 && q->size(2) == 1)) || q->size(0) != c.batch || q->size(-1) != R2O_HEAD_DIM)
+        Py_RETURN_NONE;
+    p.hq = q->size(1);
+    if (p.hq < 1 || p.hq % c.hkv || p.hq / c.hkv > R2O_MAX_GQA || !row_strides(*q, 2, p.query_strides) ||
+        !mask_args(args[5], args[6], args[7], p.window, p.sinks, p.sm_scale) ||
+        std::max(p.query_strides[0], p.query_strides[1]) > 0x7fffffff)
+        Py_RETURN_NONE;
+    if (args[4] != Py_None) {
+        if (!PyTuple_CheckExact(args[4]) || PyTuple_GET_SIZE(args[4]) != 2) Py_RETURN_NONE;
+        for (int i = 0; i < 2; ++i) {
+            const at::Tensor* t = exact_tensor(PyTuple_GET_ITEM(args[4], i));
+            if (!cache_rows(t, c, device) || !(t->dim() == 3 || (t->dim() == 4 && t->size(2) == 1)) || t->size(0) != c.batch ||
+                t->size(1) != c.hkv || t->size(-1) != R2O_HEAD_DIM || !row_strides(*t, 2, p.append_strides + 2 * i) ||
+                std::max(p.append_strides[2 * i], p.append_strides[2 * i + 1]) > 0x7fffffff)
+                Py_RETURN_NONE;
+            (i ? p.append_value : p.append_key) = static_cast<const uint16_t*>(t->data_ptr());
+        }
+    }
+    const int64_t capacity = c.max_pages * c.page_size, group = p.hq / c.hkv;
+    if (c.batch * c.hkv * div_up(capacity, 32) > 0x7fffffff - R2O_PAGED_MAX_WORKERS) Py_RETURN_NONE;
+    p.workers = paged_workers(c.batch, c.hkv, capacity, compute_units((int)device));
+    p.partial_states = (p.workers + c.batch * c.hkv) * group;
+    p.logits_floats = c.weight_pages ? c.batch * p.hq * div_up(capacity, 32) * 32 : 0;
+    const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
+    at::Tensor out = at::empty({c.batch, p.hq, R2O_HEAD_DIM}, q->options()), lse = at::empty({c.batch, p.hq}, f32);
+    at::Tensor scratch = at::empty({130 * p.partial_states + 2 + p.logits_floats}, f32);
+    p.query = static_cast<const uint16_t*>(q->data_ptr());
+    p.out = static_cast<uint16_t*>(out.data_ptr());
+    p.lse = lse.data_ptr<float>();
+    p.partial_out = scratch.data_ptr<float>();  // then the (maximum, sum) pairs and, 16-byte aligned, the logits
+    p.partial_ml = p.partial_out + 128 * p.partial_states;
+    if (p.logits_floats) p.logits = p.partial_out + div_up(130 * p.partial_states, 4) * 4;
+    return status_and(launch_on(args[0], p, device), {out, lse});
+}
+
+// paged_evict(function, cache, key pages, target, target's key pages, target's lengths, keep, sinks, recent): (status,
+// kept) or None
+PyObject* paged_evict_call(PyObject* const* args) {
+    r2o_paged_evict_params p{};
+    int64_t device;
+    const at::Tensor* lengths = exact_tensor(args[5]);
+    if (!cache_arg(args[1], args[2], p.source, device) || !cache_arg(args[3], args[4], p.target, device) || !lengths ||
+        !plain_int(args[6], p.keep) || !plain_int(args[7], p.sinks) || !plain_int(args[8], p.recent))
+        Py_RETURN_NONE;
+    const r2o_paged_cache &c = p.source, &o = p.target;
+    if (!c.weight_pages || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || c.lengths == o.lengths ||
+        c.page_table == o.page_table || p.keep < 1 || p.keep > o.max_pages * o.page_size || p.sinks < 0 || p.recent < 0 ||
+        p.sinks + p.recent > p.keep)
+        Py_RETURN_NONE;
+    at::Tensor kept = at::empty({c.batch, c.hkv, p.keep}, lengths->options());
+    p.kept = kept.data_ptr<int32_t>();
+    p.target_lengths = lengths->data_ptr<int32_t>();
+    return status_and(launch_on(args[0], p, device), {kept});
+}
+
+template <PyObject* (*CALL)(PyObject* const*), Py_ssize_t N>
+PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != N) Py_RETURN_NONE;
+    try {
+        return CALL(args);
+    } catch (...) {  // no memory, or a tensor without memory of its own: the Python path's error
+        Py_RETURN_NONE;
+    }
+}
+
+template <int64_t (*RULE)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t)>
+PyObject* rule7(PyObject*, PyObject* args) {
+    long long x[7];
+    if (!PyArg_ParseTuple(args, "LLLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5, x + 6)) return nullptr;
+    return PyLong_FromLongLong(RULE(x[0], x[1], x[2], x[3], x[4], x[5], x[6]));
+}
+
+PyObject* weight_splits_rule(PyObject*, PyObject* args) {
+    long long x[6];
+    if (!PyArg_ParseTuple(args, "LLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5)) return nullptr;
+    return PyLong_FromLongLong(weight_splits(x[0], x[1], x[2], x[3], x[4], x[5]));
+}
+
+PyObject* paged_workers_rule(PyObject*, PyObject* args) {
+    long long x[4];
+    if (!PyArg_ParseTuple(args, "LLLL", x, x + 1, x + 2, x + 3)) return nullptr;
+    return PyLong_FromLongLong(paged_workers(x[0], x[1], x[2], x[3]));
+}
+
+#define FAST(call, n) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<call, n>)), METH_FASTCALL, nullptr
+
 PyMethodDef kMethods[] = {
     {"decode_handle", decode_handle, METH_VARARGS, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, nullptr},
     {"cache_build", cache_build, METH_VARARGS, nullptr},
+    {"prompt", FAST(prompt_call, 9)},
+    {"weights", FAST(weights_call, 9)},
+    {"paged_cache", FAST(paged_cache_call, 5)},
+    {"paged_extend", FAST(paged_extend_call, 7)},
+    {"paged_attention", FAST(paged_attention_call, 8)},
+    {"paged_evict", FAST(paged_evict_call, 9)},
+    {"attention_splits", rule7<attention_splits>, METH_VARARGS, nullptr},
+    {"weight_splits", weight_splits_rule, METH_VARARGS, nullptr},
+    {"paged_workers", paged_workers_rule, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

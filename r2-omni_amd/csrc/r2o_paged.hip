@@ -71,7 +71,7 @@ struct AttentionArgs {
     float *lse, *partial_out, *partial_ml, *logits;
     int k_page, k_head, k_slot, v_page, v_head, v_slot, w_page, w_head, table_stride;
     int q_batch, q_head, nk_batch, nk_head, nv_batch, nv_head;
-    int pages, last_page, shift, batch, hkv, group, window, sinks, workers;
+    int pages, last_page, shift, batch, hkv, group, window, sinks, workers, weight_blocks;
     float c2;  // scale, in log2 units
 };
 
@@ -178,9 +178,11 @@ __device__ __forceinline__ int tiles_before(Args& a, int b) {
     return before * a.hkv;
 }
 
+// Nontemporal: each row is read once a call.  The ragged decode of 252 MB takes 76 us with plain loads, 68 so.
 __device__ __forceinline__ void load_lds16(const void* gsrc, unsigned char* lds) {
+    constexpr int kNT = 2;
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gsrc,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+                                     (__attribute__((address_space(3))) void*)lds, 16, 0, kNT);
 }
 
 constexpr int vmcnt_imm(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4) | (0xF << 8); }
@@ -485,8 +487,8 @@ __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count,
     return {m, l};
 }
 
-// Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: the
-// share of one worker again, whose slots' weights grow by their probabilities.
+// Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: an even
+// share of all tiles each, whose slots' weights grow by their probabilities.
 template <int RF>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
     Args& a = kernel_args();
@@ -534,10 +536,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
         return;
     }
     // weights
-    const int worker = blockIdx.x - heads;
-    if (worker >= share.workers || share.total == 0) return;
-    int u = share.begin(worker);
-    const int u_end = share.begin(worker + 1);
+    const int block = blockIdx.x - heads;
+    int u = (int)((int64_t)share.total * block / a.weight_blocks);
+    const int u_end = (int)((int64_t)share.total * (block + 1) / a.weight_blocks);
+    if (u >= u_end) return;
     int base;
     int b = request_of(a, u, base);
     Tiles t = tiles_of(a, load_uniform(a.lengths + b));
@@ -590,10 +592,17 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return w != w ? kNaN : k;
 }
 
+// Sum over the wave, by moves between lanes through the VALU.
 __device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, R2O_WAVE);
-    return x;
+    x += __float_as_int(r2o_lane_xor<1>(__int_as_float(x)));
+    x += __float_as_int(r2o_lane_xor<2>(__int_as_float(x)));
+    x += __float_as_int(r2o_lane_xor<4>(__int_as_float(x)));
+    x += __float_as_int(r2o_lane_xor<8>(__int_as_float(x)));
+    float a, b;
+    r2o_row_swap<16>(__int_as_float(x), a, b);
+    x = __float_as_int(a) + __float_as_int(b);
+    r2o_row_swap<32>(__int_as_float(x), a, b);
+    return __float_as_int(a) + __float_as_int(b);
 }
 
 // Sum over the workgroup's waves of a wave-uniform count; `slot` alternates, so that one barrier does.
@@ -620,6 +629,7 @@ template <int E>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_evict_params p) {
     __shared__ __align__(16) int counts[2][kSelectWaves];
     __shared__ int before[kSelectWaves][2];
+    __shared__ int ids[kSelectWaves][(4 * E + 64) / 64 * 64];
     const r2o_paged_cache& c = p.source;
     const int h = blockIdx.x % (int)c.hkv, b = blockIdx.x / (int)c.hkv, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -649,38 +659,36 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_
         const int page = page_at(j);
         return key_of(j, page, weight_at(j, page));
     };
-    // the wave's page ids, at most 4 E of them, lie in its lanes; then all weights are in flight together
-    constexpr int kPageRegs = (4 * E + 63) / 64;
+    // the wave's page ids, at most 4 E of them and one more where pages are larger than its first slot's alignment
     const int page0 = (first - lane) >> shift, last = (n - 1) >> shift;
-    int ids[kPageRegs];
 #pragma unroll
-    for (int i = 0; i < kPageRegs; ++i) ids[i] = r2o_ldg(table + min(page0 + 64 * i + lane, last));
-    auto page_in = [&](int j, int i) {  // of slot j, in row i
-        const int at = (j >> shift) - page0;
-        int id = __shfl(ids[0], at & 63, R2O_WAVE);
-#pragma unroll
-        for (int x = 1; x < kPageRegs; ++x) {
-            if (4 * i < 64 * x) break;  // 16 slots a page: row i is in register 4 i / 64, with larger pages in one before
-            const int y = __shfl(ids[x], at & 63, R2O_WAVE);
-            id = (at >> 6) == x ? y : id;
-        }
-        return id;
-    };
+    for (int i = 0; i < (4 * E + 64) / 64; ++i) ids[wave][64 * i + lane] = r2o_ldg(table + min(page0 + 64 * i + lane, last));
+    __builtin_amdgcn_wave_barrier();
+    // a wave behind the filled slots reads its first id
+    auto page_in = [&](int j) { return ids[wave][max((min(j, n - 1) >> shift) - page0, 0)]; };
     uint32_t keys[E];
     int from = first;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        asm volatile("" : "+v"(from));  // each place forms its slots anew: kept, they would spill
-        const int j = min(from + 64 * i, n - 1);
-        keys[i] = __float_as_uint(weight_at(j, page_in(j, i)));
-        __builtin_amdgcn_sched_barrier(0);  // row after row: what all of them need at once would spill
+    for (int i0 = 0; i0 < E; i0 += 8) {  // eight rows at a time: what all of them need at once would spill
+        int page[8];
+        asm volatile("" : "+v"(from));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) page[i] = page_in(from + 64 * (i0 + i));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) keys[i0 + i] = __float_as_uint(weight_at(from + 64 * (i0 + i), page[i]));
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
+    for (int i0 = 0; i0 < E; i0 += 8) {
+        int page[8];
         asm volatile("" : "+v"(from));
-        const int j = from + 64 * i;
-        keys[i] = key_of(j, page_in(min(j, n - 1), i), __uint_as_float(keys[i]));
-        asm volatile("" : "+v"(keys[i]));  // one key whole before the next
+#pragma unroll
+        for (int i = 0; i < 8; ++i) page[i] = page_in(from + 64 * (i0 + i));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            keys[i0 + i] = key_of(from + 64 * (i0 + i), page[i], __uint_as_float(keys[i0 + i]));
+            asm volatile("" : "+v"(keys[i0 + i]));  // one key whole before the next
+        }
     }
 
     int slot = 0, reach = n;  // keys >= t
@@ -856,9 +864,10 @@ int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream) {
     a.window = p->window ? (int)std::min<int64_t>(p->window, kNoWindow) : kNoWindow;
     a.sinks = p->window ? (int)p->sinks : 0;
     a.workers = (int)p->workers;
+    a.weight_blocks = 4 * a.workers;  // short work each, bound by the latency of its loads: twice and four times measure the same
     a.c2 = p->sm_scale * kLog2e;
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)p->workers), join((unsigned)(c.batch * p->hq + (c.weight_pages ? p->workers : 0)));
+    const dim3 grid((unsigned)p->workers), join((unsigned)(c.batch * p->hq + (c.weight_pages ? a.weight_blocks : 0)));
     auto launch = [&](auto partial, auto join_kernel) {
         hipLaunchKernelGGL(partial, grid, dim3(256), 0, st, a);
         if (hipGetLastError() != hipSuccess) return R2O_ELAUNCH;

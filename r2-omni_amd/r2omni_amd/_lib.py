@@ -259,6 +259,17 @@ def address(name: str) -> int:
     return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
 
 
+_ENTRIES: dict[str, int] = {}
+
+
+def entry(name: str) -> int:
+    """``address``, looked up once for each name."""
+    found = _ENTRIES.get(name)
+    if found is None:
+        found = _ENTRIES[name] = address(name)
+    return found
+
+
 def check(rc: int, name: str) -> None:
     if rc == 0:
         return

@@ -47,10 +47,14 @@ class PagedCache:
     page_table: torch.Tensor                    # int32 [B, max_pages]
     lengths: torch.Tensor                       # int32 [B]
     weight_pages: torch.Tensor | None = None    # fp32 [pages, Hkv, page_size]: accumulated attention weight
-    _c: _lib.PagedCacheParams = field(init=False, repr=False)
+    _c: bytes = field(init=False, repr=False)  # r2o_paged_cache
 
     def __post_init__(self) -> None:
         k, v, table, n, w = self.key_pages, self.value_pages, self.page_table, self.lengths, self.weight_pages
+        made = _lib.host().paged_cache(k, v, table, n, w)
+        if made is not None:
+            object.__setattr__(self, "_c", made)
+            return
         if k.ndim != 4 or k.shape[-1] != 128 or min(k.shape) < 1 or v.shape != k.shape:
             raise ValueError("paged cache needs key and value pages [pages,Hkv,page_size,128] of one shape")
         if k.shape[2] not in PAGE_SIZES:
@@ -71,17 +75,21 @@ class PagedCache:
                               or any(not 0 < st < 1 << 31 for st, size in zip(w.stride(), w.shape) if size > 1) or w.stride(2) != 1):
             raise ValueError("weight_pages must be fp32 [pages,Hkv,page_size] on the cache's device with unit-strided slots")
         _lib.require_device(k, "paged cache")
-        object.__setattr__(self, "_c", _lib.PagedCacheParams(
+        object.__setattr__(self, "_c", bytes(_lib.PagedCacheParams(
             key_pages=k.data_ptr(), value_pages=v.data_ptr(), weight_pages=_lib.ptr(w), page_table=table.data_ptr(),
             lengths=n.data_ptr(), key_strides=_strides(k, 3), value_strides=_strides(v, 3),
             weight_strides=(0, 0) if w is None else _strides(w, 2), table_stride=max(table.stride(0), table.shape[1]),
             pages=k.shape[0], max_pages=table.shape[1], page_size=k.shape[2], batch=table.shape[0], hkv=k.shape[1],
-            dtype=dtype))
+            dtype=dtype)))
 
     @property
     def capacity(self) -> int:
         """Slots that a row of the page table can hold."""
         return int(self.page_table.shape[1]) * int(self.key_pages.shape[2])
+
+
+def _params_of(cache: PagedCache) -> _lib.PagedCacheParams:
+    return _lib.PagedCacheParams.from_buffer_copy(cache._c)
 
 
 def _check_new_rows(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, what: str) -> None:
@@ -99,6 +107,9 @@ def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, c
     ``cache.lengths`` already counts them: row i of request b goes to slot ``lengths[b] - n + i``, where n is S or,
     for a padded batch, ``counts[b]`` (int32 [B]; rows behind it are not used).  Where the cache keeps weights, the
     slots get ``weights`` (fp32 [B, Hkv, S], as ``attention_weights`` returns them) or 0."""
+    made = _lib.host().paged_extend(_lib.entry("r2o_paged_extend"), cache._c, cache.key_pages, key, value, counts, weights)
+    if made is not None:
+        return _lib.check(made[0], "r2o_paged_extend")
     batch, hkv = int(cache.page_table.shape[0]), int(cache.key_pages.shape[1])
     if key.ndim != 4 or key.shape[0] != batch or key.shape[1] != hkv or key.shape[2] < 1 or key.shape[3] != 128:
         raise ValueError("paged extend requires key and value [B,Hkv,S,128] of the cache's requests and heads")
@@ -114,16 +125,10 @@ def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, c
         if weights.stride(2) != 1 and weights.shape[2] > 1 or min(weights.stride()) < 0:
             weights = weights.contiguous()
     key, value = _rows(key), _rows(value)
-    p = _lib.PagedExtend(cache=cache._c, key=key.data_ptr(), value=value.data_ptr(), weights=_lib.ptr(weights),
+    p = _lib.PagedExtend(cache=_params_of(cache), key=key.data_ptr(), value=value.data_ptr(), weights=_lib.ptr(weights),
                          counts=_lib.ptr(counts), key_strides=_strides(key, 3), value_strides=_strides(value, 3),
                          weights_strides=(0, 0) if weights is None else _strides(weights, 2), rows=key.shape[2])
     _lib.launch("r2o_paged_extend", p, key.device)
-
-
-def paged_workers(batch: int, hkv: int, capacity: int, num_cus: int) -> int:
-    """Workgroups that share the slots of a call: two a compute unit, fewer when the page tables hold fewer than
-    four tiles of 32 slots for each."""
-    return max(1, min(2 * num_cus, batch * hkv * -(-capacity // 128)))
 
 
 def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[torch.Tensor, torch.Tensor] | None = None,
@@ -138,6 +143,12 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
     grows by its probability summed over the query heads of its group (the appended slot's is set to it); a
     ``dataclasses.replace(cache, weight_pages=None)`` leaves them alone.  A request that sees no slot (an idle one of
     length 0) gets 0 and lse -inf.  ``output``: the two contiguous result tensors."""
+    if output is None:
+        made = _lib.host().paged_attention(_lib.entry("r2o_paged_attention"), cache._c, cache.key_pages, query, append, window,
+                                           sinks, sm_scale)
+        if made is not None:
+            _lib.check(made[0], "r2o_paged_attention")
+            return made[1], made[2]
     batch, hkv = int(cache.page_table.shape[0]), int(cache.key_pages.shape[1])
     if query.ndim == 4 and query.shape[2] == 1:
         query = query[:, :, 0]
@@ -166,7 +177,7 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
             raise ValueError("paged attention output must be contiguous [B,Hq,128] of the query's dtype and device")
         if tuple(lse.shape) != (batch, hq) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
             raise ValueError("paged attention lse output must be contiguous fp32 [B,Hq] on the query's device")
-    p = _lib.PagedAttention(cache=cache._c, query=query.data_ptr(), query_strides=_strides(query, 2), hq=hq, window=w,
+    p = _lib.PagedAttention(cache=_params_of(cache), query=query.data_ptr(), query_strides=_strides(query, 2), hq=hq, window=w,
                             sinks=s, sm_scale=scale, out=out.data_ptr(), lse=lse.data_ptr())
     if append is not None:
         rows = []
@@ -180,7 +191,7 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
         _check_new_rows(cache, key, value, "paged attention append")
         p.append_key, p.append_value = key.data_ptr(), value.data_ptr()
         p.append_strides = (*_strides(key, 2), *_strides(value, 2))
-    p.workers = paged_workers(batch, hkv, cache.capacity, _lib.num_cus(dev))
+    p.workers = _lib.host().paged_workers(batch, hkv, cache.capacity, _lib.num_cus(dev))
     p.partial_states = (p.workers + batch * hkv) * (hq // hkv)
     p.logits_floats = batch * hq * (-(-cache.capacity // 32) * 32) if cache.weight_pages is not None else 0
     # partial outputs, (maximum, sum) pairs, logits
@@ -202,6 +213,11 @@ def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int 
     ``weight_pages``.  The target may lie in the same pools, in pages that the source's table does not name; the
     source is left as it is, for its pages to be handed back.  Returns the kept source slots, int32 [B, Hkv, keep]
     in ascending order, -1 behind a request's length."""
+    made = _lib.host().paged_evict(_lib.entry("r2o_paged_evict"), cache._c, cache.key_pages, target._c, target.key_pages,
+                                   target.lengths, keep, sinks, recent)
+    if made is not None:
+        _lib.check(made[0], "r2o_paged_evict")
+        return made[1]
     keep, sinks, recent = int(keep), int(sinks), int(recent)
     if cache.weight_pages is None:
         raise ValueError("paged evict needs a cache with weight_pages")
@@ -217,7 +233,7 @@ def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int 
         raise ValueError("sinks and recent must be non-negative and together at most keep")
     dev = cache.key_pages.device
     kept = torch.empty((cache.page_table.shape[0], cache.key_pages.shape[1], keep), dtype=torch.int32, device=dev)
-    p = _lib.PagedEvict(source=cache._c, target=target._c, keep=keep, sinks=sinks, recent=recent, kept=kept.data_ptr(),
+    p = _lib.PagedEvict(source=_params_of(cache), target=_params_of(target), keep=keep, sinks=sinks, recent=recent, kept=kept.data_ptr(),
                         target_lengths=target.lengths.data_ptr())
     _lib.launch("r2o_paged_evict", p, dev)
     return kept

@@ -86,14 +86,6 @@ def _params(query, key, window, sinks, query_lengths, key_lengths, sm_scale) -> 
         sm_scale=_scale(sm_scale))
 
 
-def attention_splits(batch: int, hq: int, hkv: int, queries: int, keys: int, window, num_cus: int) -> int:
-    """Workgroups that share the keys of one 128-row tile: enough for two a compute unit, each with at least four
-    tiles of 64 keys."""
-    row_tiles = -(-(hq // hkv) * queries // 128) * batch * hkv
-    seen = keys if window is None else min(keys, int(window) + queries + 128)
-    return max(1, min(-(-2 * num_cus // row_tiles), -(-seen // 256)))
-
-
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, window: int | None = None,
                      sinks: int = 0, query_lengths: torch.Tensor | None = None, key_lengths: torch.Tensor | None = None,
                      sm_scale: float | None = None, output: tuple[torch.Tensor, torch.Tensor] | None = None):
@@ -106,6 +98,12 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     behind its request's length, is 0 with lse -inf; values of rows behind a length are never used.  Strided views
     are read in place where the channels are unit-strided and rows 16-byte aligned (copied otherwise).  ``output``:
     the two result tensors to write, the first with such strides, neither overlapping an input."""
+    if output is None:
+        made = _lib.host().prompt(_lib.entry("r2o_prompt_attention"), query, key, value, window, sinks, query_lengths,
+                                  key_lengths, sm_scale)
+        if made is not None:
+            _lib.check(made[0], "r2o_prompt_attention")
+            return made[1], made[2]
     _check_rows(query, key, "prompt attention")
     if value.shape != key.shape or value.device != key.device or value.dtype != key.dtype:
         raise ValueError("prompt attention value must match K's shape, device and dtype")
@@ -131,7 +129,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != query.device \
                 or not lse.is_contiguous():
             raise ValueError("prompt attention lse output must be contiguous fp32 [B,Hq,Sq] on Q's device")
-    p.splits = attention_splits(batch, hq, key.shape[1], rows, key.shape[2], window, _lib.num_cus(query.device))
+    p.splits = _lib.host().attention_splits(batch, hq, key.shape[1], rows, key.shape[2], p.window, _lib.num_cus(query.device))
     scratch = None
     if p.splits > 1:
         scratch = torch.empty(130 * p.splits * batch * hq * rows, dtype=torch.float32, device=query.device)
@@ -140,14 +138,6 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     p.out, p.o_strides, p.lse = out.data_ptr(), _strides(out, 3), lse.data_ptr()
     _lib.launch("r2o_prompt_attention", p, query.device)
     return out, lse
-
-
-def weight_splits(batch: int, hq: int, hkv: int, queries: int, keys: int, num_cus: int) -> int:
-    """Workgroups that share the query rows of one key tile: enough for four a compute unit, at most one for each
-    (query head, 64-row tile) pair."""
-    tiles = -(-keys // 128) * batch * hkv
-    pairs = hq // hkv * -(-queries // 64)
-    return max(1, min(pairs, -(-4 * num_cus // tiles)))
 
 
 def attention_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, *, window: int | None = None,
@@ -160,6 +150,12 @@ def attention_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor,
     [B, Hq, Sq] fp32 their statistics from ``prompt_attention`` with the same masks; rows with lse -inf give
     nothing.  Positions, lengths, masks and strides as there.  Keys behind a length get 0.  The sums are formed in
     a fixed order: equal calls give equal bits."""
+    if output is None:
+        made = _lib.host().weights(_lib.entry("r2o_attention_weights"), query, key, lse, window, sinks, query_lengths,
+                                   key_lengths, sm_scale)
+        if made is not None:
+            _lib.check(made[0], "r2o_attention_weights")
+            return made[1]
     _check_rows(query, key, "attention weights")
     batch, hq, rows, _ = query.shape
     if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != query.device:
@@ -176,7 +172,7 @@ def attention_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor,
         raise ValueError("attention weights output must be contiguous fp32 [B,Hkv,Sk] on Q's device")
     p = _params(query, key, window, sinks, query_lengths, key_lengths, sm_scale)
     p.lse_in, p.weights = lse.data_ptr(), output.data_ptr()
-    p.splits = weight_splits(batch, hq, hkv, rows, keys, _lib.num_cus(query.device))
+    p.splits = _lib.host().weight_splits(batch, hq, hkv, rows, keys, _lib.num_cus(query.device))
     scratch = None
     if p.splits > 1:
         scratch = torch.empty(p.splits * output.numel(), dtype=torch.float32, device=query.device)
