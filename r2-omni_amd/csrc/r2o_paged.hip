@@ -197,8 +197,9 @@ __device__ __forceinline__ void tile_pages(Args& a, const int32_t* table, int j0
 }
 
 // One tile of a (request, head): its page ids and the place of its slots in LDS.  A wave's stage holds 32 K rows, then
-// 32 V rows, each row 16 chunks of 16 bytes: K row r's chunk c at place c ^ (r & 7), for reads of one chunk by 16 rows;
-// V row r's at c ^ 2 (r & 3), for transposing reads of two chunks by four rows.
+// 32 V rows, each row 16 chunks of 16 bytes: K row r's chunk c at place c ^ (r & 15), for reads of one chunk by 16 rows;
+// V row r's at c ^ 2 (r & 7), for transposing reads of two chunks by eight rows: LDS answers 256 bytes a clock where they
+// fall into different banks.
 constexpr int kStage = 2 * kSlots * 256;
 
 struct Head {
@@ -206,7 +207,7 @@ struct Head {
     int k_page, v_page;      // strides, elements
     int k_slot, v_slot;
     int shift;
-    int k_lane[2], v_lane;   // byte offsets of this lane's row and chunk among four rows (K: among four even, four odd)
+    int k_lane[4], v_lane[2];  // byte offsets of this lane's row and chunk among four rows, by where these lie among 16 (8)
 };
 
 // Asynchronous loads of one tile into a stage: 16 of 1 KB, four rows each.
@@ -218,8 +219,8 @@ __device__ __forceinline__ void load_tile(const Head& x, int j0, const int (&pag
         const unsigned char* v = reinterpret_cast<const unsigned char*>(x.v + (int64_t)id * x.v_page + (int64_t)at * x.v_slot);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            load_lds16(k + (int64_t)(8 * i) * x.k_slot + x.k_lane[i & 1], stage + 4096 * m + 1024 * i);
-            load_lds16(v + (int64_t)(8 * i) * x.v_slot + x.v_lane, stage + 8192 + 4096 * m + 1024 * i);
+            load_lds16(k + (int64_t)(8 * i) * x.k_slot + x.k_lane[i], stage + 4096 * m + 1024 * i);
+            load_lds16(v + (int64_t)(8 * i) * x.v_slot + x.v_lane[i & 1], stage + 8192 + 4096 * m + 1024 * i);
         }
     }
 }
@@ -232,20 +233,19 @@ __device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
 // assembly, with its wait: before a load from LDS that the compiler makes it waits for every asynchronous load into
 // LDS, the next tile's among them.
 __device__ __forceinline__ void read_keys(uint32_t row, uint32_t chunk, r2o_u4 (&k)[2][4]) {
-    const uint32_t a = row + chunk, b = row + (chunk ^ 64);
+    const uint32_t a = row + chunk, b = row + (chunk ^ 64), c = row + (chunk ^ 128), e = row + (chunk ^ 192);
     asm volatile(
-        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %8 offset:128\n\tds_read_b128 %3, %9 offset:128\n\t"
-        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %8 offset:4224\n\t"
-        "ds_read_b128 %7, %9 offset:4224\n\ts_waitcnt lgkmcnt(0)"
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %10 offset:4096\n\t"
+        "ds_read_b128 %7, %11 offset:4096\n\ts_waitcnt lgkmcnt(0)"
         : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]), "=&v"(k[1][1]), "=&v"(k[1][2]), "=&v"(k[1][3])
-        : "v"(a), "v"(b)
+        : "v"(a), "v"(b), "v"(c), "v"(e)
         : "memory");
 }
 
 // V rows 4 g + 0..3 and 16 more, transposed, as the A operands of channels 64 d + 16 x ..
 __device__ __forceinline__ void read_values(uint32_t row, uint32_t chunk, int d, r2o_u4 (&v)[4]) {
-    const uint32_t a = row + chunk + 128 * d, b = row + (chunk ^ 32) + 128 * d, c = row + (chunk ^ 64) + 128 * d,
-                   e = row + (chunk ^ 96) + 128 * d;
+    const uint32_t at = chunk ^ (128 * d), a = row + at, b = row + (at ^ 32), c = row + (at ^ 64), e = row + (at ^ 96);
     r2o_u2 lo[4], hi[4];
     asm volatile(
         "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %3, %11\n\t"
@@ -303,9 +303,10 @@ __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
         head.k_slot = a.k_slot;
         head.v_slot = a.v_slot;
         head.shift = a.shift;
-        head.k_lane[0] = 2 * g * a.k_slot + 16 * (l16 ^ g);
-        head.k_lane[1] = 2 * g * a.k_slot + 16 * (l16 ^ (g + 4));
-        head.v_lane = 2 * g * a.v_slot + 16 * (l16 ^ (2 * g));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) head.k_lane[i] = 2 * g * a.k_slot + 16 * (l16 ^ (4 * i + g));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) head.v_lane[i] = 2 * g * a.v_slot + 16 * (l16 ^ (8 * i + 2 * g));
         const int32_t* table = a.table + (int64_t)b * a.table_stride;
         float* logits = WEIGHTS ? a.logits + (int64_t)pair_base * group * kSlots : nullptr;
 
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
                 uint16_t* vd = e.value + (int64_t)h * e.v_head + (int64_t)page_new * e.v_page + at * e.v_slot;
                 if (lane < 32) {
                     const r2o_u4 x = r2o_ldg(reinterpret_cast<const r2o_u4*>(lane < 16 ? ks : vs) + l16);
-                    *reinterpret_cast<r2o_u4*>(stage + (lane < 16 ? 0 : 8192) + 256 * r + 16 * (l16 ^ (lane < 16 ? r & 7 : 2 * (r & 3)))) = x;
+                    *reinterpret_cast<r2o_u4*>(stage + (lane < 16 ? 0 : 8192) + 256 * r + 16 * (l16 ^ (lane < 16 ? r & 15 : 2 * (r & 7)))) = x;
                     if (page_new >= 0) r2o_store8<true>((lane < 16 ? kd : vd) + 8 * l16, x);
                 }
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
             r2o_f4 s[2] = {r2o_f4{}, r2o_f4{}};
             {
                 r2o_u4 k[2][4];
-                read_keys(lds_address(stage) + 256 * l16, (16 * g) ^ (16 * (l16 & 7)), k);
+                read_keys(lds_address(stage) + 256 * l16, 16 * (g ^ l16), k);
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
             for (int d = 0; d < 2; ++d) {
                 r2o_u4 v[4];
                 const int r = l16 >> 2;
-                read_values(lds_address(vl) + 1024 * g + 256 * r + 8 * (l16 & 1), (16 * ((l16 & 3) >> 1)) ^ (32 * r), d, v);
+                read_values(lds_address(vl) + 1024 * g + 256 * r + 8 * (l16 & 1), (16 * ((l16 & 3) >> 1)) ^ (32 * ((4 * g + r) & 7)), d, v);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) acc[4 * d + x] = mfma16<RF>(v[x], pk, acc[4 * d + x]);
             }

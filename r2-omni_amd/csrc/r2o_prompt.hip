@@ -48,15 +48,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // One wave's 16 rows of a 64-row tile, from `row0` on clamped to `last`, into registers, and from there into LDS: a row is
 // 16 chunks of 16 bytes, chunk c of row r at place c ^ swizzle(r); lane l writes at 16 l, so the swizzle is made by which
-// chunk it reads.  SWZ 0: r & 7, for reads of one chunk by 32 rows; 1: 2 (r & 3), for transposing reads of two chunks
-// by 4 rows.
+// chunk it reads.  LDS answers 256 bytes a clock, so 16 lanes' 16-byte reads, or 32 lanes' 8-byte ones, have to fall into
+// 256 different ones.  SWZ 0: r & 15, for reads of one chunk by 32 rows (4.1 clocks a wave; r & 7 takes 8.1); 1: 4 (r & 3),
+// for transposing reads of four chunks by 4 rows (3.0 clocks; 2 (r & 3) takes 4.1).
 template <int SWZ>
 __device__ __forceinline__ void load_rows(const uint16_t* base, int stride, int row0, int last, r2o_u4 (&x)[4], int wave, int lane) {
     const int r4 = lane >> 4, place = lane & 15;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r0 = min(row0 + 16 * wave + 4 * i, last);
-        const int c = place ^ (SWZ == 0 ? (4 * i + r4) & 7 : 2 * r4);
+        const int c = place ^ (SWZ == 0 ? 4 * i + r4 : 4 * r4);
         const uint32_t at = (uint32_t)(2 * min(r4, last - r0) * stride + 16 * c);
         x[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(reinterpret_cast<const unsigned char*>(base + (int64_t)r0 * stride) + at));
     }
@@ -70,7 +71,7 @@ __device__ __forceinline__ void store_rows(unsigned char* lds, const r2o_u4 (&x)
 // 32 rows of a staged tile (SWZ 0) as the A operand of step t (channels 16 t ..).
 __device__ __forceinline__ r2o_u4 read_rows(const unsigned char* tile, int block, int t, int lane) {
     const int r = lane & 31, c = 2 * t + (lane >> 5);
-    return *reinterpret_cast<const r2o_u4*>(tile + (32 * block + r) * 256 + 16 * (c ^ (r & 7)));
+    return *reinterpret_cast<const r2o_u4*>(tile + (32 * block + r) * 256 + 16 * (c ^ (r & 15)));
 }
 
 // 16 keys from 16 kb on, transposed, as the A operand of channels 32 db ..: lane half h holds keys 4 h + 0..3 and
@@ -78,7 +79,7 @@ __device__ __forceinline__ r2o_u4 read_rows(const unsigned char* tile, int block
 __device__ __forceinline__ r2o_u4 read_values(const unsigned char* tile, int kb, int db, int lane) {
     const int i = lane & 15, r = i >> 2;
     const int c = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-    const unsigned char* p = tile + (16 * kb + 4 * (lane >> 5) + r) * 256 + 16 * (c ^ (2 * r)) + 8 * (i & 1);
+    const unsigned char* p = tile + (16 * kb + 4 * (lane >> 5) + r) * 256 + 16 * (c ^ (4 * r)) + 8 * (i & 1);
     typedef __attribute__((address_space(3))) s4v lds4;
     const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
     const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * 256));
