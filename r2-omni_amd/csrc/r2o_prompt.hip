@@ -164,8 +164,8 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
 // (maximum, sum, products) in scratch for prompt_join_kernel.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
-    __shared__ __align__(16) unsigned char k_lds[2][kTileBytes], v_lds[2][kTileBytes];
-    __shared__ int any_bad;
+    // K tiles t and t + 1, V tiles t to t + 2: two workgroups fill a compute unit's 160 KB
+    __shared__ __align__(16) unsigned char k_lds[2][kTileBytes], v_lds[3][kTileBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     Args& a = kernel_args();
     const int kvh = (int)blockIdx.z % a.hkv, b = (int)blockIdx.z / a.hkv, group = a.group, rows = a.queries * group;
@@ -183,7 +183,6 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
 #pragma unroll
         for (int t = 0; t < 8; ++t) q[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
     }
-    if (threadIdx.x == 0) any_bad = 0;
 
     // positions of the workgroup's rows and of this wave's
     const int wg_first = row0 / group, wg_last = min(row0 + kRows - 1, rows - 1) / group;
@@ -215,34 +214,32 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
         load_rows<0>(kbase, k_row, kt, last, kx, wave, lane);
         load_rows<1>(vbase, v_row, kt, last, vx, wave, lane);
     };
-    auto store = [&](int it) {
-        if (seen_in_part(tile_key(it)) && zero_not_finite<RF>(vx)) any_bad = 1;
+    bool bad = false;
+    auto store = [&](int it, int v_at) {
+        if (seen_in_part(tile_key(it))) bad |= zero_not_finite<RF>(vx);
         store_rows(k_lds[it & 1], kx, wave, lane);
-        store_rows(v_lds[it & 1], vx, wave, lane);
+        store_rows(v_lds[v_at], vx, wave, lane);
     };
-    auto compute = [&](int kt, const unsigned char* kl, const unsigned char* vl) __attribute__((always_inline)) {
-        if (kt > pmax || (kt + kTile - 1 <= pmin - window && kt >= sinks)) return;  // nothing for this wave
-        f16v sc[2] = {f16v{}, f16v{}};
+    // S^T of 32 keys x 32 rows
+    auto products = [&](const unsigned char* kl, int sub) __attribute__((always_inline)) {
+        f16v x = f16v{};
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
+        for (int t = 0; t < 8; ++t) x = mfma32<RF>(read_rows(kl, sub, t, lane), q[t], x);
+        return x;
+    };
+    // masks, and the running maximum raised where it has to be
+    auto top_of = [&](f16v& x, int from_key) __attribute__((always_inline)) {
+        if (!(from_key + 31 <= pmin && (from_key > pmax - window || from_key + 32 <= sinks))) {
+            const int from = from_key + 4 * half, back = pv - from, sink = min(sinks, pv + 1) - 1 - from;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) sc[kb] = mfma32<RF>(read_rows(kl, kb, t, lane), q[t], sc[kb]);
-        if (!(kt + kTile - 1 <= pmin && (kt > pmax - window || kt + kTile <= sinks))) {
-            const int from = kt + 4 * half, back = pv - from, sink = min(sinks, pv + 1) - 1 - from;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    sc[kb][i] = sees_from(back, sink, 32 * kb + 8 * (i >> 2) + (i & 3), window) ? sc[kb][i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) x[i] = sees_from(back, sink, 8 * (i >> 2) + (i & 3), window) ? x[i] : -INFINITY;
         }
-        float tmax = fmaxf(sc[0][0], sc[1][0]);
+        float tmax = fmaxf(x[0], x[1]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, fmaxf(sc[0][i], sc[1][i]));
-        {
-            float x, y;
-            r2o_row_swap<32>(tmax, x, y);
-            tmax = fmaxf(x, y) * c2;  // -inf stays (c2 > 0)
-        }
+        for (int i = 2; i < 16; i += 2) tmax = fmaxf(tmax, fmaxf(x[i], x[i + 1]));
+        float y, z;
+        r2o_row_swap<32>(tmax, y, z);
+        tmax = fmaxf(y, z) * c2;  // -inf stays (c2 > 0)
         if (__any(tmax > m + kSlack)) {
             // of the rows that exceed it alone: a row's result does not depend on its neighbours
             const float m_new = tmax > m + kSlack ? tmax : m;
@@ -252,34 +249,53 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
             for (int db = 0; db < 4; ++db) acc[db] *= alpha;
             m = m_new;
         }
+    };
+    auto probabilities = [&](const f16v& x, r2o_u4 (&pk)[2]) __attribute__((always_inline)) {
         const float mm = m == -INFINITY ? 0.f : m;
-        r2o_u4 pk[4];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c2, -mm));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], c2, -mm));
+            l += e0 + e1;
+            pk[i >> 3][(i & 7) >> 1] = pack2<RF>(e0, e1);
+        }
+    };
+    auto values = [&](const unsigned char* vl, int sub, const r2o_u4 (&pk)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i], c2, -mm));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i + 1], c2, -mm));
-                l += e0 + e1;
-                pk[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<RF>(e0, e1);
-            }
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-            for (int db = 0; db < 4; ++db) acc[db] = mfma32<RF>(read_values(vl, kb, db, lane), pk[kb], acc[db]);
+            for (int db = 0; db < 4; ++db) acc[db] = mfma32<RF>(read_values(vl, 2 * sub + kb, db, lane), pk[kb], acc[db]);
     };
-    __syncthreads();
+    // A tile is two halves of 32 keys; the products of the half that follows run beside the exponentials of the one
+    // before it.
     if (begin < tiles) {
         load(begin);
-        store(begin);
-    }
-    for (int it = begin; it < tiles; ++it) {
-        __syncthreads();  // the tile is there, and every wave is done with the one before
-        if (it + 1 < tiles) load(it + 1);
-        compute(tile_key(it), k_lds[it & 1], v_lds[it & 1]);
-        if (it + 1 < tiles) store(it + 1);
+        store(begin, 0);
+        __syncthreads();
+        f16v even = products(k_lds[begin & 1], 0);
+        for (int it = begin, v_at = 0; it < tiles; ++it) {
+            const int kt = tile_key(it), v_next = v_at == 2 ? 0 : v_at + 1;
+            if (it + 1 < tiles) load(it + 1);
+            r2o_u4 pk[2];
+            top_of(even, kt);
+            f16v odd = products(k_lds[it & 1], 1);
+            probabilities(even, pk);
+            values(v_lds[v_at], 0, pk);
+            top_of(odd, kt + 32);
+            if (it + 1 < tiles) store(it + 1, v_next);
+            __syncthreads();  // the next tile is there; this one's V stays till every wave is past the next barrier
+            even = products(k_lds[(it + 1) & 1], 0);  // behind the last tile: what lies there, not used
+            probabilities(odd, pk);
+            values(v_lds[v_at], 1, pk);
+            v_at = v_next;
+        }
     }
     __syncthreads();
+    int* const flags = reinterpret_cast<int*>(k_lds[0]);
+    const bool wave_bad = __any(bad);
+    if (lane == 0) flags[wave] = wave_bad;
+    __syncthreads();
+    const bool any_bad = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
     if (any_bad) {  // what was taken out, for the rows that see it
         for (int it = begin; it < tiles; ++it) {
             const int kt = tile_key(it);
