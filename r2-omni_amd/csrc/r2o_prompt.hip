@@ -131,7 +131,7 @@ struct PromptArgs {
     const float* lse_in;
     float *weights, *partial_out, *partial_ml;
     int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head, o_batch, o_head;
-    int q_row, k_row, v_row, o_row, hq, hkv, group, queries, keys, window, sinks;
+    int q_row, k_row, v_row, o_row, hq, hkv, pairs, group, queries, keys, window, sinks;
     float c2;  // scale, in log2 units
 };
 
@@ -157,19 +157,42 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
     return s;
 }
 
+// Blocks go to the 8 dies (XCDs) in turn, and a die's L2 is its own: where the pairs allow it, a die works through the
+// row tiles of one pair after the other (or shares a pair with some), so that its workgroups read the same keys.  The
+// longest rows first.  False for a block that only fills the grid up.
+__device__ __forceinline__ bool place(int block, int tiles, int pairs, int& pair, int& tile) {
+    const int die = block & 7, i = block >> 3;
+    int rank;
+    if ((pairs & 7) == 0) {
+        pair = die + 8 * (i / tiles);
+        rank = i % tiles;
+    } else if (pairs == 1 || pairs == 2 || pairs == 4) {
+        const int dies = 8 / pairs;
+        pair = die / dies;
+        rank = i * dies + die % dies;
+    } else {
+        pair = block / tiles;
+        rank = block % tiles;
+    }
+    tile = tiles - 1 - rank;
+    return rank < tiles && pair < pairs;
+}
+
 // ------------------------------------------------------------------------------ prompt attention
 // The rows of a KV head's query heads are one list, packed row r = (row r / group, head r % group): a workgroup's 128
 // stand at 128 / group neighbouring positions, so its last tiles are masked in part for few of them, and a chunk of few
-// rows fills it.  grid: (row tiles, splits, batch * hkv); with splits each takes a share of the key tiles and leaves
-// (maximum, sum, products) in scratch for prompt_join_kernel.
+// rows fills it.  grid: (row tiles x pairs of request and KV head, splits); with splits each takes a share of the key tiles and
+// leaves (maximum, sum, products) in scratch for prompt_join_kernel.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     // K tiles t and t + 1, V tiles t to t + 2: two workgroups fill a compute unit's 160 KB
     __shared__ __align__(16) unsigned char k_lds[2][kTileBytes], v_lds[3][kTileBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     Args& a = kernel_args();
-    const int kvh = (int)blockIdx.z % a.hkv, b = (int)blockIdx.z / a.hkv, group = a.group, rows = a.queries * group;
-    const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kRows;  // the longest rows first
+    const int group = a.group, rows = a.queries * group;
+    int pair, row_tile;
+    if (!place(blockIdx.x, (rows + kRows - 1) / kRows, a.pairs, pair, row_tile)) return;
+    const int kvh = pair % a.hkv, b = pair / a.hkv, row0 = row_tile * kRows;
     const Lengths s = request_lengths(a, b);
     const int window = a.window, sinks = a.sinks;
     const uint16_t* kbase = a.key + b * a.k_batch + kvh * a.k_head;
@@ -322,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     if (packed >= rows) return;
     Args& e = kernel_args();
     if (gridDim.y > 1) {
-        const int64_t at = ((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * rows + packed;
+        const int64_t at = ((int64_t)blockIdx.y * e.pairs + pair) * rows + packed;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -518,6 +541,7 @@ PromptArgs kernel_arguments(const r2o_prompt_params* p) {
     a.o_row = (int)p->o_strides[2];
     a.hq = (int)p->hq;
     a.hkv = (int)p->hkv;
+    a.pairs = (int)(p->batch * p->hkv);
     a.group = (int)(p->hq / p->hkv);
     a.queries = (int)p->queries;
     a.keys = (int)p->keys;
@@ -538,7 +562,10 @@ int r2o_prompt_attention(const r2o_prompt_params* p, void* stream) {
     const int64_t rows = p->queries * (p->hq / p->hkv), pairs = p->batch * p->hkv;
     if (rows > (1 << 30) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
     if (p->splits > 1 && (!aligned({p->scratch}, 16) || p->scratch_floats < p->splits * pairs * rows * 130)) return R2O_EINVAL;
-    const dim3 grid((unsigned)((rows + kRows - 1) / kRows), (unsigned)p->splits, (unsigned)pairs);
+    const int64_t tiles = (rows + kRows - 1) / kRows, dies = pairs == 1 || pairs == 2 || pairs == 4 ? 8 / pairs : 1;
+    const int64_t blocks = (tiles + dies - 1) / dies * dies * pairs;  // tiles in whole turns of the dies that share a pair
+    if (blocks > 0x7fffffff) return R2O_EINVAL;
+    const dim3 grid((unsigned)blocks, (unsigned)p->splits);
     const dim3 join((unsigned)((rows + 7) / 8), (unsigned)pairs);
     const hipStream_t st = (hipStream_t)stream;
     PromptArgs a = kernel_arguments(p);
