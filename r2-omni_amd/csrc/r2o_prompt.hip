@@ -131,7 +131,7 @@ struct PromptArgs {
     const float* lse_in;
     float *weights, *partial_out, *partial_ml;
     int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head, o_batch, o_head;
-    int q_row, k_row, v_row, o_row, hq, hkv, pairs, group, queries, keys, window, sinks;
+    int q_row, k_row, v_row, o_row, hq, hkv, pairs, splits, group, queries, keys, window, sinks;
     float c2;  // scale, in log2 units
 };
 
@@ -158,24 +158,25 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
 }
 
 // Blocks go to the 8 dies (XCDs) in turn, and a die's L2 is its own: where the pairs allow it, a die works through the
-// row tiles of one pair after the other (or shares a pair with some), so that its workgroups read the same keys.  The
-// longest rows first.  False for a block that only fills the grid up.
-__device__ __forceinline__ bool place(int block, int tiles, int pairs, int& pair, int& tile) {
-    const int die = block & 7, i = block >> 3;
+// tiles of one pair after the other (or shares a pair with some), so that its workgroups read the same rows.  Tile by
+// tile, a tile's splits together: the caller's first tiles are the longest.  False for a block that only fills the grid up.
+__device__ __forceinline__ bool place(int block, int tiles, int splits, int pairs, int& pair, int& tile, int& split) {
+    const int die = block & 7, i = block >> 3, items = tiles * splits;
     int rank;
     if ((pairs & 7) == 0) {
-        pair = die + 8 * (i / tiles);
-        rank = i % tiles;
+        pair = die + 8 * (i / items);
+        rank = i % items;
     } else if (pairs == 1 || pairs == 2 || pairs == 4) {
         const int dies = 8 / pairs;
         pair = die / dies;
         rank = i * dies + die % dies;
     } else {
-        pair = block / tiles;
-        rank = block % tiles;
+        pair = block / items;
+        rank = block % items;
     }
-    tile = tiles - 1 - rank;
-    return rank < tiles && pair < pairs;
+    tile = rank / splits;
+    split = rank - tile * splits;
+    return rank < items && pair < pairs;
 }
 
 // ------------------------------------------------------------------------------ prompt attention
@@ -190,9 +191,10 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     Args& a = kernel_args();
     const int group = a.group, rows = a.queries * group;
-    int pair, row_tile;
-    if (!place(blockIdx.x, (rows + kRows - 1) / kRows, a.pairs, pair, row_tile)) return;
-    const int kvh = pair % a.hkv, b = pair / a.hkv, row0 = row_tile * kRows;
+    const int row_tiles = (rows + kRows - 1) / kRows, splits = a.splits;
+    int pair, row_tile, split;
+    if (!place(blockIdx.x, row_tiles, splits, a.pairs, pair, row_tile, split)) return;
+    const int kvh = pair % a.hkv, b = pair / a.hkv, row0 = (row_tiles - 1 - row_tile) * kRows;  // the last rows see most
     const Lengths s = request_lengths(a, b);
     const int window = a.window, sinks = a.sinks;
     const uint16_t* kbase = a.key + b * a.k_batch + kvh * a.k_head;
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     const int end = wg_first < s.q && top >= 0 ? top / kTile + 1 : 0;
     const int sink_tiles = end ? min((sinks + kTile - 1) / kTile, min(first, end)) : 0;
     const int all = sink_tiles + max(0, end - first);
-    const int begin = (int)((int64_t)all * blockIdx.y / gridDim.y), tiles = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
+    const int begin = (int)((int64_t)all * split / splits), tiles = (int)((int64_t)all * (split + 1) / splits);
     const int last = max(s.n - 1, 0);
 
     const float c2 = a.c2;
@@ -344,8 +346,8 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     }
     if (packed >= rows) return;
     Args& e = kernel_args();
-    if (gridDim.y > 1) {
-        const int64_t at = ((int64_t)blockIdx.y * e.pairs + pair) * rows + packed;
+    if (splits > 1) {
+        const int64_t at = ((int64_t)split * e.pairs + pair) * rows + packed;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -405,20 +407,25 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits
 }
 
 // ----------------------------------------------------------------------------- attention weights
-constexpr int kWeightKeys = 128;  // keys of a workgroup: 4 waves of 32, whose rows stay in registers
+constexpr int kWeightKeys = 256;  // keys of a workgroup: 4 waves of 64, whose rows stay in registers
 
-// grid: (key tiles, splits, batch * hkv).  A split takes a share of the (query head, 64-row tile) pairs that see
-// the key tile; its sums go to `weights` ([splits, batch, hkv, keys]; the result itself where there is one split).
+// A split takes a share of the (query head, 64-row tile) pairs that see the key tile;
+// its sums go to `weights` ([splits, batch, hkv, keys]; the result itself where there is one split).  S = Q K^T: a lane
+// sums its own two keys.  A row tile is two halves of 32; the products of the half that follows run beside the
+// exponentials of the one before it.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     __shared__ __align__(16) unsigned char q_lds[2][kTileBytes];
-    __shared__ __align__(16) float lse_lds[2][kTile];
+    __shared__ __align__(16) float lse_lds[3][kTile];
     Args& a = kernel_args();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-    const int kvh = (int)blockIdx.z % a.hkv, b = (int)blockIdx.z / a.hkv, group = a.group;
+    const int group = a.group, key_tiles = (a.keys + kWeightKeys - 1) / kWeightKeys;
+    int pair, key_tile, split;
+    if (!place(blockIdx.x, key_tiles, a.splits, a.pairs, pair, key_tile, split)) return;
+    const int kvh = pair % a.hkv, b = pair / a.hkv, key0 = key_tile * kWeightKeys;  // the first keys have most rows
     const Lengths s = request_lengths(a, b);
     const int window = a.window, sinks = a.sinks;
-    const int key0 = blockIdx.x * kWeightKeys, kw = key0 + 32 * wave, j = kw + col;
+    const int kw = key0 + 64 * wave, j = kw + col;  // this lane's keys: j and j + 32
 
     // rows that see any of the tile's keys: p >= key0, and without a sink among them p < last key + window
     const int last_key = min(key0 + kWeightKeys, s.n) - 1;
@@ -426,67 +433,99 @@ __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     const int row_hi = key0 < sinks ? s.q : min((int64_t)s.q, (int64_t)last_key + window - s.off);
     const int first = row_lo / kTile, per_head = key0 < s.n ? max(0, (row_hi + kTile - 1) / kTile - first) : 0;
     const int64_t pairs = (int64_t)per_head * group;
-    const int begin = (int)(pairs * blockIdx.y / gridDim.y), end = (int)(pairs * (blockIdx.y + 1) / gridDim.y);
+    const int begin = (int)(pairs * split / a.splits), end = (int)(pairs * (split + 1) / a.splits);
 
-    float sum = 0.f, lost = 0.f;  // of up to hq / hkv * queries terms: what each addition loses is kept
+    float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};  // of up to hq / hkv * queries terms: what each addition loses is kept
     if (begin < end) {
         const float c2 = a.c2;
-        r2o_u4 k[8];
-        const uint16_t* src = a.key + b * a.k_batch + kvh * a.k_head + (int64_t)min(j, s.n - 1) * a.k_row + 8 * half;
+        r2o_u4 k[2][8];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) k[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
+        for (int n = 0; n < 2; ++n) {
+            const uint16_t* src = a.key + b * a.k_batch + kvh * a.k_head + (int64_t)min(j + 32 * n, s.n - 1) * a.k_row + 8 * half;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) k[n][t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
+        }
         r2o_u4 qx[4];
         float lse_next = 0.f;
-        auto tile_row = [&](int it) { return (first + it % per_head) * kTile; };
-        auto load = [&](int it) {
-            const int h = kvh * group + it / per_head, r0 = tile_row(it);
-            lse_next = r2o_ldg(a.lse_in + ((int64_t)b * a.hq + h) * a.queries + min(r0 + ((int)threadIdx.x & (kTile - 1)), s.q - 1));
-            load_rows<0>(a.query + b * a.q_batch + h * a.q_head, a.q_row, r0, s.q - 1, qx, wave, lane);
+        // the head and row tile of the tile that is loaded next, of the one that is stored and of the one computed on
+        int head = begin / per_head, row_tile = begin - head * per_head;
+        auto load = [&](int h, int r) {
+            lse_next = r2o_ldg(a.lse_in + ((int64_t)b * a.hq + kvh * group + h) * a.queries + min((first + r) * kTile + ((int)threadIdx.x & (kTile - 1)), s.q - 1));
+            load_rows<0>(a.query + b * a.q_batch + (kvh * group + h) * a.q_head, a.q_row, (first + r) * kTile, s.q - 1, qx, wave, lane);
         };
-        auto store = [&](int it, int buf) {  // rows behind the request, and those that saw no key, give exp2(-inf)
-            store_rows(q_lds[buf], qx, wave, lane);
-            const bool none = tile_row(it) + (int)threadIdx.x >= s.q || lse_next == -INFINITY;
-            if (threadIdx.x < kTile) lse_lds[buf][threadIdx.x] = none ? INFINITY : lse_next * kLog2e;
+        auto store = [&](int r, int q_at, int lse_at) {  // rows behind the request, and those that saw no key, give exp2(-inf)
+            store_rows(q_lds[q_at], qx, wave, lane);
+            const bool none = (first + r) * kTile + (int)threadIdx.x >= s.q || lse_next == -INFINITY;
+            if (threadIdx.x < kTile) lse_lds[lse_at][threadIdx.x] = none ? INFINITY : lse_next * kLog2e;
         };
-        auto tile = [&](int it, const unsigned char* ql, const float* lse) __attribute__((always_inline)) {
-            const int p0 = s.off + (first + it % per_head) * kTile;
-            if (p0 + kTile - 1 < kw || (kw + 31 <= p0 - window && kw >= sinks)) return;
-            const bool full = p0 >= kw + 31 && (kw > p0 + kTile - 1 - window || kw + 32 <= sinks);
-            float part = 0.f;
+        auto products = [&](const unsigned char* ql, int rb, f16v (&x)[2]) __attribute__((always_inline)) {
+            x[0] = x[1] = f16v{};
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                f16v sc = f16v{};
+            for (int t = 0; t < 8; ++t) {
+                const r2o_u4 q = read_rows(ql, rb, t, lane);
 #pragma unroll
-                for (int t = 0; t < 8; ++t) sc = mfma32<RF>(read_rows(ql, rb, t, lane), k[t], sc);
+                for (int n = 0; n < 2; ++n) x[n] = mfma32<RF>(q, k[n][t], x[n]);
+            }
+        };
+        auto add = [&](const f16v (&x)[2], const float* lse, int p0) __attribute__((always_inline)) {  // p0: position of the half's first row
+            const bool full = p0 >= kw + 63 && (kw > p0 + 31 - window || kw + 64 <= sinks);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const r2o_f4 x = *reinterpret_cast<const r2o_f4*>(&lse[32 * rb + 8 * g + 4 * half]);
+            for (int n = 0; n < 2; ++n) {
+                float part[2] = {0.f, 0.f};
+                if (full) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * g + i], c2, -x[i]));
-                        if (full) part += e;
-                        else part += sees(p0 + 32 * rb + 8 * g + 4 * half + i, j, window, sinks) ? e : 0.f;
+                    for (int g = 0; g < 4; ++g) {
+                        const r2o_f4 y = *reinterpret_cast<const r2o_f4*>(lse + 8 * g + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) part[i & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][4 * g + i], c2, -y[i]));
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const r2o_f4 y = *reinterpret_cast<const r2o_f4*>(lse + 8 * g + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][4 * g + i], c2, -y[i]));
+                            part[i & 1] += sees(p0 + 8 * g + 4 * half + i, j + 32 * n, window, sinks) ? e : 0.f;
+                        }
                     }
                 }
+                const float term = part[0] + part[1] - lost[n], next = sum[n] + term;
+                lost[n] = (next - sum[n]) - term;
+                sum[n] = next;
             }
-            const float add = part - lost, next = sum + add;
-            lost = (next - sum) - add;
-            sum = next;
         };
-        load(begin);
-        store(begin, 0);
-        for (int it = begin, buf = 0; it < end; ++it, buf ^= 1) {
+        load(head, row_tile);
+        store(row_tile, 0, 0);
+        __syncthreads();
+        f16v even[2], odd[2];
+        products(q_lds[0], 0, even);
+        for (int it = begin, q_at = 0, lse_at = 0; it < end; ++it, q_at ^= 1) {
+            const int p0 = s.off + (first + row_tile) * kTile, lse_to = lse_at == 2 ? 0 : lse_at + 1;
+            if (++row_tile == per_head) {
+                row_tile = 0;
+                ++head;
+            }
+            if (it + 1 < end) load(head, row_tile);
+            products(q_lds[q_at], 1, odd);
+            add(even, lse_lds[lse_at], p0);
+            if (it + 1 < end) store(row_tile, q_at ^ 1, lse_to);
             __syncthreads();
-            if (it + 1 < end) load(it + 1);
-            tile(it, q_lds[buf], lse_lds[buf]);
-            if (it + 1 < end) store(it + 1, buf ^ 1);
+            products(q_lds[q_at ^ 1], 0, even);  // behind the last tile: what lies there, not used
+            add(odd, lse_lds[lse_at] + 32, p0 + 32);
+            lse_at = lse_to;
         }
-        float x, y;
-        r2o_row_swap<32>(sum, x, y);
-        sum = x + y;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float x, y;
+            r2o_row_swap<32>(sum[n], x, y);
+            sum[n] = x + y;
+        }
     }
-    if (half == 0 && j < a.keys)
-        a.weights[((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * a.keys + j] = j < s.n ? sum : 0.f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+        if (half == n && j + 32 * n < a.keys)
+            a.weights[((int64_t)split * a.pairs + pair) * a.keys + j + 32 * n] = j + 32 * n < s.n ? sum[n] : 0.f;
 }
 
 __global__ __launch_bounds__(256) void weights_join_kernel(const float* src, float* dst, int64_t n, int splits) {
@@ -517,6 +556,12 @@ bool shapes_ok(const r2o_prompt_params* p) {
            reinterpret_cast<uintptr_t>(p->query_lengths) % 4 == 0 && reinterpret_cast<uintptr_t>(p->key_lengths) % 4 == 0;
 }
 
+// Blocks of `place`: the items in whole turns of the dies that share a pair.
+int64_t grid_blocks(int64_t tiles, int64_t splits, int64_t pairs) {
+    const int64_t dies = pairs == 1 || pairs == 2 || pairs == 4 ? 8 / pairs : 1;
+    return (tiles * splits + dies - 1) / dies * dies * pairs;
+}
+
 PromptArgs kernel_arguments(const r2o_prompt_params* p) {
     PromptArgs a{};
     a.query = p->query;
@@ -542,6 +587,7 @@ PromptArgs kernel_arguments(const r2o_prompt_params* p) {
     a.hq = (int)p->hq;
     a.hkv = (int)p->hkv;
     a.pairs = (int)(p->batch * p->hkv);
+    a.splits = (int)p->splits;
     a.group = (int)(p->hq / p->hkv);
     a.queries = (int)p->queries;
     a.keys = (int)p->keys;
@@ -562,10 +608,9 @@ int r2o_prompt_attention(const r2o_prompt_params* p, void* stream) {
     const int64_t rows = p->queries * (p->hq / p->hkv), pairs = p->batch * p->hkv;
     if (rows > (1 << 30) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
     if (p->splits > 1 && (!aligned({p->scratch}, 16) || p->scratch_floats < p->splits * pairs * rows * 130)) return R2O_EINVAL;
-    const int64_t tiles = (rows + kRows - 1) / kRows, dies = pairs == 1 || pairs == 2 || pairs == 4 ? 8 / pairs : 1;
-    const int64_t blocks = (tiles + dies - 1) / dies * dies * pairs;  // tiles in whole turns of the dies that share a pair
+    const int64_t blocks = grid_blocks((rows + kRows - 1) / kRows, p->splits, pairs);
     if (blocks > 0x7fffffff) return R2O_EINVAL;
-    const dim3 grid((unsigned)blocks, (unsigned)p->splits);
+    const dim3 grid((unsigned)blocks);
     const dim3 join((unsigned)((rows + 7) / 8), (unsigned)pairs);
     const hipStream_t st = (hipStream_t)stream;
     PromptArgs a = kernel_arguments(p);
@@ -586,8 +631,9 @@ int r2o_attention_weights(const r2o_prompt_params* p, void* stream) {
     if (!shapes_ok(p) || !aligned({p->lse_in, p->weights}, 4) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
     const int64_t n = p->batch * p->hkv * p->keys;
     if (p->splits > 1 && (!aligned({p->scratch}, 4) || p->scratch_floats < p->splits * n)) return R2O_EINVAL;
-    if ((n + 255) / 256 > 0x7fffffff) return R2O_EINVAL;
-    const dim3 grid((unsigned)((p->keys + kWeightKeys - 1) / kWeightKeys), (unsigned)p->splits, (unsigned)(p->batch * p->hkv));
+    const int64_t blocks = grid_blocks((p->keys + kWeightKeys - 1) / kWeightKeys, p->splits, p->batch * p->hkv);
+    if ((n + 255) / 256 > 0x7fffffff || blocks > 0x7fffffff) return R2O_EINVAL;
+    const dim3 grid((unsigned)blocks);
     const hipStream_t st = (hipStream_t)stream;
     PromptArgs a = kernel_arguments(p);
     a.weights = p->splits > 1 ? p->scratch : p->weights;
