@@ -429,11 +429,12 @@ int64_t attention_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries
     return std::max<int64_t>(1, std::min(cus / tiles, div_up(seen, 256)));
 }
 
-// Workgroups that share the query rows of one key tile: enough for four a compute unit, at most one for each (query
-// head, 64-row tile) pair.
+// Workgroups that share the query rows of one key tile: as many as give a compute unit three, at most one for each (query
+// head, 64-row tile) pair.  8192 rows of 16 heads over as many keys take 173 us in 12 splits (three a compute unit), 181 in
+// 16, 237 in 8; 64 rows of 28 heads over 32641 keys 30 us in one (two a compute unit), 37 in two.
 int64_t weight_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries, int64_t keys, int64_t cus) {
     const int64_t tiles = div_up(keys, 256) * batch * hkv, pairs = hq / hkv * div_up(queries, 64);
-    return std::max<int64_t>(1, std::min(pairs, div_up(4 * cus, tiles)));
+    return std::max<int64_t>(1, std::min(pairs, 3 * cus / tiles));
 }
 
 // Workgroups that share the slots of a call: one a compute unit (their LDS fills it), fewer when the page tables hold

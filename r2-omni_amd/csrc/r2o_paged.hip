@@ -582,7 +582,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
 }
 
 // ------------------------------------------------------------------------------------------ evict
-constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / 64;
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins = 4 * kSelectThreads;
 
 // Slots in the order in which they stay, as integers: protected ones, then weights (NaN first, -0 equal to 0), then
 // those of no page; 0 behind the filled ones.
@@ -606,31 +606,52 @@ __device__ __forceinline__ int wave_sum(int x) {
     return __float_as_int(a) + __float_as_int(b);
 }
 
-// Sum over the workgroup's waves of a wave-uniform count; `slot` alternates, so that one barrier does.
-__device__ __forceinline__ int block_sum(int x, int (*counts)[kSelectWaves], int& slot, int wave) {
-    if ((threadIdx.x & 63) == 0) counts[slot][wave] = x;
-    __syncthreads();
-    const int4* c = reinterpret_cast<const int4*>(counts[slot]);
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < kSelectWaves / 4; ++i) {
-        const int4 y = c[i];
-        sum += y.x + y.y + y.z + y.w;
-    }
-    slot ^= 1;
-    return __builtin_amdgcn_readfirstlane(sum);
+// Least over the wave of unsigned words.
+__device__ __forceinline__ uint32_t wave_least(uint32_t x) {
+    x = min(x, __float_as_uint(r2o_lane_xor<1>(__uint_as_float(x))));
+    x = min(x, __float_as_uint(r2o_lane_xor<2>(__uint_as_float(x))));
+    x = min(x, __float_as_uint(r2o_lane_xor<4>(__uint_as_float(x))));
+    x = min(x, __float_as_uint(r2o_lane_xor<8>(__uint_as_float(x))));
+    float a, b;
+    r2o_row_swap<16>(__uint_as_float(x), a, b);
+    x = min(__float_as_uint(a), __float_as_uint(b));
+    r2o_row_swap<32>(__uint_as_float(x), a, b);
+    return min(__float_as_uint(a), __float_as_uint(b));
 }
 
-// One workgroup a (request, head).  A wave holds a run of neighbouring slots, E keys a lane in registers (the ones
-// behind 64 E are read again when they are needed).  The key of the last slot that stays is found bit by bit: the
-// largest T that at least `keep` keys reach, each step one comparison a key and one barrier, ending early when exactly
-// `keep` reach it.  Then every wave knows how many slots before its own stay, and writes its own in order: those above
-// T, and of the equal ones the first.  Bound by those steps' latency; no atomics.
+// Sums up to each lane of the wave: shifts within rows of 16 lanes, then the rows' last lanes handed on.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
+    return x;
+}
+
+// Of the waves' numbers, one a lane: the sum of those before `wave`, and of all.
+__device__ __forceinline__ int waves_before(int x, int wave, int& all) {
+    const int upto = wave_scan((threadIdx.x & 63) < kSelectWaves ? x : 0);
+    all = __builtin_amdgcn_readlane(upto, kSelectWaves - 1);
+    return __builtin_amdgcn_readlane(upto, wave) - __builtin_amdgcn_readlane(x, wave);
+}
+
+// One workgroup a (request, head).  A wave holds a run of neighbouring slots as rows of 256, four neighbours a lane, E keys
+// a lane in registers (the rows behind are read again when they are needed).  The key of the last slot that stays, the
+// largest T that at least `keep` keys reach, is found by counting keys in parts of their range, 4096 a round, at most three
+// rounds.  Then every wave knows how many slots before its own stay, and writes its own in order: those above T, and of
+// the equal ones the first.  The counts do not depend on the order of their additions.
+// Bound by one compute unit's instructions: 8 rows of 65409 slots take 30 us (16 waves a row; loads 1.2 us of it, forming
+// the keys 3, counting 12, their places 8), of 2112 slots 8 us.  Comparing all keys with one trial after another, 13 to 20
+// times, took 45 us; narrowing by trials and then among 8192 listed ones 43 us.  Rows of one compute unit's registers stay
+// within one kernel: counts joined over several would cost a launch, some 4 us, a round.
 template <int E>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_evict_params p) {
-    __shared__ __align__(16) int counts[2][kSelectWaves];
+    constexpr int kQuads = E / 4;
+    __shared__ __align__(16) int bins[kBins];
+    __shared__ int found[3];
     __shared__ int before[kSelectWaves][2];
-    __shared__ int ids[kSelectWaves][(4 * E + 64) / 64 * 64];
     const r2o_paged_cache& c = p.source;
     const int h = blockIdx.x % (int)c.hkv, b = blockIdx.x / (int)c.hkv, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -641,84 +662,156 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_
         for (int i = tid; i < keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
         return;
     }
-    const int per_wave = max(E, (n + kSelectThreads - 1) / kSelectThreads), first = wave * per_wave * 64 + lane;
+    const int quads = max(kQuads, (n + 4 * kSelectThreads - 1) / (4 * kSelectThreads)), first = wave * quads * 256 + 4 * lane;
     const int shift = shift_of(c), mask = (1 << shift) - 1, lo = (int)p.sinks, hi = n - (int)p.recent;  // [lo, hi) may go
     const int32_t* table = c.page_table + b * c.table_stride;
     const float* weights = c.weight_pages + h * c.weight_strides[1];
     const int pages = (int)c.pages, w_page = (int)c.weight_strides[0];
+    // four neighbours lie in one page; a quad behind the filled slots reads the last filled one's
     auto page_at = [&](int j) { return r2o_ldg(table + (min(j, n - 1) >> shift)); };
-    auto weight_at = [&](int j, int page) {
-        const int id = (uint32_t)page < (uint32_t)pages ? page : 0;
-        return r2o_ldg(weights + (int64_t)id * w_page + (min(j, n - 1) & mask));
+    auto weights_at = [&](int j, int page, float (&w)[4]) {
+        const float* src = weights + (int64_t)((uint32_t)page < (uint32_t)pages ? page : 0) * w_page + (min(j, (n - 1) & ~3) & mask);
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // slots are unit-strided, rows may start anywhere
+        const f4 y = *(const R2O_GLOBAL f4*)src;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = y[x];
     };
-    auto key_of = [&](int j, int page, float w) {
-        uint32_t k = (uint32_t)page < (uint32_t)pages ? order_key(w) : kNoPage;
+    auto placed = [&](int j, uint32_t k) {  // what a slot's place says over its weight
         k = j < lo || j >= hi ? kProtected : k;
         return j < n ? k : 0u;
     };
-    auto key_at = [&](int j) {
+    auto quad_at = [&](int j, uint32_t (&k)[4]) {
+        float w[4];
         const int page = page_at(j);
-        return key_of(j, page, weight_at(j, page));
+        weights_at(j, page, w);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) k[x] = placed(j + x, (uint32_t)page < (uint32_t)pages ? order_key(w[x]) : kNoPage);
     };
-    // the wave's page ids, at most 4 E of them and one more where pages are larger than its first slot's alignment
-    const int page0 = (first - lane) >> shift, last = (n - 1) >> shift;
+    uint32_t keys[kQuads][4];
+    uint32_t most = 0, least = 0xffffffffu;
+    int page[kQuads], from = first;
 #pragma unroll
-    for (int i = 0; i < (4 * E + 64) / 64; ++i) ids[wave][64 * i + lane] = r2o_ldg(table + min(page0 + 64 * i + lane, last));
-    __builtin_amdgcn_wave_barrier();
-    // a wave behind the filled slots reads its first id
-    auto page_in = [&](int j) { return ids[wave][max((min(j, n - 1) >> shift) - page0, 0)]; };
-    uint32_t keys[E];
-    int from = first;
+    for (int i = 0; i < kQuads; ++i) page[i] = page_at(first + 256 * i);
 #pragma unroll
-    for (int i0 = 0; i0 < E; i0 += 8) {  // eight rows at a time: what all of them need at once would spill
-        int page[8];
-        asm volatile("" : "+v"(from));
+    for (int i = 0; i < kQuads; ++i) {
+        float w[4];
+        weights_at(first + 256 * i, page[i], w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) page[i] = page_in(from + 64 * (i0 + i));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) keys[i0 + i] = __float_as_uint(weight_at(from + 64 * (i0 + i), page[i]));
-        __builtin_amdgcn_sched_barrier(0);
+        for (int x = 0; x < 4; ++x) keys[i][x] = __float_as_uint(w[x]);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // what all rows need at once would spill
     }
 #pragma unroll
-    for (int i0 = 0; i0 < E; i0 += 8) {
-        int page[8];
-        asm volatile("" : "+v"(from));
+    for (int i = 0; i < kQuads; ++i) {
+        asm volatile("" : "+v"(from));  // each place forms its slots anew: kept, they would spill
+        const int row = wave * quads * 256 + 256 * i;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) page[i] = page_in(from + 64 * (i0 + i));
+        for (int x = 0; x < 4; ++x) {
+            keys[i][x] = order_key(__uint_as_float(keys[i][x]));
+            asm volatile("" : "+v"(keys[i][x]));  // one key whole before the next
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            keys[i0 + i] = key_of(from + 64 * (i0 + i), page[i], __uint_as_float(keys[i0 + i]));
-            asm volatile("" : "+v"(keys[i0 + i]));  // one key whole before the next
+        for (int x = 0; x < 4; x += 2) {  // of all slots read: bounds may be wide
+            most = max(most, max(keys[i][x], keys[i][x + 1]));
+            least = min(least, min(keys[i][x], keys[i][x + 1]));
+        }
+        asm volatile("" : "+v"(most), "+v"(least), "+v"(page[i]));  // now, not when all keys are formed
+        const bool mapped = (uint32_t)page[i] < (uint32_t)pages;
+        if (row < lo || row + 256 > hi || !__all(mapped)) {
+            least = mapped ? least : kNoPage;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) keys[i][x] = placed(from + 256 * i + x, mapped ? keys[i][x] : kNoPage);
         }
     }
 
-    int slot = 0, reach = n;  // keys >= t
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0 && reach > keep; --bit) {
-        const uint32_t trial = t | (1u << bit);
-        int x = 0;
+    auto each = [&](auto&& f) {  // of this thread's keys, four by four
 #pragma unroll
-        for (int i = 0; i < E; ++i) x += keys[i] >= trial ? 1 : 0;
-#pragma unroll 8
-        for (int i = E; i < per_wave; ++i) x += key_at(first + 64 * i) >= trial ? 1 : 0;
-        x = block_sum(wave_sum(x), counts, slot, wave);
-        if (x >= keep) {
-            t = trial;
-            reach = x;
+        for (int i = 0; i < kQuads; ++i) f(keys[i]);
+        for (int i = kQuads; i < quads; ++i) {
+            uint32_t k[4];
+            quad_at(first + 256 * i, k);
+            f(k);
+        }
+    };
+    for (int i = kQuads; i < quads; ++i) {
+        uint32_t k[4];
+        quad_at(first + 256 * i, k);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            most = max(most, k[x] == kProtected ? 0u : k[x]);
+            least = min(least, k[x] ? k[x] : kProtected);
         }
     }
-    t = (uint32_t)__builtin_amdgcn_readfirstlane((int)t);
+    least = wave_least(least);
+    most = ~wave_least(~most);
+    if (lane == 0) {
+        before[wave][0] = (int)least;
+        before[wave][1] = (int)most;
+    }
+    *reinterpret_cast<int4*>(bins + 4 * tid) = int4{0, 0, 0, 0};
+    __syncthreads();
+    least = wave_least((uint32_t)before[lane % kSelectWaves][0]);
+    most = ~wave_least(~(uint32_t)before[lane % kSelectWaves][1]);
+    // The key of the last slot that stays lies in [lo, hi): `reach` keys are at least lo, `keep` or more, and `past` at
+    // least hi, fewer.  A round counts the keys in 4096 parts of the range and goes on in the part that holds it.  The
+    // lowest part is not counted but what is left: slots that no query weighs, all equal, would queue for one counter.
+    uint32_t lo_key = (uint32_t)__builtin_amdgcn_readfirstlane((int)least), hi_key = (uint32_t)__builtin_amdgcn_readfirstlane((int)most) + 1;
+    int reach = n, past = (int)p.sinks + (int)p.recent;
+    if (past == keep) {  // the protected ones alone
+        lo_key = kProtected;
+        reach = keep;
+    }
+    while (reach > keep && hi_key - lo_key > 1) {
+        const uint32_t span = hi_key - lo_key;
+        const int part = max(0, 20 - __builtin_clz(span - 1));  // a part holds 2^part keys
+        const uint32_t bottom = lo_key + (1u << part), counted = span - (1u << part);
+        __syncthreads();  // the counters are clear, and the waves' words read
+        each([&](const uint32_t (&k)[4]) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (k[x] - bottom < counted) atomicAdd(&bins[(k[x] - lo_key) >> part], 1);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        __syncthreads();
+        int4* own = reinterpret_cast<int4*>(bins + kBins - 4 - 4 * tid);  // the highest parts are the first thread's
+        const int4 c4 = *own;
+        *own = int4{0, 0, 0, 0};
+        const int upto = wave_scan(c4.x + c4.y + c4.z + c4.w);
+        if (lane == 63) before[wave][0] = upto;
+        if (tid == 0) found[0] = 0;
+        __syncthreads();
+        int all;
+        int at = past + upto - (c4.x + c4.y + c4.z + c4.w) + waves_before(before[lane % kSelectWaves][0], wave, all);
+        all += past;
+        const int c[4] = {c4.w, c4.z, c4.y, c4.x};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (at < keep && at + c[x] >= keep) {  // of one thread at most
+                found[0] = kBins - 1 - 4 * tid - x;
+                found[1] = at;
+                found[2] = at + c[x];
+            }
+            at += c[x];
+        }
+        __syncthreads();
+        const int bin = __builtin_amdgcn_readfirstlane(found[0]);
+        past = bin ? __builtin_amdgcn_readfirstlane(found[1]) : __builtin_amdgcn_readfirstlane(all);
+        reach = bin ? __builtin_amdgcn_readfirstlane(found[2]) : reach;
+        lo_key += (uint32_t)bin << part;
+        hi_key = min(hi_key - lo_key, 1u << part) + lo_key;
+    }
+    __syncthreads();  // the waves' words are read
+    uint32_t t = (uint32_t)__builtin_amdgcn_readfirstlane((int)lo_key);
     if (reach == keep) --t;  // all that reach it stay, as those above t - 1
     const uint32_t equal = reach == keep ? 0u : t;  // no key at all, or the key whose first slots fill up
     int sures = 0, equals = 0;
-    auto count = [&](uint32_t k) {
-        sures += k > t ? 1 : 0;
-        equals += k == equal ? 1 : 0;
-        __builtin_amdgcn_sched_barrier(0);
-    };
+    each([&](const uint32_t (&k)[4]) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) count(keys[i]);
-    for (int i = E; i < per_wave; ++i) count(key_at(first + 64 * i));
+        for (int x = 0; x < 4; ++x) {
+            sures += k[x] > t ? 1 : 0;
+            equals += k[x] == equal ? 1 : 0;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    });
     sures = wave_sum(sures);
     equals = wave_sum(equals);
     if (lane == 0) {
@@ -726,29 +819,36 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_
         before[wave][1] = equals;
     }
     __syncthreads();
-    int sure_at = 0, equal_at = 0, sure_all = 0;
-    for (int x = 0; x < kSelectWaves; ++x) {
-        sure_all += before[x][0];
-        if (x < wave) {
-            sure_at += before[x][0];
-            equal_at += before[x][1];
-        }
-    }
+    int sure_all, equal_all;
+    int sure_at = waves_before(before[lane % kSelectWaves][0], wave, sure_all);
+    int equal_at = waves_before(before[lane % kSelectWaves][1], wave, equal_all);
     const int still = keep - sure_all;  // of the equal ones; 0 where just `keep` reached
     uint32_t above = t, same = equal;  // values of their own: the comparisons above are made again, not kept
     asm volatile("" : "+s"(above), "+s"(same), "+v"(from));
-    auto write = [&](int j, uint32_t k) {
-        const bool sure = k > above, eq = k == same;
-        const uint64_t s = __ballot(sure), e = __ballot(eq), below = ((uint64_t)1 << lane) - 1;
-        const int e_at = equal_at + __popcll(e & below);
-        if (sure || (eq && e_at < still)) kept[sure_at + __popcll(s & below) + min(e_at, still)] = j;
-        sure_at += __popcll(s);
-        equal_at += __popcll(e);
+    auto write = [&](int j, const uint32_t (&k)[4]) {
+        int mine = 0;  // sure ones, and equal ones above 16 bits
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mine += (k[x] > above ? 1 : 0) + (k[x] == same ? 1 << 16 : 0);
+        const int upto = wave_scan(mine), all = __builtin_amdgcn_readlane(upto, 63);
+        int s = sure_at + ((upto - mine) & 0xffff), e = equal_at + ((upto - mine) >> 16);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const bool sure = k[x] > above, eq = k[x] == same;
+            if (sure || (eq && e < still)) kept[s + min(e, still)] = j + x;
+            s += sure ? 1 : 0;
+            e += eq ? 1 : 0;
+        }
+        sure_at += all & 0xffff;
+        equal_at += all >> 16;
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
-    for (int i = 0; i < E; ++i) write(from + 64 * i, keys[i]);
-    for (int i = E; i < per_wave; ++i) write(from + 64 * i, key_at(from + 64 * i));
+    for (int i = 0; i < kQuads; ++i) write(from + 256 * i, keys[i]);
+    for (int i = kQuads; i < quads; ++i) {
+        uint32_t k[4];
+        quad_at(from + 256 * i, k);
+        write(from + 256 * i, k);
+    }
 }
 
 // 16 lanes move one kept slot's K and V row and its weight.
@@ -892,9 +992,9 @@ int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     const dim3 rows((unsigned)(c.batch * c.hkv)), threads(kSelectThreads);
     const int64_t most = c.max_pages * c.page_size;  // slots that a lane holds: those of the longest request there can be
-    if (most <= 8 * kSelectThreads) hipLaunchKernelGGL(paged_select_kernel<8>, rows, threads, 0, st, *p);
-    else if (most <= 32 * kSelectThreads) hipLaunchKernelGGL(paged_select_kernel<32>, rows, threads, 0, st, *p);
-    else hipLaunchKernelGGL(paged_select_kernel<128>, rows, threads, 0, st, *p);
+    if (most <= 4 * kSelectThreads) hipLaunchKernelGGL(paged_select_kernel<4>, rows, threads, 0, st, *p);
+    else if (most <= 16 * kSelectThreads) hipLaunchKernelGGL(paged_select_kernel<16>, rows, threads, 0, st, *p);
+    else hipLaunchKernelGGL(paged_select_kernel<64>, rows, threads, 0, st, *p);
     R2O_CHECK_LAUNCH();
     hipLaunchKernelGGL(paged_compact_kernel, dim3((unsigned)((p->keep + 15) / 16), (unsigned)c.hkv, (unsigned)c.batch), dim3(256), 0,
                        st, *p);
