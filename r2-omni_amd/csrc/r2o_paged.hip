@@ -512,8 +512,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
         const int u = base + h * t.count, w0 = share.worker(u), count = share.worker(u + t.count - 1) - w0 + 1;
         const int64_t slot0 = (int64_t)w0 + b * hkv + h;
         const Ml ml = join_ml(a.partial_ml, slot0, count, group, head);
-        const bool live = ml.m != -INFINITY;
-        const float ms = live ? ml.m : 0.f;
+        const bool live = !(ml.l == 0.f);  // no slot seen; NaN logits leave m, and a NaN sum
+        const float ms = ml.m == -INFINITY ? 0.f : ml.m;
         const int row = threadIdx.x >> 5, d4 = threadIdx.x & 31;
         r2o_f4 o{};
         for (int i = row; i < count; i += 8) {
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
         const int w0 = share.worker(pair_base), count = share.worker(pair_base + t.count - 1) - w0 + 1;
         for (int head = wave; head < group; head += 4) {
             const Ml ml = join_ml(a.partial_ml, (int64_t)w0 + b * hkv + h, count, group, head);
-            if (lane == 0) lse2[head] = ml.m == -INFINITY ? INFINITY : ml.m + __builtin_amdgcn_logf(ml.l);
+            if (lane == 0) lse2[head] = ml.l == 0.f ? INFINITY : ml.m + __builtin_amdgcn_logf(ml.l);
         }
         __syncthreads();
         const int32_t* table = a.table + (int64_t)b * a.table_stride;

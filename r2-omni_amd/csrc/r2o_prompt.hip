@@ -356,11 +356,11 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
                     r2o_f4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
         if (half == 0) {
             e.partial_ml[2 * at] = row < s.q ? m : -INFINITY;
-            e.partial_ml[2 * at + 1] = l;
+            e.partial_ml[2 * at + 1] = row < s.q ? l : 0.f;
         }
         return;
     }
-    const bool live = row < s.q && m != -INFINITY;
+    const bool live = row < s.q && !(l == 0.f);  // no key seen; NaN logits leave m, and a NaN sum
     const float inv = live ? 1.f / l : 0.f;
     uint16_t* dst = e.out + b * e.o_batch + (kvh * group + head) * e.o_head + (int64_t)row * e.o_row;
 #pragma unroll
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits
         o = m2 == -INFINITY ? o : o * f + o2 * f2;
         m = mn;
     }
-    const bool live = m != -INFINITY;
+    const bool live = !(l == 0.f);
     const float inv = live ? 1.f / l : 0.f;
     r2o_u2 w{};
     if (live) w = r2o_u2{pack2<RF>(o[0] * inv, o[1] * inv), pack2<RF>(o[2] * inv, o[3] * inv)};

@@ -147,7 +147,7 @@ def attention_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor,
     heads of its group.
 
     ``query`` holds the rows that count (all of a prompt's, or the last ones of an observation window) and ``lse``
-    [B, Hq, Sq] fp32 their statistics from ``prompt_attention`` with the same masks; rows with lse -inf give
+    [B, Hq, Sq] fp32 their statistics from ``prompt_attention`` with the same masks; finite rows with lse -inf give
     nothing.  Positions, lengths, masks and strides as there.  Keys behind a length get 0.  The sums are formed in
     a fixed order: equal calls give equal bits."""
     if output is None:
