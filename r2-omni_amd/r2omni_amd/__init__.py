@@ -38,6 +38,7 @@ from .policy import (
     build_layer_compression_plan,
     build_page_table,
     plan_from_pages,
+    project_attention_weights_to_pages,
     project_token_bits_to_pages,
 )
 from .prompt import attention_weights, prompt_attention

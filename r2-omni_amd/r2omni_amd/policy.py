@@ -7,7 +7,8 @@ Same names, fields and error behaviour as the reference's policy/runtime types t
   build_page_table           page_assignment.py:63-137  (pages never cross a modality change)
   project_token_bits_to_pages page_assignment.py:36-60   (16 > 4 > 2 > 0 bits per page)
   LayerCompressionPlan, build_layer_compression_plan  r2omni/sspa/runtime/cache_plan.py:11-52
-The precision policy that decides the bits (scoring, allocation) is not part of the decode path.
+The reference's precision policy (scoring, allocation) is not part of the decode path; without it,
+``project_attention_weights_to_pages`` decides by the attention that the prompt's own rows paid to each page.
 """
 from __future__ import annotations
 
@@ -124,6 +125,40 @@ def project_token_bits_to_pages(page_table: PageTable, token_bits: torch.Tensor)
     dev = bits.device
     zeros = torch.zeros(page_table.num_pages, device=dev, dtype=torch.float32)
     return PageAssignment(page_table, torch.tensor(classes, dtype=torch.int8, device=dev), zeros, zeros, zeros)
+
+
+def project_attention_weights_to_pages(page_table: PageTable, weights: torch.Tensor, *, fp_tokens: int, int4_tokens: int,
+                                       int2_tokens: int) -> PageAssignment:
+    """Page classes from one request's attention weights, [Hkv, S] or [S] as ``attention_weights`` returns them.
+
+    Pages that are protected or recent stay FP.  The others are taken by their weight a token (summed over the heads,
+    in 64 bits; equal ones in the order of the table, NaN as the largest) and become FP, INT4 and INT2 pages as long
+    as a page fits into what is left of that class's tokens; what fits into none is evicted.  The assignment's
+    ``attention_scores`` are the weights a token, on the table's device."""
+    tokens = int(page_table.token_indices.numel())
+    if weights.ndim not in (1, 2) or weights.shape[-1] != tokens or not weights.is_floating_point():
+        raise ValueError("weights must be a floating-point [Hkv,S] or [S] with one value per page-table token")
+    left = [int(fp_tokens), int(int4_tokens), int(int2_tokens)]
+    if min(left) < 0:
+        raise ValueError("fp_tokens, int4_tokens and int2_tokens must be non-negative")
+    per_token = weights.detach().to(device="cpu", dtype=torch.float64).reshape(-1, tokens).sum(0)
+    lengths = page_table.lengths.tolist()
+    scores = torch.stack([run.mean() for run in per_token.split(lengths)]) if lengths else per_token
+    classes = [int(PageClass.EVICTED_PAGE)] * len(lengths)
+    protected, recent = page_table.protected.tolist(), page_table.recent.tolist()
+    for page in scores.sort(descending=True, stable=True).indices.tolist():
+        if protected[page] or recent[page]:
+            classes[page] = int(PageClass.PROTECTED_FP_PAGE if protected[page] else PageClass.RECENT_FP_PAGE)
+            continue
+        for i, cls in enumerate((PageClass.FP_PAGE, PageClass.INT4_PAGE, PageClass.INT2_PAGE)):
+            if lengths[page] <= left[i]:
+                left[i] -= lengths[page]
+                classes[page] = int(cls)
+                break
+    dev = page_table.offsets.device
+    attention = scores.to(device=dev, dtype=torch.float32)
+    zeros = torch.zeros_like(attention)
+    return PageAssignment(page_table, torch.tensor(classes, dtype=torch.int8, device=dev), attention, zeros, zeros)
 
 
 @dataclass(frozen=True)
