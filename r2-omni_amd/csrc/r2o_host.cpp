@@ -593,7 +593,7 @@ bool cache_arg(PyObject* bytes, PyObject* keys, r2o_paged_cache& c, int64_t& dev
 }
 
 bool cache_rows(const at::Tensor* t, const r2o_paged_cache& c, int64_t device) {
-    return t && on_device(*t, device) && row_code(*t) == c.dtype;
+    return t && on_device(*t, device) && row_code(*t) == c.dtype && !needs_grad(*t);
 }
 
 // paged_extend(function, cache, key pages, key, value, counts, weights): (status,) or None
@@ -629,7 +629,7 @@ PyObject* paged_attention_call(PyObject* const* args) {
     r2o_paged_cache& c = p.cache;
     int64_t device;
     const at::Tensor* q = exact_tensor(args[3]);
-    if (!cache_arg(args[1], args[2], c, device) || !cache_rows(q, c, device) || needs_grad(*q) ||
+    if (!cache_arg(args[1], args[2], c, device) || !cache_rows(q, c, device) ||
         !(q->dim() == 3 || (q->dim() == 4 && q->size(2) == 1)) || q->size(0) != c.batch || q->size(-1) != R2O_HEAD_DIM)
         Py_RETURN_NONE;
     p.hq = q->size(1);
@@ -675,7 +675,7 @@ PyObject* paged_evict_call(PyObject* const* args) {
         !plain_int(args[6], p.keep) || !plain_int(args[7], p.sinks) || !plain_int(args[8], p.recent))
         Py_RETURN_NONE;
     const r2o_paged_cache &c = p.source, &o = p.target;
-    if (!c.weight_pages || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || c.lengths == o.lengths ||
+    if (!c.weight_pages || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || std::abs(c.lengths - o.lengths) < c.batch ||
         c.page_table == o.page_table || p.keep < 1 || p.keep > o.max_pages * o.page_size || p.sinks < 0 || p.recent < 0 ||
         p.sinks + p.recent > p.keep)
         Py_RETURN_NONE;

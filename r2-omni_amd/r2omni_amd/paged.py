@@ -98,6 +98,8 @@ def _check_new_rows(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, w
     for t in (key, value):
         if t.dtype != cache.key_pages.dtype or t.device != cache.key_pages.device:
             raise ValueError(f"{what} rows must match the cache's dtype and device")
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
 def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, counts: torch.Tensor | None = None,
@@ -225,7 +227,7 @@ def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int 
         raise ValueError("paged evict target must have the source's requests and heads")
     if cache.key_pages.dtype != target.key_pages.dtype or cache.key_pages.device != target.key_pages.device:
         raise ValueError("paged evict target must match the source's dtype and device")
-    if cache.lengths.data_ptr() == target.lengths.data_ptr() or cache.page_table.data_ptr() == target.page_table.data_ptr():
+    if abs(cache.lengths.data_ptr() - target.lengths.data_ptr()) < 4 * cache.lengths.numel() or cache.page_table.data_ptr() == target.page_table.data_ptr():
         raise ValueError("paged evict target needs a page table and lengths of its own")
     if not 1 <= keep <= target.capacity:
         raise ValueError("keep must be positive and at most what the target's page table holds")

@@ -151,3 +151,9 @@ def test_the_longest_scratch_is_joined_in_one_order():
     torch.cuda.synchronize()
     for out, lse, w in got:
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and torch.equal(w, weights)
+
+
+def test_evict_short_requests_of_long_tables():
+    """What a lane holds goes by the request, not by what the table could hold."""
+    cache = _cache(_cuda(), (20000, 4096, 4097, 16384, 16385, 50), 1, 128, BF16, seed=10, weights=True)
+    _check_evict(cache, 100, 4, 20)

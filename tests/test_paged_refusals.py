@@ -208,3 +208,25 @@ def test_struct_layouts_match_the_header(tmp_path):
         offsets, size = _c_layout(struct, names, tmp_path)
         assert [getattr(cls, n).offset for n in names] == offsets, struct
         assert ctypes.sizeof(cls) == size, struct
+
+
+def test_rows_that_need_a_gradient_are_refused(cache):
+    plain, grad = _rows(2, 2, 5, 128), _rows(2, 2, 5, 128).requires_grad_()
+    for key, value in ((grad, plain), (plain, grad)):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            ro.paged_extend(cache, key, value)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            ro.paged_attention(_rows(2, 4, 128), cache, append=(key[:, :, 0], value[:, :, 0]))
+        with torch.no_grad(), pytest.raises(AssertionError, match="launched"):
+            ro.paged_extend(cache, key, value)
+
+
+def test_evictions_into_overlapping_lengths_are_refused(cache):
+    both = torch.zeros(3, dtype=I32)
+    source = ro.PagedCache(**_tensors(lengths=both[:2]))
+    target = ro.PagedCache(**_tensors(lengths=both[1:]))
+    with pytest.raises(ValueError, match="lengths of its own"):
+        ro.paged_evict(source, target, 8)
+    lib = _lib.load()
+    assert lib.r2o_paged_evict(ctypes.byref(_evict(target_lengths=0x5004)), None) == 1
+    assert lib.r2o_paged_evict(ctypes.byref(_evict(target_lengths=0x4ffc)), None) == 1
