@@ -35,7 +35,8 @@ __device__ __forceinline__ int page_of(const r2o_paged_cache& c, int b, int slot
 }
 
 // ---------------------------------------------------------------------------------------- extend
-// 16 lanes move one K and one V row.  Bound by the rows' bytes for a prompt, by the launch for a step.
+// 16 lanes move one K and one V row.  Bound by the rows' bytes for a prompt (32641 rows of 8 heads: 52 us, 5.2 TB/s read and written), by the
+// launch for a step (5 us).
 __global__ __launch_bounds__(256) void paged_extend_kernel(r2o_paged_extend_params p) {
     const r2o_paged_cache& c = p.cache;
     const int h = blockIdx.y, b = blockIdx.z, l16 = threadIdx.x & 15;
@@ -263,6 +264,9 @@ __device__ __forceinline__ void read_values(uint32_t row, uint32_t chunk, int d,
 // two LDS stages: the next tile's loads go out before this one's products, its page ids one tile earlier still.
 // S^T = K Q^T (16 slots x 16 heads a product), O^T += V^T P^T; P^T's operand is the C registers of S^T as they are: the
 // slots of a product are summed in that order on both sides.
+// Bound by the rows' bytes: a ragged batch of 252 MB takes 50 us, 5.0 TB/s of the 5.9 that a streaming read reaches, about
+// 5 of it the first loads and the last join.  One workgroup a compute unit, whose LDS it fills: with twice as many, a
+// windowed batch of 251 MB takes 54.3 us instead of 51.2.
 template <int RF, bool WEIGHTS>
 __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
     __shared__ __align__(16) unsigned char lds[kWaves][2][kStage];
@@ -490,7 +494,8 @@ __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count,
 }
 
 // Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: an even
-// share of all tiles each, whose slots' weights grow by their probabilities.
+// share of all tiles each, whose slots' weights grow by their probabilities.  Bound by its launch and two round trips: 5
+// us for a call without weights, 11.6 for a ragged batch of 252 MB with them.
 template <int RF>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
     Args& a = kernel_args();
@@ -869,7 +874,8 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(r2o_paged_
     select_row<64>(p, lds, h, b, n);
 }
 
-// 16 lanes move one kept slot's K and V row and its weight.
+// 16 lanes move one kept slot's K and V row and its weight.  Bound by the rows' bytes: eight requests of 2048 slots and 4
+// heads take 13.5 us, 5.0 TB/s read and written, what a large copy reaches.
 __global__ __launch_bounds__(256) void paged_compact_kernel(r2o_paged_evict_params p) {
     const r2o_paged_cache &c = p.source, &o = p.target;
     const int h = blockIdx.y, b = blockIdx.z, l16 = threadIdx.x & 15, i = blockIdx.x * 16 + (threadIdx.x >> 4);

@@ -184,6 +184,11 @@ __device__ __forceinline__ bool place(int block, int tiles, int splits, int pair
 // stand at 128 / group neighbouring positions, so its last tiles are masked in part for few of them, and a chunk of few
 // rows fills it.  grid: (row tiles x pairs of request and KV head, splits); with splits each takes a share of the key tiles and
 // leaves (maximum, sum, products) in scratch for prompt_join_kernel.
+// 16384 rows of 28 heads over 4: 2105 us, 914 TFLOP/s (bf16; a large library product reaches 1270 to 1380); 8192, 5003 and
+// 1231 rows of 32 heads with a window of 1024 and four sinks: 376 us (fp16); 257 rows of 16 heads over 4097 keys: 27 us in 7 splits and 7 for
+// the join.  Bound by what runs beside the matrix instructions: without LDS reads and writes the first takes 1463 us, without
+// the maximum as well 1070.  A wave of 64 rows reads half as much from LDS, but its 512 registers leave one wave a SIMD: 2693
+// us; 256 rows a workgroup (8 waves) 1953 against 2009, but 386 against 365 for the windowed batch and 39 against 33 for the 257 rows.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     // K tiles t and t + 1, V tiles t to t + 2: two workgroups fill a compute unit's 160 KB
@@ -379,7 +384,8 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
         e.lse[((int64_t)b * e.hq + kvh * group + head) * e.queries + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
-// 32 lanes a packed row: its splits' states, joined in order.
+// 32 lanes a packed row: its splits' states, joined in order.  Bound by its launch and one round trip to the partial
+// states: 257 rows of 16 heads in 7 splits (15 MB) take 7 us.
 template <int RF>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits) {
     Args& a = kernel_args();
@@ -411,10 +417,11 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits
 // ----------------------------------------------------------------------------- attention weights
 constexpr int kWeightKeys = 256;  // keys of a workgroup: 4 waves of 64, whose rows stay in registers
 
-// A split takes a share of the (query head, 64-row tile) pairs that see the key tile;
-// its sums go to `weights` ([splits, batch, hkv, keys]; the result itself where there is one split).  S = Q K^T: a lane
+// A split takes a share of the (query head, 64-row tile) pairs that see the key tile; its sums go to `weights` ([splits, batch, hkv, keys]; the result itself where there is one split).  S = Q K^T: a lane
 // sums its own two keys.  A row tile is two halves of 32; the products of the half that follows run beside the
-// exponentials of the one before it.
+// exponentials of the one before it.  The sums carry what an addition rounds off along: 8192 terms of very different size.
+// Bound by the exponentials and additions beside the matrix instructions: 8192 rows of 16 heads over as many keys take 177
+// us, 780 TFLOP/s of products; with 32 keys a wave, that is twice the reads of Q, 320.  64 rows of 28 heads over 32641 keys: 30 us.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     __shared__ __align__(16) unsigned char q_lds[2][kTileBytes];
