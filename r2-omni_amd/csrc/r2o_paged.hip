@@ -34,6 +34,17 @@ __device__ __forceinline__ int page_of(const r2o_paged_cache& c, int b, int slot
     return (uint32_t)page < (uint32_t)c.pages ? page : -1;
 }
 
+// Sums up to each lane of the wave: shifts within rows of 16 lanes, then the rows' last lanes handed on.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
+    return x;
+}
+
 // ---------------------------------------------------------------------------------------- extend
 // 16 lanes move one K and one V row.  Bound by the rows' bytes for a prompt (32641 rows of 8 heads: 52 us, 5.2 TB/s read and written), by the
 // launch for a step (5 us).
@@ -135,12 +146,7 @@ __device__ __forceinline__ Lane lane_tiles(Args& a, int b0) {
     const int lane = threadIdx.x & 63, b = b0 + lane;
     Lane x;
     x.count = b < a.batch ? tiles_of(a, r2o_ldg(a.lengths + b)).count : 0;
-    x.upto = x.count;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int y = __shfl_up(x.upto, m, R2O_WAVE);
-        if (lane >= m) x.upto += y;
-    }
+    x.upto = wave_scan(x.count);
     return x;
 }
 
@@ -488,8 +494,17 @@ __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count,
         const float* s = ml + ((slot0 + i) * group + head) * 2;
         join_states(m, l, r2o_ldg(s), r2o_ldg(s + 1));
     }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) join_states(m, l, __shfl_xor(m, x, R2O_WAVE), __shfl_xor(l, x, R2O_WAVE));
+    join_states(m, l, r2o_lane_xor<1>(m), r2o_lane_xor<1>(l));
+    join_states(m, l, r2o_lane_xor<2>(m), r2o_lane_xor<2>(l));
+    join_states(m, l, r2o_lane_xor<4>(m), r2o_lane_xor<4>(l));
+    join_states(m, l, r2o_lane_xor<8>(m), r2o_lane_xor<8>(l));
+    float m2, l2;
+    r2o_row_swap<16>(m, m, m2);
+    r2o_row_swap<16>(l, l, l2);
+    join_states(m, l, m2, l2);
+    r2o_row_swap<32>(m, m, m2);
+    r2o_row_swap<32>(l, l, l2);
+    join_states(m, l, m2, l2);
     return {m, l};
 }
 
@@ -517,12 +532,24 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
         }
         const int u = base + h * t.count, w0 = share.worker(u), count = share.worker(u + t.count - 1) - w0 + 1;
         const int64_t slot0 = (int64_t)w0 + b * hkv + h;
+        // the first 32 partial outputs go out with the states that weigh them
+        const int row = threadIdx.x >> 5, d4 = threadIdx.x & 31;
+        r2o_f4 part[4];
+        float part_m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t at = (slot0 + min(row + 8 * k, count - 1)) * group + head;
+            part_m[k] = r2o_ldg(a.partial_ml + at * 2);
+            part[k] = r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4);
+        }
         const Ml ml = join_ml(a.partial_ml, slot0, count, group, head);
         const bool live = !(ml.l == 0.f);  // no slot seen; NaN logits leave m, and a NaN sum
         const float ms = ml.m == -INFINITY ? 0.f : ml.m;
-        const int row = threadIdx.x >> 5, d4 = threadIdx.x & 31;
         r2o_f4 o{};
-        for (int i = row; i < count; i += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (row + 8 * k < count) o += __builtin_amdgcn_exp2f(part_m[k] - ms) * part[k];
+        for (int i = row + 32; i < count; i += 8) {
             const int64_t at = (slot0 + i) * group + head;
             const float f = __builtin_amdgcn_exp2f(r2o_ldg(a.partial_ml + at * 2) - ms);
             o += f * r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4);
@@ -623,17 +650,6 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t x) {
     x = min(__float_as_uint(a), __float_as_uint(b));
     r2o_row_swap<32>(__uint_as_float(x), a, b);
     return min(__float_as_uint(a), __float_as_uint(b));
-}
-
-// Sums up to each lane of the wave: shifts within rows of 16 lanes, then the rows' last lanes handed on.
-__device__ __forceinline__ int wave_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
-    return x;
 }
 
 // Of the waves' numbers, one a lane: the sum of those before `wave`, and of all.
