@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstdlib>
 #include <initializer_list>
+#include <type_traits>
 
 #include "r2o_common.hpp"
 
@@ -621,10 +622,14 @@ constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins =
 // those of no page; 0 behind the filled ones.
 constexpr uint32_t kProtected = 0xffffffffu, kNaN = 0xfffffffeu, kNoPage = 1u;
 
-__device__ __forceinline__ uint32_t order_key(float w) {
-    const uint32_t u = __float_as_uint(w + 0.f), k = (u & 0x80000000u) ? ~u : u | 0x80000000u;  // -inf: 0x007fffff, inf: 0xff800000
-    return w != w ? kNaN : k;
+__device__ __forceinline__ uint32_t number_key(float w) {  // -inf: 0x007fffff, inf: 0xff800000, NaN beyond either
+    const int u = __float_as_int(w + 0.f);
+    return (uint32_t)(u ^ ((u >> 31) | (int)0x80000000));
 }
+
+constexpr uint32_t kLeastNumber = 0x007fffffu, kMostNumber = 0xff800000u;
+
+__device__ __forceinline__ uint32_t order_key(float w) { return w != w ? kNaN : number_key(w); }
 
 // Sum over the wave, by moves between lanes through the VALU.
 __device__ __forceinline__ int wave_sum(int x) {
@@ -664,8 +669,8 @@ __device__ __forceinline__ int waves_before(int x, int wave, int& all) {
 // largest T that at least `keep` keys reach, is found by counting keys in parts of their range, 4096 a round, at most three
 // rounds.  Then every wave knows how many slots before its own stay, and writes its own in order: those above T, and of
 // the equal ones the first.  The counts do not depend on the order of their additions.
-// Bound by one compute unit's instructions: 8 rows of 65409 slots take 30 us (16 waves a row; loads 1.2 us of it, forming
-// the keys 3, counting 12, their places 8), of 2112 slots 8 us.  Comparing all keys with one trial after another, 13 to 20
+// Bound by one compute unit's instructions: 8 rows of 65409 slots take 25 us (16 waves a row; loads 1.3 us of it, forming
+// the keys 5, three rounds 11, places 6), of 2112 slots 8 us.  Comparing all keys with one trial after another, 13 to 20
 // times, took 45 us; narrowing by trials and then among 8192 listed ones 43 us.  Rows of one compute unit's registers stay
 // within one kernel: counts joined over several would cost a launch, some 4 us, a round.
 struct SelectLds {
@@ -727,21 +732,27 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
         const int row = wave * quads * 256 + 256 * i;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            keys[i][x] = order_key(__uint_as_float(keys[i][x]));
+            keys[i][x] = number_key(__uint_as_float(keys[i][x]));
             asm volatile("" : "+v"(keys[i][x]));  // one key whole before the next
         }
-#pragma unroll
-        for (int x = 0; x < 4; x += 2) {  // of all slots read: bounds may be wide
-            most = max(most, max(keys[i][x], keys[i][x + 1]));
-            least = min(least, min(keys[i][x], keys[i][x + 1]));
-        }
-        asm volatile("" : "+v"(most), "+v"(least), "+v"(page[i]));  // now, not when all keys are formed
+        uint32_t high = max(max(keys[i][0], keys[i][1]), max(keys[i][2], keys[i][3]));
+        uint32_t low = min(min(keys[i][0], keys[i][1]), min(keys[i][2], keys[i][3]));
+        asm volatile("" : "+v"(page[i]), "+v"(high), "+v"(low));
         const bool mapped = (uint32_t)page[i] < (uint32_t)pages;
-        if (row < lo || row + 256 > hi || !__all(mapped)) {
-            least = mapped ? least : kNoPage;
+        if (row < lo || row + 256 > hi || !__all(mapped && low >= kLeastNumber && high <= kMostNumber)) {
+            high = 0;
+            low = kProtected;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) keys[i][x] = placed(from + 256 * i + x, mapped ? keys[i][x] : kNoPage);
+            for (int x = 0; x < 4; ++x) {
+                const bool number = keys[i][x] >= kLeastNumber && keys[i][x] <= kMostNumber;
+                keys[i][x] = placed(from + 256 * i + x, !mapped ? kNoPage : number ? keys[i][x] : kNaN);
+                high = max(high, keys[i][x] == kProtected ? 0u : keys[i][x]);
+                low = min(low, keys[i][x] ? keys[i][x] : kProtected);
+            }
         }
+        most = max(most, high);
+        least = min(least, low);
+        asm volatile("" : "+v"(most), "+v"(least));  // now, not when all keys are formed
     }
 
     auto each = [&](auto&& f) {  // of this thread's keys, four by four
@@ -827,12 +838,15 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
     int sures = 0, equals = 0;
     each([&](const uint32_t (&k)[4]) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            sures += k[x] > t ? 1 : 0;
-            equals += k[x] == equal ? 1 : 0;
-        }
+        for (int x = 0; x < 4; ++x) sures += k[x] > t ? 1 : 0;
         __builtin_amdgcn_sched_barrier(0);
     });
+    if (equal)
+        each([&](const uint32_t (&k)[4]) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) equals += k[x] == equal ? 1 : 0;
+            __builtin_amdgcn_sched_barrier(0);
+        });
     sures = wave_sum(sures);
     equals = wave_sum(equals);
     if (lane == 0) {
@@ -844,32 +858,37 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
     int sure_at = waves_before(before[lane % kSelectWaves][0], wave, sure_all);
     int equal_at = waves_before(before[lane % kSelectWaves][1], wave, equal_all);
     const int still = keep - sure_all;  // of the equal ones; 0 where just `keep` reached
-    uint32_t above = t, same = equal;  // values of their own: the comparisons above are made again, not kept
+    // values of their own: the comparisons above are made again, not kept
+    uint32_t above = (uint32_t)__builtin_amdgcn_readfirstlane((int)t), same = (uint32_t)__builtin_amdgcn_readfirstlane((int)equal);
     asm volatile("" : "+s"(above), "+s"(same), "+v"(from));
-    auto write = [&](int j, const uint32_t (&k)[4]) {
-        int mine = 0;  // sure ones, and equal ones above 16 bits
+    auto write_all = [&](auto ties) {
+        auto write = [&](int j, const uint32_t (&k)[4]) {
+            int mine = 0;  // sure ones, and equal ones above 16 bits
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mine += (k[x] > above ? 1 : 0) + (k[x] == same ? 1 << 16 : 0);
-        const int upto = wave_scan(mine), all = __builtin_amdgcn_readlane(upto, 63);
-        int s = sure_at + ((upto - mine) & 0xffff), e = equal_at + ((upto - mine) >> 16);
+            for (int x = 0; x < 4; ++x) mine += (k[x] > above ? 1 : 0) + (ties && k[x] == same ? 1 << 16 : 0);
+            const int upto = wave_scan(mine), all = __builtin_amdgcn_readlane(upto, 63);
+            int s = sure_at + ((upto - mine) & 0xffff), e = equal_at + ((upto - mine) >> 16);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const bool sure = k[x] > above, eq = k[x] == same;
-            if (sure || (eq && e < still)) kept[s + min(e, still)] = j + x;
-            s += sure ? 1 : 0;
-            e += eq ? 1 : 0;
+            for (int x = 0; x < 4; ++x) {
+                const bool sure = k[x] > above, eq = ties && k[x] == same;
+                if (sure || (eq && e < still)) kept[ties ? s + min(e, still) : s] = j + x;
+                s += sure ? 1 : 0;
+                e += eq ? 1 : 0;
+            }
+            sure_at += all & 0xffff;
+            equal_at += all >> 16;
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) write(from + 256 * i, keys[i]);
+        for (int i = kQuads; i < quads; ++i) {
+            uint32_t k[4];
+            quad_at(from + 256 * i, k);
+            write(from + 256 * i, k);
         }
-        sure_at += all & 0xffff;
-        equal_at += all >> 16;
-        __builtin_amdgcn_sched_barrier(0);
     };
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) write(from + 256 * i, keys[i]);
-    for (int i = kQuads; i < quads; ++i) {
-        uint32_t k[4];
-        quad_at(from + 256 * i, k);
-        write(from + 256 * i, k);
-    }
+    if (equal) write_all(std::true_type());
+    else write_all(std::false_type());
 }
 
 // E: for the longest request that the page table can hold; a shorter one takes as few keys a lane as it needs.
