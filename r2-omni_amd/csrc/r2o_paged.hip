@@ -669,8 +669,8 @@ __device__ __forceinline__ int waves_before(int x, int wave, int& all) {
 // largest T that at least `keep` keys reach, is found by counting keys in parts of their range, 4096 a round, at most three
 // rounds.  Then every wave knows how many slots before its own stay, and writes its own in order: those above T, and of
 // the equal ones the first.  The counts do not depend on the order of their additions.
-// Bound by one compute unit's instructions: 8 rows of 65409 slots take 25 us (16 waves a row; loads 1.3 us of it, forming
-// the keys 5, three rounds 11, places 6), of 2112 slots 8 us.  Comparing all keys with one trial after another, 13 to 20
+// Bound by one compute unit's instructions: 8 rows of 65409 slots take 23 us (16 waves a row; loads 1.3 us of it, forming
+// the keys 5, three rounds 10, places 6), of 2112 slots 6.6 us.  Comparing all keys with one trial after another, 13 to 20
 // times, took 45 us; narrowing by trials and then among 8192 listed ones 43 us.  Rows of one compute unit's registers stay
 // within one kernel: counts joined over several would cost a launch, some 4 us, a round.
 struct SelectLds {
@@ -784,8 +784,8 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
     least = wave_least((uint32_t)before[lane % kSelectWaves][0]);
     most = ~wave_least(~(uint32_t)before[lane % kSelectWaves][1]);
     // The key of the last slot that stays lies in [lo, hi): `reach` keys are at least lo, `keep` or more, and `past` at
-    // least hi, fewer.  A round counts the keys in 4096 parts of the range and goes on in the part that holds it.  The
-    // lowest part is not counted but what is left: slots that no query weighs, all equal, would queue for one counter.
+    // least hi, fewer.  A round counts the keys above lo in 4096 parts of the range and goes on in the part that holds it.
+    // Those equal to lo are not counted but what is left: slots that no query weighs would queue for one counter.
     uint32_t lo_key = (uint32_t)__builtin_amdgcn_readfirstlane((int)least), hi_key = (uint32_t)__builtin_amdgcn_readfirstlane((int)most) + 1;
     int reach = n, past = (int)p.sinks + (int)p.recent;
     if (past == keep) {  // the protected ones alone
@@ -795,12 +795,12 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
     while (reach > keep && hi_key - lo_key > 1) {
         const uint32_t span = hi_key - lo_key;
         const int part = max(0, 20 - __builtin_clz(span - 1));  // a part holds 2^part keys
-        const uint32_t bottom = lo_key + (1u << part), counted = span - (1u << part);
+        const uint32_t bottom = lo_key + 1, counted = span - 1;
         __syncthreads();  // the counters are clear, and the waves' words read
         each([&](const uint32_t (&k)[4]) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-                if (k[x] - bottom < counted) atomicAdd(&bins[(k[x] - lo_key) >> part], 1);
+                if (k[x] - bottom < counted) atomicAdd(&bins[(k[x] - bottom) >> part], 1);
             __builtin_amdgcn_sched_barrier(0);
         });
         __syncthreads();
@@ -809,7 +809,7 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
         *own = int4{0, 0, 0, 0};
         const int upto = wave_scan(c4.x + c4.y + c4.z + c4.w);
         if (lane == 63) before[wave][0] = upto;
-        if (tid == 0) found[0] = 0;
+        if (tid == 0) found[0] = -1;
         __syncthreads();
         int all;
         int at = past + upto - (c4.x + c4.y + c4.z + c4.w) + waves_before(before[lane % kSelectWaves][0], wave, all);
@@ -826,10 +826,15 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
         }
         __syncthreads();
         const int bin = __builtin_amdgcn_readfirstlane(found[0]);
-        past = bin ? __builtin_amdgcn_readfirstlane(found[1]) : __builtin_amdgcn_readfirstlane(all);
-        reach = bin ? __builtin_amdgcn_readfirstlane(found[2]) : reach;
-        lo_key += (uint32_t)bin << part;
-        hi_key = min(hi_key - lo_key, 1u << part) + lo_key;
+        if (bin < 0) {  // lo itself
+            past = __builtin_amdgcn_readfirstlane(all);
+            hi_key = lo_key + 1;
+        } else {
+            past = __builtin_amdgcn_readfirstlane(found[1]);
+            reach = __builtin_amdgcn_readfirstlane(found[2]);
+            lo_key = bottom + ((uint32_t)bin << part);
+            hi_key = min(hi_key - lo_key, 1u << part) + lo_key;
+        }
     }
     __syncthreads();  // the waves' words are read
     uint32_t t = (uint32_t)__builtin_amdgcn_readfirstlane((int)lo_key);

@@ -77,6 +77,21 @@ def test_evict_when_nearly_all_weights_are_equal(n):
     _check_evict(cache, 40, 10, 30)
 
 
+@pytest.mark.parametrize("n", [200, 5000, 20000])
+def test_evict_nan_of_every_sign_and_payload(n):
+    """All NaN are equal and the largest, the earlier first; what lies behind the filled slots may be any of them."""
+    dev = _cuda()
+    cache = _cache(dev, (n,), 1, 64, BF16, seed=11, weights=True)
+    w, ids = cache.weight_pages.view(torch.int32), cache.page_table[0].long()
+    for i, bits in enumerate((0x7FFFFFFF, -1, -0x400000, 0x7F800001, 0x7FC00000)):
+        j = (6101 * (i + 1)) % n
+        w[ids[j // 64], 0, j % 64] = bits
+    if n % 64:
+        w[ids[-1], 0, n % 64 :] = torch.tensor([0x7FFFFFFF, -1], dtype=torch.int32, device=dev).repeat(32)[: 64 - n % 64]
+    for keep in (1, 3, 5, 6, 70):
+        _check_evict(cache, keep)
+
+
 def test_more_requests_than_lanes_with_windows_sinks_and_weights():
     dev = _cuda()
     lengths = tuple((37 * i) % 130 for i in range(150))
