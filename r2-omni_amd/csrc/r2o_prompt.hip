@@ -46,21 +46,21 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return RF == 0 ? r2o_pack_bf2(lo, hi) : r2o_pack_h2(lo, hi);
 }
 
-// One wave's 16 rows of a 64-row tile, from `row0` on clamped to `last`, into registers, and from there into LDS: a row is
-// 16 chunks of 16 bytes, chunk c of row r at place c ^ swizzle(r); lane l writes at 16 l, so the swizzle is made by which
-// chunk it reads.  LDS answers 256 bytes a clock, so 16 lanes' 16-byte reads, or 32 lanes' 8-byte ones, have to fall into
-// 256 different ones.  SWZ 0: r & 15, for reads of one chunk by 32 rows (4.1 clocks a wave; r & 7 takes 8.1); 1: 4 (r & 3),
-// for transposing reads of four chunks by 4 rows (3.0 clocks; 2 (r & 3) takes 4.1).
+// A staged tile's row is 16 chunks of 16 bytes, chunk c of row r at place c ^ swizzle(r).  LDS answers 256 bytes a clock,
+// so 16 lanes' 16-byte reads, or 32 lanes' 8-byte ones, have to fall into 256 different ones.  SWZ 0: r & 15, for reads
+// of one chunk by 32 rows (4.1 clocks a wave; r & 7 takes 8.1); 1: 4 (r & 3), for transposing reads of four chunks by 4
+// rows (3.0 clocks; 2 (r & 3) takes 4.1).  A wave brings 16 rows, four at a time: lane l writes at 16 l, so the swizzle is
+// made by which chunk it reads.  This lane's chunk of four rows from r0 on, clamped to `last`:
 template <int SWZ>
+__device__ __forceinline__ const unsigned char* row_chunk(const uint16_t* base, int stride, int r0, int last, int i, int lane) {
+    const int r4 = lane >> 4, place = lane & 15, c = place ^ (SWZ == 0 ? 4 * i + r4 : 4 * r4);
+    return reinterpret_cast<const unsigned char*>(base + (int64_t)r0 * stride) + (uint32_t)(2 * min(r4, last - r0) * stride + 16 * c);
+}
+
+// Into registers, and from there into LDS.
 __device__ __forceinline__ void load_rows(const uint16_t* base, int stride, int row0, int last, r2o_u4 (&x)[4], int wave, int lane) {
-    const int r4 = lane >> 4, place = lane & 15;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r0 = min(row0 + 16 * wave + 4 * i, last);
-        const int c = place ^ (SWZ == 0 ? 4 * i + r4 : 4 * r4);
-        const uint32_t at = (uint32_t)(2 * min(r4, last - r0) * stride + 16 * c);
-        x[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(reinterpret_cast<const unsigned char*>(base + (int64_t)r0 * stride) + at));
-    }
+    for (int i = 0; i < 4; ++i) x[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(row_chunk<0>(base, stride, min(row0 + 16 * wave + 4 * i, last), last, i, lane)));
 }
 
 __device__ __forceinline__ void store_rows(unsigned char* lds, const r2o_u4 (&x)[4], int wave, int lane) {
@@ -72,6 +72,36 @@ __device__ __forceinline__ void store_rows(unsigned char* lds, const r2o_u4 (&x)
 __device__ __forceinline__ r2o_u4 read_rows(const unsigned char* tile, int block, int t, int lane) {
     const int r = lane & 31, c = 2 * t + (lane >> 5);
     return *reinterpret_cast<const r2o_u4*>(tile + (32 * block + r) * 256 + 16 * (c ^ (r & 15)));
+}
+
+// Straight into LDS, asynchronously.
+template <int SWZ>
+__device__ __forceinline__ void stage_rows(const uint16_t* base, int stride, int row0, int last, unsigned char* lds, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)row_chunk<SWZ>(base, stride, min(row0 + 16 * wave + 4 * i, last), last, i, lane),
+            (__attribute__((address_space(3))) void*)(lds + (16 * wave + 4 * i) * 256), 16, 0, 0);
+}
+
+__device__ __forceinline__ void wait_staged() { __builtin_amdgcn_s_waitcnt(0xF70); }  // vmcnt(0), the other counters left alone
+
+__device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)p;
+}
+
+// 32 rows of a staged tile (SWZ 0) as the A operands of all eight steps, in assembly, with its wait: before a load from LDS
+// that the compiler makes it waits for every asynchronous load into LDS.
+__device__ __forceinline__ void read_all_rows(const unsigned char* tile, int block, int lane, r2o_u4 (&k)[8]) {
+    const int r = lane & 31;
+    const uint32_t a = lds_address(tile) + (32 * block + r) * 256 + 16 * ((lane >> 5) ^ (r & 15));
+    asm volatile(
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+        "ds_read_b128 %4, %12\n\tds_read_b128 %5, %13\n\tds_read_b128 %6, %14\n\tds_read_b128 %7, %15\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0]), "=&v"(k[1]), "=&v"(k[2]), "=&v"(k[3]), "=&v"(k[4]), "=&v"(k[5]), "=&v"(k[6]), "=&v"(k[7])
+        : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "v"(a ^ 128), "v"(a ^ 160), "v"(a ^ 192), "v"(a ^ 224)
+        : "memory");
 }
 
 // 16 keys from 16 kb on, transposed, as the A operand of channels 32 db ..: lane half h holds keys 4 h + 0..3 and
@@ -105,7 +135,7 @@ __device__ __forceinline__ bool not_finite(uint32_t bits16) {
 }
 
 // In a tile that some row of the workgroup sees in part, a masked key's probability is 0, but 0 times an infinite
-// or NaN value is NaN: such elements become zero before they reach LDS; true if there was one.
+// or NaN value is NaN: such elements become zero before any product; true if there was one.
 template <int RF>
 __device__ __forceinline__ bool zero_not_finite(r2o_u4 (&x)[4]) {
     constexpr uint32_t e = RF == 0 ? 0x7f807f80u : 0x7c007c00u, one = RF == 0 ? 0x00800080u : 0x04000400u;
@@ -184,11 +214,12 @@ __device__ __forceinline__ bool place(int block, int tiles, int splits, int pair
 // stand at 128 / group neighbouring positions, so its last tiles are masked in part for few of them, and a chunk of few
 // rows fills it.  grid: (row tiles x pairs of request and KV head, splits); with splits each takes a share of the key tiles and
 // leaves (maximum, sum, products) in scratch for prompt_join_kernel.
-// 16384 rows of 28 heads over 4: 2105 us, 914 TFLOP/s (bf16; a large library product reaches 1270 to 1380); 8192, 5003 and
-// 1231 rows of 32 heads with a window of 1024 and four sinks: 376 us (fp16); 257 rows of 16 heads over 4097 keys: 27 us in 7 splits and 7 for
-// the join.  Bound by what runs beside the matrix instructions: without LDS reads and writes the first takes 1463 us, without
-// the maximum as well 1070.  A wave of 64 rows reads half as much from LDS, but its 512 registers leave one wave a SIMD: 2693
-// us; 256 rows a workgroup (8 waves) 1953 against 2009, but 386 against 365 for the windowed batch and 39 against 33 for the 257 rows.
+// 16384 rows of 28 heads over 4: 1983 us, 970 TFLOP/s (bf16; a large library product reaches 1270 to 1380); 8192, 5003 and
+// 1231 rows of 32 heads with a window of 1024 and four sinks: 365 us (fp16); 257 rows of 16 heads over 4097 keys: 26 us in 7
+// splits and 7 for the join.  Bound by what runs beside the matrix instructions (staged through registers, the first took 2009
+// us, without LDS reads and writes 1463, without the maximum as well 1070).  A wave of 64 rows reads half as much from LDS,
+// but its 512 registers leave one wave a SIMD: 2693 us; 256 rows a workgroup (8 waves) 1953 against 2009, but 386 against
+// 365 for the windowed batch and 39 against 33 for the 257 rows.  All of a half's V operands read at once, as K's are: 2001.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     // K tiles t and t + 1, V tiles t to t + 2: two workgroups fill a compute unit's 160 KB
@@ -236,26 +267,34 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
 
     auto tile_key = [&](int it) { return (it < sink_tiles ? it : first + it - sink_tiles) * kTile; };
     auto seen_in_part = [&](int kt) { return !(kt + kTile - 1 <= wg_min && (kt > wg_max - window || kt + kTile <= sinks)); };
-    // The next tile but one is on its way into registers while this one is computed on, from the moment that the next
-    // one's have gone to LDS: 16384 rows of 28 heads take 2105 us, 2137 with the loads half a tile later.  Loads straight
-    // into LDS would save the registers, but the compiler waits for all of them before the transposing reads.
-    r2o_u4 kx[4], vx[4];
-    auto load = [&](int it) {
-        const int kt = tile_key(it);
-        load_rows<0>(kbase, k_row, kt, last, kx, wave, lane);
-        load_rows<1>(vbase, v_row, kt, last, vx, wave, lane);
-    };
+    // The next tile but one goes straight into LDS while the next one is computed on: K into the buffer that every wave
+    // has left behind the last barrier, V into the third one.  The transposing reads that follow wait for it, long after
+    // it went out.  16384 rows of 28 heads take 1983 us so, 2057 through registers.
     bool bad = false;
-    auto store = [&](int it, int v_at) {
-        if (seen_in_part(tile_key(it))) bad |= zero_not_finite<RF>(vx);
-        store_rows(k_lds[it & 1], kx, wave, lane);
-        store_rows(v_lds[v_at], vx, wave, lane);
+    auto stage = [&](int it, int v_at) {
+        stage_rows<0>(kbase, k_row, tile_key(it), last, k_lds[it & 1], wave, lane);
+        stage_rows<1>(vbase, v_row, tile_key(it), last, v_lds[v_at], wave, lane);
+    };
+    // this wave's rows of a staged tile that some row of the workgroup sees in part
+    auto clean = [&](int it, int v_at) {
+        if (!seen_in_part(tile_key(it))) return;
+        r2o_u4* at = reinterpret_cast<r2o_u4*>(v_lds[v_at] + 16 * wave * 256) + lane;
+        r2o_u4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = at[64 * i];
+        if (zero_not_finite<RF>(x)) {
+            bad = true;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) at[64 * i] = x[i];
+        }
     };
     // S^T of 32 keys x 32 rows
     auto products = [&](const unsigned char* kl, int sub) __attribute__((always_inline)) {
         f16v x = f16v{};
+        r2o_u4 k[8];
+        read_all_rows(kl, sub, lane, k);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) x = mfma32<RF>(read_rows(kl, sub, t, lane), q[t], x);
+        for (int t = 0; t < 8; ++t) x = mfma32<RF>(k[t], q[t], x);
         return x;
     };
     // masks, and the running maximum raised where it has to be
@@ -300,9 +339,10 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     // A tile is two halves of 32 keys; the products of the half that follows run beside the exponentials of the one
     // before it.
     if (begin < tiles) {
-        load(begin);
-        store(begin, 0);
-        if (begin + 1 < tiles) load(begin + 1);
+        stage(begin, 0);
+        if (begin + 1 < tiles) stage(begin + 1, 1);
+        wait_staged();
+        clean(begin, 0);
         __syncthreads();
         f16v even = products(k_lds[begin & 1], 0);
         for (int it = begin, v_at = 0; it < tiles; ++it) {
@@ -313,12 +353,13 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
             probabilities(even, pk);
             values(v_lds[v_at], 0, pk);
             top_of(odd, kt + 32);
-            if (it + 1 < tiles) store(it + 1, v_next);
-            if (it + 2 < tiles) load(it + 2);
+            wait_staged();
+            if (it + 1 < tiles) clean(it + 1, v_next);
             __syncthreads();  // the next tile is there; this one's V stays till every wave is past the next barrier
             even = products(k_lds[(it + 1) & 1], 0);  // behind the last tile: what lies there, not used
             probabilities(odd, pk);
             values(v_lds[v_at], 1, pk);
+            if (it + 2 < tiles) stage(it + 2, v_next == 2 ? 0 : v_next + 1);
             v_at = v_next;
         }
     }
@@ -460,7 +501,7 @@ __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
         int head = begin / per_head, row_tile = begin - head * per_head;
         auto load = [&](int h, int r) {
             lse_next = r2o_ldg(a.lse_in + ((int64_t)b * a.hq + kvh * group + h) * a.queries + min((first + r) * kTile + ((int)threadIdx.x & (kTile - 1)), s.q - 1));
-            load_rows<0>(a.query + b * a.q_batch + (kvh * group + h) * a.q_head, a.q_row, (first + r) * kTile, s.q - 1, qx, wave, lane);
+            load_rows(a.query + b * a.q_batch + (kvh * group + h) * a.q_head, a.q_row, (first + r) * kTile, s.q - 1, qx, wave, lane);
         };
         auto store = [&](int r, int q_at, int lse_at) {  // rows behind the request, and those that saw no key, give exp2(-inf)
             store_rows(q_lds[q_at], qx, wave, lane);
