@@ -510,8 +510,8 @@ __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count,
 }
 
 // Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: an even
-// share of all tiles each, whose slots' weights grow by their probabilities.  Bound by its launch and two round trips: 5
-// us for a call without weights, 11.6 for a ragged batch of 252 MB with them.
+// share of all tiles each, whose slots' weights grow by their probabilities.  Bound by its launch and its round trips: 5
+// us for a call without weights, 11.1 for a ragged batch of 252 MB with them.
 template <int RF>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
     Args& a = kernel_args();
