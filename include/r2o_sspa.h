@@ -501,7 +501,7 @@ typedef struct r2o_prompt_params {
 int r2o_prompt_attention(const r2o_prompt_params* p, void* stream);
 
 /* weights[b, h, j] = sum over KV head h's query heads and the rows that see key j of
- * exp(sm_scale q . k_j - lse_in); 0 behind a request's length.  Rows with lse_in -inf give nothing.  The sums of
+ * exp(sm_scale q . k_j - lse_in); 0 behind a request's length.  Finite rows with lse_in -inf give nothing.  The sums of
  * the splits are joined in order. */
 int r2o_attention_weights(const r2o_prompt_params* p, void* stream);
 
@@ -513,8 +513,9 @@ int r2o_attention_weights(const r2o_prompt_params* p, void* stream);
 
 /* Slot j of request b is slot j % page_size of page page_table[b][j / page_size], for every KV head; lengths[b]
  * slots are filled (clamped to max_pages * page_size).  Slots of a page id outside [0, pages) are not seen and not
- * written.  K and V rows as above with element strides (page, head, slot) below 2^31, the slots' at most 2^24; weight_pages (may be NULL): fp32 with
- * element strides (page, head), slots unit-strided. */
+ * written.  K and V rows as above with element strides (page, head, slot) below 2^31, the slots' at most 2^24;
+ * weight_pages (may be NULL): fp32 with element strides (page, head), slots unit-strided.  A page whose rows or weights are
+ * written stands in the tables once. */
 typedef struct r2o_paged_cache {
     uint16_t* key_pages;      /* [pages, hkv, page_size, 128] */
     uint16_t* value_pages;
@@ -565,7 +566,8 @@ int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream);
 
 /* Of each (request, KV head) of `source` that holds more than `keep` slots, the first `sinks`, the last `recent` and
  * those of largest weight stay (ties to the lower slot, NaN above all), in order; they are copied, with their
- * weights where the target keeps them, into slots 0.. of `target`, whose pages must not be the source's.
+ * weights where the target keeps them, into slots 0.. of `target`, whose pages must not be the source's (target_lengths
+ * must not overlap its lengths).
  * target_lengths[b] = min(lengths[b], keep), kept [batch, hkv, keep] = the source slots in order, then -1. */
 typedef struct r2o_paged_evict_params {
     r2o_paged_cache source, target;

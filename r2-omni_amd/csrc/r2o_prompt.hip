@@ -458,11 +458,12 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits
 // ----------------------------------------------------------------------------- attention weights
 constexpr int kWeightKeys = 256;  // keys of a workgroup: 4 waves of 64, whose rows stay in registers
 
-// A split takes a share of the (query head, 64-row tile) pairs that see the key tile; its sums go to `weights` ([splits, batch, hkv, keys]; the result itself where there is one split).  S = Q K^T: a lane
-// sums its own two keys.  A row tile is two halves of 32; the products of the half that follows run beside the
+// A split takes a share of the (query head, 64-row tile) pairs that see the key tile; its sums go to `weights` ([splits,
+// batch, hkv, keys]; the result itself where there is one split).  S = Q K^T: a lane sums its own two keys.  A row tile is two halves of 32; the products of the half that follows run beside the
 // exponentials of the one before it.  The sums carry what an addition rounds off along: 8192 terms of very different size.
 // Bound by vector instructions, of which an exponential, its argument and an addition a pair alone take 125 us of the
-// 169 that 8192 rows of 16 heads take over as many keys (813 TFLOP/s of products); with 32 keys a wave, that is twice the reads of Q, 320.  64 rows of 28 heads over 32641 keys: 30 us.
+// 169 that 8192 rows of 16 heads take over as many keys (813 TFLOP/s of products); with 32 keys a wave, that is twice the
+// reads of Q, 320.  64 rows of 28 heads over 32641 keys: 30 us.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     __shared__ __align__(16) unsigned char q_lds[2][kTileBytes];
