@@ -172,3 +172,58 @@ def test_evict_short_requests_of_long_tables():
     """What a lane holds goes by the request, not by what the table could hold."""
     cache = _cache(_cuda(), (20000, 4096, 4097, 16384, 16385, 50), 1, 128, BF16, seed=10, weights=True)
     _check_evict(cache, 100, 4, 20)
+
+
+def test_pages_whose_offsets_pass_32_bits():
+    """The same rows in a small pool and in one whose pages lie 2^30 elements apart: equal bits from every call."""
+    import r2omni_amd as ro
+
+    dev, n, page = _cuda(), 280, 64
+    small = _cache(dev, (n,), 2, page, BF16, seed=12, weights=True, spare=0)
+    pages, stride = small.key_pages.shape[0], 1 << 30
+    wide = []
+    for pool in (small.key_pages, small.value_pages):
+        big = torch.empty((pages - 1) * stride + 2 * page * 128, dtype=BF16, device=dev)
+        view = big.as_strided(pool.shape, (stride, page * 128, 128, 1))
+        view.copy_(pool)
+        wide.append(view)
+    assert 2 * (pages - 1) * stride > 1 << 32
+    table, lengths = small.page_table, small.lengths
+    large = ro.PagedCache(*wide, table, lengths.clone(), small.weight_pages.clone())
+    q, new = _query(dev, 1, 8, BF16, 12), _append(dev, 1, 2, BF16, 12)
+    k, v = (torch.randn(1, 2, 70, 128, device=dev).to(BF16) for _ in range(2))
+    results = []
+    for cache in (small, large):
+        ro.paged_extend(cache, k, v, weights=torch.ones(1, 2, 70, device=dev))
+        out = ro.paged_attention(q, cache, append=new)
+        target = _cache(dev, (64,), 2, page, BF16, seed=13, weights=True)
+        kept = ro.paged_evict(cache, target, 64, sinks=2, recent=5)
+        results.append((*out, kept, target.key_pages.view(torch.int16), target.value_pages.view(torch.int16), target.weight_pages[:1]))
+    torch.cuda.synchronize()
+    for x, y in zip(*results):
+        assert torch.equal(x, y) or (x.is_floating_point() and torch.equal(x.nan_to_num(), y.nan_to_num()))
+    for pool, view in zip((small.key_pages, small.value_pages), wide):
+        assert torch.equal(pool.view(torch.int16), view.contiguous().view(torch.int16))
+
+
+def test_requests_whose_offsets_pass_32_bits():
+    """A prompt's requests 2^31 elements apart, and rows 2^24 apart: the bits of compact ones."""
+    import r2omni_amd as ro
+
+    q, k, v = _rows(_cuda(), 2, 4, 2, 90, 200, BF16, seed=13)
+    want = ro.prompt_attention(q, k, v)
+    weights = ro.attention_weights(q, k, want[1])
+
+    def spread(t, strides):
+        big = torch.empty(sum((n - 1) * s for n, s in zip(t.shape, strides)) + 1, dtype=t.dtype, device=t.device)
+        view = big.as_strided(t.shape, strides)
+        view.copy_(t)
+        return view
+
+    for far in ((1 << 31, 200 * 128, 128, 1), (128, 256, 1 << 24, 1)):
+        k2, v2 = spread(k, far), spread(v, far)
+        q2 = spread(q, (1 << 31, 90 * 128, 128, 1))
+        got = ro.prompt_attention(q2, k2, v2)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert torch.equal(ro.attention_weights(q2, k2, got[1]), weights)
+        del k2, v2, q2
