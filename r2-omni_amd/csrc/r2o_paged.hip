@@ -132,7 +132,8 @@ __device__ __forceinline__ Tiles tiles_of(Args& a, int length) {
 struct Share {
     int total, workers, each, more;
     __device__ __forceinline__ int begin(int i) const { return i * each + min(i, more); }
-    __device__ __forceinline__ int worker(int u) const {  // the one that takes tile u
+    __device__ __forceinline__ int worker(int at) const {  // the one that takes tile `at`, or the last tile
+        const int u = min(at, total - 1);
         const int wide = more * (each + 1);
         return u < wide ? (int)((uint32_t)u / (uint32_t)(each + 1)) : more + (int)((uint32_t)(u - wide) / (uint32_t)each);
     }
@@ -162,10 +163,10 @@ __device__ __forceinline__ Share make_share(Args& a) {
     return s;
 }
 
-// The request that holds tile u, and the tiles before it.
+// The request that holds tile u, and the tiles before it; `batch` if lengths that change meanwhile leave none.
 __device__ __forceinline__ int request_of(Args& a, int u, int& before) {
     before = 0;
-    for (int b0 = 0;; b0 += 64) {
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Lane x = lane_tiles(a, b0);
         const int all = __builtin_amdgcn_readlane(x.upto, 63) * a.hkv;
         if (u < before + all) {
@@ -175,6 +176,7 @@ __device__ __forceinline__ int request_of(Args& a, int u, int& before) {
         }
         before += all;
     }
+    return a.batch;
 }
 
 // The tiles of the requests before b.
@@ -288,13 +290,15 @@ __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
         u = share.begin(worker);
         u_end = share.begin(worker + 1);
         b = request_of(a, u, base);
+        if (b >= a.batch) return;
     }
     while (u < u_end) {
         Args& a = kernel_args();
         Tiles t = tiles_of(a, load_uniform(a.lengths + b));
         while (u >= base + t.count * a.hkv) {
             base += t.count * a.hkv;
-            t = tiles_of(a, load_uniform(a.lengths + ++b));
+            if (++b >= a.batch) return;
+            t = tiles_of(a, load_uniform(a.lengths + b));
         }
         const int h = (int)((uint32_t)(u - base) / (uint32_t)t.count), pair_base = base + h * t.count;
         const int t0 = u - pair_base, t1 = min(t.count, u_end - pair_base), group = a.group, sinks = min(a.sinks, t.n);
@@ -526,7 +530,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
         const Tiles t = tiles_of(a, load_uniform(a.lengths + b));
         float* lse = a.lse + blockIdx.x;
         uint16_t* dst = a.out + (int64_t)blockIdx.x * 128;
-        if (t.count == 0) {
+        if (t.count == 0 || share.total == 0) {
             if (threadIdx.x < 64) reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = 0;
             if (threadIdx.x == 0) *lse = -INFINITY;
             return;
@@ -577,11 +581,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
     if (u >= u_end) return;
     int base;
     int b = request_of(a, u, base);
+    if (b >= a.batch) return;
     Tiles t = tiles_of(a, load_uniform(a.lengths + b));
     while (u < u_end) {
         while (u >= base + t.count * hkv) {
             base += t.count * hkv;
-            t = tiles_of(a, load_uniform(a.lengths + ++b));
+            if (++b >= a.batch) return;
+            t = tiles_of(a, load_uniform(a.lengths + b));
         }
         const int h = (int)((uint32_t)(u - base) / (uint32_t)t.count), pair_base = base + h * t.count;
         const int stop = min(pair_base + t.count, u_end);
@@ -863,11 +869,12 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
     int sure_at = waves_before(before[lane % kSelectWaves][0], wave, sure_all);
     int equal_at = waves_before(before[lane % kSelectWaves][1], wave, equal_all);
     const int still = keep - sure_all;  // of the equal ones; 0 where just `keep` reached
+    if (still < 0) return;  // rows read again have changed meanwhile: no place is left for the answer
     // values of their own: the comparisons above are made again, not kept
     uint32_t above = (uint32_t)__builtin_amdgcn_readfirstlane((int)t), same = (uint32_t)__builtin_amdgcn_readfirstlane((int)equal);
     asm volatile("" : "+s"(above), "+s"(same), "+v"(from));
     auto write_all = [&](auto ties) {
-        auto write = [&](int j, const uint32_t (&k)[4]) {
+        auto write = [&](int j, const uint32_t (&k)[4], auto again) {
             int mine = 0;  // sure ones, and equal ones above 16 bits
 #pragma unroll
             for (int x = 0; x < 4; ++x) mine += (k[x] > above ? 1 : 0) + (ties && k[x] == same ? 1 << 16 : 0);
@@ -876,7 +883,8 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const bool sure = k[x] > above, eq = ties && k[x] == same;
-                if (sure || (eq && e < still)) kept[ties ? s + min(e, still) : s] = j + x;
+                const int to = ties ? s + min(e, still) : s;
+                if ((sure || (eq && e < still)) && (!again || to < keep)) kept[to] = j + x;
                 s += sure ? 1 : 0;
                 e += eq ? 1 : 0;
             }
@@ -885,11 +893,11 @@ __device__ __forceinline__ void select_row(const r2o_paged_evict_params& p, Sele
             __builtin_amdgcn_sched_barrier(0);
         };
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) write(from + 256 * i, keys[i]);
+        for (int i = 0; i < kQuads; ++i) write(from + 256 * i, keys[i], std::false_type());
         for (int i = kQuads; i < quads; ++i) {
             uint32_t k[4];
             quad_at(from + 256 * i, k);
-            write(from + 256 * i, k);
+            write(from + 256 * i, k, std::true_type());
         }
     };
     if (equal) write_all(std::true_type());
@@ -921,7 +929,7 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(r2o_paged_evict_para
     const int h = blockIdx.y, b = blockIdx.z, l16 = threadIdx.x & 15, i = blockIdx.x * 16 + (threadIdx.x >> 4);
     if (i >= (int)p.keep || i >= (int)(o.max_pages * o.page_size)) return;
     const int j = r2o_ldg(p.kept + ((int64_t)b * c.hkv + h) * p.keep + i);
-    if (j < 0) return;
+    if ((uint32_t)j >= (uint32_t)(c.max_pages * c.page_size)) return;  // -1 behind the request's length
     const int shift = shift_of(c), to_shift = shift_of(o), at = j & ((1 << shift) - 1), to_at = i & ((1 << to_shift) - 1);
     const int page = page_of(c, b, j, shift), to = page_of(o, b, i, to_shift);
     if (to < 0) return;
