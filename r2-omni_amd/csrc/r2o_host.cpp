@@ -538,41 +538,60 @@ PyObject* weights_call(PyObject* const* args) {
     return status_and(launch_on(args[0], p, device), {out});
 }
 
-// paged_cache(key pages, value pages, page table, lengths, weight pages or None): the r2o_paged_cache as bytes, or None
-PyObject* paged_cache_call(PyObject* const* args) {
-    const at::Tensor *k = exact_tensor(args[0]), *v = exact_tensor(args[1]), *table = exact_tensor(args[2]), *n = exact_tensor(args[3]);
-    const at::Tensor* w = args[4] == Py_None ? nullptr : exact_tensor(args[4]);
-    if (!k || !v || !table || !n || (args[4] != Py_None && !w) || k->dim() != 4 || k->device().type() != at::kCUDA) Py_RETURN_NONE;
-    const int64_t device = k->device().index();
+PyObject* const kCacheFields[5] = {PyUnicode_InternFromString("key_pages"), PyUnicode_InternFromString("value_pages"),
+                                   PyUnicode_InternFromString("page_table"), PyUnicode_InternFromString("lengths"),
+                                   PyUnicode_InternFromString("weight_pages")};
+
+// A PagedCache's tensors, held for a call, and where they lie now: nothing is kept from its making, so a copy, a loaded
+// one and one whose tensors got other memory are what they say.
+struct Cache {
+    PyObject* fields[5] = {};
     r2o_paged_cache c{};
+    int64_t device = -1;
+    ~Cache() {
+        for (PyObject* o : fields) Py_XDECREF(o);
+    }
+    bool read(PyObject* cache);  // false for what the Python path has to look at
+};
+
+bool Cache::read(PyObject* cache) {
+    for (int i = 0; i < 5; ++i)
+        if (!(fields[i] = PyObject_GetAttr(cache, kCacheFields[i]))) {
+            PyErr_Clear();
+            return false;
+        }
+    const at::Tensor *k = exact_tensor(fields[0]), *v = exact_tensor(fields[1]), *table = exact_tensor(fields[2]), *n = exact_tensor(fields[3]);
+    const at::Tensor* w = fields[4] == Py_None ? nullptr : exact_tensor(fields[4]);
+    if (!k || !v || !table || !n || (fields[4] != Py_None && !w) || k->dim() != 4 || k->device().type() != at::kCUDA) return false;
+    device = k->device().index();
     c.pages = k->size(0);
     c.hkv = k->size(1);
     c.page_size = k->size(2);
     c.dtype = row_code(*k);
     for (const at::Tensor* t : {k, v, table, n})
-        if (!on_device(*t, device)) Py_RETURN_NONE;
+        if (!on_device(*t, device)) return false;
     if (c.dtype < 0 || k->size(3) != R2O_HEAD_DIM || c.pages < 1 || c.pages > 0x7fffffff || c.hkv < 1 || c.hkv > 1024 ||
         v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() ||
         (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128))
-        Py_RETURN_NONE;
-    if (!row_strides(*k, 3, c.key_strides, true) || !row_strides(*v, 3, c.value_strides, true)) Py_RETURN_NONE;
+        return false;
+    if (!row_strides(*k, 3, c.key_strides, true) || !row_strides(*v, 3, c.value_strides, true)) return false;
     for (int i = 0; i < 3; ++i)
-        if (std::max(c.key_strides[i], c.value_strides[i]) > (i == 2 ? R2O_PAGED_MAX_SLOT_STRIDE : 0x7fffffff)) Py_RETURN_NONE;
+        if (std::max(c.key_strides[i], c.value_strides[i]) > (i == 2 ? R2O_PAGED_MAX_SLOT_STRIDE : 0x7fffffff)) return false;
     if (table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) < 1 || table->size(1) < 1 ||
         (table->size(1) > 1 && table->stride(1) != 1) || n->scalar_type() != at::kInt || n->dim() != 1 || n->size(0) != table->size(0) ||
         !n->is_contiguous())
-        Py_RETURN_NONE;
+        return false;
     c.batch = table->size(0);
     c.max_pages = table->size(1);
     c.table_stride = std::max(table->stride(0), c.max_pages);
-    if (c.batch > R2O_PAGED_MAX_BATCH || c.max_pages * c.page_size > (1 << 29) || c.table_stride > 0x7fffffff) Py_RETURN_NONE;
+    if (c.batch > R2O_PAGED_MAX_BATCH || c.max_pages * c.page_size > (1 << 29) || c.table_stride > 0x7fffffff) return false;
     if (w) {
         if (!on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != c.pages || w->size(1) != c.hkv ||
             w->size(2) != c.page_size || w->stride(2) != 1)
-            Py_RETURN_NONE;
+            return false;
         for (int i = 0; i < 2; ++i) {
             c.weight_strides[i] = w->size(i) > 1 ? w->stride(i) : 0;
-            if (w->size(i) > 1 && (c.weight_strides[i] < 1 || c.weight_strides[i] > 0x7fffffff)) Py_RETURN_NONE;
+            if (w->size(i) > 1 && (c.weight_strides[i] < 1 || c.weight_strides[i] > 0x7fffffff)) return false;
         }
         c.weight_pages = w->data_ptr<float>();
     }
@@ -580,37 +599,38 @@ PyObject* paged_cache_call(PyObject* const* args) {
     c.value_pages = static_cast<uint16_t*>(v->data_ptr());
     c.page_table = table->data_ptr<int32_t>();
     c.lengths = n->data_ptr<int32_t>();
-    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&c), sizeof(c));
+    return true;
 }
 
-// The cache's fields, if its tensors lie on the current device.
-bool cache_arg(PyObject* bytes, PyObject* keys, r2o_paged_cache& c, int64_t& device) {
-    const at::Tensor* k = exact_tensor(keys);
-    device = current_device();
-    if (!PyBytes_CheckExact(bytes) || PyBytes_GET_SIZE(bytes) != (Py_ssize_t)sizeof(c) || !k || !on_device(*k, device)) return false;
-    std::memcpy(&c, PyBytes_AS_STRING(bytes), sizeof(c));
-    return true;
+// paged_cache(cache): True if its tensors need no look by the Python path, or None
+PyObject* paged_cache_call(PyObject* const* args) {
+    Cache cache;
+    if (!cache.read(args[0])) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
 }
 
 bool cache_rows(const at::Tensor* t, const r2o_paged_cache& c, int64_t device) {
     return t && on_device(*t, device) && row_code(*t) == c.dtype && !needs_grad(*t);
 }
 
-// paged_extend(function, cache, key pages, key, value, counts, weights): (status,) or None
+// paged_extend(function, cache, key, value, counts, weights): (status,) or None
 PyObject* paged_extend_call(PyObject* const* args) {
     r2o_paged_extend_params p{};
-    int64_t device;
-    const at::Tensor *k = exact_tensor(args[3]), *v = exact_tensor(args[4]);
-    if (!cache_arg(args[1], args[2], p.cache, device) || !cache_rows(k, p.cache, device) || !cache_rows(v, p.cache, device) ||
+    Cache cache;
+    const at::Tensor *k = exact_tensor(args[2]), *v = exact_tensor(args[3]);
+    if (!cache.read(args[1]) || cache.device != current_device()) Py_RETURN_NONE;
+    const int64_t device = cache.device;
+    p.cache = cache.c;
+    if (!cache_rows(k, p.cache, device) || !cache_rows(v, p.cache, device) ||
         k->dim() != 4 || k->size(0) != p.cache.batch || k->size(1) != p.cache.hkv || k->size(3) != R2O_HEAD_DIM || v->sizes() != k->sizes())
         Py_RETURN_NONE;
     p.rows = k->size(2);
     if (p.rows < 1 || p.rows > p.cache.max_pages * p.cache.page_size || !row_strides(*k, 3, p.key_strides) ||
         !row_strides(*v, 3, p.value_strides) || p.key_strides[2] > R2O_MAX_ROW_STRIDE || p.value_strides[2] > R2O_MAX_ROW_STRIDE ||
-        !lengths_arg(args[5], p.cache.batch, device, p.counts))
+        !lengths_arg(args[4], p.cache.batch, device, p.counts))
         Py_RETURN_NONE;
-    if (args[6] != Py_None) {
-        const at::Tensor* w = exact_tensor(args[6]);
+    if (args[5] != Py_None) {
+        const at::Tensor* w = exact_tensor(args[5]);
         if (!w || !p.cache.weight_pages || !on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 ||
             w->size(0) != k->size(0) || w->size(1) != k->size(1) || w->size(2) != k->size(2) || !w->is_contiguous())
             Py_RETURN_NONE;
@@ -623,24 +643,27 @@ PyObject* paged_extend_call(PyObject* const* args) {
     return status_and(launch_on(args[0], p, device), {});
 }
 
-// paged_attention(function, cache, key pages, query, append or None, window, sinks, scale): (status, out, lse) or None
+// paged_attention(function, cache, query, append or None, window, sinks, scale): (status, out, lse) or None
 PyObject* paged_attention_call(PyObject* const* args) {
     r2o_paged_attention_params p{};
     r2o_paged_cache& c = p.cache;
-    int64_t device;
-    const at::Tensor* q = exact_tensor(args[3]);
-    if (!cache_arg(args[1], args[2], c, device) || !cache_rows(q, c, device) ||
+    Cache cache;
+    const at::Tensor* q = exact_tensor(args[2]);
+    if (!cache.read(args[1]) || cache.device != current_device()) Py_RETURN_NONE;
+    const int64_t device = cache.device;
+    c = cache.c;
+    if (!cache_rows(q, c, device) ||
         !(q->dim() == 3 || (q->dim() == 4 && q->size(2) == 1)) || q->size(0) != c.batch || q->size(-1) != R2O_HEAD_DIM)
         Py_RETURN_NONE;
     p.hq = q->size(1);
     if (p.hq < 1 || p.hq % c.hkv || p.hq / c.hkv > R2O_MAX_GQA || !row_strides(*q, 2, p.query_strides) ||
-        !mask_args(args[5], args[6], args[7], p.window, p.sinks, p.sm_scale) ||
+        !mask_args(args[4], args[5], args[6], p.window, p.sinks, p.sm_scale) ||
         std::max(p.query_strides[0], p.query_strides[1]) > 0x7fffffff)
         Py_RETURN_NONE;
-    if (args[4] != Py_None) {
-        if (!PyTuple_CheckExact(args[4]) || PyTuple_GET_SIZE(args[4]) != 2) Py_RETURN_NONE;
+    if (args[3] != Py_None) {
+        if (!PyTuple_CheckExact(args[3]) || PyTuple_GET_SIZE(args[3]) != 2) Py_RETURN_NONE;
         for (int i = 0; i < 2; ++i) {
-            const at::Tensor* t = exact_tensor(PyTuple_GET_ITEM(args[4], i));
+            const at::Tensor* t = exact_tensor(PyTuple_GET_ITEM(args[3], i));
             if (!cache_rows(t, c, device) || !(t->dim() == 3 || (t->dim() == 4 && t->size(2) == 1)) || t->size(0) != c.batch ||
                 t->size(1) != c.hkv || t->size(-1) != R2O_HEAD_DIM || !row_strides(*t, 2, p.append_strides + 2 * i) ||
                 std::max(p.append_strides[2 * i], p.append_strides[2 * i + 1]) > 0x7fffffff)
@@ -665,24 +688,23 @@ PyObject* paged_attention_call(PyObject* const* args) {
     return status_and(launch_on(args[0], p, device), {out, lse});
 }
 
-// paged_evict(function, cache, key pages, target, target's key pages, target's lengths, keep, sinks, recent): (status,
-// kept) or None
+// paged_evict(function, cache, target, keep, sinks, recent): (status, kept) or None
 PyObject* paged_evict_call(PyObject* const* args) {
     r2o_paged_evict_params p{};
-    int64_t device;
-    const at::Tensor* lengths = exact_tensor(args[5]);
-    if (!cache_arg(args[1], args[2], p.source, device) || !cache_arg(args[3], args[4], p.target, device) || !lengths ||
-        !plain_int(args[6], p.keep) || !plain_int(args[7], p.sinks) || !plain_int(args[8], p.recent))
+    Cache source, target;
+    if (!source.read(args[1]) || !target.read(args[2]) || source.device != target.device || source.device != current_device() ||
+        !plain_int(args[3], p.keep) || !plain_int(args[4], p.sinks) || !plain_int(args[5], p.recent))
         Py_RETURN_NONE;
-    const r2o_paged_cache &c = p.source, &o = p.target;
+    const r2o_paged_cache &c = p.source = source.c, &o = p.target = target.c;
     if (!c.weight_pages || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || std::abs(c.lengths - o.lengths) < c.batch ||
         c.page_table == o.page_table || p.keep < 1 || p.keep > o.max_pages * o.page_size || p.sinks < 0 || p.recent < 0 ||
         p.sinks + p.recent > p.keep)
         Py_RETURN_NONE;
-    at::Tensor kept = at::empty({c.batch, c.hkv, p.keep}, lengths->options());
+    const at::Tensor& lengths = THPVariable_Unpack(target.fields[3]);
+    at::Tensor kept = at::empty({c.batch, c.hkv, p.keep}, lengths.options());
     p.kept = kept.data_ptr<int32_t>();
-    p.target_lengths = lengths->data_ptr<int32_t>();
-    return status_and(launch_on(args[0], p, device), {kept});
+    p.target_lengths = lengths.data_ptr<int32_t>();
+    return status_and(launch_on(args[0], p, source.device), {kept});
 }
 
 template <PyObject* (*CALL)(PyObject* const*), Py_ssize_t N>
@@ -722,10 +744,10 @@ PyMethodDef kMethods[] = {
     {"cache_build", cache_build, METH_VARARGS, nullptr},
     {"prompt", FAST(prompt_call, 9)},
     {"weights", FAST(weights_call, 9)},
-    {"paged_cache", FAST(paged_cache_call, 5)},
-    {"paged_extend", FAST(paged_extend_call, 7)},
-    {"paged_attention", FAST(paged_attention_call, 8)},
-    {"paged_evict", FAST(paged_evict_call, 9)},
+    {"paged_cache", FAST(paged_cache_call, 1)},
+    {"paged_extend", FAST(paged_extend_call, 6)},
+    {"paged_attention", FAST(paged_attention_call, 7)},
+    {"paged_evict", FAST(paged_evict_call, 6)},
     {"attention_splits", rule7<attention_splits>, METH_VARARGS, nullptr},
     {"weight_splits", weight_splits_rule, METH_VARARGS, nullptr},
     {"paged_workers", paged_workers_rule, METH_VARARGS, nullptr},

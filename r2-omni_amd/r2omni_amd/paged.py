@@ -15,7 +15,7 @@ keeps no unpacked cache once a prompt is packed.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 
@@ -34,7 +34,7 @@ def _pool_ok(t: torch.Tensor) -> bool:
 
 @dataclass(frozen=True, eq=False)
 class PagedCache:
-    """Views of the tensors that hold one layer's cache; the calls write them in place.
+    """The tensors that hold one layer's cache; the calls write them in place, where they lie at the time of the call.
 
     Slot j of request b is slot ``j % page_size`` of page ``page_table[b, j // page_size]``, for every KV head, and
     the first ``lengths[b]`` slots are filled.  A page id outside the pool (such as -1 for a page not handed out)
@@ -47,40 +47,10 @@ class PagedCache:
     page_table: torch.Tensor                    # int32 [B, max_pages]
     lengths: torch.Tensor                       # int32 [B]
     weight_pages: torch.Tensor | None = None    # fp32 [pages, Hkv, page_size]: accumulated attention weight
-    _c: bytes = field(init=False, repr=False)  # r2o_paged_cache
 
     def __post_init__(self) -> None:
-        k, v, table, n, w = self.key_pages, self.value_pages, self.page_table, self.lengths, self.weight_pages
-        made = _lib.host().paged_cache(k, v, table, n, w)
-        if made is not None:
-            object.__setattr__(self, "_c", made)
-            return
-        if k.ndim != 4 or k.shape[-1] != 128 or min(k.shape) < 1 or v.shape != k.shape:
-            raise ValueError("paged cache needs key and value pages [pages,Hkv,page_size,128] of one shape")
-        if k.shape[2] not in PAGE_SIZES:
-            raise ValueError("page_size must be one of 16, 32, 64, or 128")
-        dtype = _lib.dtype_code(k.dtype)
-        if v.dtype != k.dtype or any(t.device != k.device for t in (v, table, n)):
-            raise ValueError("paged cache tensors must share a device and K/V a dtype")
-        if not _pool_ok(k) or not _pool_ok(v):
-            raise ValueError("paged cache pages need unit channel stride and 16-byte aligned rows of their own")
-        if table.dtype != torch.int32 or table.ndim != 2 or min(table.shape) < 1 or table.stride(1) != 1 and table.shape[1] > 1:
-            raise ValueError("page_table must be int32 [B,max_pages] with unit-strided rows")
-        if n.dtype != torch.int32 or tuple(n.shape) != (table.shape[0],) or not n.is_contiguous():
-            raise ValueError("lengths must be contiguous int32 [B]")
-        if table.shape[0] > MAX_BATCH or table.shape[1] * k.shape[2] > 1 << 29 or k.shape[0] >= 1 << 31 or k.shape[1] > 1024 \
-                or table.stride(0) >= 1 << 31:
-            raise ValueError("paged cache takes at most 1024 requests, 1024 heads and 2^29 slots a request")
-        if w is not None and (w.shape != k.shape[:3] or w.dtype != torch.float32 or w.device != k.device
-                              or any(not 0 < st < 1 << 31 for st, size in zip(w.stride(), w.shape) if size > 1) or w.stride(2) != 1):
-            raise ValueError("weight_pages must be fp32 [pages,Hkv,page_size] on the cache's device with unit-strided slots")
-        _lib.require_device(k, "paged cache")
-        object.__setattr__(self, "_c", bytes(_lib.PagedCacheParams(
-            key_pages=k.data_ptr(), value_pages=v.data_ptr(), weight_pages=_lib.ptr(w), page_table=table.data_ptr(),
-            lengths=n.data_ptr(), key_strides=_strides(k, 3), value_strides=_strides(v, 3),
-            weight_strides=(0, 0) if w is None else _strides(w, 2), table_stride=max(table.stride(0), table.shape[1]),
-            pages=k.shape[0], max_pages=table.shape[1], page_size=k.shape[2], batch=table.shape[0], hkv=k.shape[1],
-            dtype=dtype)))
+        if _lib.host().paged_cache(self) is None:
+            _params_of(self)
 
     @property
     def capacity(self) -> int:
@@ -89,7 +59,35 @@ class PagedCache:
 
 
 def _params_of(cache: PagedCache) -> _lib.PagedCacheParams:
-    return _lib.PagedCacheParams.from_buffer_copy(cache._c)
+    """Where the cache's tensors lie now, checked.  Nothing is kept from one call for the next: a copied cache has tensors
+    of its own, and ``t.data = ...`` gives one other memory."""
+    k, v, table, n, w = cache.key_pages, cache.value_pages, cache.page_table, cache.lengths, cache.weight_pages
+    if k.ndim != 4 or k.shape[-1] != 128 or min(k.shape) < 1 or v.shape != k.shape:
+        raise ValueError("paged cache needs key and value pages [pages,Hkv,page_size,128] of one shape")
+    if k.shape[2] not in PAGE_SIZES:
+        raise ValueError("page_size must be one of 16, 32, 64, or 128")
+    dtype = _lib.dtype_code(k.dtype)
+    if v.dtype != k.dtype or any(t.device != k.device for t in (v, table, n)):
+        raise ValueError("paged cache tensors must share a device and K/V a dtype")
+    if not _pool_ok(k) or not _pool_ok(v):
+        raise ValueError("paged cache pages need unit channel stride and 16-byte aligned rows of their own")
+    if table.dtype != torch.int32 or table.ndim != 2 or min(table.shape) < 1 or table.stride(1) != 1 and table.shape[1] > 1:
+        raise ValueError("page_table must be int32 [B,max_pages] with unit-strided rows")
+    if n.dtype != torch.int32 or tuple(n.shape) != (table.shape[0],) or not n.is_contiguous():
+        raise ValueError("lengths must be contiguous int32 [B]")
+    if table.shape[0] > MAX_BATCH or table.shape[1] * k.shape[2] > 1 << 29 or k.shape[0] >= 1 << 31 or k.shape[1] > 1024 \
+            or table.stride(0) >= 1 << 31:
+        raise ValueError("paged cache takes at most 1024 requests, 1024 heads and 2^29 slots a request")
+    if w is not None and (w.shape != k.shape[:3] or w.dtype != torch.float32 or w.device != k.device
+                          or any(not 0 < st < 1 << 31 for st, size in zip(w.stride(), w.shape) if size > 1) or w.stride(2) != 1):
+        raise ValueError("weight_pages must be fp32 [pages,Hkv,page_size] on the cache's device with unit-strided slots")
+    _lib.require_device(k, "paged cache")
+    return _lib.PagedCacheParams(
+        key_pages=k.data_ptr(), value_pages=v.data_ptr(), weight_pages=_lib.ptr(w), page_table=table.data_ptr(),
+        lengths=n.data_ptr(), key_strides=_strides(k, 3), value_strides=_strides(v, 3),
+        weight_strides=(0, 0) if w is None else _strides(w, 2), table_stride=max(table.stride(0), table.shape[1]),
+        pages=k.shape[0], max_pages=table.shape[1], page_size=k.shape[2], batch=table.shape[0], hkv=k.shape[1],
+        dtype=dtype)
 
 
 def _check_new_rows(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, what: str) -> None:
@@ -109,7 +107,7 @@ def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, c
     ``cache.lengths`` already counts them: row i of request b goes to slot ``lengths[b] - n + i``, where n is S or,
     for a padded batch, ``counts[b]`` (int32 [B]; rows behind it are not used).  Where the cache keeps weights, the
     slots get ``weights`` (fp32 [B, Hkv, S], as ``attention_weights`` returns them) or 0."""
-    made = _lib.host().paged_extend(_lib.entry("r2o_paged_extend"), cache._c, cache.key_pages, key, value, counts, weights)
+    made = _lib.host().paged_extend(_lib.entry("r2o_paged_extend"), cache, key, value, counts, weights)
     if made is not None:
         return _lib.check(made[0], "r2o_paged_extend")
     batch, hkv = int(cache.page_table.shape[0]), int(cache.key_pages.shape[1])
@@ -146,8 +144,7 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
     ``dataclasses.replace(cache, weight_pages=None)`` leaves them alone.  A request that sees no slot (an idle one of
     length 0) gets 0 and lse -inf.  ``output``: the two contiguous result tensors."""
     if output is None:
-        made = _lib.host().paged_attention(_lib.entry("r2o_paged_attention"), cache._c, cache.key_pages, query, append, window,
-                                           sinks, sm_scale)
+        made = _lib.host().paged_attention(_lib.entry("r2o_paged_attention"), cache, query, append, window, sinks, sm_scale)
         if made is not None:
             _lib.check(made[0], "r2o_paged_attention")
             return made[1], made[2]
@@ -215,8 +212,7 @@ def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int 
     ``weight_pages``.  The target may lie in the same pools, in pages that the source's table does not name; the
     source is left as it is, for its pages to be handed back.  Returns the kept source slots, int32 [B, Hkv, keep]
     in ascending order, -1 behind a request's length."""
-    made = _lib.host().paged_evict(_lib.entry("r2o_paged_evict"), cache._c, cache.key_pages, target._c, target.key_pages,
-                                   target.lengths, keep, sinks, recent)
+    made = _lib.host().paged_evict(_lib.entry("r2o_paged_evict"), cache, target, keep, sinks, recent)
     if made is not None:
         _lib.check(made[0], "r2o_paged_evict")
         return made[1]
