@@ -520,7 +520,7 @@ typedef struct r2o_paged_cache {
     uint16_t* key_pages;      /* [pages, hkv, page_size, 128] */
     uint16_t* value_pages;
     float* weight_pages;      /* [pages, hkv, page_size] */
-    const int32_t* page_table; /* [batch, max_pages], rows table_stride apart */
+    const int32_t* page_table; /* [batch, max_pages], rows table_stride apart; 0: one row for all, whose pages no call writes */
     const int32_t* lengths;   /* [batch] */
     int64_t key_strides[3], value_strides[3], weight_strides[2];
     int64_t table_stride, pages, max_pages, page_size, batch, hkv, dtype;

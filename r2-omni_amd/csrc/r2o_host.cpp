@@ -583,7 +583,8 @@ bool Cache::read(PyObject* cache) {
         return false;
     c.batch = table->size(0);
     c.max_pages = table->size(1);
-    c.table_stride = std::max(table->stride(0), c.max_pages);
+    c.table_stride = c.batch > 1 ? table->stride(0) : c.max_pages;
+    if (c.table_stride && c.table_stride < c.max_pages) return false;  // rows that overlap
     if (c.batch > R2O_PAGED_MAX_BATCH || c.max_pages * c.page_size > (1 << 29) || c.table_stride > 0x7fffffff) return false;
     if (w) {
         if (!on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != c.pages || w->size(1) != c.hkv ||
@@ -601,6 +602,9 @@ bool Cache::read(PyObject* cache) {
     c.lengths = n->data_ptr<int32_t>();
     return true;
 }
+
+// One row of page ids for all requests (an expanded table): their pages may be read, not written.
+bool one_row(const r2o_paged_cache& c) { return c.batch > 1 && c.table_stride == 0; }
 
 // paged_cache(cache): True if its tensors need no look by the Python path, or None
 PyObject* paged_cache_call(PyObject* const* args) {
@@ -621,6 +625,7 @@ PyObject* paged_extend_call(PyObject* const* args) {
     if (!cache.read(args[1]) || cache.device != current_device()) Py_RETURN_NONE;
     const int64_t device = cache.device;
     p.cache = cache.c;
+    if (one_row(p.cache)) Py_RETURN_NONE;
     if (!cache_rows(k, p.cache, device) || !cache_rows(v, p.cache, device) ||
         k->dim() != 4 || k->size(0) != p.cache.batch || k->size(1) != p.cache.hkv || k->size(3) != R2O_HEAD_DIM || v->sizes() != k->sizes())
         Py_RETURN_NONE;
@@ -652,6 +657,7 @@ PyObject* paged_attention_call(PyObject* const* args) {
     if (!cache.read(args[1]) || cache.device != current_device()) Py_RETURN_NONE;
     const int64_t device = cache.device;
     c = cache.c;
+    if (one_row(c) && (c.weight_pages || args[3] != Py_None)) Py_RETURN_NONE;
     if (!cache_rows(q, c, device) ||
         !(q->dim() == 3 || (q->dim() == 4 && q->size(2) == 1)) || q->size(0) != c.batch || q->size(-1) != R2O_HEAD_DIM)
         Py_RETURN_NONE;
@@ -696,7 +702,7 @@ PyObject* paged_evict_call(PyObject* const* args) {
         !plain_int(args[3], p.keep) || !plain_int(args[4], p.sinks) || !plain_int(args[5], p.recent))
         Py_RETURN_NONE;
     const r2o_paged_cache &c = p.source = source.c, &o = p.target = target.c;
-    if (!c.weight_pages || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || std::abs(c.lengths - o.lengths) < c.batch ||
+    if (!c.weight_pages || one_row(o) || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || std::abs(c.lengths - o.lengths) < c.batch ||
         c.page_table == o.page_table || p.keep < 1 || p.keep > o.max_pages * o.page_size || p.sinks < 0 || p.recent < 0 ||
         p.sinks + p.recent > p.keep)
         Py_RETURN_NONE;

@@ -961,18 +961,21 @@ bool cache_ok(const r2o_paged_cache& c) {
     return slots_ok(c) && (c.dtype == 0 || c.dtype == 1) && aligned(c.key_pages, 16) && aligned(c.value_pages, 16) && aligned(c.page_table, 4) &&
            aligned(c.lengths, 4) && reinterpret_cast<uintptr_t>(c.weight_pages) % 4 == 0 && rows_ok(c.key_strides, 3) &&
            rows_ok(c.value_strides, 3) && c.weight_strides[0] >= 0 && c.weight_strides[0] <= 0x7fffffff && c.weight_strides[1] >= 0 &&
-           c.weight_strides[1] <= 0x7fffffff && c.table_stride >= c.max_pages && c.table_stride <= 0x7fffffff &&
+           c.weight_strides[1] <= 0x7fffffff && (c.table_stride >= c.max_pages || c.table_stride == 0) && c.table_stride <= 0x7fffffff &&
            c.pages >= 1 && c.pages <= 0x7fffffff && c.max_pages >= 1 && c.batch >= 1 && c.batch <= R2O_PAGED_MAX_BATCH &&
            c.hkv >= 1 && c.hkv <= 1024 &&
            (c.page_size == 16 || c.page_size == 32 || c.page_size == 64 || c.page_size == 128) && c.max_pages <= (1 << 29) / c.page_size;
 }
+
+// One row of page ids for all requests: their pages may be read, not written.
+bool one_row(const r2o_paged_cache& c) { return c.batch > 1 && c.table_stride == 0; }
 
 }  // namespace
 
 extern "C" {
 
 int r2o_paged_extend(const r2o_paged_extend_params* p, void* stream) {
-    if (!p || !cache_ok(p->cache) || !aligned(p->key, 16) || !aligned(p->value, 16) || !rows_ok(p->key_strides, 3) ||
+    if (!p || !cache_ok(p->cache) || one_row(p->cache) || !aligned(p->key, 16) || !aligned(p->value, 16) || !rows_ok(p->key_strides, 3) ||
         !rows_ok(p->value_strides, 3) || p->rows < 1 || p->rows > (1 << 29) || reinterpret_cast<uintptr_t>(p->counts) % 4 ||
         reinterpret_cast<uintptr_t>(p->weights) % 4 || p->weights_strides[0] < 0 || p->weights_strides[1] < 0 ||
         (p->weights && !p->cache.weight_pages))
@@ -993,6 +996,7 @@ int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream) {
         !aligned(p->partial_ml, 8) || p->partial_states < (p->workers + pairs) * group)
         return R2O_EINVAL;
     if ((p->append_key == nullptr) != (p->append_value == nullptr)) return R2O_EINVAL;
+    if (one_row(c) && (p->append_key || c.weight_pages)) return R2O_EINVAL;
     if (p->append_key && (!aligned(p->append_key, 16) || !aligned(p->append_value, 16) || !rows_ok(p->append_strides, 4)))
         return R2O_EINVAL;
     // every slot that the page tables can hold has room for its logits, whatever the lengths on the device say
@@ -1059,7 +1063,7 @@ int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream) {
 int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream) {
     if (!p || !cache_ok(p->source) || !cache_ok(p->target)) return R2O_EINVAL;
     const r2o_paged_cache &c = p->source, &o = p->target;
-    if (!c.weight_pages || c.dtype != o.dtype || c.batch != o.batch || c.hkv != o.hkv || p->keep < 1 ||
+    if (!c.weight_pages || one_row(o) || c.dtype != o.dtype || c.batch != o.batch || c.hkv != o.hkv || p->keep < 1 ||
         p->keep > o.max_pages * o.page_size || p->sinks < 0 || p->recent < 0 || p->sinks + p->recent > p->keep ||
         !aligned(p->kept, 4) || !aligned(p->target_lengths, 4) || std::abs(p->target_lengths - c.lengths) < c.batch)
         return R2O_EINVAL;

@@ -38,8 +38,8 @@ class PagedCache:
 
     Slot j of request b is slot ``j % page_size`` of page ``page_table[b, j // page_size]``, for every KV head, and
     the first ``lengths[b]`` slots are filled.  A page id outside the pool (such as -1 for a page not handed out)
-    makes its slots invisible: they are neither read nor written.  Requests may share pages that no call writes to;
-    a page whose rows or weights are written stands in the tables once.  Pool and head strides are free (views of one
+    makes its slots invisible: they are neither read nor written.  Requests may share pages that no call writes to
+    (one row of ids expanded for all of them serves); a page whose rows or weights are written stands in the tables once.  Pool and head strides are free (views of one
     pool for both, or for all layers, serve), as long as channels are unit-strided and rows 16-byte aligned."""
 
     key_pages: torch.Tensor                     # bf16 / fp16 [pages, Hkv, page_size, 128]
@@ -73,10 +73,13 @@ def _params_of(cache: PagedCache) -> _lib.PagedCacheParams:
         raise ValueError("paged cache pages need unit channel stride and 16-byte aligned rows of their own")
     if table.dtype != torch.int32 or table.ndim != 2 or min(table.shape) < 1 or table.stride(1) != 1 and table.shape[1] > 1:
         raise ValueError("page_table must be int32 [B,max_pages] with unit-strided rows")
+    table_stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    if 0 < table_stride < table.shape[1]:
+        raise ValueError("page_table rows must not overlap (one expanded row for all requests is taken)")
     if n.dtype != torch.int32 or tuple(n.shape) != (table.shape[0],) or not n.is_contiguous():
         raise ValueError("lengths must be contiguous int32 [B]")
     if table.shape[0] > MAX_BATCH or table.shape[1] * k.shape[2] > 1 << 29 or k.shape[0] >= 1 << 31 or k.shape[1] > 1024 \
-            or table.stride(0) >= 1 << 31:
+            or table_stride >= 1 << 31:
         raise ValueError("paged cache takes at most 1024 requests, 1024 heads and 2^29 slots a request")
     if w is not None and (w.shape != k.shape[:3] or w.dtype != torch.float32 or w.device != k.device
                           or any(not 0 < st < 1 << 31 for st, size in zip(w.stride(), w.shape) if size > 1) or w.stride(2) != 1):
@@ -85,9 +88,14 @@ def _params_of(cache: PagedCache) -> _lib.PagedCacheParams:
     return _lib.PagedCacheParams(
         key_pages=k.data_ptr(), value_pages=v.data_ptr(), weight_pages=_lib.ptr(w), page_table=table.data_ptr(),
         lengths=n.data_ptr(), key_strides=_strides(k, 3), value_strides=_strides(v, 3),
-        weight_strides=(0, 0) if w is None else _strides(w, 2), table_stride=max(table.stride(0), table.shape[1]),
+        weight_strides=(0, 0) if w is None else _strides(w, 2), table_stride=table_stride,
         pages=k.shape[0], max_pages=table.shape[1], page_size=k.shape[2], batch=table.shape[0], hkv=k.shape[1],
         dtype=dtype)
+
+
+def _check_written(cache: PagedCache, what: str) -> None:
+    if cache.page_table.shape[0] > 1 and cache.page_table.stride(0) == 0:
+        raise ValueError(f"{what} would write one page for several requests: the page table is one expanded row")
 
 
 def _check_new_rows(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, what: str) -> None:
@@ -114,6 +122,7 @@ def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, c
     if key.ndim != 4 or key.shape[0] != batch or key.shape[1] != hkv or key.shape[2] < 1 or key.shape[3] != 128:
         raise ValueError("paged extend requires key and value [B,Hkv,S,128] of the cache's requests and heads")
     _check_new_rows(cache, key, value, "paged extend")
+    _check_written(cache, "paged extend")
     if key.shape[2] > cache.capacity:
         raise ValueError("paged extend has more rows than the page table holds")
     counts = _lengths(counts, batch, key.device, "counts")
@@ -164,6 +173,8 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
         raise ValueError("paged attention takes at most 2^36 slots over all requests and heads")
     w, s = _window(window, sinks)
     scale = _scale(sm_scale)
+    if append is not None or cache.weight_pages is not None:
+        _check_written(cache, "paged attention with an append or weights")
     dev = query.device
     query = _rows(query)
     if output is None:
@@ -229,6 +240,7 @@ def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int 
         raise ValueError("keep must be positive and at most what the target's page table holds")
     if sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError("sinks and recent must be non-negative and together at most keep")
+    _check_written(target, "paged evict")
     dev = cache.key_pages.device
     kept = torch.empty((cache.page_table.shape[0], cache.key_pages.shape[1], keep), dtype=torch.int32, device=dev)
     p = _lib.PagedEvict(source=_params_of(cache), target=_params_of(target), keep=keep, sinks=sinks, recent=recent, kept=kept.data_ptr(),

@@ -36,3 +36,29 @@ def test_calls_on_a_copy_leave_the_original_alone(how):
     assert (target.lengths == 40).all() and torch.equal(kept[0, 0, 31:], torch.arange(61, 70, dtype=torch.int32, device=dev))
     for t, before in zip(memory, was):
         assert torch.equal(t.nan_to_num(), before.nan_to_num())
+
+
+def test_requests_that_read_one_expanded_row_of_pages():
+    """One prefix for four requests of different lengths, by a row of ids expanded for them: the bits of a whole table."""
+    import dataclasses
+
+    import r2omni_amd as ro
+
+    dev = _cuda()
+    cache = _cache(dev, (3001,), 2, 32, BF16, seed=3, weights=True)
+    lengths = torch.tensor([3001, 17, 0, 1500], dtype=torch.int32, device=dev)
+    shared = dataclasses.replace(cache, page_table=cache.page_table.expand(4, -1), lengths=lengths)
+    whole = dataclasses.replace(shared, page_table=shared.page_table.contiguous())
+    assert shared.page_table.stride(0) == 0 and whole.page_table.stride(0) > 0
+    q = _query(dev, 4, 8, BF16, 3)
+    plain = dataclasses.replace(shared, weight_pages=None)
+    got = _check(q, plain)
+    want = ro.paged_attention(q, dataclasses.replace(whole, weight_pages=None))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    targets = [_cache(dev, (64,) * 4, 2, 32, BF16, seed=4, weights=True) for _ in range(2)]
+    kept = [ro.paged_evict(c, t, 64, sinks=2, recent=5) for c, t in zip((shared, whole), targets)]
+    assert torch.equal(*kept)
+    assert torch.equal(*(t.key_pages.view(torch.int16) for t in targets))
+    for write in (lambda: ro.paged_attention(q, shared), lambda: ro.paged_evict(whole, dataclasses.replace(shared, lengths=lengths.clone()), 64)):
+        with pytest.raises(ValueError, match="one page for several requests"):
+            write()

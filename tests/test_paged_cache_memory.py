@@ -1,6 +1,7 @@
 """Which memory a paged call uses: that of the cache's tensors at the time of the call.  On the CPU; what would be
 launched is looked at instead."""
 import copy
+import ctypes
 import io
 import pickle
 
@@ -95,3 +96,50 @@ def test_tensors_that_no_longer_make_a_cache_are_refused(launched):
             with pytest.raises(ValueError):
                 call()
     assert not launched
+
+
+@pytest.mark.parametrize("stride,ok", [(0, True), (1, False), (2, False), (3, True), (7, True)])
+def test_page_table_strides_are_the_tables_own(stride, ok, launched):
+    """Requests' rows lie where the table says; a row read by all is expanded, rows that overlap are refused."""
+    table = torch.zeros(3 + 3 * stride, dtype=I32).as_strided((4, 3), (stride, 1))
+    change = dict(page_table=table, lengths=torch.zeros(4, dtype=I32), weight_pages=None)
+    if not ok:
+        with pytest.raises(ValueError, match="overlap"):
+            _cache(**change)
+        return
+    ro.paged_attention(torch.zeros(4, 2, 128, dtype=BF16), _cache(**change))
+    assert launched[0].cache.table_stride == stride and launched[0].cache.batch == 4
+
+
+def test_one_request_has_any_table_stride(launched):
+    table = torch.zeros(3, dtype=I32).as_strided((1, 3), (1, 1))
+    ro.paged_attention(torch.zeros(1, 2, 128, dtype=BF16), _cache(page_table=table, lengths=torch.zeros(1, dtype=I32), weight_pages=None))
+    assert launched[0].cache.table_stride >= 3
+
+
+def test_pages_of_an_expanded_table_are_not_written(launched):
+    cache = _cache(page_table=torch.zeros(1, 3, dtype=I32).expand(2, -1))
+    plain = _cache(page_table=torch.zeros(1, 3, dtype=I32).expand(2, -1), weight_pages=None)
+    rows = torch.zeros(2, 2, 5, 128, dtype=BF16)
+    for call in (lambda: ro.paged_extend(cache, rows, rows), lambda: ro.paged_attention(rows[:, :, 0], cache),
+                 lambda: ro.paged_attention(rows[:, :, 0], plain, append=(rows[:, :, 0], rows[:, :, 0])),
+                 lambda: ro.paged_evict(_cache(), cache, 8)):
+        with pytest.raises(ValueError, match="one page for several requests"):
+            call()
+    assert not launched
+    ro.paged_evict(cache, _cache(), 8)  # reads them
+    assert launched[0].source.table_stride == 0
+
+
+def test_c_abi_takes_one_row_for_reading_alone():
+    """What is refused before a launch; the stride itself, and each call that writes."""
+    from test_paged_refusals import _attention, _c_cache, _evict, _extend
+
+    lib, one = _lib.load(), dict(table_stride=0)
+    for overlapping in (1, 2, -3):
+        assert lib.r2o_paged_attention(ctypes.byref(_attention(cache=_c_cache(table_stride=overlapping))), None) == 1
+    assert lib.r2o_paged_extend(ctypes.byref(_extend(cache=_c_cache(**one))), None) == 1
+    assert lib.r2o_paged_attention(ctypes.byref(_attention(cache=_c_cache(**one))), None) == 1
+    plain = _attention(cache=_c_cache(weight_pages=None, **one), append_key=0xC000, append_value=0xD000)
+    assert lib.r2o_paged_attention(ctypes.byref(plain), None) == 1
+    assert lib.r2o_paged_evict(ctypes.byref(_evict(target=_c_cache(page_table=0x6000, lengths=0x7000, **one))), None) == 1
