@@ -381,7 +381,8 @@ int64_t compute_units(int device) {
     return known[device];
 }
 
-bool needs_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// A derivative through the tensor, of either mode, would be lost.
+bool needs_grad(const at::Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
 
 // Strides of the axes before the channels: multiples of 8 elements, the rows' within 32-bit offsets; 0 for an axis of one.
 bool row_strides(const at::Tensor& t, int64_t n, int64_t* out, bool own_memory = false) {
@@ -523,7 +524,7 @@ PyObject* weights_call(PyObject* const* args) {
     int64_t device;
     const at::Tensor *q = exact_tensor(args[1]), *k = exact_tensor(args[2]), *lse = exact_tensor(args[3]);
     if (!prompt_operands(q, k, args + 4, p, device) || !lse || !on_device(*lse, device) || lse->scalar_type() != at::kFloat ||
-        lse->dim() != 3 || lse->size(0) != p.batch || lse->size(1) != p.hq || lse->size(2) != p.queries || !lse->is_contiguous())
+        lse->dim() != 3 || lse->size(0) != p.batch || lse->size(1) != p.hq || lse->size(2) != p.queries || !lse->is_contiguous() || needs_grad(*lse))
         Py_RETURN_NONE;
     const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
     at::Tensor out = at::empty({p.batch, p.hkv, p.keys}, f32), scratch;
@@ -552,6 +553,12 @@ struct Cache {
         for (PyObject* o : fields) Py_XDECREF(o);
     }
     bool read(PyObject* cache);  // false for what the Python path has to look at
+    bool callable() const {      // in a call: the tensors lie on the current device, and no derivative would be lost
+        if (device != current_device()) return false;
+        for (int i : {0, 1, 4})
+            if (fields[i] != Py_None && needs_grad(THPVariable_Unpack(fields[i]))) return false;
+        return true;
+    }
 };
 
 bool Cache::read(PyObject* cache) {
@@ -622,7 +629,7 @@ PyObject* paged_extend_call(PyObject* const* args) {
     r2o_paged_extend_params p{};
     Cache cache;
     const at::Tensor *k = exact_tensor(args[2]), *v = exact_tensor(args[3]);
-    if (!cache.read(args[1]) || cache.device != current_device()) Py_RETURN_NONE;
+    if (!cache.read(args[1]) || !cache.callable()) Py_RETURN_NONE;
     const int64_t device = cache.device;
     p.cache = cache.c;
     if (one_row(p.cache)) Py_RETURN_NONE;
@@ -636,7 +643,7 @@ PyObject* paged_extend_call(PyObject* const* args) {
         Py_RETURN_NONE;
     if (args[5] != Py_None) {
         const at::Tensor* w = exact_tensor(args[5]);
-        if (!w || !p.cache.weight_pages || !on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 ||
+        if (!w || !p.cache.weight_pages || needs_grad(*w) || !on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 ||
             w->size(0) != k->size(0) || w->size(1) != k->size(1) || w->size(2) != k->size(2) || !w->is_contiguous())
             Py_RETURN_NONE;
         p.weights = w->data_ptr<float>();
@@ -654,7 +661,7 @@ PyObject* paged_attention_call(PyObject* const* args) {
     r2o_paged_cache& c = p.cache;
     Cache cache;
     const at::Tensor* q = exact_tensor(args[2]);
-    if (!cache.read(args[1]) || cache.device != current_device()) Py_RETURN_NONE;
+    if (!cache.read(args[1]) || !cache.callable()) Py_RETURN_NONE;
     const int64_t device = cache.device;
     c = cache.c;
     if (one_row(c) && (c.weight_pages || args[3] != Py_None)) Py_RETURN_NONE;
@@ -698,7 +705,7 @@ PyObject* paged_attention_call(PyObject* const* args) {
 PyObject* paged_evict_call(PyObject* const* args) {
     r2o_paged_evict_params p{};
     Cache source, target;
-    if (!source.read(args[1]) || !target.read(args[2]) || source.device != target.device || source.device != current_device() ||
+    if (!source.read(args[1]) || !target.read(args[2]) || !source.callable() || !target.callable() ||
         !plain_int(args[3], p.keep) || !plain_int(args[4], p.sinks) || !plain_int(args[5], p.recent))
         Py_RETURN_NONE;
     const r2o_paged_cache &c = p.source = source.c, &o = p.target = target.c;

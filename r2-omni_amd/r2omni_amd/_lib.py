@@ -304,6 +304,17 @@ def num_cus(device: torch.device) -> int:
     return _NUM_CUS[index]
 
 
+def refuse_gradients(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raise if a derivative through one of the tensors would be lost: the operators have none, in either mode."""
+    for t in tensors:
+        if t is None:
+            continue
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: pass tensors without tangents")
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

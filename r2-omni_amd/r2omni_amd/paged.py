@@ -93,6 +93,10 @@ def _params_of(cache: PagedCache) -> _lib.PagedCacheParams:
         dtype=dtype)
 
 
+def _pools(cache: PagedCache) -> tuple[torch.Tensor | None, ...]:
+    return cache.key_pages, cache.value_pages, cache.weight_pages
+
+
 def _check_written(cache: PagedCache, what: str) -> None:
     if cache.page_table.shape[0] > 1 and cache.page_table.stride(0) == 0:
         raise ValueError(f"{what} would write one page for several requests: the page table is one expanded row")
@@ -104,8 +108,7 @@ def _check_new_rows(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, w
     for t in (key, value):
         if t.dtype != cache.key_pages.dtype or t.device != cache.key_pages.device:
             raise ValueError(f"{what} rows must match the cache's dtype and device")
-        if torch.is_grad_enabled() and t.requires_grad:
-            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    _lib.refuse_gradients(what, key, value)
 
 
 def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, counts: torch.Tensor | None = None,
@@ -133,6 +136,7 @@ def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, c
             raise ValueError("paged extend weights must be fp32 [B,Hkv,S] on the rows' device")
         if weights.stride(2) != 1 and weights.shape[2] > 1 or min(weights.stride()) < 0:
             weights = weights.contiguous()
+    _lib.refuse_gradients("paged extend", weights, *_pools(cache))
     key, value = _rows(key), _rows(value)
     p = _lib.PagedExtend(cache=_params_of(cache), key=key.data_ptr(), value=value.data_ptr(), weights=_lib.ptr(weights),
                          counts=_lib.ptr(counts), key_strides=_strides(key, 3), value_strides=_strides(value, 3),
@@ -167,8 +171,7 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
         raise ValueError(f"GQA requires Hq divisible by Hkv, at most {_lib.MAX_GQA} query heads a KV head")
     if query.dtype != cache.key_pages.dtype or query.device != cache.key_pages.device:
         raise ValueError("paged attention query must match the cache's dtype and device")
-    if torch.is_grad_enabled() and query.requires_grad:
-        raise RuntimeError("paged attention has no backward pass: call it under torch.no_grad()")
+    _lib.refuse_gradients("paged attention", query, *_pools(cache), *(output or ()))
     if batch * hkv * (-(-cache.capacity // 32)) > (1 << 31) - 4097:
         raise ValueError("paged attention takes at most 2^36 slots over all requests and heads")
     w, s = _window(window, sinks)
@@ -241,6 +244,7 @@ def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int 
     if sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError("sinks and recent must be non-negative and together at most keep")
     _check_written(target, "paged evict")
+    _lib.refuse_gradients("paged evict", *_pools(cache), *_pools(target))
     dev = cache.key_pages.device
     kept = torch.empty((cache.page_table.shape[0], cache.key_pages.shape[1], keep), dtype=torch.int32, device=dev)
     p = _lib.PagedEvict(source=_params_of(cache), target=_params_of(target), keep=keep, sinks=sinks, recent=recent, kept=kept.data_ptr(),

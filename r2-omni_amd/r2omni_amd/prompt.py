@@ -73,8 +73,7 @@ def _check_rows(query: torch.Tensor, key: torch.Tensor, what: str) -> None:
     if query.device != key.device or query.dtype != key.dtype:
         raise ValueError("Q/K device and dtype must match")
     _lib.dtype_code(query.dtype)
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    _lib.refuse_gradients(what, query, key)
 
 
 def _params(query, key, window, sinks, query_lengths, key_lengths, sm_scale) -> _lib.PromptParams:
@@ -107,8 +106,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     _check_rows(query, key, "prompt attention")
     if value.shape != key.shape or value.device != key.device or value.dtype != key.dtype:
         raise ValueError("prompt attention value must match K's shape, device and dtype")
-    if torch.is_grad_enabled() and value.requires_grad:
-        raise RuntimeError("prompt attention has no backward pass: call it under torch.no_grad()")
+    _lib.refuse_gradients("prompt attention", value, *(output or ()))
     batch, hq, rows, _ = query.shape
     query_lengths = _lengths(query_lengths, batch, query.device, "query_lengths")
     key_lengths = _lengths(key_lengths, batch, query.device, "key_lengths")
@@ -160,6 +158,7 @@ def attention_weights(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor,
     batch, hq, rows, _ = query.shape
     if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != query.device:
         raise ValueError("attention weights lse must be fp32 [B,Hq,Sq] on Q's device")
+    _lib.refuse_gradients("attention weights", lse, output)
     query_lengths = _lengths(query_lengths, batch, query.device, "query_lengths")
     key_lengths = _lengths(key_lengths, batch, query.device, "key_lengths")
     _lib.require_device(query, "attention weights input")
