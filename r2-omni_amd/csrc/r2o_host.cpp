@@ -711,7 +711,7 @@ PyObject* paged_evict_call(PyObject* const* args) {
     const r2o_paged_cache &c = p.source = source.c, &o = p.target = target.c;
     if (!c.weight_pages || one_row(o) || c.batch != o.batch || c.hkv != o.hkv || c.dtype != o.dtype || std::abs(c.lengths - o.lengths) < c.batch ||
         c.page_table == o.page_table || p.keep < 1 || p.keep > o.max_pages * o.page_size || p.sinks < 0 || p.recent < 0 ||
-        p.sinks + p.recent > p.keep)
+        p.sinks > p.keep || p.recent > p.keep - p.sinks)
         Py_RETURN_NONE;
     const at::Tensor& lengths = THPVariable_Unpack(target.fields[3]);
     at::Tensor kept = at::empty({c.batch, c.hkv, p.keep}, lengths.options());

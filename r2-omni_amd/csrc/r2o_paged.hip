@@ -1064,7 +1064,7 @@ int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream) {
     if (!p || !cache_ok(p->source) || !cache_ok(p->target)) return R2O_EINVAL;
     const r2o_paged_cache &c = p->source, &o = p->target;
     if (!c.weight_pages || one_row(o) || c.dtype != o.dtype || c.batch != o.batch || c.hkv != o.hkv || p->keep < 1 ||
-        p->keep > o.max_pages * o.page_size || p->sinks < 0 || p->recent < 0 || p->sinks + p->recent > p->keep ||
+        p->keep > o.max_pages * o.page_size || p->sinks < 0 || p->recent < 0 || p->sinks > p->keep || p->recent > p->keep - p->sinks ||
         !aligned(p->kept, 4) || !aligned(p->target_lengths, 4) || std::abs(p->target_lengths - c.lengths) < c.batch)
         return R2O_EINVAL;
     const hipStream_t st = (hipStream_t)stream;

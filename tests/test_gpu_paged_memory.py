@@ -62,3 +62,14 @@ def test_requests_that_read_one_expanded_row_of_pages():
     for write in (lambda: ro.paged_attention(q, shared), lambda: ro.paged_evict(whole, dataclasses.replace(shared, lengths=lengths.clone()), 64)):
         with pytest.raises(ValueError, match="one page for several requests"):
             write()
+
+
+@pytest.mark.parametrize("sinks,recent", [(1 << 62, 1 << 62), ((1 << 63) - 1, 1), (1 << 64, 0)])
+def test_protected_slots_past_every_number_are_refused(sinks, recent):
+    """By the host module's checks too, whose sums are 64-bit."""
+    import r2omni_amd as ro
+
+    dev = _cuda()
+    cache, target = (_cache(dev, (70, 90), 2, 16, BF16, seed=s, weights=True) for s in (5, 6))
+    with pytest.raises(ValueError, match="at most keep"):
+        ro.paged_evict(cache, target, 40, sinks=sinks, recent=recent)
