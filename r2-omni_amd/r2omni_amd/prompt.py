@@ -44,12 +44,12 @@ def _scale(sm_scale) -> float:
 
 
 def _window(window, sinks) -> tuple[int, int]:
-    """(window, sinks) as the kernels take them: a window of 0 is none."""
+    """(window, sinks) as the kernels take them: a window of 0 is none, one past every length is any such."""
     if window is not None and int(window) < 1:
         raise ValueError("window must be None or at least one token")
     if int(sinks) < 0:
         raise ValueError("sinks must be non-negative")
-    return (0 if window is None else int(window)), min(int(sinks), _MOST_ROWS)
+    return (0 if window is None else min(int(window), 2 * _MOST_ROWS)), min(int(sinks), _MOST_ROWS)
 
 
 def _lengths(t, batch: int, device: torch.device, what: str):
