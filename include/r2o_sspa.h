@@ -496,7 +496,8 @@ typedef struct r2o_prompt_params {
 } r2o_prompt_params;
 
 /* out = softmax(sm_scale q k^T) v over the keys that each row sees, and lse = log of the sum of exponentials.
- * Every row is written: one that sees no key, or lies behind its request's length, is 0 with lse -inf.  The states of
+ * Every row is written: one that sees no key, or lies behind its request's length, is 0 with lse -inf.  Infinite and NaN
+ * values that a row sees add up to its channel, however small their weights.  The states of
  * the splits are joined in order: equal calls give equal bits. */
 int r2o_prompt_attention(const r2o_prompt_params* p, void* stream);
 
@@ -544,7 +545,7 @@ int r2o_paged_extend(const r2o_paged_extend_params* p, void* stream);
  * last `window` and the first `sinks` ones.  append_key / append_value (both or neither): the rows of slot lengths[b]
  * - 1, which are attended and written into their page.  Where the cache keeps weights, the weight of each slot seen
  * grows by the sum of its probabilities over the KV head's query heads; the appended slot's is set to it.  A request
- * without a slot to see gets 0 and lse -inf.  Two launches; no atomics, so equal calls give equal bits. */
+ * without a slot to see gets 0 and lse -inf.  Infinite and NaN values as in r2o_prompt_attention.  Two launches; no atomics, so equal calls give equal bits. */
 typedef struct r2o_paged_attention_params {
     r2o_paged_cache cache;
     const uint16_t* query;    /* [batch, hq, 128], element strides (batch, head) */

@@ -513,6 +513,48 @@ __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count,
     return {m, l};
 }
 
+// The infinite and NaN values of channels 2 lane and 2 lane + 1 that a request's token sees, added up; 0 where there are
+// none.  By one wave, 16 rows in flight.
+template <int RF>
+__device__ __forceinline__ void seen_not_finite(int b, int h, float& x, float& y) {
+    Args& a = kernel_args();
+    const Tiles t = tiles_of(a, load_uniform(a.lengths + b));
+    const int lane = threadIdx.x & 63;
+    const int32_t* table = a.table + (int64_t)b * a.table_stride;
+    const uint16_t* rows = a.value + (int64_t)h * a.v_head + 8 * (lane & 15);
+    float sum[8] = {};
+#pragma unroll 1
+    for (int half = 0; half < 2 * t.count; ++half) {
+        r2o_u4 v[4];
+        bool seen[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // four rows a load
+            const int j = t.slot(half >> 1) + 16 * (half & 1) + 4 * i + (lane >> 4);
+            const int page = r2o_ldg(table + min(j >> a.shift, a.last_page));
+            seen[i] = t.sees(j, a.sinks) && (uint32_t)page < (uint32_t)a.pages;
+            v[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(rows + (int64_t)(seen[i] ? page : 0) * a.v_page + (int64_t)(j & ((1 << a.shift) - 1)) * a.v_slot));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t bits = v[i][k >> 1] >> (16 * (k & 1)) & 0xffffu;
+                const float f = RF == 0 ? r2o_bf16_to_f32(bits) : r2o_f16_to_f32(bits);
+                sum[k] += seen[i] && !__builtin_isfinite(f) ? f : 0.f;
+            }
+    }
+    x = y = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        float p, q;
+        r2o_row_swap<16>(sum[k], p, q);
+        r2o_row_swap<32>(p + q, p, q);
+        const float all = __shfl(p + q, lane >> 2);  // chunk lane / 4 holds this lane's channels, its elements 2 (lane % 4) ..
+        x = k == 2 * (lane & 3) ? all : x;
+        y = k == 2 * (lane & 3) + 1 ? all : y;
+    }
+}
+
 // Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: an even
 // share of all tiles each, whose slots' weights grow by their probabilities.  Bound by its launch and its round trips: 5
 // us for a call without weights, 11.1 for a ragged batch of 252 MB with them.
@@ -569,7 +611,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
                 x += red[i][2 * threadIdx.x];
                 y += red[i][2 * threadIdx.x + 1];
             }
-            reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = live ? pack2<RF>(x * inv, y * inv) : 0u;
+            x *= inv;
+            y *= inv;
+            // A channel is infinite or NaN where a slot that the token sees is, however small that slot's weight: not NaN where
+            // the weight is rounded to 0 on its way to a product or a state's factor is 0, which depends on the workers' shares.
+            // A NaN sum, of a NaN logit, makes the whole row NaN.
+            if (__any(live && ml.l == ml.l && !(__builtin_isfinite(x) && __builtin_isfinite(y)))) {
+                float x2, y2;
+                seen_not_finite<RF>(b, h, x2, y2);
+                x = __builtin_isfinite(x2) ? x : x2;
+                y = __builtin_isfinite(y2) ? y : y2;
+            }
+            reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = live ? pack2<RF>(x, y) : 0u;
             if (threadIdx.x == 0) *lse = live ? (ml.m + __builtin_amdgcn_logf(ml.l)) * kLn2 : -INFINITY;
         }
         return;

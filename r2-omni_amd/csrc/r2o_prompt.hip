@@ -134,6 +134,17 @@ __device__ __forceinline__ bool not_finite(uint32_t bits16) {
     return (bits16 & e) == e;
 }
 
+template <int RF>
+__device__ __forceinline__ bool any_not_finite(r2o_u4 x) {
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) any |= not_finite<RF>(x[k]) | not_finite<RF>(x[k] >> 16);
+    return any;
+}
+
+// A partial output by the factor of its state: infinite and NaN ones stay, where a factor of 0 would make them NaN.
+__device__ __forceinline__ float weighed(float x, float f) { return __builtin_isfinite(x) ? x * f : x; }
+
 // In a tile that some row of the workgroup sees in part, a masked key's probability is 0, but 0 times an infinite
 // or NaN value is NaN: such elements become zero before any product; true if there was one.
 template <int RF>
@@ -369,28 +380,54 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     if (lane == 0) flags[wave] = wave_bad;
     __syncthreads();
     const bool any_bad = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
-    if (any_bad) {  // what was taken out, for the rows that see it
-        for (int it = begin; it < tiles; ++it) {
-            const int kt = tile_key(it);
-            if (!seen_in_part(kt)) continue;
-            for (int j = kt; j < min(kt + kTile, s.n); ++j) {
-                if (!sees(pv, j, window, sinks)) continue;
-                const uint16_t* src = vbase + (int64_t)j * v_row + 4 * half;
-#pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint32_t x = r2o_ldg(src + 32 * db + 8 * (i >> 2) + (i & 3));
-                        if (not_finite<RF>(x)) acc[db][i] += RF == 0 ? r2o_bf16_to_f32(x) : r2o_f16_to_f32(x);
-                    }
-            }
-        }
-    }
-
     {
         float x, y;
         r2o_row_swap<32>(l, x, y);
         l = x + y;
+    }
+    // A row's channel is infinite or NaN where a key that it sees is, however small that key's weight: not NaN where the
+    // weight is rounded to 0 on its way to the product, which depends on the maximum so far.  Those channels are formed
+    // again from the values alone: over all tiles where a product has met one, else over those where some were taken out.
+    float odd[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) odd[db] = __builtin_fmaf(acc[db][i], 0.f, odd[db]);  // NaN where one is not finite
+    const float any_odd = odd[0] + odd[1] + odd[2] + odd[3];
+    const bool met = __any(any_odd != any_odd && l == l && row < s.q);  // a NaN sum, of a NaN logit, makes the whole row NaN
+    if (any_bad || met) {
+        f16v extra[4];
+#pragma unroll
+        for (int db = 0; db < 4; ++db) extra[db] = f16v{};
+        for (int it = begin; it < tiles; ++it) {
+            const int kt = tile_key(it);
+            if (!met && !seen_in_part(kt)) continue;
+            for (int j16 = kt; j16 < kt + kTile; j16 += 16) {
+                r2o_u4 chunk[4];  // of four rows each
+                bool any = false;
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    chunk[n] = r2o_ldg(reinterpret_cast<const r2o_u4*>(vbase + (int64_t)min(j16 + 4 * n + (lane >> 4), last) * v_row) + (lane & 15));
+#pragma unroll
+                for (int n = 0; n < 4; ++n) any |= any_not_finite<RF>(chunk[n]);
+                if (!__any(any)) continue;
+                for (int j = j16; j < min(j16 + 16, s.n); ++j) {
+                    if (!sees(pv, j, window, sinks)) continue;
+                    const uint16_t* src = vbase + (int64_t)j * v_row + 4 * half;
+#pragma unroll
+                    for (int db = 0; db < 4; ++db)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t x = r2o_ldg(src + 32 * db + 8 * (i >> 2) + (i & 3));
+                            if (not_finite<RF>(x)) extra[db][i] += RF == 0 ? r2o_bf16_to_f32(x) : r2o_f16_to_f32(x);
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[db][i] = __builtin_isfinite(extra[db][i]) ? acc[db][i] : extra[db][i];
     }
     if (packed >= rows) return;
     Args& e = kernel_args();
@@ -444,7 +481,8 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits
         const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
         const float f = __builtin_amdgcn_exp2f(m - ms), f2 = __builtin_amdgcn_exp2f(m2 - ms);
         l = l * f + l2 * f2;
-        o = m2 == -INFINITY ? o : o * f + o2 * f2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = weighed(o[k], f) + weighed(o2[k], f2);
         m = mn;
     }
     const bool live = !(l == 0.f);
