@@ -14,6 +14,7 @@
 #include <initializer_list>
 
 #include "r2o_common.hpp"
+#include "r2o_place.hpp"
 
 namespace {
 
@@ -172,7 +173,7 @@ struct PromptArgs {
     const float* lse_in;
     float *weights, *partial_out, *partial_ml;
     int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head, o_batch, o_head;
-    int q_row, k_row, v_row, o_row, hq, hkv, pairs, splits, group, queries, keys, window, sinks;
+    int q_row, k_row, v_row, o_row, batches, hq, hkv, pairs, splits, group, queries, keys, window, sinks;
     float c2;  // scale, in log2 units
 };
 
@@ -198,28 +199,6 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
     return s;
 }
 
-// Blocks go to the 8 dies (XCDs) in turn, and a die's L2 is its own: where the pairs allow it, a die works through the
-// tiles of one pair after the other (or shares a pair with some), so that its workgroups read the same rows.  Tile by
-// tile, a tile's splits together: the caller's first tiles are the longest.  False for a block that only fills the grid up.
-__device__ __forceinline__ bool place(int block, int tiles, int splits, int pairs, int& pair, int& tile, int& split) {
-    const int die = block & 7, i = block >> 3, items = tiles * splits;
-    int rank;
-    if ((pairs & 7) == 0) {
-        pair = die + 8 * (i / items);
-        rank = i % items;
-    } else if (pairs == 1 || pairs == 2 || pairs == 4) {
-        const int dies = 8 / pairs;
-        pair = die / dies;
-        rank = i * dies + die % dies;
-    } else {
-        pair = block / items;
-        rank = block % items;
-    }
-    tile = rank / splits;
-    split = rank - tile * splits;
-    return rank < items && pair < pairs;
-}
-
 // ------------------------------------------------------------------------------ prompt attention
 // The rows of a KV head's query heads are one list, packed row r = (row r / group, head r % group): a workgroup's 128
 // stand at 128 / group neighbouring positions, so its last tiles are masked in part for few of them, and a chunk of few
@@ -239,9 +218,10 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     Args& a = kernel_args();
     const int group = a.group, rows = a.queries * group;
     const int row_tiles = (rows + kRows - 1) / kRows, splits = a.splits;
-    int pair, row_tile, split;
-    if (!place(blockIdx.x, row_tiles, splits, a.pairs, pair, row_tile, split)) return;
-    const int kvh = pair % a.hkv, b = pair / a.hkv, row0 = (row_tiles - 1 - row_tile) * kRows;  // the last rows see most
+    const R2oPlace at_block = r2o_place(blockIdx.x, row_tiles, splits, a.batches, a.pairs / a.batches);
+    if (!at_block.valid) return;
+    const int pair = at_block.pair, split = at_block.split;
+    const int kvh = pair % a.hkv, b = pair / a.hkv, row0 = (row_tiles - 1 - at_block.tile) * kRows;  // the last rows see most
     const Lengths s = request_lengths(a, b);
     const int window = a.window, sinks = a.sinks;
     const uint16_t* kbase = a.key + b * a.k_batch + kvh * a.k_head;
@@ -509,9 +489,10 @@ __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     Args& a = kernel_args();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int group = a.group, key_tiles = (a.keys + kWeightKeys - 1) / kWeightKeys;
-    int pair, key_tile, split;
-    if (!place(blockIdx.x, key_tiles, a.splits, a.pairs, pair, key_tile, split)) return;
-    const int kvh = pair % a.hkv, b = pair / a.hkv, key0 = key_tile * kWeightKeys;  // the first keys have most rows
+    const R2oPlace at_block = r2o_place(blockIdx.x, key_tiles, a.splits, 1, a.pairs);
+    if (!at_block.valid) return;
+    const int pair = at_block.pair, split = at_block.split;
+    const int kvh = pair % a.hkv, b = pair / a.hkv, key0 = at_block.tile * kWeightKeys;  // the first keys have most rows
     const Lengths s = request_lengths(a, b);
     const int window = a.window, sinks = a.sinks;
     const int kw = key0 + 64 * wave, j = kw + col;  // this lane's keys: j and j + 32
@@ -645,12 +626,6 @@ bool shapes_ok(const r2o_prompt_params* p) {
            reinterpret_cast<uintptr_t>(p->query_lengths) % 4 == 0 && reinterpret_cast<uintptr_t>(p->key_lengths) % 4 == 0;
 }
 
-// Blocks of `place`: the items in whole turns of the dies that share a pair.
-int64_t grid_blocks(int64_t tiles, int64_t splits, int64_t pairs) {
-    const int64_t dies = pairs == 1 || pairs == 2 || pairs == 4 ? 8 / pairs : 1;
-    return (tiles * splits + dies - 1) / dies * dies * pairs;
-}
-
 PromptArgs kernel_arguments(const r2o_prompt_params* p) {
     PromptArgs a{};
     a.query = p->query;
@@ -697,12 +672,16 @@ int r2o_prompt_attention(const r2o_prompt_params* p, void* stream) {
     const int64_t rows = p->queries * (p->hq / p->hkv), pairs = p->batch * p->hkv;
     if (rows > (1 << 30) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
     if (p->splits > 1 && (!aligned({p->scratch}, 16) || p->scratch_floats < p->splits * pairs * rows * 130)) return R2O_EINVAL;
-    const int64_t blocks = grid_blocks((rows + kRows - 1) / kRows, p->splits, pairs);
+    // Requests of one length keep their pairs to dies of their own (four of 4096 rows, 16 heads over 2: 292 us, spread 311);
+    // of lengths that may differ, each is spread over all dies (8192, 2048, 1024 and 512 rows: 384 us, pinned 1100).
+    const int64_t batches = p->query_lengths || p->key_lengths ? p->batch : 1;
+    const int64_t blocks = r2o_place_blocks((rows + kRows - 1) / kRows, p->splits, batches, pairs / batches);
     if (blocks > 0x7fffffff) return R2O_EINVAL;
     const dim3 grid((unsigned)blocks);
     const dim3 join((unsigned)((rows + 7) / 8), (unsigned)pairs);
     const hipStream_t st = (hipStream_t)stream;
     PromptArgs a = kernel_arguments(p);
+    a.batches = (int)batches;
     a.partial_out = p->scratch;
     a.partial_ml = p->scratch + p->splits * pairs * rows * 128;
     if (p->dtype == 0) hipLaunchKernelGGL(prompt_attention_kernel<0>, grid, dim3(256), 0, st, a);
@@ -720,7 +699,9 @@ int r2o_attention_weights(const r2o_prompt_params* p, void* stream) {
     if (!shapes_ok(p) || !aligned({p->lse_in, p->weights}, 4) || p->splits < 1 || p->splits > 65535) return R2O_EINVAL;
     const int64_t n = p->batch * p->hkv * p->keys;
     if (p->splits > 1 && (!aligned({p->scratch}, 4) || p->scratch_floats < p->splits * n)) return R2O_EINVAL;
-    const int64_t blocks = grid_blocks((p->keys + kWeightKeys - 1) / kWeightKeys, p->splits, p->batch * p->hkv);
+    // Pairs keep to dies of their own here, whatever the lengths: 8192 and 1024 rows of 28 heads over 4 take 568 us, spread
+    // 563, two requests of 8192 rows 572 and 659.
+    const int64_t blocks = r2o_place_blocks((p->keys + kWeightKeys - 1) / kWeightKeys, p->splits, 1, p->batch * p->hkv);
     if ((n + 255) / 256 > 0x7fffffff || blocks > 0x7fffffff) return R2O_EINVAL;
     const dim3 grid((unsigned)blocks);
     const hipStream_t st = (hipStream_t)stream;
