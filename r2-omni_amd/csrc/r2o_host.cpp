@@ -422,11 +422,14 @@ bool mask_args(PyObject* window_o, PyObject* sinks_o, PyObject* scale_o, int64_t
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Workgroups that share the keys of one 128-row tile: as many as give a compute unit one, each with at least four tiles
-// of 64 keys.  257 rows of 16 heads over 4097 keys take 34 us in 6 splits (one a compute unit), 41 in 16, 102 in one.
-int64_t attention_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries, int64_t keys, int64_t window, int64_t cus) {
-    const int64_t tiles = div_up(hq / hkv * queries, 128) * batch * hkv;
-    const int64_t seen = window ? std::min(keys, std::min(window, keys) + queries + 128) : keys;
+// Workgroups that share the keys of one tile of 128 packed rows: as many as give a compute unit one, at most one for each 256
+// keys, begun ones among them, that the tile sees: its rows stand at 128 / group neighbouring positions, so with a window
+// these are the window's, as many more, the sinks, and what the first key tile holds before them.  257 rows of 16 heads over
+// 4097 keys take 28.4 us in 7 splits (one a compute unit), 30 in 6, 32 in 8, 91 in one; 512 rows of 16 heads with a window of
+// 256 15.9 in 2, 19.8 in 4, 14.0 in one; one row of 28 heads over 300 keys 10.7 in 2, 11.2 in one.
+int64_t attention_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries, int64_t keys, int64_t window, int64_t sinks, int64_t cus) {
+    const int64_t group = hq / hkv, tiles = div_up(group * queries, 128) * batch * hkv;
+    const int64_t seen = window ? std::min(keys, std::min(window, keys) + div_up(128, group) + std::min(sinks, keys) + 64) : keys;
     return std::max<int64_t>(1, std::min(cus / tiles, div_up(seen, 256)));
 }
 
@@ -506,7 +509,7 @@ PyObject* prompt_call(PyObject* const* args) {
     if (!row_strides(out, 3, p.o_strides, true) || p.o_strides[2] > R2O_MAX_ROW_STRIDE) Py_RETURN_NONE;
     const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
     at::Tensor lse = at::empty({p.batch, p.hq, p.queries}, f32), scratch;
-    p.splits = attention_splits(p.batch, p.hq, p.hkv, p.queries, p.keys, p.window, compute_units((int)device));
+    p.splits = attention_splits(p.batch, p.hq, p.hkv, p.queries, p.keys, p.window, p.sinks, compute_units((int)device));
     if (p.splits > 1) {
         p.scratch_floats = 130 * p.splits * p.batch * p.hq * p.queries;
         scratch = at::empty({p.scratch_floats}, f32);
@@ -730,11 +733,10 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
-template <int64_t (*RULE)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t)>
-PyObject* rule7(PyObject*, PyObject* args) {
-    long long x[7];
-    if (!PyArg_ParseTuple(args, "LLLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5, x + 6)) return nullptr;
-    return PyLong_FromLongLong(RULE(x[0], x[1], x[2], x[3], x[4], x[5], x[6]));
+PyObject* attention_splits_rule(PyObject*, PyObject* args) {
+    long long x[8];
+    if (!PyArg_ParseTuple(args, "LLLLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5, x + 6, x + 7)) return nullptr;
+    return PyLong_FromLongLong(attention_splits(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]));
 }
 
 PyObject* weight_splits_rule(PyObject*, PyObject* args) {
@@ -761,7 +763,7 @@ PyMethodDef kMethods[] = {
     {"paged_extend", FAST(paged_extend_call, 6)},
     {"paged_attention", FAST(paged_attention_call, 7)},
     {"paged_evict", FAST(paged_evict_call, 6)},
-    {"attention_splits", rule7<attention_splits>, METH_VARARGS, nullptr},
+    {"attention_splits", attention_splits_rule, METH_VARARGS, nullptr},
     {"weight_splits", weight_splits_rule, METH_VARARGS, nullptr},
     {"paged_workers", paged_workers_rule, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

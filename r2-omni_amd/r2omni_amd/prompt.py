@@ -127,7 +127,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != query.device \
                 or not lse.is_contiguous():
             raise ValueError("prompt attention lse output must be contiguous fp32 [B,Hq,Sq] on Q's device")
-    p.splits = _lib.host().attention_splits(batch, hq, key.shape[1], rows, key.shape[2], p.window, _lib.num_cus(query.device))
+    p.splits = _lib.host().attention_splits(batch, hq, key.shape[1], rows, key.shape[2], p.window, p.sinks, _lib.num_cus(query.device))
     scratch = None
     if p.splits > 1:
         scratch = torch.empty(130 * p.splits * batch * hq * rows, dtype=torch.float32, device=query.device)
