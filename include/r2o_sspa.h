@@ -532,7 +532,7 @@ typedef struct r2o_paged_cache {
  * zeros where the cache keeps weights and none are given. */
 typedef struct r2o_paged_extend_params {
     r2o_paged_cache cache;
-    const uint16_t* key;      /* [batch, hkv, rows, 128], element strides (batch, head, row) */
+    const uint16_t* key;      /* [batch, hkv, rows, 128], element strides (batch, head, row), 64-bit */
     const uint16_t* value;
     const float* weights;
     const int32_t* counts;

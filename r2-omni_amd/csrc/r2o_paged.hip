@@ -1007,6 +1007,13 @@ bool rows_ok(const int64_t* st, int n) {  // the kernels hold strides in 32 bits
     return true;
 }
 
+// The extend kernel multiplies in 64 bits: a prompt's requests, heads and rows may lie anywhere.
+bool new_rows_ok(const int64_t* st) {
+    for (int i = 0; i < 3; ++i)
+        if (st[i] < 0 || st[i] % 8) return false;
+    return true;
+}
+
 // One slot's rows lie within 32-bit offsets of the next ones'.
 bool slots_ok(const r2o_paged_cache& c) { return c.key_strides[2] <= R2O_PAGED_MAX_SLOT_STRIDE && c.value_strides[2] <= R2O_PAGED_MAX_SLOT_STRIDE; }
 
@@ -1028,8 +1035,8 @@ bool one_row(const r2o_paged_cache& c) { return c.batch > 1 && c.table_stride ==
 extern "C" {
 
 int r2o_paged_extend(const r2o_paged_extend_params* p, void* stream) {
-    if (!p || !cache_ok(p->cache) || one_row(p->cache) || !aligned(p->key, 16) || !aligned(p->value, 16) || !rows_ok(p->key_strides, 3) ||
-        !rows_ok(p->value_strides, 3) || p->rows < 1 || p->rows > (1 << 29) || reinterpret_cast<uintptr_t>(p->counts) % 4 ||
+    if (!p || !cache_ok(p->cache) || one_row(p->cache) || !aligned(p->key, 16) || !aligned(p->value, 16) || !new_rows_ok(p->key_strides) ||
+        !new_rows_ok(p->value_strides) || p->rows < 1 || p->rows > (1 << 29) || reinterpret_cast<uintptr_t>(p->counts) % 4 ||
         reinterpret_cast<uintptr_t>(p->weights) % 4 || p->weights_strides[0] < 0 || p->weights_strides[1] < 0 ||
         (p->weights && !p->cache.weight_pages))
         return R2O_EINVAL;

@@ -58,6 +58,12 @@ class PagedCache:
         return int(self.page_table.shape[1]) * int(self.key_pages.shape[2])
 
 
+def _token_rows(t: torch.Tensor) -> torch.Tensor:
+    """``_rows`` of [B, H, 128]; copied too where they lie farther apart than the kernels' 32 bits of elements."""
+    t = _rows(t)
+    return t.clone(memory_format=torch.contiguous_format) if any(st >= 1 << 31 for st, n in zip(t.stride(), t.shape) if n > 1) else t
+
+
 def _params_of(cache: PagedCache) -> _lib.PagedCacheParams:
     """Where the cache's tensors lie now, checked.  Nothing is kept from one call for the next: a copied cache has tensors
     of its own, and ``t.data = ...`` gives one other memory."""
@@ -179,7 +185,7 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
     if append is not None or cache.weight_pages is not None:
         _check_written(cache, "paged attention with an append or weights")
     dev = query.device
-    query = _rows(query)
+    query = _token_rows(query)
     if output is None:
         out = torch.empty((batch, hq, 128), dtype=query.dtype, device=dev)
         lse = torch.empty((batch, hq), dtype=torch.float32, device=dev)
@@ -199,7 +205,7 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
                 t = t[:, :, 0]
             if tuple(t.shape) != (batch, hkv, 128):
                 raise ValueError("paged attention append requires key and value [B,Hkv,128]")
-            rows.append(_rows(t))
+            rows.append(_token_rows(t))
         key, value = rows
         _check_new_rows(cache, key, value, "paged attention append")
         p.append_key, p.append_value = key.data_ptr(), value.data_ptr()

@@ -73,3 +73,29 @@ def test_protected_slots_past_every_number_are_refused(sinks, recent):
     cache, target = (_cache(dev, (70, 90), 2, 16, BF16, seed=s, weights=True) for s in (5, 6))
     with pytest.raises(ValueError, match="at most keep"):
         ro.paged_evict(cache, target, 40, sinks=sinks, recent=recent)
+
+
+def test_new_rows_whose_offsets_pass_32_bits():
+    """A layer's rows as slices of a tensor that holds all layers of long requests, and a token's as a slice of a long prompt:
+    requests 2^31 elements apart give the bits of compact ones."""
+    import dataclasses
+
+    import r2omni_amd as ro
+
+    dev, far = _cuda(), 1 << 31
+    big = torch.empty(2 * far + 4096, dtype=BF16, device=dev)
+    small = torch.randn(2, 2, 7, 128, device=dev).to(BF16)
+    rows = big.as_strided(small.shape, (far, 7 * 128, 128, 1))
+    rows.copy_(small)
+    caches = [_cache(dev, (70, 90), 2, 16, BF16, seed=7, weights=True) for _ in range(2)]
+    for cache, new in zip(caches, (small, rows)):
+        ro.paged_extend(cache, new, new)
+    for name in ("key_pages", "value_pages"):
+        assert torch.equal(*(getattr(c, name).view(torch.int16) for c in caches))
+    near = _query(dev, 2, 4, BF16, 7)
+    query = big.as_strided(near.shape, (far, 128, 1), 2048)
+    query.copy_(near)
+    plain = dataclasses.replace(caches[0], weight_pages=None)
+    want = ro.paged_attention(near, plain, append=(small[:, :, 0], small[:, :, 1]))
+    got = ro.paged_attention(query, plain, append=(rows[:, :, 0], rows[:, :, 1]))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
