@@ -514,34 +514,45 @@ __device__ __forceinline__ Ml join_ml(const float* ml, int64_t slot0, int count,
 }
 
 // The infinite and NaN values of channels 2 lane and 2 lane + 1 that a request's token sees, added up; 0 where there are
-// none.  By one wave, 16 rows in flight.
+// none.  By one wave, in the tiles of the workers whose products met one (first: the pair's first tile of all, w0 its
+// worker, of `count`), 16 rows in flight, till every channel is NaN.
 template <int RF>
-__device__ __forceinline__ void seen_not_finite(int b, int h, float& x, float& y) {
+__device__ __forceinline__ void seen_not_finite(const Tiles& t, const Share& share, int first, int w0, int count, int b, int h, int head, float& x, float& y) {
     Args& a = kernel_args();
-    const Tiles t = tiles_of(a, load_uniform(a.lengths + b));
     const int lane = threadIdx.x & 63;
     const int32_t* table = a.table + (int64_t)b * a.table_stride;
     const uint16_t* rows = a.value + (int64_t)h * a.v_head + 8 * (lane & 15);
     float sum[8] = {};
+    bool more = true;
 #pragma unroll 1
-    for (int half = 0; half < 2 * t.count; ++half) {
-        r2o_u4 v[4];
-        bool seen[4];
+    for (int w = w0; w < w0 + count && more; ++w) {
+        const float* part = a.partial_out + (((int64_t)w + b * a.hkv + h) * a.group + head) * 128 + 2 * lane;
+        if (!__any(!(__builtin_isfinite(r2o_ldg(part)) && __builtin_isfinite(r2o_ldg(part + 1))))) continue;
+        const int stop = 2 * (min(share.begin(w + 1), first + t.count) - first);
+#pragma unroll 1
+        for (int half = 2 * (max(share.begin(w), first) - first); half < stop && more; ++half) {
+            r2o_u4 v[4];
+            bool seen[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // four rows a load
-            const int j = t.slot(half >> 1) + 16 * (half & 1) + 4 * i + (lane >> 4);
-            const int page = r2o_ldg(table + min(j >> a.shift, a.last_page));
-            seen[i] = t.sees(j, a.sinks) && (uint32_t)page < (uint32_t)a.pages;
-            v[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(rows + (int64_t)(seen[i] ? page : 0) * a.v_page + (int64_t)(j & ((1 << a.shift) - 1)) * a.v_slot));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {  // four rows a load
+                const int j = t.slot(half >> 1) + 16 * (half & 1) + 4 * i + (lane >> 4);
+                const int page = r2o_ldg(table + min(j >> a.shift, a.last_page));
+                seen[i] = t.sees(j, a.sinks) && (uint32_t)page < (uint32_t)a.pages;
+                v[i] = r2o_ldg(reinterpret_cast<const r2o_u4*>(rows + (int64_t)(seen[i] ? page : 0) * a.v_page + (int64_t)(j & ((1 << a.shift) - 1)) * a.v_slot));
+            }
+            bool all_nan = true;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const uint32_t bits = v[i][k >> 1] >> (16 * (k & 1)) & 0xffffu;
-                const float f = RF == 0 ? r2o_bf16_to_f32(bits) : r2o_f16_to_f32(bits);
-                sum[k] += seen[i] && !__builtin_isfinite(f) ? f : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bits = v[i][k >> 1] >> (16 * (k & 1)) & 0xffffu;
+                    const float f = RF == 0 ? r2o_bf16_to_f32(bits) : r2o_f16_to_f32(bits);
+                    sum[k] += seen[i] && !__builtin_isfinite(f) ? f : 0.f;
+                }
+                all_nan &= sum[k] != sum[k];
             }
+            more = !__all(all_nan);
+        }
     }
     x = y = 0.f;
 #pragma unroll
@@ -618,7 +629,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
             // A NaN sum, of a NaN logit, makes the whole row NaN.
             if (__any(live && ml.l == ml.l && !(__builtin_isfinite(x) && __builtin_isfinite(y)))) {
                 float x2, y2;
-                seen_not_finite<RF>(b, h, x2, y2);
+                seen_not_finite<RF>(t, share, u, w0, count, b, h, head, x2, y2);
                 x = __builtin_isfinite(x2) ? x : x2;
                 y = __builtin_isfinite(y2) ? y : y2;
             }

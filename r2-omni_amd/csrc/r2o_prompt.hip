@@ -379,10 +379,11 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
         f16v extra[4];
 #pragma unroll
         for (int db = 0; db < 4; ++db) extra[db] = f16v{};
-        for (int it = begin; it < tiles; ++it) {
+        bool more = true;  // till every row has NaN alone
+        for (int it = begin; it < tiles && more; ++it) {
             const int kt = tile_key(it);
             if (!met && !seen_in_part(kt)) continue;
-            for (int j16 = kt; j16 < kt + kTile; j16 += 16) {
+            for (int j16 = kt; j16 < kt + kTile && more; j16 += 16) {
                 r2o_u4 chunk[4];  // of four rows each
                 bool any = false;
 #pragma unroll
@@ -402,6 +403,12 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
                             if (not_finite<RF>(x)) extra[db][i] += RF == 0 ? r2o_bf16_to_f32(x) : r2o_f16_to_f32(x);
                         }
                 }
+                bool all_nan = true;
+#pragma unroll
+                for (int db = 0; db < 4; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) all_nan &= extra[db][i] != extra[db][i];
+                more = !__all(all_nan || row >= s.q);
             }
         }
 #pragma unroll

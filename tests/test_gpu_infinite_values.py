@@ -167,3 +167,21 @@ def test_a_nan_token_beside_infinite_values():
     rest[3] = False
     assert (out[0, [0, 1, 2], 100] == math.inf).all()
     assert torch.isfinite(out[0, 4:]).all() and torch.isfinite(out[1]).all() and torch.isfinite(out[0, rest][:, :100]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_nan_alone_beside_rows_that_see_less(dtype):
+    """The search for such values may end early where everything is NaN: not before rows that see other ones are done."""
+    import r2omni_amd as ro
+
+    dev = _cuda()
+    q, k, v = _rows(dev, 1, 4, 2, 400, 400, dtype, seed=11)
+    clean, _ = ro.prompt_attention(q, k, v, window=90, sinks=3)
+    v[:, :, 100:140] = math.nan
+    v[:, :, 250, 3], v[:, :, 310, 3], v[:, :, 2, 9] = math.inf, -math.inf, -math.inf
+    for window, sinks in ((90, 3), (None, 0)):
+        out, _ = ro.prompt_attention(q, k, v, window=window, sinks=sinks)
+        seen = visible(400, 400, 400, 400, window, sinks, dev)
+        for h in range(4):
+            want = _want(clean[0, h] if window else out[0, h].nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), seen, v[0, h // 2])
+            _same(out[0, h], want)
