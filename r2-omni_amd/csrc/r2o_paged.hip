@@ -273,9 +273,11 @@ __device__ __forceinline__ void read_values(uint32_t row, uint32_t chunk, int d,
 // two LDS stages: the next tile's loads go out before this one's products, its page ids one tile earlier still.
 // S^T = K Q^T (16 slots x 16 heads a product), O^T += V^T P^T; P^T's operand is the C registers of S^T as they are: the
 // slots of a product are summed in that order on both sides.
-// Bound by the rows' bytes: a ragged batch of 252 MB takes 50 us, 5.0 TB/s of the 5.9 that a streaming read reaches, about
-// 5 of it the first loads and the last join.  One workgroup a compute unit, whose LDS it fills: with twice as many, a
-// windowed batch of 251 MB takes 54.3 us instead of 51.2.
+// Bound by the rows' bytes: a ragged batch of 252 MB takes 51 us, 4.9 TB/s of the 5.9 that a streaming read reaches (52 in
+// turn with four other caches, 1.3 GB in all), about 5 of it the first loads and the last join.  One workgroup a compute unit,
+// whose LDS it fills: with twice as many, a windowed batch of 251 MB takes 54.3 us instead of 51.2.
+// The probabilities are rounded to the rows' 16 bits for the product with V, whose two operands are of one type; their sum
+// and the slots' weights take them unrounded.  The results' error against 64 bits is that of their own rounding.
 template <int RF, bool WEIGHTS>
 __global__ __launch_bounds__(256, 1) void paged_partial_kernel(AttentionArgs) {
     __shared__ __align__(16) unsigned char lds[kWaves][2][kStage];
@@ -568,7 +570,7 @@ __device__ __forceinline__ void seen_not_finite(const Tiles& t, const Share& sha
 
 // Blocks below batch x hq: one (request, query head) each, the partial outputs joined.  Blocks behind them: an even
 // share of all tiles each, whose slots' weights grow by their probabilities.  Bound by its launch and its round trips: 5
-// us for a call without weights, 11.1 for a ragged batch of 252 MB with them.
+// us for a call without weights, 10.9 for a ragged batch of 252 MB with them.
 template <int RF>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttentionArgs) {
     Args& a = kernel_args();
@@ -740,7 +742,8 @@ __device__ __forceinline__ int waves_before(int x, int wave, int& all) {
 // rounds.  Then every wave knows how many slots before its own stay, and writes its own in order: those above T, and of
 // the equal ones the first.  The counts do not depend on the order of their additions.
 // Bound by one compute unit's instructions: 8 rows of 65409 slots take 23 us (16 waves a row; loads 1.3 us of it, forming
-// the keys 5, three rounds 10, places 6), of 2112 slots 6.6 us.  Comparing all keys with one trial after another, 13 to 20
+// the keys 5, three rounds 10, places 6), of 2112 slots 6.6 us.  Rows past 65536 slots are read again in each pass: a call on
+// 8 rows of 131072 slots takes 95 us, on 8 of 65409 35.  Comparing all keys with one trial after another, 13 to 20
 // times, took 45 us; narrowing by trials and then among 8192 listed ones 43 us.  Rows of one compute unit's registers stay
 // within one kernel: counts joined over several would cost a launch, some 4 us, a round.
 struct SelectLds {

@@ -204,12 +204,16 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
 // stand at 128 / group neighbouring positions, so its last tiles are masked in part for few of them, and a chunk of few
 // rows fills it.  grid: (row tiles x pairs of request and KV head, splits); with splits each takes a share of the key tiles and
 // leaves (maximum, sum, products) in scratch for prompt_join_kernel.
-// 16384 rows of 28 heads over 4: 1983 us, 970 TFLOP/s (bf16; a large library product reaches 1270 to 1380); 8192, 5003 and
-// 1231 rows of 32 heads with a window of 1024 and four sinks: 365 us (fp16); 257 rows of 16 heads over 4097 keys: 26 us in 7
-// splits and 7 for the join.  Bound by what runs beside the matrix instructions (staged through registers, the first took 2009
-// us, without LDS reads and writes 1463, without the maximum as well 1070).  A wave of 64 rows reads half as much from LDS,
-// but its 512 registers leave one wave a SIMD: 2693 us; 256 rows a workgroup (8 waves) 1953 against 2009, but 386 against
-// 365 for the windowed batch and 39 against 33 for the 257 rows.  All of a half's V operands read at once, as K's are: 2001.
+// 16384 rows of 28 heads over 4: 1950 us, 987 TFLOP/s (bf16; a large library product reaches 1270 to 1380); 8192, 5003 and
+// 1231 rows of 32 heads with a window of 1024 and four sinks: 366 us (fp16); 257 rows of 16 heads over 4097 keys: 26.5 us in
+// 7 splits and 5.2 for the join.  Bound by what runs beside the matrix instructions.  Of 1968 us (same box), it takes without
+// its reads of LDS 1810, without the loads into it 1715, without either 1568, without the maximum 1841, without all three
+// 1418, without exponentials 1866.  A wave of 64 rows reads half as much from LDS, but its 512 registers leave one wave a
+// SIMD: 2693 us; 256 rows a workgroup (8 waves) 1953 against 2009 then, but 386 against 365 for the windowed batch and 39
+// against 33 for the 257 rows.  All of a half's V operands read at once, as K's are: 2001 against 1999.
+// The probabilities are rounded to the rows' 16 bits, at most half a step each, for the product with V, whose two operands
+// are of one type; their sum takes them unrounded.  The results' error against 64 bits is that of their own rounding: 1.7e-3
+// (bf16) and 2.1e-4 (fp16), as with probabilities of 32 bits.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     // K tiles t and t + 1, V tiles t to t + 2: two workgroups fill a compute unit's 160 KB
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
     auto seen_in_part = [&](int kt) { return !(kt + kTile - 1 <= wg_min && (kt > wg_max - window || kt + kTile <= sinks)); };
     // The next tile but one goes straight into LDS while the next one is computed on: K into the buffer that every wave
     // has left behind the last barrier, V into the third one.  The transposing reads that follow wait for it, long after
-    // it went out.  16384 rows of 28 heads take 1983 us so, 2057 through registers.
+    // it went out.  16384 rows of 28 heads took 1983 us so, 2057 through registers.
     bool bad = false;
     auto stage = [&](int it, int v_at) {
         stage_rows<0>(kbase, k_row, tile_key(it), last, k_lds[it & 1], wave, lane);
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(PromptArgs) {
 }
 
 // 32 lanes a packed row: its splits' states, joined in order.  Bound by its launch and one round trip to the partial
-// states: 257 rows of 16 heads in 7 splits (15 MB) take 7 us.
+// states: 257 rows of 16 heads in 7 splits (15 MB) take 5.2 us.
 template <int RF>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs, int splits) {
     Args& a = kernel_args();
@@ -486,9 +490,11 @@ constexpr int kWeightKeys = 256;  // keys of a workgroup: 4 waves of 64, whose r
 // A split takes a share of the (query head, 64-row tile) pairs that see the key tile; its sums go to `weights` ([splits,
 // batch, hkv, keys]; the result itself where there is one split).  S = Q K^T: a lane sums its own two keys.  A row tile is two halves of 32; the products of the half that follows run beside the
 // exponentials of the one before it.  The sums carry what an addition rounds off along: 8192 terms of very different size.
-// Bound by vector instructions, of which an exponential, its argument and an addition a pair alone take 125 us of the
-// 169 that 8192 rows of 16 heads take over as many keys (813 TFLOP/s of products); with 32 keys a wave, that is twice the
-// reads of Q, 320.  64 rows of 28 heads over 32641 keys: 30 us.
+// Bound by the sum of what each pair needs, no one part of it: 8192 rows of 16 heads over as many keys take 172 us (799
+// TFLOP/s of products), without the products 128, without exponentials 153, without their arguments as well 134, without
+// the reads of Q from LDS 157, without the load of K 165; with 32 keys a wave, that is twice the reads of Q, 320 against 236
+// then.  64 rows of 28 heads over 32641 keys: 30 to 32 us, of which 10.5 are the launch, K's load, the first row tile and the
+// sums' way out, 21 the other row tiles; without the products 24.5, without the load of K 28.4.
 template <int RF>
 __global__ __launch_bounds__(256, 2) void attention_weights_kernel(PromptArgs) {
     __shared__ __align__(16) unsigned char q_lds[2][kTileBytes];

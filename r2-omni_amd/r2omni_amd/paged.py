@@ -161,7 +161,8 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
     ``window`` and the first ``sinks`` slots are seen.  Where the cache keeps weights, the weight of every slot seen
     grows by its probability summed over the query heads of its group (the appended slot's is set to it); a
     ``dataclasses.replace(cache, weight_pages=None)`` leaves them alone.  A request that sees no slot (an idle one of
-    length 0) gets 0 and lse -inf.  ``output``: the two contiguous result tensors."""
+    length 0) gets 0 and lse -inf; infinite and NaN values count as in ``prompt_attention``.  ``output``: the two
+    contiguous result tensors."""
     if output is None:
         made = _lib.host().paged_attention(_lib.entry("r2o_paged_attention"), cache, query, append, window, sinks, sm_scale)
         if made is not None:

@@ -94,7 +94,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     The last query row of a request stands at its last key, so Sq < Sk is a chunk of a longer prompt.
     ``query_lengths`` / ``key_lengths`` (int32 [B] on the device): the rows of each request of a padded batch.
     With ``window``, a row sees its last ``window`` keys and the first ``sinks``.  A row that sees no key, or lies
-    behind its request's length, is 0 with lse -inf; values of rows behind a length are never used.  Strided views
+    behind its request's length, is 0 with lse -inf; values of rows behind a length are never used.  A value that is
+    infinite or NaN in a row that counts is its channel's result there, however small its weight.  Strided views
     are read in place where the channels are unit-strided and rows 16-byte aligned (copied otherwise).  ``output``:
     the two result tensors to write, the first with such strides, neither overlapping an input."""
     if output is None:
