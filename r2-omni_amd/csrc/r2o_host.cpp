@@ -424,7 +424,7 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Workgroups that share the keys of one tile of 128 packed rows: as many as give a compute unit one, at most one for each 256
 // keys, begun ones among them, that the tile sees: its rows stand at 128 / group neighbouring positions, so with a window
-// these are the window's, as many more, the sinks, and what the first key tile holds before them.  257 rows of 16 heads over
+// these are the window's, 128 / group more, the sinks and what else the first of its key tiles holds.  257 rows of 16 heads over
 // 4097 keys take 28.4 us in 7 splits (one a compute unit), 30 in 6, 32 in 8, 91 in one; 512 rows of 16 heads with a window of
 // 256 15.9 in 2, 19.8 in 4, 14.0 in one; one row of 28 heads over 300 keys 10.7 in 2, 11.2 in one.
 int64_t attention_splits(int64_t batch, int64_t hq, int64_t hkv, int64_t queries, int64_t keys, int64_t window, int64_t sinks, int64_t cus) {

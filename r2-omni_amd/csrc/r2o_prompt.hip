@@ -206,7 +206,7 @@ __device__ __forceinline__ Lengths request_lengths(Args& a, int b) {
 // leaves (maximum, sum, products) in scratch for prompt_join_kernel.
 // 16384 rows of 28 heads over 4: 1950 us, 987 TFLOP/s (bf16; a large library product reaches 1270 to 1380); 8192, 5003 and
 // 1231 rows of 32 heads with a window of 1024 and four sinks: 366 us (fp16); 257 rows of 16 heads over 4097 keys: 26.5 us in
-// 7 splits and 5.2 for the join.  Bound by what runs beside the matrix instructions.  Of 1968 us (same box), it takes without
+// 7 splits and 5.2 for the join.  Bound by what runs beside the matrix instructions.  Of 1968 us (one card), it takes without
 // its reads of LDS 1810, without the loads into it 1715, without either 1568, without the maximum 1841, without all three
 // 1418, without exponentials 1866.  A wave of 64 rows reads half as much from LDS, but its 512 registers leave one wave a
 // SIMD: 2693 us; 256 rows a workgroup (8 waves) 1953 against 2009 then, but 386 against 365 for the windowed batch and 39

@@ -39,8 +39,9 @@ class PagedCache:
     Slot j of request b is slot ``j % page_size`` of page ``page_table[b, j // page_size]``, for every KV head, and
     the first ``lengths[b]`` slots are filled.  A page id outside the pool (such as -1 for a page not handed out)
     makes its slots invisible: they are neither read nor written.  Requests may share pages that no call writes to
-    (one row of ids expanded for all of them serves); a page whose rows or weights are written stands in the tables once.  Pool and head strides are free (views of one
-    pool for both, or for all layers, serve), as long as channels are unit-strided and rows 16-byte aligned."""
+    (one row of ids expanded for all of them serves); a page whose rows or weights are written stands in the tables
+    once.  Pool and head strides are free (views of one pool for both, or for all layers, serve), as long as channels
+    are unit-strided and rows 16-byte aligned."""
 
     key_pages: torch.Tensor                     # bf16 / fp16 [pages, Hkv, page_size, 128]
     value_pages: torch.Tensor
