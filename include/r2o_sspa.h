@@ -578,6 +578,78 @@ typedef struct r2o_paged_evict_params {
 } r2o_paged_evict_params;
 int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream);
 
+/* Attention of each request's newest rows over a prefix that it shares with its neighbours and over its own slots.
+ * Requests 0 .. members[0] - 1 share prefix 0, the next members[1] prefix 1, and so on (counts below 0, or past the batch's
+ * end, are cut off there; members NULL: all share prefix 0); requests behind the last have none.  `cache` holds the
+ * requests' own slots (lengths count the new rows), `prefix` the prefixes', its table's rows and lengths one a prefix; batch 0:
+ * there is none, and its other fields are not looked at.  Both keep no weights, and have the same heads and type; pools, page sizes
+ * and tables may differ.  Row i of a request with q rows (query_lengths [batch], NULL for all; clamped) and n slots of its own
+ * sees every slot of its prefix and its own slots j <= n - q + i; slots without a page are not seen.  Every row is written: one that
+ * sees no slot, or lies behind q, is 0 with lse -inf.  Infinite and NaN values as in r2o_prompt_attention.  Two launches; no
+ * atomics, so equal calls give equal bits. */
+typedef struct r2o_paged_prefix_params {
+    r2o_paged_cache cache, prefix;
+    const int32_t* members;   /* [prefix.batch] */
+    const int32_t* query_lengths;
+    const uint16_t* query;    /* [batch, hq, rows, 128], element strides (batch, head, row), the rows' at most 2^24 */
+    uint16_t* out;            /* as query */
+    float* lse;               /* [batch, hq, rows], contiguous */
+    int64_t q_strides[3], o_strides[3];
+    int64_t hq, rows;         /* batch * hq * rows at most 2^30 */
+    float sm_scale;           /* positive and finite */
+    float* scratch;           /* 16-byte aligned */
+    int64_t scratch_floats;   /* at least 130 (256 workers + r), r = 2 batch hq rows with prefixes and hq / hkv * rows < 128, else 0 */
+    int64_t workers;          /* workgroups that share the slots */
+} r2o_paged_prefix_params;
+int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream);
+
+/* -------------------------------------------------------- rotation by positions ---- */
+
+/* Channel pair (i, i + 64) of a row turns by the angle position * inv_freq[i] of its axis: axis 1 or 2 where bit i of pairs_1
+ * or pairs_2 is set (both never are), axis 0 elsewhere.  Angles are formed in 64 bits; cosine and sine are
+ * multiplied by `scaling`.  With q_weight and k_weight (both or neither, [128], the rows' type) a row is first divided by
+ * sqrt(mean of squares + eps) and multiplied by its weights.  All in fp32, one rounding at the end. */
+typedef struct r2o_rotation {
+    const void* positions;    /* integers of position_bytes (4 or 8) bytes, element strides (axis, batch, token) */
+    int64_t position_strides[3], position_bytes, axes; /* 1 to 3 */
+    const void* inv_freq;     /* [64], fp32 or fp64: freq_bytes 4 or 8 */
+    int64_t freq_bytes;
+    uint64_t pairs_1, pairs_2;
+    const uint16_t* q_weight;
+    const uint16_t* k_weight;
+    float eps, scaling;       /* finite; eps at least 0 */
+} r2o_rotation;
+
+/* Q and K rotated, optionally followed by the orthonormal FWHT-128.  Element strides (batch, head, token), multiples of 8;
+ * rows 16-byte aligned with unit-strided channels, dtype 0 = bf16, 1 = fp16.  A result may be its operand, in place. */
+typedef struct r2o_position_rope_params {
+    r2o_rotation rotation;
+    const uint16_t* query;    /* [batch, hq, tokens, 128] */
+    const uint16_t* key;      /* [batch, hkv, tokens, 128] */
+    uint16_t* query_out;
+    uint16_t* key_out;
+    int64_t q_strides[3], k_strides[3], qo_strides[3], ko_strides[3];
+    int64_t batch, hq, hkv, tokens, dtype, hadamard;
+} r2o_position_rope_params;
+int r2o_position_rope(const r2o_position_rope_params* p, void* stream);
+
+/* r2o_paged_extend of rotated keys, and their queries rotated: row i of request b (i < counts[b], all `rows` without counts) is
+ * its slot lengths[b] - counts[b] + i.  positions NULL: a row's slot is its position on every axis.  Query rows behind a
+ * request's count are 0 in query_out. */
+typedef struct r2o_paged_rope_extend_params {
+    r2o_paged_cache cache;
+    r2o_rotation rotation;
+    const uint16_t* query;    /* [batch, hq, rows, 128]; strides as above */
+    const uint16_t* key;      /* [batch, hkv, rows, 128] */
+    const uint16_t* value;
+    uint16_t* query_out;
+    const float* weights;     /* fp32 [batch, hkv, rows], element strides (batch, head), or NULL */
+    const int32_t* counts;
+    int64_t q_strides[3], k_strides[3], v_strides[3], qo_strides[3], weights_strides[2];
+    int64_t hq, rows;
+} r2o_paged_rope_extend_params;
+int r2o_paged_rope_extend(const r2o_paged_rope_extend_params* p, void* stream);
+
 /* Library identification: returns the gfx target the code objects were built for. */
 const char* r2o_build_target(void);
 

@@ -723,6 +723,209 @@ PyObject* paged_evict_call(PyObject* const* args) {
     return status_and(launch_on(args[0], p, source.device), {kept});
 }
 
+// ------------------------------------------------------------------------ positions and prefixes
+PyObject* const kZero = PyLong_FromLong(0);
+PyObject* const kRotaryFields[7] = {PyUnicode_InternFromString("inv_freq"),      PyUnicode_InternFromString("mrope_section"),
+                                    PyUnicode_InternFromString("interleaved"),   PyUnicode_InternFromString("scaling"),
+                                    PyUnicode_InternFromString("q_norm_weight"), PyUnicode_InternFromString("k_norm_weight"),
+                                    PyUnicode_InternFromString("eps")};
+
+bool plain_float(PyObject* o, float& v) {
+    if (!PyFloat_CheckExact(o)) return false;
+    v = (float)PyFloat_AS_DOUBLE(o);
+    return std::isfinite(v);
+}
+
+// A PositionRotary's fields, held for a call.
+struct Rotary {
+    PyObject* fields[7] = {};
+    r2o_rotation r{};
+    ~Rotary() {
+        for (PyObject* o : fields) Py_XDECREF(o);
+    }
+    bool read(PyObject* rotary, int dtype, int64_t device);  // false for what the Python path has to look at
+    bool place(PyObject* positions, int64_t batch, int64_t tokens, int64_t device);
+};
+
+bool Rotary::read(PyObject* rotary, int dtype, int64_t device) {
+    for (int i = 0; i < 7; ++i)
+        if (!(fields[i] = PyObject_GetAttr(rotary, kRotaryFields[i]))) {
+            PyErr_Clear();
+            return false;
+        }
+    const at::Tensor* freq = exact_tensor(fields[0]);
+    if (!freq || !on_device(*freq, device) || freq->dim() != 1 || freq->size(0) != 64 || !freq->is_contiguous() || needs_grad(*freq) ||
+        (freq->scalar_type() != at::kFloat && freq->scalar_type() != at::kDouble))
+        return false;
+    r.inv_freq = freq->data_ptr();
+    r.freq_bytes = freq->scalar_type() == at::kDouble ? 8 : 4;
+    if (!PyTuple_CheckExact(fields[1]) || !PyBool_Check(fields[2]) || !plain_float(fields[3], r.scaling) || !plain_float(fields[6], r.eps) || r.eps < 0.f)
+        return false;
+    r.axes = PyTuple_GET_SIZE(fields[1]);
+    if (r.axes < 1 || r.axes > 3) return false;
+    int64_t n[3] = {}, sum = 0;
+    for (int i = 0; i < r.axes; ++i) {
+        if (!plain_int(PyTuple_GET_ITEM(fields[1], i), n[i]) || n[i] < 0 || n[i] > 64) return false;
+        sum += n[i];
+    }
+    if (sum != 64) return false;
+    const bool interleaved = fields[2] == Py_True;
+    int64_t taken[3] = {};
+    for (int i = 0; i < 64; ++i) {
+        const int axis = interleaved ? (i % 3 < r.axes && i < 3 * n[i % 3] ? i % 3 : 0) : (i < n[0] ? 0 : (i < n[0] + n[1] ? 1 : 2));
+        ++taken[axis];
+        if (axis) (axis == 1 ? r.pairs_1 : r.pairs_2) |= (uint64_t)1 << i;
+    }
+    for (int i = 0; i < r.axes; ++i)
+        if (taken[i] != n[i]) return false;
+    if ((fields[4] == Py_None) != (fields[5] == Py_None)) return false;
+    if (fields[4] == Py_None) return true;
+    for (int i : {4, 5}) {
+        const at::Tensor* w = exact_tensor(fields[i]);
+        if (!w || !on_device(*w, device) || row_code(*w) != dtype || w->dim() != 1 || w->size(0) != R2O_HEAD_DIM || !w->is_contiguous() ||
+            !aligned16(*w) || needs_grad(*w))
+            return false;
+        (i == 4 ? r.q_weight : r.k_weight) = static_cast<const uint16_t*>(w->data_ptr());
+    }
+    return true;
+}
+
+bool Rotary::place(PyObject* positions, int64_t batch, int64_t tokens, int64_t device) {
+    const at::Tensor* t = exact_tensor(positions);
+    if (!t || !on_device(*t, device) || (t->scalar_type() != at::kLong && t->scalar_type() != at::kInt)) return false;
+    const int64_t axes = t->dim() == 3 ? t->size(0) : 1, first = t->dim() - 2;
+    if ((t->dim() != 3 && t->dim() != 2) || axes != r.axes || t->size(first) != batch || t->size(first + 1) != tokens) return false;
+    r.positions = t->data_ptr();
+    r.position_bytes = t->scalar_type() == at::kLong ? 8 : 4;
+    for (int64_t i = 0; i < t->dim(); ++i) r.position_strides[3 - t->dim() + i] = t->size(i) > 1 ? t->stride(i) : 0;
+    return true;
+}
+
+// Q [B, Hq, S, 128] and K [B, Hkv, S, 128] in place, and a result like Q.
+bool heads_arg(const at::Tensor* t, int64_t device, int64_t* strides) {
+    return t && t->dim() == 4 && t->size(3) == R2O_HEAD_DIM && t->size(0) > 0 && t->size(1) > 0 && t->size(2) > 0 && on_device(*t, device) &&
+           row_code(*t) >= 0 && !needs_grad(*t) && row_strides(*t, 3, strides) && strides[2] <= R2O_MAX_ROW_STRIDE;
+}
+
+// position_rope(function, query, key, positions, rotary, hadamard): (status, query, key) or None
+PyObject* position_rope_call(PyObject* const* args) {
+    r2o_position_rope_params p{};
+    const int64_t device = current_device();
+    const at::Tensor *q = exact_tensor(args[1]), *k = exact_tensor(args[2]);
+    if (!heads_arg(q, device, p.q_strides) || !heads_arg(k, device, p.k_strides) || q->scalar_type() != k->scalar_type() ||
+        q->size(0) != k->size(0) || q->size(2) != k->size(2) || !PyBool_Check(args[5]))
+        Py_RETURN_NONE;
+    p.dtype = row_code(*q);
+    p.batch = q->size(0);
+    p.hq = q->size(1);
+    p.hkv = k->size(1);
+    p.tokens = q->size(2);
+    p.hadamard = args[5] == Py_True;
+    Rotary rotary;
+    if (!rotary.read(args[4], (int)p.dtype, device) || !rotary.place(args[3], p.batch, p.tokens, device) || p.batch * p.tokens > 0x7fffffff)
+        Py_RETURN_NONE;
+    p.rotation = rotary.r;
+    at::Tensor q_out = at::empty_like(*q), k_out = at::empty_like(*k);
+    if (!row_strides(q_out, 3, p.qo_strides, true) || !row_strides(k_out, 3, p.ko_strides, true)) Py_RETURN_NONE;
+    p.query = static_cast<const uint16_t*>(q->data_ptr());
+    p.key = static_cast<const uint16_t*>(k->data_ptr());
+    p.query_out = static_cast<uint16_t*>(q_out.data_ptr());
+    p.key_out = static_cast<uint16_t*>(k_out.data_ptr());
+    return status_and(launch_on(args[0], p, device), {q_out, k_out});
+}
+
+// paged_rope_extend(function, cache, query, key, value, rotary, positions, counts, weights): (status, query) or None
+PyObject* paged_rope_extend_call(PyObject* const* args) {
+    r2o_paged_rope_extend_params p{};
+    Cache cache;
+    if (!cache.read(args[1]) || !cache.callable()) Py_RETURN_NONE;
+    const int64_t device = cache.device;
+    const r2o_paged_cache& c = p.cache = cache.c;
+    const at::Tensor *q = exact_tensor(args[2]), *k = exact_tensor(args[3]), *v = exact_tensor(args[4]);
+    if (one_row(c) || !heads_arg(q, device, p.q_strides) || !heads_arg(k, device, p.k_strides) || !heads_arg(v, device, p.v_strides) ||
+        row_code(*q) != c.dtype || row_code(*k) != c.dtype || row_code(*v) != c.dtype || q->size(0) != c.batch || k->size(0) != c.batch ||
+        k->size(1) != c.hkv || q->size(2) != k->size(2) || v->sizes() != k->sizes())
+        Py_RETURN_NONE;
+    p.hq = q->size(1);
+    p.rows = q->size(2);
+    if (p.rows > c.max_pages * c.page_size || c.batch * p.rows > 0x7fffffff || !lengths_arg(args[7], c.batch, device, p.counts)) Py_RETURN_NONE;
+    if (args[8] != Py_None) {
+        const at::Tensor* w = exact_tensor(args[8]);
+        if (!w || !c.weight_pages || needs_grad(*w) || !on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 ||
+            w->size(0) != c.batch || w->size(1) != c.hkv || w->size(2) != p.rows || !w->is_contiguous())
+            Py_RETURN_NONE;
+        p.weights = w->data_ptr<float>();
+        p.weights_strides[0] = w->stride(0);
+        p.weights_strides[1] = w->stride(1);
+    }
+    Rotary rotary;
+    if (!rotary.read(args[5], (int)c.dtype, device) || (args[6] != Py_None && !rotary.place(args[6], c.batch, p.rows, device))) Py_RETURN_NONE;
+    p.rotation = rotary.r;
+    at::Tensor q_out = at::empty_like(*q);
+    if (!row_strides(q_out, 3, p.qo_strides, true)) Py_RETURN_NONE;
+    p.query = static_cast<const uint16_t*>(q->data_ptr());
+    p.key = static_cast<const uint16_t*>(k->data_ptr());
+    p.value = static_cast<const uint16_t*>(v->data_ptr());
+    p.query_out = static_cast<uint16_t*>(q_out.data_ptr());
+    return status_and(launch_on(args[0], p, device), {q_out});
+}
+
+// Key tiles of a call of the prefix attention, at most: whatever the lengths on the device say.
+bool merged_rows(int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes) { return prefixes && hq / hkv * rows < 128; }
+
+int64_t prefix_tiles(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t capacity, int64_t prefixes, int64_t prefix_capacity) {
+    const int64_t packed = hq / hkv * rows, own = div_up(capacity, 64), shared = prefixes ? div_up(prefix_capacity, 64) : 0;
+    return merged_rows(hkv, hq, rows, prefixes) ? hkv * ((batch * packed / 128 + prefixes) * shared + batch * own)
+                                                : hkv * batch * div_up(packed, 128) * (shared + own);
+}
+
+// Workgroups that share them: two a compute unit, whose LDS they fill, of two tiles at least.
+int64_t prefix_workers(int64_t tiles, int64_t cus) { return std::max<int64_t>(1, std::min(2 * cus, div_up(tiles, 2))); }
+
+int64_t prefix_scratch(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes, int64_t workers) {
+    return 130 * (256 * workers + (merged_rows(hkv, hq, rows, prefixes) ? 2 * batch * hq * rows : 0));
+}
+
+// paged_prefix_attention(function, query, cache, prefix or None, members, query_lengths, scale): (status, out, lse) or None
+PyObject* paged_prefix_attention_call(PyObject* const* args) {
+    r2o_paged_prefix_params p{};
+    Cache cache, prefix;
+    if (!cache.read(args[2]) || !cache.callable() || cache.c.weight_pages) Py_RETURN_NONE;
+    const int64_t device = cache.device;
+    const r2o_paged_cache &c = p.cache = cache.c, &f = p.prefix;
+    if (args[3] != Py_None) {
+        if (!prefix.read(args[3]) || !prefix.callable() || prefix.c.weight_pages) Py_RETURN_NONE;
+        p.prefix = prefix.c;
+        if (f.hkv != c.hkv || f.dtype != c.dtype || (f.batch > 1 && args[4] == Py_None)) Py_RETURN_NONE;
+    } else if (args[4] != Py_None) {
+        Py_RETURN_NONE;
+    }
+    const at::Tensor* q = exact_tensor(args[1]);
+    if (!cache_rows(q, c, device) || (q->dim() != 3 && q->dim() != 4) || q->size(0) != c.batch || q->size(-1) != R2O_HEAD_DIM) Py_RETURN_NONE;
+    const int64_t axes = q->dim() - 1;
+    p.hq = q->size(1);
+    p.rows = axes == 3 ? q->size(2) : 1;
+    int64_t window, sinks;
+    if (p.hq < 1 || p.hq % c.hkv || p.rows < 1 || p.hq * p.rows > (1 << 30) || c.batch * p.hq * p.rows > (1 << 30) ||
+        !row_strides(*q, axes, p.q_strides) || p.q_strides[2] > R2O_MAX_ROW_STRIDE ||
+        !mask_args(Py_None, kZero, args[6], window, sinks, p.sm_scale) || !lengths_arg(args[4], f.batch, device, p.members) ||
+        !lengths_arg(args[5], c.batch, device, p.query_lengths))
+        Py_RETURN_NONE;
+    const int64_t tiles = prefix_tiles(c.batch, c.hkv, p.hq, p.rows, c.max_pages * c.page_size, f.batch, f.max_pages * f.page_size);
+    if (tiles > 0x7fffffff - R2O_PAGED_MAX_WORKERS) Py_RETURN_NONE;
+    at::Tensor out = at::empty_like(*q);
+    if (!row_strides(out, axes, p.o_strides, true) || p.o_strides[2] > R2O_MAX_ROW_STRIDE) Py_RETURN_NONE;
+    p.workers = prefix_workers(tiles, compute_units((int)device));
+    p.scratch_floats = prefix_scratch(c.batch, c.hkv, p.hq, p.rows, f.batch, p.workers);
+    const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
+    at::Tensor lse = at::empty(q->sizes().slice(0, axes), f32), scratch = at::empty({p.scratch_floats}, f32);
+    p.query = static_cast<const uint16_t*>(q->data_ptr());
+    p.out = static_cast<uint16_t*>(out.data_ptr());
+    p.lse = lse.data_ptr<float>();
+    p.scratch = scratch.data_ptr<float>();
+    return status_and(launch_on(args[0], p, device), {out, lse});
+}
+
 template <PyObject* (*CALL)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != N) Py_RETURN_NONE;
@@ -751,6 +954,24 @@ PyObject* paged_workers_rule(PyObject*, PyObject* args) {
     return PyLong_FromLongLong(paged_workers(x[0], x[1], x[2], x[3]));
 }
 
+PyObject* prefix_tiles_rule(PyObject*, PyObject* args) {
+    long long x[7];
+    if (!PyArg_ParseTuple(args, "LLLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5, x + 6)) return nullptr;
+    return PyLong_FromLongLong(prefix_tiles(x[0], x[1], x[2], x[3], x[4], x[5], x[6]));
+}
+
+PyObject* prefix_workers_rule(PyObject*, PyObject* args) {
+    long long x[2];
+    if (!PyArg_ParseTuple(args, "LL", x, x + 1)) return nullptr;
+    return PyLong_FromLongLong(prefix_workers(x[0], x[1]));
+}
+
+PyObject* prefix_scratch_rule(PyObject*, PyObject* args) {
+    long long x[6];
+    if (!PyArg_ParseTuple(args, "LLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5)) return nullptr;
+    return PyLong_FromLongLong(prefix_scratch(x[0], x[1], x[2], x[3], x[4], x[5]));
+}
+
 #define FAST(call, n) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<call, n>)), METH_FASTCALL, nullptr
 
 PyMethodDef kMethods[] = {
@@ -763,6 +984,12 @@ PyMethodDef kMethods[] = {
     {"paged_extend", FAST(paged_extend_call, 6)},
     {"paged_attention", FAST(paged_attention_call, 7)},
     {"paged_evict", FAST(paged_evict_call, 6)},
+    {"position_rope", FAST(position_rope_call, 6)},
+    {"paged_rope_extend", FAST(paged_rope_extend_call, 9)},
+    {"paged_prefix_attention", FAST(paged_prefix_attention_call, 7)},
+    {"prefix_tiles", prefix_tiles_rule, METH_VARARGS, nullptr},
+    {"prefix_workers", prefix_workers_rule, METH_VARARGS, nullptr},
+    {"prefix_scratch", prefix_scratch_rule, METH_VARARGS, nullptr},
     {"attention_splits", attention_splits_rule, METH_VARARGS, nullptr},
     {"weight_splits", weight_splits_rule, METH_VARARGS, nullptr},
     {"paged_workers", paged_workers_rule, METH_VARARGS, nullptr},

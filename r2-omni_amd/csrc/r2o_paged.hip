@@ -9,6 +9,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "r2o_cache_check.hpp"
 #include "r2o_common.hpp"
 
 namespace {
@@ -1013,14 +1014,6 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(r2o_paged_evict_para
 }
 
 // ------------------------------------------------------------------------------------ host checks
-bool aligned(const void* p, uintptr_t n) { return p && reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-bool rows_ok(const int64_t* st, int n) {  // the kernels hold strides in 32 bits and multiply into 64
-    for (int i = 0; i < n; ++i)
-        if (st[i] < 0 || st[i] % 8 || st[i] > 0x7fffffff) return false;
-    return true;
-}
-
 // The extend kernel multiplies in 64 bits: a prompt's requests, heads and rows may lie anywhere.
 bool new_rows_ok(const int64_t* st) {
     for (int i = 0; i < 3; ++i)
@@ -1028,28 +1021,12 @@ bool new_rows_ok(const int64_t* st) {
     return true;
 }
 
-// One slot's rows lie within 32-bit offsets of the next ones'.
-bool slots_ok(const r2o_paged_cache& c) { return c.key_strides[2] <= R2O_PAGED_MAX_SLOT_STRIDE && c.value_strides[2] <= R2O_PAGED_MAX_SLOT_STRIDE; }
-
-bool cache_ok(const r2o_paged_cache& c) {
-    return slots_ok(c) && (c.dtype == 0 || c.dtype == 1) && aligned(c.key_pages, 16) && aligned(c.value_pages, 16) && aligned(c.page_table, 4) &&
-           aligned(c.lengths, 4) && reinterpret_cast<uintptr_t>(c.weight_pages) % 4 == 0 && rows_ok(c.key_strides, 3) &&
-           rows_ok(c.value_strides, 3) && c.weight_strides[0] >= 0 && c.weight_strides[0] <= 0x7fffffff && c.weight_strides[1] >= 0 &&
-           c.weight_strides[1] <= 0x7fffffff && (c.table_stride >= c.max_pages || c.table_stride == 0) && c.table_stride <= 0x7fffffff &&
-           c.pages >= 1 && c.pages <= 0x7fffffff && c.max_pages >= 1 && c.batch >= 1 && c.batch <= R2O_PAGED_MAX_BATCH &&
-           c.hkv >= 1 && c.hkv <= 1024 &&
-           (c.page_size == 16 || c.page_size == 32 || c.page_size == 64 || c.page_size == 128) && c.max_pages <= (1 << 29) / c.page_size;
-}
-
-// One row of page ids for all requests: their pages may be read, not written.
-bool one_row(const r2o_paged_cache& c) { return c.batch > 1 && c.table_stride == 0; }
-
 }  // namespace
 
 extern "C" {
 
 int r2o_paged_extend(const r2o_paged_extend_params* p, void* stream) {
-    if (!p || !cache_ok(p->cache) || one_row(p->cache) || !aligned(p->key, 16) || !aligned(p->value, 16) || !new_rows_ok(p->key_strides) ||
+    if (!p || !r2o_paged_cache_ok(p->cache) || r2o_one_row(p->cache) || !r2o_aligned(p->key, 16) || !r2o_aligned(p->value, 16) || !new_rows_ok(p->key_strides) ||
         !new_rows_ok(p->value_strides) || p->rows < 1 || p->rows > (1 << 29) || reinterpret_cast<uintptr_t>(p->counts) % 4 ||
         reinterpret_cast<uintptr_t>(p->weights) % 4 || p->weights_strides[0] < 0 || p->weights_strides[1] < 0 ||
         (p->weights && !p->cache.weight_pages))
@@ -1061,22 +1038,22 @@ int r2o_paged_extend(const r2o_paged_extend_params* p, void* stream) {
 }
 
 int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream) {
-    if (!p || !cache_ok(p->cache)) return R2O_EINVAL;
+    if (!p || !r2o_paged_cache_ok(p->cache)) return R2O_EINVAL;
     const r2o_paged_cache& c = p->cache;
     const int64_t group = p->hq / c.hkv, pairs = c.batch * c.hkv;
-    if (p->hq < c.hkv || p->hq % c.hkv || group > R2O_MAX_GQA || !aligned(p->query, 16) || !rows_ok(p->query_strides, 2) ||
-        !aligned(p->out, 16) || !aligned(p->lse, 4) || p->window < 0 || p->sinks < 0 || p->sinks > (1 << 29) || !(p->sm_scale > 0.f) ||
-        !(p->sm_scale < INFINITY) || p->workers < 1 || p->workers > R2O_PAGED_MAX_WORKERS || !aligned(p->partial_out, 16) ||
-        !aligned(p->partial_ml, 8) || p->partial_states < (p->workers + pairs) * group)
+    if (p->hq < c.hkv || p->hq % c.hkv || group > R2O_MAX_GQA || !r2o_aligned(p->query, 16) || !r2o_strides_ok(p->query_strides, 2, 0x7fffffff) ||
+        !r2o_aligned(p->out, 16) || !r2o_aligned(p->lse, 4) || p->window < 0 || p->sinks < 0 || p->sinks > (1 << 29) || !(p->sm_scale > 0.f) ||
+        !(p->sm_scale < INFINITY) || p->workers < 1 || p->workers > R2O_PAGED_MAX_WORKERS || !r2o_aligned(p->partial_out, 16) ||
+        !r2o_aligned(p->partial_ml, 8) || p->partial_states < (p->workers + pairs) * group)
         return R2O_EINVAL;
     if ((p->append_key == nullptr) != (p->append_value == nullptr)) return R2O_EINVAL;
-    if (one_row(c) && (p->append_key || c.weight_pages)) return R2O_EINVAL;
-    if (p->append_key && (!aligned(p->append_key, 16) || !aligned(p->append_value, 16) || !rows_ok(p->append_strides, 4)))
+    if (r2o_one_row(c) && (p->append_key || c.weight_pages)) return R2O_EINVAL;
+    if (p->append_key && (!r2o_aligned(p->append_key, 16) || !r2o_aligned(p->append_value, 16) || !r2o_strides_ok(p->append_strides, 4, 0x7fffffff)))
         return R2O_EINVAL;
     // every slot that the page tables can hold has room for its logits, whatever the lengths on the device say
     const int64_t tiles = (c.max_pages * c.page_size + kSlots - 1) / kSlots;
     if (pairs * tiles > 0x7fffffff - R2O_PAGED_MAX_WORKERS) return R2O_EINVAL;
-    if (c.weight_pages && (!aligned(p->logits, 16) || p->logits_floats < pairs * tiles * kSlots * group)) return R2O_EINVAL;
+    if (c.weight_pages && (!r2o_aligned(p->logits, 16) || p->logits_floats < pairs * tiles * kSlots * group)) return R2O_EINVAL;
     AttentionArgs a{};
     a.key = c.key_pages;
     a.value = c.value_pages;
@@ -1135,11 +1112,11 @@ int r2o_paged_attention(const r2o_paged_attention_params* p, void* stream) {
 }
 
 int r2o_paged_evict(const r2o_paged_evict_params* p, void* stream) {
-    if (!p || !cache_ok(p->source) || !cache_ok(p->target)) return R2O_EINVAL;
+    if (!p || !r2o_paged_cache_ok(p->source) || !r2o_paged_cache_ok(p->target)) return R2O_EINVAL;
     const r2o_paged_cache &c = p->source, &o = p->target;
-    if (!c.weight_pages || one_row(o) || c.dtype != o.dtype || c.batch != o.batch || c.hkv != o.hkv || p->keep < 1 ||
+    if (!c.weight_pages || r2o_one_row(o) || c.dtype != o.dtype || c.batch != o.batch || c.hkv != o.hkv || p->keep < 1 ||
         p->keep > o.max_pages * o.page_size || p->sinks < 0 || p->recent < 0 || p->sinks > p->keep || p->recent > p->keep - p->sinks ||
-        !aligned(p->kept, 4) || !aligned(p->target_lengths, 4) || std::abs(p->target_lengths - c.lengths) < c.batch)
+        !r2o_aligned(p->kept, 4) || !r2o_aligned(p->target_lengths, 4) || std::abs(p->target_lengths - c.lengths) < c.batch)
         return R2O_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
     const dim3 rows((unsigned)(c.batch * c.hkv)), threads(kSelectThreads);

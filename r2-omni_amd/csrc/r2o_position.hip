@@ -1,0 +1,277 @@
+// Queries and keys rotated by their positions on up to three axes, for gfx950: into tensors, or the keys, with their
+// values, into their slots of the paged cache.
+//
+// Channel pair (i, i + 64) of a token's row turns by the angle a = position[axis of i] * inv_freq[i]:
+//     y_i = c x_i - s x_{i+64},  y_{i+64} = c x_{i+64} + s x_i,  c = scaling cos a, s = scaling sin a
+// in fp32, with x = w x / sqrt(mean x^2 + eps) before where there are norm weights, and one rounding at the end.
+//
+// A row (128 channels of one (request, head, token)) is 16 lanes of 8 channels, one 16-byte load and store; a channel's
+// partner is lane ^ 8, read by DPP.  A wave takes 4 tokens and walks a run of heads: the 64 angles of a token are formed once
+// for all of them, and 4 heads' rows are in flight at a time.
+#include <algorithm>
+#include <initializer_list>
+
+#include "r2o_cache_check.hpp"
+#include "r2o_common.hpp"
+
+namespace {
+
+struct RotateArgs {
+    r2o_rotation rotation;
+    const uint16_t *q, *k, *v;
+    uint16_t *q_out, *k_out;
+    int64_t q_strides[3], k_strides[3], v_strides[3], qo_strides[3], ko_strides[3], weights_strides[2];
+    r2o_paged_cache cache;  // of a paged call
+    const float* weights;
+    const int32_t* counts;
+    uint32_t items, tokens;  // items: batch * tokens
+    int hq, hkv, heads, heads_per_wave, hadamard;
+};
+
+// cos and sin of 2 pi turns, |turns| at most 1/2.  The quarter turn that is nearest is taken off (exact), the rest, x in
+// [-pi/4, pi/4], goes through the Taylor polynomials of degree 9 and 8: off by at most x^11 / 11! = 1.8e-9 and x^10 / 10! =
+// 2.5e-8, below half a step of fp32 at the cosine's least value there.
+__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
+    const double quarters = 4.0 * turns, n = __builtin_rint(quarters);
+    const float x = (float)((quarters - n) * 1.5707963267948966), x2 = x * x;
+    float p = __builtin_fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);
+    p = __builtin_fmaf(x2, p, 8.3333333e-3f);
+    p = __builtin_fmaf(x2, p, -0.16666667f);
+    const float sx = __builtin_fmaf(x * x2, p, x);
+    float r = __builtin_fmaf(x2, 2.4801587e-5f, -1.3888889e-3f);
+    r = __builtin_fmaf(x2, r, 4.1666667e-2f);
+    r = __builtin_fmaf(x2, r, -0.5f);
+    const float cx = __builtin_fmaf(x2, r, 1.f);
+    const int q = (int)n & 3;
+    const float a = q & 1 ? sx : cx, b = q & 1 ? cx : sx;
+    c = q == 1 || q == 2 ? -a : a;
+    s = q & 2 ? -b : b;
+}
+
+// The position of a token on an axis.
+__device__ __forceinline__ int64_t position_at(const r2o_rotation& r, int axis, int64_t b, int64_t token) {
+    const int64_t at = axis * r.position_strides[0] + b * r.position_strides[1] + token * r.position_strides[2];
+    return r.position_bytes == 8 ? r2o_ldg(reinterpret_cast<const int64_t*>(r.positions) + at)
+                                 : (int64_t)r2o_ldg(reinterpret_cast<const int32_t*>(r.positions) + at);
+}
+
+// cos and sin of the lane's channels 8 c8 .. 8 c8 + 7, the sine with its channel's sign.  A turn is position * (inv_freq / 2
+// pi) without its whole part, in 64 bits: a position of 2^31 leaves it 2^-24 exact.
+__device__ __forceinline__ void angles(const r2o_rotation& r, int64_t b, int64_t token, int64_t slot, int c8, float (&c)[8], float (&s)[8]) {
+    const int d0 = 8 * (c8 & 7);
+    double p0, p1 = 0.0, p2 = 0.0;
+    if (r.positions) {
+        p0 = (double)position_at(r, 0, b, token);
+        if (r.axes > 1) p1 = (double)position_at(r, 1, b, token);
+        if (r.axes > 2) p2 = (double)position_at(r, 2, b, token);
+    } else {
+        p0 = p1 = p2 = (double)slot;
+    }
+    const uint32_t m1 = (uint32_t)(r.pairs_1 >> d0) & 255u, m2 = (uint32_t)(r.pairs_2 >> d0) & 255u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double f = r.freq_bytes == 8 ? r2o_ldg(reinterpret_cast<const double*>(r.inv_freq) + d0 + i)
+                                           : (double)r2o_ldg(reinterpret_cast<const float*>(r.inv_freq) + d0 + i);
+        const double p = m1 >> i & 1 ? p1 : (m2 >> i & 1 ? p2 : p0), t = p * (f * 0.15915494309189535);
+        cos_sin(t - __builtin_rint(t), c[i], s[i]);
+        c[i] *= r.scaling;
+        s[i] *= c8 < 8 ? -r.scaling : r.scaling;
+    }
+}
+
+// One row in place; sn carries the sign of its channel.
+template <bool NORM>
+__device__ __forceinline__ void rotate_row(float (&x)[8], const float (&cs)[8], const float (&sn)[8], const float (&weight)[8], float eps) {
+    if constexpr (NORM) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x[i], x[i], s);
+        s += r2o_lane_xor<8>(s);
+        s += r2o_lane_xor<4>(s);
+        s += r2o_lane_xor<2>(s);
+        s += r2o_lane_xor<1>(s);
+        const float inv = __fdiv_rn(1.f, __fsqrt_rn(__builtin_fmaf(s, 1.f / 128.f, eps)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * weight[i];
+    }
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(r2o_lane_xor<8>(x[i]), sn[i], x[i] * cs[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i];
+}
+
+constexpr int kHeadsInFlight = 4;
+
+// grid (ceil(items / 16), ceil(heads / heads_per_wave)), block 256.  Lanes past the last item work on it again and store
+// nothing: the exchanges need every lane of the wave.
+template <int DT, bool NORM, bool PAGED>
+__global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
+    const int lane = threadIdx.x & 63, c8 = lane & 15;
+    const uint32_t item = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
+    bool live = item < a.items;
+    const uint32_t at = live ? item : a.items - 1, b = at / a.tokens, token = at - b * a.tokens;
+    // of a paged call: whether the row counts, its slot, and where that lies
+    bool counts = true;
+    int64_t slot = 0, key_at = -1, value_at = 0, weight_at = 0;
+    if constexpr (PAGED) {
+        const r2o_paged_cache& c = a.cache;
+        const int n = a.counts ? min(max(r2o_ldg(a.counts + b), 0), (int)a.tokens) : (int)a.tokens;
+        counts = (int)token < n;
+        slot = (int64_t)r2o_ldg(c.lengths + b) - n + token;
+        if (live && counts && slot >= 0 && slot < c.max_pages * c.page_size) {
+            const int shift = 31 - __builtin_clz((int)c.page_size);
+            const int page = r2o_ldg(c.page_table + b * c.table_stride + (slot >> shift));
+            if ((uint32_t)page < (uint32_t)c.pages) {
+                const int64_t in_page = slot & (c.page_size - 1);
+                key_at = page * c.key_strides[0] + in_page * c.key_strides[2] + 8 * c8;
+                value_at = page * c.value_strides[0] + in_page * c.value_strides[2] + 8 * c8;
+                weight_at = page * c.weight_strides[0] + in_page;
+            }
+        }
+    }
+    float cs[8], sn[8], wq[8], wk[8];
+    angles(a.rotation, b, token, slot, c8, cs, sn);
+    if constexpr (NORM) {
+        r2o_unpack8<DT>(r2o_load8<true>(a.rotation.q_weight + 8 * c8), wq);
+        r2o_unpack8<DT>(r2o_load8<true>(a.rotation.k_weight + 8 * c8), wk);
+    }
+    auto in_head = [&](const int64_t (&st)[3]) { return b * st[0] + token * st[2] + 8 * c8; };
+    const int64_t q0 = in_head(a.q_strides), k0 = in_head(a.k_strides), v0 = PAGED ? in_head(a.v_strides) : 0;
+    const int64_t qo0 = in_head(a.qo_strides), ko0 = PAGED ? 0 : in_head(a.ko_strides);
+    const int h_end = min(a.heads, (int)(blockIdx.y + 1) * a.heads_per_wave);
+    for (int h0 = blockIdx.y * a.heads_per_wave; h0 < h_end; h0 += kHeadsInFlight) {
+        r2o_u4 raw[kHeadsInFlight];
+#pragma unroll
+        for (int u = 0; u < kHeadsInFlight; ++u) {  // h is wave-uniform
+            const int h = min(h0 + u, h_end - 1);
+            if (h < a.hq) raw[u] = r2o_load8<true>(a.q + q0 + h * a.q_strides[1]);
+            else if (!PAGED || h < a.hq + a.hkv) raw[u] = r2o_load8<true>(a.k + k0 + (h - a.hq) * a.k_strides[1]);
+            else raw[u] = r2o_load8<true>(a.v + v0 + (h - a.hq - a.hkv) * a.v_strides[1]);
+        }
+#pragma unroll
+        for (int u = 0; u < kHeadsInFlight; ++u) {
+            const int h = h0 + u;
+            if (h >= h_end) break;
+            if (PAGED && h >= a.hq + a.hkv) {
+                if (key_at >= 0) r2o_store8<true>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
+                continue;
+            }
+            float x[8];
+            r2o_unpack8<DT>(raw[u], x);
+            rotate_row<NORM>(x, cs, sn, h < a.hq ? wq : wk, a.rotation.eps);
+            if (!PAGED && a.hadamard) r2o_fwht_row8(x, c8);
+            r2o_u4 y = r2o_pack8<DT>(x);
+            if (h < a.hq) {
+                if (PAGED && !counts) y = r2o_u4{};
+                if (live) r2o_store8<true>(a.q_out + qo0 + h * a.qo_strides[1], y);
+            } else if constexpr (PAGED) {
+                const int64_t kv = h - a.hq;
+                if (key_at >= 0) {
+                    r2o_store8<true>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
+                    if (a.cache.weight_pages && c8 == 0)
+                        a.cache.weight_pages[weight_at + kv * a.cache.weight_strides[1]] =
+                            a.weights ? r2o_ldg(a.weights + b * a.weights_strides[0] + kv * a.weights_strides[1] + token) : 0.f;
+                }
+            } else if (live) {
+                r2o_store8<true>(a.k_out + ko0 + (h - a.hq) * a.ko_strides[1], y);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ host checks
+bool rows_ok(const void* p, const int64_t (&st)[3]) { return r2o_strides_ok(st, 3, INT64_MAX) && r2o_aligned(p, 16); }
+
+bool rotation_ok(const r2o_rotation& r, bool slots) {
+    if (r.axes < 1 || r.axes > 3 || (r.freq_bytes != 4 && r.freq_bytes != 8) || !r2o_aligned(r.inv_freq, r.freq_bytes) || (r.pairs_1 & r.pairs_2) ||
+        (r.axes < 2 && r.pairs_1) || (r.axes < 3 && r.pairs_2) || !(r.eps >= 0.f) || !(r.eps < INFINITY) || !(r.scaling > -INFINITY) ||
+        !(r.scaling < INFINITY) || (r.q_weight == nullptr) != (r.k_weight == nullptr) || (r.q_weight && (!r2o_aligned(r.q_weight, 16) || !r2o_aligned(r.k_weight, 16))))
+        return false;
+    if (!r.positions) return slots;
+    for (int64_t s : r.position_strides)
+        if (s < 0) return false;
+    return (r.position_bytes == 4 || r.position_bytes == 8) && r2o_aligned(r.positions, r.position_bytes);
+}
+
+// Heads of a wave: all of them share its angles, but a call of few tokens is spread over the chip first.  kFullWaves waves are
+// 8 for each SIMD.
+constexpr int64_t kFullWaves = 8192;
+
+template <bool PAGED>
+int launch(RotateArgs& a, int64_t dtype, int64_t batch, int64_t tokens, int64_t heads, hipStream_t st) {
+    const int64_t items = batch * tokens;
+    if (heads > 0x7fffffff / 2 || tokens > 0x7fffffff || batch > 0x7fffffff || items > 0x7fffffff) return R2O_EINVAL;
+    a.items = (uint32_t)items;
+    a.tokens = (uint32_t)tokens;
+    a.heads = (int)heads;
+    const int64_t token_waves = (items + 3) / 4;
+    int64_t per = std::max<int64_t>(1, std::min((heads * token_waves + kFullWaves - 1) / kFullWaves, heads));
+    per = std::max(per, (heads + 65534) / 65535);  // the grid's second dimension
+    a.heads_per_wave = (int)per;
+    const dim3 grid((unsigned)((items + 15) / 16), (unsigned)((heads + per - 1) / per));
+    const bool norm = a.rotation.q_weight != nullptr;
+    if (dtype == 0) {
+        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<0, true, PAGED>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rotate_by_position_kernel<0, false, PAGED>), grid, dim3(256), 0, st, a);
+    } else {
+        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<1, true, PAGED>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rotate_by_position_kernel<1, false, PAGED>), grid, dim3(256), 0, st, a);
+    }
+    R2O_CHECK_LAUNCH();
+    return R2O_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int r2o_position_rope(const r2o_position_rope_params* p, void* stream) {
+    if (!p || !rotation_ok(p->rotation, false) || !rows_ok(p->query, p->q_strides) || !rows_ok(p->key, p->k_strides) ||
+        !rows_ok(p->query_out, p->qo_strides) || !rows_ok(p->key_out, p->ko_strides) || (p->dtype != 0 && p->dtype != 1) || p->batch < 1 ||
+        p->hq < 1 || p->hkv < 1 || p->tokens < 1 || p->hq > 0x3fffffff || p->hkv > 0x3fffffff)
+        return R2O_EINVAL;
+    RotateArgs a{};
+    a.rotation = p->rotation;
+    a.q = p->query;
+    a.k = p->key;
+    a.q_out = p->query_out;
+    a.k_out = p->key_out;
+    std::copy_n(p->q_strides, 3, a.q_strides);
+    std::copy_n(p->k_strides, 3, a.k_strides);
+    std::copy_n(p->qo_strides, 3, a.qo_strides);
+    std::copy_n(p->ko_strides, 3, a.ko_strides);
+    a.hq = (int)p->hq;
+    a.hkv = (int)p->hkv;
+    a.hadamard = p->hadamard ? 1 : 0;
+    return launch<false>(a, p->dtype, p->batch, p->tokens, p->hq + p->hkv, (hipStream_t)stream);
+}
+
+int r2o_paged_rope_extend(const r2o_paged_rope_extend_params* p, void* stream) {
+    if (!p) return R2O_EINVAL;
+    const r2o_paged_cache& c = p->cache;
+    if (!r2o_paged_cache_ok(c) || r2o_one_row(c) || !rotation_ok(p->rotation, true) || !rows_ok(p->query, p->q_strides) ||
+        !rows_ok(p->key, p->k_strides) || !rows_ok(p->value, p->v_strides) || !rows_ok(p->query_out, p->qo_strides) || p->hq < 1 ||
+        p->hq > 0x3fffffff || p->rows < 1 || p->rows > (1 << 29) || reinterpret_cast<uintptr_t>(p->counts) % 4 ||
+        reinterpret_cast<uintptr_t>(p->weights) % 4 || p->weights_strides[0] < 0 || p->weights_strides[1] < 0 || (p->weights && !c.weight_pages))
+        return R2O_EINVAL;
+    RotateArgs a{};
+    a.rotation = p->rotation;
+    a.cache = c;
+    a.q = p->query;
+    a.k = p->key;
+    a.v = p->value;
+    a.q_out = p->query_out;
+    a.weights = p->weights;
+    a.counts = p->counts;
+    std::copy_n(p->q_strides, 3, a.q_strides);
+    std::copy_n(p->k_strides, 3, a.k_strides);
+    std::copy_n(p->v_strides, 3, a.v_strides);
+    std::copy_n(p->qo_strides, 3, a.qo_strides);
+    std::copy_n(p->weights_strides, 2, a.weights_strides);
+    a.hq = (int)p->hq;
+    a.hkv = (int)c.hkv;
+    return launch<true>(a, c.dtype, c.batch, p->rows, p->hq + 2 * c.hkv, (hipStream_t)stream);
+}
+
+}  // extern "C"

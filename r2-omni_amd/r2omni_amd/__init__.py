@@ -29,7 +29,7 @@ from .cache import (
     precision_cache_active_storage_breakdown,
     precision_cache_storage_breakdown,
 )
-from .paged import PagedCache, paged_attention, paged_evict, paged_extend
+from .paged import PagedCache, paged_attention, paged_evict, paged_extend, paged_prefix_attention
 from .policy import (
     LayerCompressionPlan,
     PageAssignment,
@@ -41,6 +41,7 @@ from .policy import (
     project_attention_weights_to_pages,
     project_token_bits_to_pages,
 )
+from .position import PositionRotary, paged_rope_extend, qk_position_rope
 from .prompt import attention_weights, prompt_attention
 from .reference import normalized_fwht, triton_mixed_reference
 from .rope import FusedQwen3Rotary, FusedRotary, qwen3_qk_norm_rope, qwen_qk_mrope

@@ -177,6 +177,38 @@ class PagedEvict(ctypes.Structure):  # r2o_paged_evict_params
     ]
 
 
+class PagedPrefix(ctypes.Structure):  # r2o_paged_prefix_params
+    _fields_ = [
+        ("cache", PagedCacheParams), ("prefix", PagedCacheParams), ("members", c_vp), ("query_lengths", c_vp), ("query", c_vp),
+        ("out", c_vp), ("lse", c_vp), ("q_strides", c_i64 * 3), ("o_strides", c_i64 * 3), ("hq", c_i64), ("rows", c_i64),
+        ("sm_scale", ctypes.c_float), ("scratch", c_vp), ("scratch_floats", c_i64), ("workers", c_i64),
+    ]
+
+
+class Rotation(ctypes.Structure):  # r2o_rotation
+    _fields_ = [
+        ("positions", c_vp), ("position_strides", c_i64 * 3), ("position_bytes", c_i64), ("axes", c_i64), ("inv_freq", c_vp),
+        ("freq_bytes", c_i64), ("pairs_1", ctypes.c_uint64), ("pairs_2", ctypes.c_uint64), ("q_weight", c_vp), ("k_weight", c_vp),
+        ("eps", ctypes.c_float), ("scaling", ctypes.c_float),
+    ]
+
+
+class PositionRope(ctypes.Structure):  # r2o_position_rope_params
+    _fields_ = [
+        ("rotation", Rotation), ("query", c_vp), ("key", c_vp), ("query_out", c_vp), ("key_out", c_vp), ("q_strides", c_i64 * 3),
+        ("k_strides", c_i64 * 3), ("qo_strides", c_i64 * 3), ("ko_strides", c_i64 * 3), ("batch", c_i64), ("hq", c_i64),
+        ("hkv", c_i64), ("tokens", c_i64), ("dtype", c_i64), ("hadamard", c_i64),
+    ]
+
+
+class PagedRopeExtend(ctypes.Structure):  # r2o_paged_rope_extend_params
+    _fields_ = [
+        ("cache", PagedCacheParams), ("rotation", Rotation), ("query", c_vp), ("key", c_vp), ("value", c_vp), ("query_out", c_vp),
+        ("weights", c_vp), ("counts", c_vp), ("q_strides", c_i64 * 3), ("k_strides", c_i64 * 3), ("v_strides", c_i64 * 3),
+        ("qo_strides", c_i64 * 3), ("weights_strides", c_i64 * 2), ("hq", c_i64), ("rows", c_i64),
+    ]
+
+
 _SIGNATURES = {
     "r2o_plan_work_items": (ctypes.POINTER(PlanRun), c_i64, ctypes.POINTER(PlanConfig), c_vp, c_i64, c_i64, c_i64,
                             c_vp, c_i64, c_vp, c_i64, ctypes.POINTER(c_i64)),
@@ -203,6 +235,9 @@ _SIGNATURES = {
     "r2o_paged_extend": (ctypes.POINTER(PagedExtend), c_vp),
     "r2o_paged_attention": (ctypes.POINTER(PagedAttention), c_vp),
     "r2o_paged_evict": (ctypes.POINTER(PagedEvict), c_vp),
+    "r2o_paged_prefix_attention": (ctypes.POINTER(PagedPrefix), c_vp),
+    "r2o_position_rope": (ctypes.POINTER(PositionRope), c_vp),
+    "r2o_paged_rope_extend": (ctypes.POINTER(PagedRopeExtend), c_vp),
     "r2o_fwht128": (c_vp, c_vp, c_i64, c_i64, c_vp),
     "r2o_qk_mrope": (c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp,
                      c_i64, c_i64, c_i64, c_vp),

@@ -6,6 +6,8 @@ pages that a server hands out, and gives up the tokens that received the least a
 * ``paged_extend`` (``r2o_paged_extend``): a prompt's rows, or a chunk of them, into their slots.
 * ``paged_attention`` (``r2o_paged_attention``): one new token per request over its filled slots, its own K and V
   rows appended by the same call, and the cache's accumulated weights advanced.
+* ``paged_prefix_attention`` (``r2o_paged_prefix_attention``): the newest rows of each request (a step's token, or a
+  question's) over a prefix that many requests share, whose rows are read once for all of them, and over its own slots.
 * ``paged_evict`` (``r2o_paged_evict``): the tokens of largest accumulated weight, with the first and the newest
   ones, compacted in order into another page table.
 
@@ -20,7 +22,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .prompt import _lengths, _rows, _scale, _strides, _window
+from .prompt import _check_like, _lengths, _like, _rows, _scale, _strides, _window
 
 PAGE_SIZES = (16, 32, 64, 128)
 MAX_BATCH = 1024
@@ -118,6 +120,17 @@ def _check_new_rows(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, w
     _lib.refuse_gradients(what, key, value)
 
 
+def _row_weights(cache: PagedCache, key: torch.Tensor, weights: torch.Tensor | None, what: str) -> torch.Tensor | None:
+    """The new rows' weights, checked; unit-strided along the rows."""
+    if weights is None:
+        return None
+    if cache.weight_pages is None:
+        raise ValueError(f"{what} weights need a cache with weight_pages")
+    if weights.shape != key.shape[:3] or weights.dtype != torch.float32 or weights.device != key.device:
+        raise ValueError(f"{what} weights must be fp32 [B,Hkv,S] on the rows' device")
+    return weights.contiguous() if weights.stride(2) != 1 and weights.shape[2] > 1 or min(weights.stride()) < 0 else weights
+
+
 def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, counts: torch.Tensor | None = None,
                  weights: torch.Tensor | None = None) -> None:
     """Write rows of key and value [B, Hkv, S, 128] into each request's newest slots.
@@ -136,13 +149,7 @@ def paged_extend(cache: PagedCache, key: torch.Tensor, value: torch.Tensor, *, c
     if key.shape[2] > cache.capacity:
         raise ValueError("paged extend has more rows than the page table holds")
     counts = _lengths(counts, batch, key.device, "counts")
-    if weights is not None:
-        if cache.weight_pages is None:
-            raise ValueError("paged extend weights need a cache with weight_pages")
-        if weights.shape != key.shape[:3] or weights.dtype != torch.float32 or weights.device != key.device:
-            raise ValueError("paged extend weights must be fp32 [B,Hkv,S] on the rows' device")
-        if weights.stride(2) != 1 and weights.shape[2] > 1 or min(weights.stride()) < 0:
-            weights = weights.contiguous()
+    weights = _row_weights(cache, key, weights, "paged extend")
     _lib.refuse_gradients("paged extend", weights, *_pools(cache))
     key, value = _rows(key), _rows(value)
     p = _lib.PagedExtend(cache=_params_of(cache), key=key.data_ptr(), value=value.data_ptr(), weights=_lib.ptr(weights),
@@ -223,6 +230,84 @@ def paged_attention(query: torch.Tensor, cache: PagedCache, *, append: tuple[tor
         p.logits = base + (520 * p.partial_states + 15) // 16 * 16
     _lib.launch("r2o_paged_attention", p, dev)
     return out, lse
+
+
+def paged_prefix_attention(query: torch.Tensor, cache: PagedCache, prefix: PagedCache | None = None, *,
+                           members: torch.Tensor | None = None, query_lengths: torch.Tensor | None = None,
+                           sm_scale: float | None = None, output: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """Attention of each request's newest rows, query [B, Hq, S, 128] (or [B, Hq, 128] for one token), over the prefix that it
+    shares and over its own slots; returns (out like query, lse fp32 [B, Hq, S] or [B, Hq]).
+
+    ``prefix`` is a cache whose table has a row, and whose lengths have an entry, for each prefix; its pages may lie in
+    ``cache``'s pools or others (of one type and head count; page sizes may differ).  ``members`` (int32 [prefixes] on the device):
+    requests 0 .. members[0] - 1 share prefix 0, the next members[1] prefix 1, and so on, requests behind the last share
+    none; without it all share the one prefix there is.  Counts past the batch's end are cut off.  Row i of a request with q
+    query rows (S, or ``query_lengths[b]``) and n = ``cache.lengths[b]`` slots, the new ones among them, sees all of its
+    prefix and its own slots j <= n - q + i.  A row that sees nothing, or lies behind its request's rows, is 0 with lse
+    -inf; infinite and NaN values count as in ``prompt_attention``.  Without a prefix it is causal attention of a chunk over
+    its paged cache.  Caches that keep weights are refused: ``dataclasses.replace(cache, weight_pages=None)``.  ``output``:
+    the two result tensors, the first with unit-strided channels and 16-byte aligned rows, neither overlapping an input."""
+    if output is None:
+        made = _lib.host().paged_prefix_attention(_lib.entry("r2o_paged_prefix_attention"), query, cache, prefix, members,
+                                                  query_lengths, sm_scale)
+        if made is not None:
+            _lib.check(made[0], "r2o_paged_prefix_attention")
+            return made[1], made[2]
+    what = "paged prefix attention"
+    batch, hkv, dev = int(cache.page_table.shape[0]), int(cache.key_pages.shape[1]), cache.key_pages.device
+    token = query.ndim == 3
+    if token:
+        query = query[:, :, None]
+        output = None if output is None else (output[0][:, :, None], output[1][..., None])
+    if query.ndim != 4 or query.shape[0] != batch or query.shape[3] != 128 or min(query.shape) < 1:
+        raise ValueError("paged prefix attention requires query [B,Hq,S,128] or [B,Hq,128] of the cache's requests")
+    hq, rows = int(query.shape[1]), int(query.shape[2])
+    if hq % hkv:
+        raise ValueError("GQA requires Hq divisible by Hkv")
+    if query.dtype != cache.key_pages.dtype or query.device != dev:
+        raise ValueError("paged prefix attention query must match the cache's dtype and device")
+    if batch * hq * rows > 1 << 30:
+        raise ValueError("paged prefix attention takes at most 2^30 query rows over all heads")
+    caches = (cache,) if prefix is None else (cache, prefix)
+    if any(c.weight_pages is not None for c in caches):
+        raise ValueError("paged prefix attention does not keep weights: pass caches without weight_pages")
+    prefixes = 0
+    if prefix is not None:
+        prefixes = int(prefix.page_table.shape[0])
+        if prefix.key_pages.shape[1] != hkv or prefix.key_pages.dtype != cache.key_pages.dtype or prefix.key_pages.device != dev:
+            raise ValueError("paged prefix attention prefix must have the cache's heads, dtype and device")
+        if members is None and prefixes > 1:
+            raise ValueError("paged prefix attention of several prefixes needs members")
+    elif members is not None:
+        raise ValueError("paged prefix attention members need a prefix")
+    members = _lengths(members, prefixes, dev, "members")
+    query_lengths = _lengths(query_lengths, batch, dev, "query_lengths")
+    _lib.refuse_gradients(what, query, *(t for c in caches for t in _pools(c)), *(output or ()))
+    scale = _scale(sm_scale)
+    most = _lib.host().prefix_tiles(batch, hkv, hq, rows, cache.capacity, prefixes, prefix.capacity if prefixes else 0)
+    if most > (1 << 31) - 4097:
+        raise ValueError("paged prefix attention has more tiles of slots than it can count")
+    params = [_params_of(c) for c in caches]
+    query = _rows(query)
+    if output is None:
+        out = _like(query)
+        lse = torch.empty((batch, hq, rows), dtype=torch.float32, device=dev)
+    else:
+        out, lse = output
+        _check_like(out, query, what)
+        if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
+            raise ValueError("paged prefix attention lse output must be contiguous fp32 [B,Hq,S] on Q's device")
+    p = _lib.PagedPrefix(cache=params[0], members=_lib.ptr(members), query_lengths=_lib.ptr(query_lengths), query=query.data_ptr(),
+                         out=out.data_ptr(), lse=lse.data_ptr(), q_strides=_strides(query, 3), o_strides=_strides(out, 3), hq=hq,
+                         rows=rows, sm_scale=scale)
+    if prefixes:
+        p.prefix = params[1]
+    p.workers = _lib.host().prefix_workers(most, _lib.num_cus(dev))
+    p.scratch_floats = _lib.host().prefix_scratch(batch, hkv, hq, rows, prefixes, p.workers)
+    scratch = torch.empty(p.scratch_floats, dtype=torch.float32, device=dev)
+    p.scratch = scratch.data_ptr()
+    _lib.launch("r2o_paged_prefix_attention", p, dev)
+    return (out[:, :, 0], lse[..., 0]) if token else (out, lse)
 
 
 def paged_evict(cache: PagedCache, target: PagedCache, keep: int, *, sinks: int = 0, recent: int = 0) -> torch.Tensor:

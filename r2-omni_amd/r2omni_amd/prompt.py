@@ -31,6 +31,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An empty tensor laid out like ``t``, if the kernels can write that in place."""
+    out = torch.empty_like(t)
+    return out if _rows(out) is out else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _check_like(out: torch.Tensor, t: torch.Tensor, what: str, whose: str = "Q's") -> None:
+    """A result tensor that a caller gave."""
+    if out.shape != t.shape or out.dtype != t.dtype or out.device != t.device:
+        raise ValueError(f"{what} output must match {whose} shape, dtype and device")
+    if _rows(out) is not out or any(st == 0 for st, n in zip(out.stride(), out.shape) if n > 1):
+        raise ValueError(f"{what} output needs unit channel stride and 16-byte aligned rows of its own")
+
+
 def _strides(t: torch.Tensor, n: int):
     """Element strides of the first ``n`` axes; those of an axis of one do not matter and may be anything."""
     return (ctypes.c_int64 * n)(*[st if size > 1 else 0 for st, size in zip(t.stride()[:n], t.shape)])
@@ -115,16 +129,11 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     query, key, value = _rows(query), _rows(key), _rows(value)
     p = _params(query, key, window, sinks, query_lengths, key_lengths, sm_scale)
     if output is None:
-        out = torch.empty_like(query)
-        if _rows(out) is not out:
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        out = _like(query)
         lse = torch.empty((batch, hq, rows), dtype=torch.float32, device=query.device)
     else:
         out, lse = output
-        if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
-            raise ValueError("prompt attention output must match Q's shape, dtype and device")
-        if _rows(out) is not out or any(st == 0 for st, n in zip(out.stride(), out.shape) if n > 1):
-            raise ValueError("prompt attention output needs unit channel stride and 16-byte aligned rows of its own")
+        _check_like(out, query, "prompt attention")
         if tuple(lse.shape) != (batch, hq, rows) or lse.dtype != torch.float32 or lse.device != query.device \
                 or not lse.is_contiguous():
             raise ValueError("prompt attention lse output must be contiguous fp32 [B,Hq,Sq] on Q's device")
