@@ -875,15 +875,16 @@ bool merged_rows(int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes) { retu
 
 int64_t prefix_tiles(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t capacity, int64_t prefixes, int64_t prefix_capacity) {
     const int64_t packed = hq / hkv * rows, own = div_up(capacity, 64), shared = prefixes ? div_up(prefix_capacity, 64) : 0;
-    return merged_rows(hkv, hq, rows, prefixes) ? hkv * ((batch * packed / 128 + prefixes) * shared + batch * own)
-                                                : hkv * batch * div_up(packed, 128) * (shared + own);
+    return merged_rows(hkv, hq, rows, prefixes)
+               ? std::max(hkv * (batch * packed / 256 + prefixes) * shared, hkv * batch * div_up(packed, 32) * 2 * own)
+               : hkv * batch * div_up(packed, 256) * std::max<int64_t>(1, shared + own);
 }
 
-// Workgroups that share them: two a compute unit, whose LDS they fill, of two tiles at least.
-int64_t prefix_workers(int64_t tiles, int64_t cus) { return std::max<int64_t>(1, std::min(2 * cus, div_up(tiles, 2))); }
+// Workgroups that share them: one a compute unit, whose LDS it fills.
+int64_t prefix_workers(int64_t tiles, int64_t cus) { return std::max<int64_t>(1, std::min(cus, tiles)); }
 
 int64_t prefix_scratch(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes, int64_t workers) {
-    return 130 * (256 * workers + (merged_rows(hkv, hq, rows, prefixes) ? 2 * batch * hq * rows : 0));
+    return 130 * (512 * workers + (merged_rows(hkv, hq, rows, prefixes) ? 2 * batch * hq * rows : 0));
 }
 
 // paged_prefix_attention(function, query, cache, prefix or None, members, query_lengths, scale): (status, out, lse) or None
@@ -912,7 +913,7 @@ PyObject* paged_prefix_attention_call(PyObject* const* args) {
         !lengths_arg(args[5], c.batch, device, p.query_lengths))
         Py_RETURN_NONE;
     const int64_t tiles = prefix_tiles(c.batch, c.hkv, p.hq, p.rows, c.max_pages * c.page_size, f.batch, f.max_pages * f.page_size);
-    if (tiles > 0x7fffffff - R2O_PAGED_MAX_WORKERS) Py_RETURN_NONE;
+    if (tiles > 0x7fffffff - 8 * R2O_PAGED_MAX_WORKERS) Py_RETURN_NONE;
     at::Tensor out = at::empty_like(*q);
     if (!row_strides(out, axes, p.o_strides, true) || p.o_strides[2] > R2O_MAX_ROW_STRIDE) Py_RETURN_NONE;
     p.workers = prefix_workers(tiles, compute_units((int)device));

@@ -9,6 +9,7 @@
 // request of its own, each leaves (maximum, sum, products) in scratch for the join.
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "r2o_cache_check.hpp"
 #include "r2o_common.hpp"
@@ -18,8 +19,11 @@ namespace {
 
 using namespace r2o_tiles;
 
-constexpr int kRows = 128;   // rows of a workgroup: 4 waves of 32
-constexpr int kMinTiles = 2; // key tiles that a workgroup takes at least
+constexpr int kWaves = 8;    // of a workgroup, which fills a compute unit
+constexpr int kRows = 256;   // rows of a workgroup: a wave's 32 each; 128 or fewer: 32 for two waves, which share their keys
+constexpr int kMerged = 128; // packed rows of a request below which all requests of a prefix are one list
+constexpr int kWaveRows = 32, kWaveKeys = 32;  // of a wave that works by itself
+constexpr int kAhead = 4;    // tiles in LDS or on their way there, the one in use among them
 
 // One cache's rows, in the kernels' widths (the host has checked that they fit).
 struct Source {
@@ -67,62 +71,97 @@ __device__ __forceinline__ int wave_scan(int x) {
 __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
 
 __device__ __forceinline__ int filled(SourceArgs& s, int length) { return min(max(length, 0), (s.last_page + 1) << s.shift); }
-__device__ __forceinline__ int key_tiles(SourceArgs& s, int length) { return (filled(s, length) + kTile - 1) / kTile; }
 
-// ------------------------------------------------------------------------------------- the list
-// Entries: where rows are merged, each prefix (with the rows of all its requests) and then each request (its own slots);
-// otherwise each request, its prefix's slots before its own.  An entry has `heads` times its row tiles times its key tiles
-// of work.  The wave goes through them 64 at a time, one a lane.
+// ------------------------------------------------------------------------------------- the work
+// Where rows are merged there are two lists: the prefixes' (with the rows of all their requests), whose row tiles workgroups
+// take as a whole, and the requests' own slots, of few rows each, which waves take by themselves: a workgroup's eight have
+// eight requests' latencies under way at a time.  Otherwise there is one list, of the requests, a prefix's slots before the own
+// ones.  The wave goes through prefixes and requests 64 at a time, one a lane; what the first 64 hold is loaded at once and kept.
+struct Lane {
+    int members, shared, own, rows;  // as the tensors have them: a prefix's, a request's
+};
+
+__device__ __forceinline__ Lane lane_of(int i0) {
+    Args& a = kernel_args();
+    const int i = i0 + (threadIdx.x & 63);
+    Lane x{0, 0, 0, a.rows};
+    if (i < a.prefixes) {
+        x.members = a.members ? r2o_ldg(a.members + i) : a.batch;
+        x.shared = r2o_ldg(a.shared.lengths + i);
+    }
+    if (i < a.batch) {
+        x.own = r2o_ldg(a.own.lengths + i);
+        if (a.query_lengths) x.rows = r2o_ldg(a.query_lengths + i);
+    }
+    return x;
+}
+
+__device__ __forceinline__ Lane lane_at(const Lane& first, int i0) { return i0 ? lane_of(i0) : first; }
+
 struct Members {
     int first, count;  // requests of this lane's prefix
 };
 
 // Counts are cut off where the batch ends, so that whatever they hold no request has two prefixes.
-__device__ __forceinline__ Members lane_members(Args& a, int g0, int& before) {
-    const int g = g0 + (threadIdx.x & 63);
-    int m = 0;
-    if (g < a.prefixes) m = a.members ? min(max(r2o_ldg(a.members + g), 0), a.batch) : a.batch;
-    const int upto = wave_scan(m);
-    Members x;
-    x.first = min(before + upto - m, a.batch);
-    x.count = min(m, a.batch - x.first);
+__device__ __forceinline__ Members lane_members(const Lane& x, int& before) {
+    Args& a = kernel_args();
+    const int m = min(max(x.members, 0), a.batch), upto = wave_scan(m);
+    Members r;
+    r.first = min(before + upto - m, a.batch);
+    r.count = min(m, a.batch - r.first);
     before = min(before + last_lane(upto), a.batch);
-    return x;
+    return r;
 }
 
-__device__ __forceinline__ int row_tiles(int rows) { return (rows + kRows - 1) / kRows; }
-
-// Work of this lane's prefix (merged rows).
-__device__ __forceinline__ int lane_prefix_work(Args& a, int g0, const Members& x) {
-    const int g = g0 + (threadIdx.x & 63);
-    return g < a.prefixes && x.count ? a.hkv * row_tiles(x.count * a.packed) * key_tiles(a.shared, r2o_ldg(a.shared.lengths + g)) : 0;
+__device__ __forceinline__ int div_up(int x, int by) { return (x + by - 1) / by; }
+__device__ __forceinline__ int counted_rows(int rows) {
+    Args& a = kernel_args();
+    return min(max(rows, 0), a.rows);
 }
 
-// The prefix of this lane's request, -1 for none, and all lanes' members are looked at: one step a prefix.
-__device__ __forceinline__ int prefix_of(Args& a, int b) {
+// Tiles of this lane's prefix (merged rows): heads x row tiles x key tiles.
+__device__ __forceinline__ int prefix_work(const Lane& x, const Members& m) {
+    Args& a = kernel_args();
+    return m.count ? a.hkv * div_up(m.count * a.packed, kRows) * div_up(filled(a.shared, x.shared), kTile) : 0;
+}
+
+// Tiles of this lane's request's own slots (merged rows), of 32 rows and 32 keys.
+__device__ __forceinline__ int own_work(const Lane& x, int b0) {
+    Args& a = kernel_args();
+    const int b = b0 + (threadIdx.x & 63);
+    return b < a.batch ? a.hkv * div_up(a.packed, kWaveRows) * div_up(filled(a.own, x.own), kWaveKeys) : 0;
+}
+
+// The prefix of this lane's request, -1 for none, and its length: one step a prefix.
+__device__ __forceinline__ int prefix_of(const Lane& first, int b, int& length) {
+    Args& a = kernel_args();
     int of = -1, before = 0;
+    length = 0;
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
-        const Members x = lane_members(a, g0, before);
+        const Lane x = lane_at(first, g0);
+        const Members m = lane_members(x, before);
         const int here = min(64, a.prefixes - g0);
         for (int i = 0; i < here; ++i) {
-            const int first = __builtin_amdgcn_readlane(x.first, i), count = __builtin_amdgcn_readlane(x.count, i);
-            of = (uint32_t)(b - first) < (uint32_t)count ? g0 + i : of;
+            const bool mine = (uint32_t)(b - __builtin_amdgcn_readlane(m.first, i)) < (uint32_t)__builtin_amdgcn_readlane(m.count, i);
+            of = mine ? g0 + i : of;
+            length = mine ? __builtin_amdgcn_readlane(x.shared, i) : length;
         }
     }
     return of;
 }
 
-// Work of this lane's request.  Not merged, a row tile without a key has one tile, of none: its rows are written there.
-__device__ __forceinline__ int lane_request_work(Args& a, int b0) {
+// Tiles of this lane's request with its prefix (rows that are not merged).  A row tile without a key has one tile, of none: its
+// rows are written there.
+__device__ __forceinline__ int request_work(const Lane& first, const Lane& x, int b0) {
+    Args& a = kernel_args();
     const int b = b0 + (threadIdx.x & 63);
-    int tiles = b < a.batch ? key_tiles(a.own, r2o_ldg(a.own.lengths + b)) : 0;
-    if (a.merged) return a.hkv * tiles;
-    const int g = prefix_of(a, b);
-    if (g >= 0 && b < a.batch) tiles += key_tiles(a.shared, r2o_ldg(a.shared.lengths + g));
-    return b < a.batch ? a.hkv * row_tiles(a.packed) * max(tiles, 1) : 0;
+    int length;
+    prefix_of(first, b, length);
+    const int tiles = div_up(filled(a.own, x.own), kTile) + div_up(filled(a.shared, length), kTile);
+    return b < a.batch ? a.hkv * div_up(counted_rows(x.rows) * a.group, kRows) * max(tiles, 1) : 0;
 }
 
-// The list shared evenly: worker i takes `each` tiles from begin(i) on, the first `more` workers one more.
+// A list shared evenly: worker i takes `each` tiles from begin(i) on, the first `more` workers one more.
 struct Share {
     int total, workers, each, more;
     __device__ __forceinline__ int begin(int i) const { return i * each + min(i, more); }
@@ -132,53 +171,164 @@ struct Share {
     }
 };
 
-__device__ __forceinline__ Share share_of(Args& a, int total) {
+__device__ __forceinline__ Share share_of(int total, int workers) {
     Share s;
     s.total = total;
-    s.workers = max(1, min(a.workers, (total + kMinTiles - 1) / kMinTiles));
+    s.workers = max(1, min(workers, total));
     s.each = (int)((uint32_t)total / (uint32_t)s.workers);
     s.more = total - s.each * s.workers;
     return s;
 }
 
-// An entry: its place in the list, and what it is.
-struct Entry {
-    int base, work;      // tiles before it, its own
-    int prefix, request; // request -1: all of a prefix's
-    int first, members;  // of the prefix
+// Both lists of merged rows.  Workgroups 0 .. n - 1 take the prefixes', those from `own_first` on the requests', their number by
+// what the lists cost.
+struct Plan {
+    Share shared, own;  // own: waves
+    int own_first;
 };
 
-// The entry that holds tile u; the tiles of all entries, if `all`.  u = -1: none.
-__device__ __forceinline__ Entry find(Args& a, int u, int& total) {
-    Entry e{};
-    e.request = -2;
-    int at = 0;
-    const int lane = threadIdx.x & 63;
-    if (a.merged) {
-        int before = 0;
-        for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
-            const Members x = lane_members(a, g0, before);
-            const int work = lane_prefix_work(a, g0, x), upto = wave_scan(work), all = last_lane(upto);
-            if ((uint32_t)(u - at) < (uint32_t)all) {
-                const int i = __builtin_ctzll(__ballot(at + upto > u));
-                e.base = at + __builtin_amdgcn_readlane(upto - work, i);
-                e.work = __builtin_amdgcn_readlane(work, i);
-                e.prefix = g0 + i;
-                e.request = -1;
-                e.first = __builtin_amdgcn_readlane(x.first, i);
-                e.members = __builtin_amdgcn_readlane(x.count, i);
-            }
-            at += all;
+__device__ __forceinline__ Plan plan_of(Args& a, int shared, int own, float shared_cost, float own_cost) {
+    Plan p;
+    int n = __builtin_amdgcn_readfirstlane((int)(a.workers * (shared_cost / (shared_cost + own_cost)) + 0.5f));
+    n = max(min(n, a.workers - (own > 0)), (int)(shared > 0));
+    p.own_first = min(n, a.workers - 1);  // of one workgroup, which does both
+    p.shared = share_of(shared, n);
+    p.own = share_of(own, kWaves * (a.workers - p.own_first));
+    return p;
+}
+
+// What a prefix's and a request's tiles cost, in the time that a compute unit takes for its part of the memory's rate and 16 KB.
+__device__ __forceinline__ float prefix_cost(int work, int rows) { return (float)work * (rows > kRows / 2 ? 3.f : 2.f); }
+__device__ __forceinline__ float own_cost(int work) {
+    Args& a = kernel_args();
+    return (float)work + (work ? 1.f * a.hkv * div_up(a.packed, kWaveRows) : 0.f);
+}
+
+__device__ __forceinline__ float wave_total(float x) {
+    x += r2o_lane_xor<1>(x);
+    x += r2o_lane_xor<2>(x);
+    x += r2o_lane_xor<4>(x);
+    x += r2o_lane_xor<8>(x);
+    return r2o_sum_lane_pair<32>(r2o_sum_lane_pair<16>(x));
+}
+
+// An entry of a list: its place there, and what it is.
+struct Entry {
+    int base;             // tiles before it
+    int prefix, request;  // request -1: all of a prefix's; -2: no entry
+    int first, members;   // of the prefix
+    int n_shared, n_own, rows;
+};
+
+// The tiles of the lists, and where request b's parts lie in them (b -1: none).
+struct Sums {
+    int shared, own;
+    float shared_cost, own_cost;
+    Entry of_prefix, of_request;
+};
+
+__device__ __forceinline__ Sums sums_of(const Lane& first, int b) {
+    Args& a = kernel_args();
+    Sums s{};
+    s.of_prefix.prefix = -1;
+    int before = 0;
+    for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
+        const Lane x = lane_at(first, g0);
+        const Members m = lane_members(x, before);
+        const int work = prefix_work(x, m), upto = wave_scan(work);
+        const uint64_t mine = b < 0 ? 0 : __ballot((uint32_t)(b - m.first) < (uint32_t)m.count);
+        if (mine) {
+            const int i = __builtin_ctzll(mine);
+            s.of_prefix.base = s.shared + __builtin_amdgcn_readlane(upto - work, i);
+            s.of_prefix.prefix = g0 + i;
+            s.of_prefix.first = __builtin_amdgcn_readlane(m.first, i);
+            s.of_prefix.members = __builtin_amdgcn_readlane(m.count, i);
+            s.of_prefix.n_shared = filled(a.shared, __builtin_amdgcn_readlane(x.shared, i));
         }
+        s.shared_cost += wave_total(prefix_cost(work, m.count * a.packed));
+        s.shared += last_lane(upto);
     }
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int work = lane_request_work(a, b0), upto = wave_scan(work), all = last_lane(upto);
+        const Lane x = lane_at(first, b0);
+        const int work = own_work(x, b0), upto = wave_scan(work);
+        if ((uint32_t)(b - b0) < 64u) {
+            s.of_request.base = s.own + __builtin_amdgcn_readlane(upto - work, b - b0);
+            s.of_request.n_own = filled(a.own, __builtin_amdgcn_readlane(x.own, b - b0));
+            s.of_request.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, b - b0));
+        }
+        s.own_cost += wave_total(own_cost(work));
+        s.own += last_lane(upto);
+    }
+    return s;
+}
+
+// Merged rows: the prefix that holds tile u of the prefixes' list.
+__device__ __forceinline__ Entry find_prefix(const Lane& first, int u) {
+    Args& a = kernel_args();
+    Entry e{};
+    e.request = -2;
+    int at = 0, before = 0;
+    for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
+        const Lane x = lane_at(first, g0);
+        const Members m = lane_members(x, before);
+        const int work = prefix_work(x, m), upto = wave_scan(work), all = last_lane(upto);
         if ((uint32_t)(u - at) < (uint32_t)all) {
             const int i = __builtin_ctzll(__ballot(at + upto > u));
             e.base = at + __builtin_amdgcn_readlane(upto - work, i);
-            e.work = __builtin_amdgcn_readlane(work, i);
+            e.prefix = g0 + i;
+            e.request = -1;
+            e.first = __builtin_amdgcn_readlane(m.first, i);
+            e.members = __builtin_amdgcn_readlane(m.count, i);
+            e.n_shared = filled(a.shared, __builtin_amdgcn_readlane(x.shared, i));
+            e.rows = e.members * a.packed;
+        }
+        at += all;
+    }
+    return e;
+}
+
+// Merged rows: the request that holds tile u of the requests' list.
+__device__ __forceinline__ Entry find_own(const Lane& first, int u) {
+    Args& a = kernel_args();
+    Entry e{};
+    e.request = -2;
+    e.prefix = -1;
+    int at = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const Lane x = lane_at(first, b0);
+        const int work = own_work(x, b0), upto = wave_scan(work), all = last_lane(upto);
+        if ((uint32_t)(u - at) < (uint32_t)all) {
+            const int i = __builtin_ctzll(__ballot(at + upto > u));
+            e.base = at + __builtin_amdgcn_readlane(upto - work, i);
             e.request = b0 + i;
-            e.prefix = a.merged ? -1 : __builtin_amdgcn_readlane(prefix_of(a, b0 + lane), i);
+            e.n_own = filled(a.own, __builtin_amdgcn_readlane(x.own, i));
+            e.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, i));
+        }
+        at += all;
+    }
+    return e;
+}
+
+// Rows that are not merged: the request that holds tile u (-1: none), and the tiles of all.
+__device__ __forceinline__ Entry find_request(const Lane& first, int u, int& total) {
+    Args& a = kernel_args();
+    Entry e{};
+    e.request = -2;
+    e.prefix = -1;
+    int at = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const Lane x = lane_at(first, b0);
+        const int work = request_work(first, x, b0), upto = wave_scan(work), all = last_lane(upto);
+        if ((uint32_t)(u - at) < (uint32_t)all) {
+            const int i = __builtin_ctzll(__ballot(at + upto > u));
+            int length;
+            const int of = prefix_of(first, b0 + (threadIdx.x & 63), length);
+            e.base = at + __builtin_amdgcn_readlane(upto - work, i);
+            e.request = b0 + i;
+            e.prefix = __builtin_amdgcn_readlane(of, i);
+            e.n_shared = e.prefix < 0 ? 0 : filled(a.shared, __builtin_amdgcn_readlane(length, i));
+            e.n_own = filled(a.own, __builtin_amdgcn_readlane(x.own, i));
+            e.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, i)) * a.group;
         }
         at += all;
     }
@@ -186,35 +336,44 @@ __device__ __forceinline__ Entry find(Args& a, int u, int& total) {
     return e;
 }
 
-// One row tile of an entry and head, and the keys that it may see: `shared` tiles of the prefix, then `own` ones.
+// One row tile of an entry and head, and its key tiles: of a workgroup, `shared` ones of the prefix, then its own; of a
+// wave, own ones.
 struct Segment {
     int base, tiles;         // in the list
-    int head, row0, rows;    // first row in the entry's list of them, and that list's end
-    int shared, n_shared, n_own;
+    int head, row0, shared;  // row0: in the entry's rows
 };
 
-__device__ __forceinline__ Segment segment_of(Args& a, const Entry& e, int u) {
-    Segment s;
-    s.n_shared = e.prefix >= 0 ? filled(a.shared, load_uniform(a.shared.lengths + e.prefix)) : 0;
-    s.n_own = e.request >= 0 ? filled(a.own, load_uniform(a.own.lengths + e.request)) : 0;
-    s.shared = (s.n_shared + kTile - 1) / kTile;
-    s.tiles = max(1, s.shared + (s.n_own + kTile - 1) / kTile);
-    s.rows = e.request < 0 ? e.members * a.packed : a.packed;
-    const int per_head = row_tiles(s.rows), at = (int)((uint32_t)(u - e.base) / (uint32_t)s.tiles);
+__device__ __forceinline__ Segment segment_at(const Entry& e, int u, int tiles, int row_tiles, int rows) {
+    Segment s{};
+    s.tiles = max(1, tiles);
+    const int per_head = max(1, row_tiles), at = (int)((uint32_t)(u - e.base) / (uint32_t)s.tiles);
     s.head = (int)((uint32_t)at / (uint32_t)per_head);
-    s.row0 = (at - s.head * per_head) * kRows;
+    s.row0 = (at - s.head * per_head) * rows;
     s.base = e.base + at * s.tiles;
     return s;
 }
 
-// Where partial states lie: two tiles of rows for each worker, for the segments that it does not have alone (the one that
-// another began, and the one that it leaves to others), then, where rows are merged, a place for each row of the prefixes'
-// segments and of the requests'.
-__device__ __forceinline__ int64_t split_rows(int worker, bool begins) { return ((int64_t)2 * worker + begins) * kRows; }
-__device__ __forceinline__ int64_t whole_rows(Args& a, bool shared, int first, int members, int b, int head) {
-    const int64_t packed = a.packed, base = (int64_t)2 * a.workers * kRows;
-    return base + (shared ? ((int64_t)first * a.hkv + (int64_t)head * members) * packed : ((int64_t)(a.batch + b) * a.hkv + head) * packed);
+__device__ __forceinline__ Segment segment_of(const Entry& e, int u) {
+    const int shared = div_up(e.n_shared, kTile);
+    Segment s = segment_at(e, u, shared + div_up(e.n_own, kTile), div_up(e.rows, kRows), kRows);
+    s.shared = shared;
+    return s;
 }
+
+// Where partial states lie: two tiles of rows for each workgroup, or for each of its waves, for the segments that it does not
+// have alone (the one that another began, and the one that it leaves to others), then, where rows are merged, a place for
+// each row of the prefixes' segments and of the requests'.
+__device__ __forceinline__ uint32_t split_rows(int worker, bool begins) { return (2u * worker + begins) * kRows; }
+__device__ __forceinline__ uint32_t split_wave_rows(int own_first, int wave, bool begins) {  // wave: of all that take requests
+    return 2u * kRows * own_first + (2u * wave + begins) * kWaveRows;
+}
+__device__ __forceinline__ uint32_t whole_prefix_rows(Args& a, int first, int members, int head) {
+    return 2u * kRows * a.workers + ((uint32_t)first * a.hkv + (uint32_t)head * members) * a.packed;
+}
+__device__ __forceinline__ uint32_t whole_own_rows(Args& a, int b, int head) {
+    return 2u * kRows * a.workers + ((uint32_t)(a.batch + b) * a.hkv + head) * a.packed;
+}
+constexpr uint32_t kNoRow = 0xffffffffu, kResult = 0xfffffffeu;  // no row, and one whose result is written at once
 
 // ------------------------------------------------------------------------------------- the rows
 // A cache's rows of one table and head.
@@ -240,312 +399,605 @@ __device__ __forceinline__ Side side_of(SourceArgs& s, int row, int head, int n)
     return x;
 }
 
-// The page of slot j, -1 if it has none.
+// The page of slot j, -1 if it has none or is not filled.
 __device__ __forceinline__ int page_of(const Side& x, int j) {
     const int id = load_uniform(x.table + min(j >> x.shift, x.last_page));
     return j < x.n && (uint32_t)id < (uint32_t)x.pages ? id : -1;
 }
 
-// Four groups of 16 slots, each within a page: bit i for one that has a page and a filled slot.
-__device__ __forceinline__ int tile_valid(const Side& x, int j0, int wave, int& page) {
-    int valid = 0;
-    page = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int id = page_of(x, j0 + 16 * i);
-        valid |= (id >= 0) << i;
-        page = i == wave ? max(id, 0) : page;
-    }
-    return valid;
+// 64 neighbouring pages of a table, one a lane, -1 for one outside the pool.  Scalar loads of a tile's pages, one after the
+// other, took longer than the tile.
+struct Window {
+    int first, ids;
+};
+
+__device__ __forceinline__ Window window_of(SourceArgs& s, const int32_t* table, int first, int lane) {
+    const int id = r2o_ldg(table + min(first + lane, s.last_page));
+    return {first, (uint32_t)id < (uint32_t)s.pages ? id : -1};
 }
 
-// This wave's 16 rows of K and V, straight into LDS.
+// Four rows (of 16 from `base` on, the i-th four of them) straight into LDS.
 template <int SWZ>
-__device__ __forceinline__ void stage_group(const uint16_t* base, int stride, unsigned char* lds, int wave, int lane) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)row_chunk<SWZ>(base, stride, 4 * i, 15, i, lane),
-            (__attribute__((address_space(3))) void*)(lds + (16 * wave + 4 * i) * 256), 16, 0, 0);
+__device__ __forceinline__ void stage_four(const uint16_t* base, int stride, int i, unsigned char* lds, int lane) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)row_chunk<SWZ>(base, stride, 4 * i, 15, i, lane),
+                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-// One workgroup: its share of the list.  S^T = K Q^T (32 keys x 32 rows a product), O^T += V^T P^T; two tiles ahead go into LDS
-// while one is computed on.
-// The probabilities are rounded to the rows' 16 bits for the product with V, whose two operands are of one type; their sum
-// takes them unrounded.
+// Waits for this wave's loads but the last N.
+template <int N>
+__device__ __forceinline__ void wait_all_but() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 0xF70);
+    asm volatile("" ::: "memory");
+}
+
+// 16 keys from 16 kb on, transposed, as the A operands of channels 32 db ..: lane half h holds keys 4 h + 0..3 and 8 + 4 h
+// + 0..3, the order in which the products' C registers hold the probabilities.  In assembly, with its wait, as K's.
+__device__ __forceinline__ void read_value_rows(const unsigned char* tile, int kb, int lane, r2o_u4 (&v)[4]) {
+    const int i = lane & 15, r = i >> 2;
+    const uint32_t a = lds_address(tile) + (16 * kb + 4 * (lane >> 5) + r) * 256 + 64 * r + 16 * (2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + 8 * (i & 1);
+    r2o_u2 lo[4], hi[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %3, %11\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:2048\n\tds_read_b64_tr_b16 %5, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %6, %10 offset:2048\n\tds_read_b64_tr_b16 %7, %11 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+        : "v"(a), "v"(a ^ 64), "v"(a ^ 128), "v"(a ^ 192)
+        : "memory");
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = r2o_u4{lo[x][0], lo[x][1], hi[x][0], hi[x][1]};
+}
+
+// A wave's 32 rows: their query rows, and the state of their softmax and products.
+struct Rows {
+    r2o_u4 q[8];
+    f16v acc[4];
+    float m, l;
+};
+
+__device__ __forceinline__ void start_rows(Rows& w, const uint16_t* src) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) w.q[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.acc[i] = f16v{};
+    w.m = -INFINITY;
+    w.l = 0.f;
+}
+
+// The query rows, which went out before any tile: waited for here, so that nothing but tiles is counted from here on.
+__device__ __forceinline__ void wait_rows(Rows& w) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) asm volatile("" : "+v"(w.q[t]));
+}
+
+// S^T of 32 keys x 32 rows
 template <int RF>
-__global__ __launch_bounds__(256, 2) void prefix_partial_kernel(PrefixArgs) {
-    __shared__ __align__(16) unsigned char k_lds[2][kTileBytes], v_lds[3][kTileBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-    const int worker = blockIdx.x;
-    int u, u_end;
-    {
-        Args& a = kernel_args();
-        int total;
-        find(a, -1, total);
-        const Share share = share_of(a, total);
-        if (worker >= share.workers || total == 0) return;
-        u = share.begin(worker);
-        u_end = share.begin(worker + 1);
+__device__ __forceinline__ f16v products(const Rows& w, const unsigned char* kl, int sub, int lane) {
+    f16v x = f16v{};
+    r2o_u4 k[8];
+    read_all_rows(kl, sub, lane, k);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) x = mfma32<RF>(k[t], w.q[t], x);
+    return x;
+}
+
+// Masks of 32 keys from `from` on, of which `groups` (a bit for 16) have a page and which a row sees up to `seen`; and the running
+// maximum raised where it has to be.
+__device__ __forceinline__ void top_of(Rows& w, f16v& x, int from, int seen, int groups, int lane, float c2) {
+    if (groups != 3 || __any(from + 31 > seen)) {
+        const int back = seen - from - 4 * (lane >> 5), back0 = groups & 1 ? back : -1, back1 = groups & 2 ? back : -1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = (i < 8 ? back0 : back1) >= 8 * (i >> 2) + (i & 3) ? x[i] : -INFINITY;
     }
+    float tmax = fmaxf(x[0], x[1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) tmax = fmaxf(tmax, fmaxf(x[i], x[i + 1]));
+    float y, z;
+    r2o_row_swap<32>(tmax, y, z);
+    tmax = fmaxf(y, z) * c2;  // -inf stays (c2 > 0)
+    if (__any(tmax > w.m + kSlack)) {
+        // of the rows that exceed it alone: a row's result does not depend on its neighbours
+        const float m_new = tmax > w.m + kSlack ? tmax : w.m;
+        const float alpha = m_new == w.m ? 1.f : __builtin_amdgcn_exp2f(w.m - m_new);
+        w.l *= alpha;
+#pragma unroll
+        for (int db = 0; db < 4; ++db) w.acc[db] *= alpha;
+        w.m = m_new;
+    }
+}
+
+template <int RF>
+__device__ __forceinline__ void probabilities(Rows& w, const f16v& x, r2o_u4 (&pk)[2], float c2) {
+    const float mm = w.m == -INFINITY ? 0.f : w.m;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c2, -mm));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], c2, -mm));
+        w.l += e0 + e1;
+        pk[i >> 3][(i & 7) >> 1] = pack2<RF>(e0, e1);
+    }
+}
+
+template <int RF>
+__device__ __forceinline__ void values(Rows& w, const unsigned char* vl, int sub, const r2o_u4 (&pk)[2], int lane) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        r2o_u4 v[4];
+        read_value_rows(vl, 2 * sub + kb, lane, v);
+#pragma unroll
+        for (int db = 0; db < 4; ++db) w.acc[db] = mfma32<RF>(v[db], pk[kb], w.acc[db]);
+    }
+}
+
+// Whether a channel's sum is infinite or NaN in a row of this wave that counts; a NaN sum of the softmax, of a NaN logit,
+// makes the whole row NaN anyhow.
+__device__ __forceinline__ bool met_not_finite(const Rows& w, bool counts) {
+    float odd[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) odd[db] = __builtin_fmaf(w.acc[db][i], 0.f, odd[db]);  // NaN where one is not finite
+    const float any = odd[0] + odd[1] + odd[2] + odd[3];
+    return __any(any != any && w.l == w.l && counts);
+}
+
+// All bits for a finite number, none for an infinite one or NaN: by arithmetic, for 64 conditions at a time do not fit.
+__device__ __forceinline__ uint32_t finite_mask(uint32_t bits) { return (uint32_t)((int)((bits & 0x7f800000u) - 0x7f800000u) >> 31); }
+
+// A row's channel is infinite or NaN where a key that it sees is, however small that key's weight: not NaN where the weight is
+// rounded to 0 on its way to the product.  Those channels are formed again from the values alone, 32 channels (block db) at a
+// time: slots j0 .. j1 - 1 of a side added here, till every row has NaN alone.
+template <int RF>
+__device__ __forceinline__ void add_not_finite(f16v& extra, int db, const Side& x, int j0, int j1, int seen, bool counts, int lane) {
+    bool more = true;
+#pragma unroll 1
+    for (int j16 = j0; j16 < j1 && more; j16 += 16) {
+        const int page = page_of(x, j16);
+        if (page < 0) continue;
+        const uint16_t* rows = x.v + (int64_t)page * x.v_page + (int64_t)(j16 & ((1 << x.shift) - 1)) * x.v_slot;
+        r2o_u4 chunk[4];  // of four rows each
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            chunk[n] = r2o_ldg(reinterpret_cast<const r2o_u4*>(rows + (int64_t)(4 * n + (lane >> 4)) * x.v_slot) + (lane & 15));
+        if (!__any(zero_not_finite<RF>(chunk))) continue;
+        for (int j = 0; j < min(16, x.n - j16); ++j) {
+            if (j16 + j > seen) continue;
+            const uint16_t* value = rows + (int64_t)j * x.v_slot + 32 * db + 4 * (lane >> 5);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const r2o_u2 y = r2o_ldg(reinterpret_cast<const r2o_u2*>(value + 8 * g));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t bits = y[k >> 1] >> 16 * (k & 1) & 0xffffu, z = __float_as_uint(RF == 0 ? r2o_bf16_to_f32(bits) : r2o_f16_to_f32(bits));
+                    extra[4 * g + k] += __uint_as_float(z & ~finite_mask(z));
+                }
+            }
+        }
+        float number = extra[0];  // the largest that is no NaN, or NaN
+#pragma unroll
+        for (int i = 0; i < 16; ++i) number = fmaxf(number, extra[i]);
+        more = !__all(number != number || !counts);
+    }
+}
+
+__device__ __forceinline__ void take_not_finite(f16v& acc, const f16v& extra) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t x = __float_as_uint(extra[i]), keep = finite_mask(x);
+        acc[i] = __uint_as_float((__float_as_uint(acc[i]) & keep) | (x & ~keep));
+    }
+}
+
+__device__ __forceinline__ void store_state(Args& a, const Rows& w, uint32_t to, bool counts, int lane) {
+    if (to == kNoRow) return;
+    const int half = lane >> 5;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<R2O_GLOBAL r2o_f4*>((R2O_GLOBAL float*)(a.partial_out + (int64_t)to * 128 + 32 * db + 8 * g + 4 * half)) =
+                r2o_f4{w.acc[db][4 * g], w.acc[db][4 * g + 1], w.acc[db][4 * g + 2], w.acc[db][4 * g + 3]};
+    if (half == 0) {
+        a.partial_ml[2 * (int64_t)to] = counts ? w.m : -INFINITY;
+        a.partial_ml[2 * (int64_t)to + 1] = counts ? w.l : 0.f;
+    }
+}
+
+constexpr int kKeyTiles = kAhead, kValueTiles = kAhead + 1;
+typedef unsigned char Lds[kKeyTiles + kValueTiles][kTileBytes];
+
+__device__ __forceinline__ void lds_barrier() {  // of LDS alone: stores to memory are not waited for
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A workgroup's part of a list of row tiles, its own slots behind a prefix's where rows are not merged.  S^T = K Q^T (32 keys x 32
+// rows a product), O^T += V^T P^T; three tiles ahead go into LDS while one is computed on.  A tile is two halves of 32 keys: the
+// products of the half that follows run beside the exponentials of the one before it.
+template <int RF, bool MERGED>
+__device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const Lane& first, int u, int u_end) {
     while (u < u_end) {
         Args& a = kernel_args();
+        int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), worker = blockIdx.x;
+        asm("" : "+v"(lane), "+s"(wave), "+s"(worker));  // or what depends on them alone would be held from one segment to the next
         int total;
-        const Entry e = find(a, u, total);
+        const Entry e = MERGED ? find_prefix(first, u) : find_request(first, u, total);
         if (e.request == -2) return;  // lengths that change meanwhile
-        const Segment s = segment_of(a, e, u);
+        const Segment s = segment_of(e, u);
         const int begin = u - s.base, stop = min(s.tiles, u_end - s.base);
         if (begin < 0 || stop <= begin || s.head >= a.hkv) return;
 
         // this lane's row, and the last key of its own that it sees
-        const int at = min(s.row0 + 32 * wave + col, s.rows - 1), group = a.group;
-        const int rank = e.request < 0 ? at / a.packed : 0, p = at - rank * a.packed, row = p / group, head = s.head * group + p - row * group;
-        const int b = e.request < 0 ? e.first + rank : e.request;
-        const bool busy = s.row0 + 32 * wave < s.rows;  // of this wave
-        // where its partial state goes; -1 for no row, -2 for a row that is written here
-        uint32_t to = 0xffffffffu;
-        if (s.row0 + 32 * wave + col < s.rows) {
-            if (begin > 0 || stop < s.tiles) to = (uint32_t)split_rows(worker, begin == 0) + 32 * wave + col;
-            else if (a.merged) to = (uint32_t)whole_rows(a, e.request < 0, e.first, e.members, e.request, s.head) + s.row0 + 32 * wave + col;
-            else to = 0xfffffffeu;
+        int two = __builtin_amdgcn_readfirstlane(e.rows - s.row0 <= kRows / 2);  // waves share the keys of 32 rows, a half of each tile each
+        const int part = two ? wave >> 2 : 0, in_tile = 32 * (two ? wave & 3 : wave) + (lane & 31);
+        const int at = min(s.row0 + in_tile, e.rows - 1), group = a.group;
+        const int rank = MERGED ? at / a.packed : 0, p = at - rank * a.packed, row = p / group, head = s.head * group + p - row * group;
+        const int b = MERGED ? e.first + rank : e.request;
+        int busy = __builtin_amdgcn_readfirstlane(s.row0 + in_tile - (lane & 31) < e.rows);  // of this wave
+        asm("" : "+s"(two), "+s"(busy));  // compared where they are asked, not held as masks
+        uint32_t to = kNoRow;
+        if (s.row0 + in_tile < e.rows && part == 0) {
+            if (begin > 0 || stop < s.tiles) to = split_rows(worker, begin == 0) + in_tile;
+            else if (MERGED) to = whole_prefix_rows(a, e.first, e.members, s.head) + s.row0 + in_tile;
+            else to = kResult;
         }
+        Rows w;
+        start_rows(w, a.query + (int64_t)b * a.q_batch + (int64_t)head * a.q_head + (int64_t)row * a.q_row + 8 * (lane >> 5));
         int counted = a.rows;
-        if (a.query_lengths) counted = min(max(r2o_ldg(a.query_lengths + b), 0), a.rows);
-        const int off = s.n_own - counted;
-        const int see_own = min(off + row, s.n_own - 1);
-        // the least that a row of the workgroup, and of this wave, sees of them; no row of a prefix's segment has any
-        const int wg_least = __builtin_amdgcn_readfirstlane(e.request < 0 ? 0 : min(s.n_own - counted + s.row0 / group, s.n_own - 1));
-        const int most = __builtin_amdgcn_readfirstlane(
-            e.request < 0 ? -1 : min(s.n_own - counted + min(s.row0 + kRows - 1, s.rows - 1) / group, s.n_own - 1));
-        const int last = min(stop, s.shared + max(most, -1) / kTile + (most >= 0));  // tiles behind it are seen by no row
-
-        r2o_u4 q[8];
-        {
-            const uint16_t* src = a.query + (int64_t)b * a.q_batch + (int64_t)head * a.q_head + (int64_t)row * a.q_row + 8 * half;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) q[t] = r2o_ldg(reinterpret_cast<const r2o_u4*>(src + 16 * t));
-        }
-        float m = -INFINITY, l = 0.f;
-        f16v acc[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = f16v{};
+        if (a.query_lengths) counted = counted_rows(r2o_ldg(a.query_lengths + b));
+        const int see_own = min(e.n_own - counted + row, e.n_own - 1);
+        // the least and the most that a row of the workgroup sees of them; no row of a prefix's segment has any
+        const int base_row = e.n_own - __builtin_amdgcn_readfirstlane(counted);
+        const int least = MERGED ? 0 : min(base_row + s.row0 / group, e.n_own - 1);
+        const int most = MERGED ? -1 : min(base_row + min(s.row0 + kRows - 1, e.rows - 1) / group, e.n_own - 1);
+        const int last = min(stop, s.shared + (most >= 0 ? most / kTile + 1 : 0));  // tiles behind it are seen by no row
         const float c2 = a.c2;
         bool bad = false;
 
         auto side_at = [&](int it) {
             Args& x = kernel_args();
-            return it < s.shared ? side_of(x.shared, e.prefix, s.head, s.n_shared) : side_of(x.own, e.request, s.head, s.n_own);
+            return MERGED || it < s.shared ? side_of(x.shared, e.prefix, s.head, e.n_shared) : side_of(x.own, e.request, s.head, e.n_own);
         };
-        auto slot_of = [&](int it) { return (it < s.shared ? it : it - s.shared) * kTile; };
-        // Loads of a tile; which groups of 16 slots count.
-        auto stage = [&](int it, int v_at) {
-            const Side x = side_at(it);
-            const int j0 = slot_of(it), j = (j0 + 16 * wave) & ((1 << x.shift) - 1);
-            int page;
-            const int valid = tile_valid(x, j0, wave, page);
-            stage_group<0>(x.k + (int64_t)page * x.k_page + (int64_t)j * x.k_slot, x.k_slot, k_lds[it & 1], wave, lane);
-            stage_group<1>(x.v + (int64_t)page * x.v_page + (int64_t)j * x.v_slot, x.v_slot, v_lds[v_at], wave, lane);
+        auto slot_of = [&](int it) { return (MERGED || it < s.shared ? it : it - s.shared) * kTile; };
+        auto last_seen = [&](int it) { return MERGED || it < s.shared ? e.n_shared - 1 : see_own; };
+        // The side and the pages of the next tile to be staged, and its buffers.
+        Side side = side_at(begin);
+        auto window_at = [&](int it) {
+            Args& x = kernel_args();
+            return window_of(MERGED || it < s.shared ? x.shared : x.own, side.table, slot_of(it) >> side.shift, lane);
+        };
+        Window window = window_at(begin);
+        int k_at = 0, v_at = kKeyTiles;
+        asm("" : "+s"(k_at), "+s"(v_at));  // or every wave's place in each would be held in a register
+        // This wave's eight rows of K and V; which of the tile's four groups of 16 slots, each within a page, count.
+        auto stage = [&](int it) {
+            const int j0 = slot_of(it), page0 = j0 >> side.shift;
+            if (!MERGED && it == s.shared && it > begin) {
+                side = side_at(it);
+                window = window_at(it);
+            } else if (page0 - window.first > 63) {
+                window = window_at(it);
+            }
+            auto page_at = [&](int j) { return __builtin_amdgcn_readlane(window.ids, (j >> side.shift) - window.first); };
+            int valid = 0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) valid |= (page_at(j0 + 16 * g) >= 0 && j0 + 16 * g < side.n) << g;
+            const int j1 = j0 + 16 * (wave >> 1), i0 = 2 * (wave & 1), j = j1 & ((1 << side.shift) - 1), id = max(page_at(j1), 0);
+            const uint16_t* k = side.k + (int64_t)id * side.k_page + (int64_t)j * side.k_slot;
+            const uint16_t* v = side.v + (int64_t)id * side.v_page + (int64_t)j * side.v_slot;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                stage_four<0>(k, side.k_slot, i0 + i, lds[k_at] + (8 * wave + 4 * i) * 256, lane);
+                stage_four<1>(v, side.v_slot, i0 + i, lds[v_at] + (8 * wave + 4 * i) * 256, lane);
+            }
+            k_at = k_at == kKeyTiles - 1 ? 0 : k_at + 1;
+            v_at = v_at == kKeyTiles + kValueTiles - 1 ? kKeyTiles : v_at + 1;
             return valid;
         };
-        auto last_seen = [&](int it) { return it < s.shared ? s.n_shared - 1 : see_own; };
-        // This wave's 16 value rows of a staged tile.  Rows that no row of the workgroup sees may hold anything: zero.  Where some see
-        // a row that others do not, 0 times an infinite or NaN value would be NaN: those become zero before any product.
-        auto clean = [&](int it, int v_at, int valid) {
-            const int n = it < s.shared ? s.n_shared : s.n_own, j0 = slot_of(it) + 16 * wave;
-            const bool some = it >= s.shared && slot_of(it) + kTile - 1 > wg_least && wg_least < n - 1;
-            const bool ends = j0 + 16 > n || !(valid >> wave & 1);
-            if (!some && !ends) return;
-            r2o_u4* at_lds = reinterpret_cast<r2o_u4*>(v_lds[v_at] + 16 * wave * 256) + lane;
-            r2o_u4 x[4];
+        // This wave's eight value rows of a staged tile.  Rows that no row of the workgroup sees may hold anything: zero.  Where some
+        // see a row that others do not, 0 times an infinite or NaN value would be NaN: those become zero before any product.
+        auto clean = [&](int it, int v_buffer, int valid) {
+            const int n = MERGED || it < s.shared ? e.n_shared : e.n_own, j0 = slot_of(it);
+            const bool some = !MERGED && it >= s.shared && j0 + kTile - 1 > least && least < n - 1;
+            if (valid == 15 && j0 + kTile <= n && !some) return;  // the same for all waves
+            r2o_u4* at_lds = reinterpret_cast<r2o_u4*>(lds[v_buffer] + 8 * wave * 256) + lane;
+            r2o_u4 x[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 x[i] = at_lds[64 * i];
-                if (!(valid >> wave & 1) || j0 + 4 * i + (lane >> 4) >= n) x[i] = r2o_u4{};
+                if (!(valid >> (wave >> 1) & 1) || j0 + 8 * wave + 4 * i + (lane >> 4) >= n) x[i] = r2o_u4{};
             }
             bad |= some && zero_not_finite<RF>(x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) at_lds[64 * i] = x[i];
+            for (int i = 0; i < 2; ++i) at_lds[64 * i] = x[i];
+            lds_barrier();
         };
-        auto products = [&](const unsigned char* kl, int sub) __attribute__((always_inline)) {
-            f16v x = f16v{};
-            r2o_u4 k[8];
-            read_all_rows(kl, sub, lane, k);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) x = mfma32<RF>(k[t], q[t], x);
-            return x;
+        // Tile `it`'s loads have landed for every wave, but for those of `behind` tiles after it.  Behind the barrier no wave reads
+        // the keys of the tile before it, nor the values of the one before that.
+        auto arrive = [&](int behind) {
+            if (behind >= 3) wait_all_but<12>();
+            else if (behind == 2) wait_all_but<8>();
+            else if (behind == 1) wait_all_but<4>();
+            else wait_all_but<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
         };
-        // masks, and the running maximum raised where it has to be
-        auto top_of = [&](f16v& x, int it, int sub, int valid) __attribute__((always_inline)) {
-            const int from = slot_of(it) + 32 * sub, seen = last_seen(it);
-            if (valid != 15 || __any(from + 31 > seen)) {
-                const int back = seen - from - 4 * half;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    x[i] = back >= 8 * (i >> 2) + (i & 3) && (valid >> (2 * sub + (i >> 3)) & 1) ? x[i] : -INFINITY;
-            }
-            float tmax = fmaxf(x[0], x[1]);
-#pragma unroll
-            for (int i = 2; i < 16; i += 2) tmax = fmaxf(tmax, fmaxf(x[i], x[i + 1]));
-            float y, z;
-            r2o_row_swap<32>(tmax, y, z);
-            tmax = fmaxf(y, z) * c2;  // -inf stays (c2 > 0)
-            if (__any(tmax > m + kSlack)) {
-                // of the rows that exceed it alone: a row's result does not depend on its neighbours
-                const float m_new = tmax > m + kSlack ? tmax : m;
-                const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-                l *= alpha;
-#pragma unroll
-                for (int db = 0; db < 4; ++db) acc[db] *= alpha;
-                m = m_new;
-            }
-        };
-        auto probabilities = [&](const f16v& x, r2o_u4 (&pk)[2]) __attribute__((always_inline)) {
-            const float mm = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c2, -mm));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], c2, -mm));
-                l += e0 + e1;
-                pk[i >> 3][(i & 7) >> 1] = pack2<RF>(e0, e1);
-            }
-        };
-        auto values = [&](const unsigned char* vl, int sub, const r2o_u4 (&pk)[2]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int db = 0; db < 4; ++db) acc[db] = mfma32<RF>(read_values(vl, 2 * sub + kb, db, lane), pk[kb], acc[db]);
-        };
-        // A tile is two halves of 32 keys; the products of the half that follows run beside the exponentials of the one
-        // before it.  A wave without rows brings its rows of the tiles alone.
+        int valid = 0;  // four bits a tile, from the current one on
+        wait_rows(w);
         if (begin < last) {
-            int valid = stage(begin, 0), next = 0, after = 0;
-            if (begin + 1 < last) next = stage(begin + 1, 1);
-            wait_staged();
-            clean(begin, 0, valid);
-            __syncthreads();
-            f16v even{};
-            if (busy) even = products(k_lds[begin & 1], 0);
-            for (int it = begin, v_at = 0; it < last; ++it) {
-                const int v_next = v_at == 2 ? 0 : v_at + 1;
-                r2o_u4 pk[2];
-                f16v odd{};
-                if (busy) {
-                    top_of(even, it, 0, valid);
-                    odd = products(k_lds[it & 1], 1);
-                    probabilities(even, pk);
-                    values(v_lds[v_at], 0, pk);
-                    top_of(odd, it, 1, valid);
+            int staged = begin;
+#pragma unroll 1
+            for (int i = 0; i < 4 * kAhead && staged < last; i += 4) {
+                valid |= stage(staged) << i;
+                ++staged;
+            }
+            arrive(staged - begin - 1);
+            int k_now = 0, v_now = kKeyTiles;
+            clean(begin, v_now, valid & 15);
+            // From tile `it` to the next one: v_last is left for the values that are still to be read.
+            int v_last = 0;
+            auto next = [&](int it) __attribute__((always_inline)) {
+                k_now = k_now == kKeyTiles - 1 ? 0 : k_now + 1;
+                v_last = v_now;
+                v_now = v_now == kKeyTiles + kValueTiles - 1 ? kKeyTiles : v_now + 1;
+                if (it + 1 < last) {
+                    arrive(staged - it - 2);
+                    if (staged < last) {
+                        valid |= stage(staged) << 4 * kAhead;
+                        ++staged;
+                    }
+                    clean(it + 1, v_now, valid >> 4 & 15);
                 }
-                wait_staged();
-                if (it + 1 < last) clean(it + 1, v_next, next);
-                __syncthreads();  // the next tile is there; this one's V stays till every wave is past the next barrier
-                if (busy) {
-                    even = products(k_lds[(it + 1) & 1], 0);  // behind the last tile: what lies there, not used
-                    probabilities(odd, pk);
-                    values(v_lds[v_at], 1, pk);
+                valid >>= 4;
+            };
+            // Behind the last tile the products are of what lies there, and not used.
+            if (!busy) {  // brings its rows of the tiles alone
+                for (int it = begin; it < last; ++it) next(it);
+            } else if (two) {
+                f16v now = products<RF>(w, lds[0], part, lane);
+                for (int it = begin; it < last; ++it) {
+                    r2o_u4 pk[2];
+                    top_of(w, now, slot_of(it) + 32 * part, last_seen(it), valid >> 2 * part & 3, lane, c2);
+                    probabilities<RF>(w, now, pk, c2);
+                    next(it);
+                    now = products<RF>(w, lds[k_now], part, lane);
+                    values<RF>(w, lds[v_last], part, pk, lane);
                 }
-                if (it + 2 < last) after = stage(it + 2, v_next == 2 ? 0 : v_next + 1);
-                valid = next;
-                next = after;
-                v_at = v_next;
+            } else {
+                f16v even = products<RF>(w, lds[0], 0, lane);
+                for (int it = begin; it < last; ++it) {
+                    r2o_u4 pk[2];
+                    top_of(w, even, slot_of(it), last_seen(it), valid & 3, lane, c2);
+                    f16v odd = products<RF>(w, lds[k_now], 1, lane);
+                    probabilities<RF>(w, even, pk, c2);
+                    values<RF>(w, lds[v_now], 0, pk, lane);
+                    top_of(w, odd, slot_of(it) + 32, last_seen(it), valid >> 2 & 3, lane, c2);
+                    next(it);
+                    even = products<RF>(w, lds[k_now], 0, lane);
+                    probabilities<RF>(w, odd, pk, c2);
+                    values<RF>(w, lds[v_last], 1, pk, lane);
+                }
             }
         }
-        __syncthreads();
-        int* const flags = reinterpret_cast<int*>(k_lds[0]);
-        const bool wave_bad = __any(bad);
-        if (lane == 0) flags[wave] = wave_bad;
-        __syncthreads();
-        const bool any_bad = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
         {
             float x, y;
-            r2o_row_swap<32>(l, x, y);
-            l = x + y;
+            r2o_row_swap<32>(w.l, x, y);
+            w.l = x + y;
         }
-        // A row's channel is infinite or NaN where a key that it sees is, however small that key's weight: not NaN where the weight
-        // is rounded to 0 on its way to the product.  Those channels are formed again from the values alone.
-        float odd_sum[4] = {};
+        const bool wave_bad = __any(bad);
+        if (lane == 0) flags[wave] = wave_bad;
+        lds_barrier();  // no wave reads a tile any more
+        if (two && part) {
+            r2o_f4* to_lds = reinterpret_cast<r2o_f4*>(lds[wave & 3]) + lane;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 16; ++i)
+                to_lds[64 * i] = r2o_f4{w.acc[i >> 2][4 * (i & 3)], w.acc[i >> 2][4 * (i & 3) + 1], w.acc[i >> 2][4 * (i & 3) + 2], w.acc[i >> 2][4 * (i & 3) + 3]};
+            float* ml = reinterpret_cast<float*>(lds[4]) + 128 * (wave & 3) + lane;
+            ml[0] = w.m;
+            ml[64] = w.l;
+        }
+        lds_barrier();
+        if (two && !part) {
+            const float* ml = reinterpret_cast<const float*>(lds[4]) + 128 * wave + lane;
+            const float m2 = ml[0], l2 = ml[64], mn = fmaxf(w.m, m2), ms = mn == -INFINITY ? 0.f : mn;
+            const float f = __builtin_amdgcn_exp2f(w.m - ms), f2 = __builtin_amdgcn_exp2f(m2 - ms);
+            const r2o_f4* from_lds = reinterpret_cast<const r2o_f4*>(lds[wave]) + lane;
 #pragma unroll
-            for (int db = 0; db < 4; ++db) odd_sum[db] = __builtin_fmaf(acc[db][i], 0.f, odd_sum[db]);  // NaN where one is not finite
-        const float any_odd = odd_sum[0] + odd_sum[1] + odd_sum[2] + odd_sum[3];
-        const bool met = __any(any_odd != any_odd && l == l && row < counted);  // a NaN sum, of a NaN logit, makes the whole row NaN
-        if (busy && (any_bad || met)) {
-            f16v extra[4];
+            for (int i = 0; i < 16; ++i) {
+                const r2o_f4 o = from_lds[64 * i];
 #pragma unroll
-            for (int db = 0; db < 4; ++db) extra[db] = f16v{};
-            bool more = true;  // till every row has NaN alone
-            for (int it = begin; it < last && more; ++it) {
-                const Side x = side_at(it);
-                const int seen = last_seen(it);
-                for (int j16 = slot_of(it); j16 < slot_of(it) + kTile && more; j16 += 16) {
-                    const int page = page_of(x, j16);
-                    if (page < 0) continue;
-                    const uint16_t* rows = x.v + (int64_t)page * x.v_page + (int64_t)(j16 & ((1 << x.shift) - 1)) * x.v_slot;
-                    r2o_u4 chunk[4];  // of four rows each
-                    bool any = false;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        chunk[n] = r2o_ldg(reinterpret_cast<const r2o_u4*>(rows + (int64_t)(4 * n + (lane >> 4)) * x.v_slot) + (lane & 15));
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) any |= any_not_finite<RF>(chunk[n]);
-                    if (!__any(any)) continue;
-                    for (int j = 0; j < min(16, x.n - j16); ++j) {
-                        if (j16 + j > seen) continue;
-                        const uint16_t* src = rows + (int64_t)j * x.v_slot + 4 * half;
-#pragma unroll
-                        for (int db = 0; db < 4; ++db)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const uint32_t y = r2o_ldg(src + 32 * db + 8 * (i >> 2) + (i & 3));
-                                if (not_finite<RF>(y)) extra[db][i] += RF == 0 ? r2o_bf16_to_f32(y) : r2o_f16_to_f32(y);
-                            }
-                    }
-                    bool all_nan = true;
-#pragma unroll
-                    for (int db = 0; db < 4; ++db)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) all_nan &= extra[db][i] != extra[db][i];
-                    more = !__all(all_nan || row >= counted);
-                }
+                for (int k = 0; k < 4; ++k) w.acc[i >> 2][4 * (i & 3) + k] = weighed(w.acc[i >> 2][4 * (i & 3) + k], f) + weighed(o[k], f2);
             }
+            w.l = w.l * f + l2 * f2;
+            w.m = mn;
+        }
+        int any_bad = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) any_bad |= flags[i];
+        const bool counts = row < counted;
+        if (busy && part == 0 && (any_bad || met_not_finite(w, counts))) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+                f16v extra = f16v{};
+#pragma unroll 1
+                for (int from = begin, to_tile; from < last; from = to_tile) {  // the prefix's, then its own
+                    to_tile = MERGED || from >= s.shared ? last : min(last, s.shared);
+                    add_not_finite<RF>(extra, db, side_at(from), slot_of(from), slot_of(from) + (to_tile - from) * kTile, last_seen(from), counts, lane);
+                }
+                take_not_finite(w.acc[db], extra);
+            }
+        }
+        if (!MERGED && to == kResult) {
+            Args& x = kernel_args();
+            const bool live = counts && !(w.l == 0.f);  // no key seen; NaN logits leave m, and a NaN sum
+            const float inv = live ? 1.f / w.l : 0.f;
+            uint16_t* dst = x.out + (int64_t)b * x.o_batch + (int64_t)head * x.o_head + (int64_t)row * x.o_row;
 #pragma unroll
             for (int db = 0; db < 4; ++db)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[db][i] = __builtin_isfinite(extra[db][i]) ? acc[db][i] : extra[db][i];
-        }
-        if (to != 0xffffffffu) {
-            Args& x = kernel_args();
-            if (to == 0xfffffffeu) {
-                const bool live = row < counted && !(l == 0.f);  // no key seen; NaN logits leave m, and a NaN sum
-                const float inv = live ? 1.f / l : 0.f;
-                uint16_t* dst = x.out + (int64_t)b * x.o_batch + (int64_t)head * x.o_head + (int64_t)row * x.o_row;
+                for (int g = 0; g < 4; ++g) {
+                    r2o_u2 y;
 #pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        r2o_u2 w;
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            w[k] = live ? pack2<RF>(acc[db][4 * g + 2 * k] * inv, acc[db][4 * g + 2 * k + 1] * inv) : 0u;
-                        *reinterpret_cast<R2O_GLOBAL r2o_u2*>((R2O_GLOBAL uint16_t*)(dst + 32 * db + 8 * g + 4 * half)) = w;
-                    }
-                if (half == 0) x.lse[((int64_t)b * x.hq + head) * x.rows + row] = live ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-            } else {
-#pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        *reinterpret_cast<R2O_GLOBAL r2o_f4*>((R2O_GLOBAL float*)(x.partial_out + (int64_t)to * 128 + 32 * db + 8 * g + 4 * half)) =
-                            r2o_f4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
-                if (half == 0) {
-                    x.partial_ml[2 * (int64_t)to] = row < counted ? m : -INFINITY;
-                    x.partial_ml[2 * (int64_t)to + 1] = row < counted ? l : 0.f;
+                    for (int k = 0; k < 2; ++k)
+                        y[k] = live ? pack2<RF>(w.acc[db][4 * g + 2 * k] * inv, w.acc[db][4 * g + 2 * k + 1] * inv) : 0u;
+                    *reinterpret_cast<R2O_GLOBAL r2o_u2*>((R2O_GLOBAL uint16_t*)(dst + 32 * db + 8 * g + 4 * (lane >> 5))) = y;
                 }
-            }
+            if (lane < 32) x.lse[((int64_t)b * x.hq + head) * x.rows + row] = live ? (w.m + __builtin_amdgcn_logf(w.l)) * kLn2 : -INFINITY;
+        } else {
+            store_state(kernel_args(), w, to, counts, lane);
         }
         u = s.base + stop;
-        __syncthreads();  // the flags lie where the next tiles go
+        lds_barrier();  // flags and states lie where the next segment's go
+    }
+}
+
+// A wave's part of the requests' own slots (merged rows), in tiles of 32 rows and 32 keys, without a barrier: the next tile's
+// keys go out when this one's products have read theirs, its values when these have been.
+template <int RF>
+__device__ __forceinline__ void work_on_own(Lds& lds, const Lane& first, int own_first, int index, int u, int u_end) {
+    while (u < u_end) {
+        Args& a = kernel_args();
+        int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        asm("" : "+v"(lane), "+s"(wave));
+        const Entry e = find_own(first, u);
+        if (e.request == -2) return;  // lengths that change meanwhile
+        const Segment s = segment_at(e, u, div_up(e.n_own, kWaveKeys), div_up(a.packed, kWaveRows), kWaveRows);
+        const int begin = u - s.base, stop = min(s.tiles, u_end - s.base);
+        if (begin < 0 || stop <= begin || s.head >= a.hkv) return;
+        const int p = min(s.row0 + (lane & 31), a.packed - 1), row = p / a.group, head = s.head * a.group + p - row * a.group;
+        uint32_t to = kNoRow;
+        if (s.row0 + (lane & 31) < a.packed)
+            to = (begin > 0 || stop < s.tiles ? split_wave_rows(own_first, index, begin == 0) : whole_own_rows(a, e.request, s.head) + s.row0) + (lane & 31);
+        Rows w;
+        start_rows(w, a.query + (int64_t)e.request * a.q_batch + (int64_t)head * a.q_head + (int64_t)row * a.q_row + 8 * (lane >> 5));
+        const int off = e.n_own - e.rows, seen = min(off + row, e.n_own - 1);
+        const int least = min(off + s.row0 / a.group, e.n_own - 1), most = min(off + min(s.row0 + kWaveRows - 1, a.packed - 1) / a.group, e.n_own - 1);
+        const int last = min(stop, most >= 0 ? most / kWaveKeys + 1 : 0);  // tiles behind it are seen by no row
+        const float c2 = a.c2;
+        const Side side = side_of(a.own, e.request, s.head, e.n_own);
+        Window window = window_of(a.own, side.table, begin * kWaveKeys >> side.shift, lane);
+        unsigned char *const kl = lds[wave], *const vl = kl + kTileBytes / 2;
+        bool bad = false;
+        // The page of a tile's group of 16 slots, -1 for none; windows are as wide as whole tiles.
+        auto page_at = [&](int j) {
+            if ((j >> side.shift) - window.first > 63) window = window_of(kernel_args().own, side.table, j >> side.shift, lane);
+            const int id = __builtin_amdgcn_readlane(window.ids, (j >> side.shift) - window.first);
+            return j < side.n ? id : -1;
+        };
+        auto stage = [&](const uint16_t* base, int page_stride, int slot_stride, int id, int j, auto swizzle, unsigned char* to_lds) {
+            const uint16_t* rows = base + (int64_t)max(id, 0) * page_stride + (int64_t)(j & ((1 << side.shift) - 1)) * slot_stride;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) stage_four<decltype(swizzle)::value>(rows, slot_stride, i, to_lds + 4 * i * 256, lane);
+        };
+        auto stage_keys = [&](int j, int id0, int id1) {
+            stage(side.k, side.k_page, side.k_slot, id0, j, std::integral_constant<int, 0>(), kl);
+            stage(side.k, side.k_page, side.k_slot, id1, j + 16, std::integral_constant<int, 0>(), kl + 4096);
+        };
+        auto stage_values = [&](int j, int id0, int id1) {
+            stage(side.v, side.v_page, side.v_slot, id0, j, std::integral_constant<int, 1>(), vl);
+            stage(side.v, side.v_page, side.v_slot, id1, j + 16, std::integral_constant<int, 1>(), vl + 4096);
+        };
+        wait_rows(w);
+        if (begin < last) {
+            int id0 = page_at(begin * kWaveKeys), id1 = page_at(begin * kWaveKeys + 16);
+            stage_keys(begin * kWaveKeys, id0, id1);
+            stage_values(begin * kWaveKeys, id0, id1);
+            for (int it = begin; it < last; ++it) {
+                const int j0 = it * kWaveKeys;
+                const bool more = it + 1 < last;
+                int next0 = -1, next1 = -1;
+                if (more) {
+                    next0 = page_at(j0 + kWaveKeys);
+                    next1 = page_at(j0 + kWaveKeys + 16);
+                }
+                wait_all_but<8>();
+                f16v x = products<RF>(w, kl, 0, lane);
+                if (more) stage_keys(j0 + kWaveKeys, next0, next1);
+                top_of(w, x, j0, seen, (id0 >= 0) | (id1 >= 0) << 1, lane, c2);
+                r2o_u4 pk[2];
+                probabilities<RF>(w, x, pk, c2);
+                if (more) wait_all_but<8>();
+                else wait_all_but<0>();
+                // rows that no row of the wave sees, or some do and others do not, as a workgroup has it
+                const bool some = j0 + kWaveKeys - 1 > least && least < side.n - 1;
+                if (some || id0 < 0 || id1 < 0 || j0 + kWaveKeys > side.n) {
+                    r2o_u4* at_lds = reinterpret_cast<r2o_u4*>(vl) + lane;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        r2o_u4 y[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            y[i] = at_lds[256 * g + 64 * i];
+                            if ((g ? id1 : id0) < 0 || j0 + 16 * g + 4 * i + (lane >> 4) >= side.n) y[i] = r2o_u4{};
+                        }
+                        bad |= some && zero_not_finite<RF>(y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) at_lds[256 * g + 64 * i] = y[i];
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+                values<RF>(w, vl, 0, pk, lane);
+                if (more) stage_values(j0 + kWaveKeys, next0, next1);
+                id0 = next0;
+                id1 = next1;
+            }
+        }
+        {
+            float x, y;
+            r2o_row_swap<32>(w.l, x, y);
+            w.l = x + y;
+        }
+        const bool counts = row < e.rows;
+        if (__any(bad) || met_not_finite(w, counts)) {
+            const Side x = side_of(kernel_args().own, e.request, s.head, e.n_own);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+                f16v extra = f16v{};
+                add_not_finite<RF>(extra, db, x, begin * kWaveKeys, last * kWaveKeys, seen, counts, lane);
+                take_not_finite(w.acc[db], extra);
+            }
+        }
+        store_state(kernel_args(), w, to, counts, lane);
+        u = s.base + stop;
+    }
+}
+
+// The probabilities are rounded to the rows' 16 bits for the product with V, whose two operands are of one type; their sum
+// takes them unrounded.
+template <int RF, bool MERGED>
+__global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixArgs) {
+    __shared__ __align__(1024) Lds lds;
+    __shared__ int flags[kWaves];
+    Args& a = kernel_args();
+    const Lane first = lane_of(0);
+    int u = 0, u_end = 0;
+    if constexpr (MERGED) {
+        int own_first, index, v = 0, v_end = 0;
+        {
+            const Sums sums = sums_of(first, -1);
+            const Plan plan = plan_of(a, sums.shared, sums.own, sums.shared_cost, sums.own_cost);
+            if (sums.shared > 0 && (int)blockIdx.x < plan.shared.workers) {
+                u = plan.shared.begin(blockIdx.x);
+                u_end = plan.shared.begin(blockIdx.x + 1);
+            }
+            own_first = plan.own_first;
+            index = kWaves * ((int)blockIdx.x - own_first) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            if (sums.own > 0 && index >= 0 && index < plan.own.workers) {
+                v = plan.own.begin(index);
+                v_end = plan.own.begin(index + 1);
+            }
+        }
+        work_on_row_tiles<RF, true>(lds, flags, first, u, u_end);
+        work_on_own<RF>(lds, first, own_first, index, v, v_end);
+    } else {
+        int total;
+        find_request(first, -1, total);
+        const Share share = share_of(total, a.workers);
+        if (total > 0 && (int)blockIdx.x < share.workers) {
+            u = share.begin(blockIdx.x);
+            u_end = share.begin(blockIdx.x + 1);
+        }
+        work_on_row_tiles<RF, false>(lds, flags, first, u, u_end);
     }
 }
 
@@ -564,7 +1016,8 @@ __device__ __forceinline__ void join_state(State& s, float m2, float l2, const r
     s.m = mn;
 }
 
-__device__ __forceinline__ void join_partial(Args& a, State& s, int64_t at, int d4) {
+__device__ __forceinline__ void join_partial(Args& a, State& s, uint32_t row, int d4) {
+    const int64_t at = row;
     const float m2 = r2o_ldg(a.partial_ml + 2 * at), l2 = r2o_ldg(a.partial_ml + 2 * at + 1);
     join_state(s, m2, l2, r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4));
 }
@@ -579,29 +1032,46 @@ __device__ __forceinline__ void write_row(Args& a, const State& s, int b, int he
     if (d4 == 0) a.lse[((int64_t)b * a.hq + head) * a.rows + row] = live ? (s.m + __builtin_amdgcn_logf(s.l)) * kLn2 : -INFINITY;
 }
 
-// Rows that are not merged: the workgroups (w, .) join the segment that worker w is the second to work on, 32 lanes a row.
+// Rows that are not merged.  Workgroups (w, .) join the segment that worker w + 1 is the second to work on, 32 lanes a row;
+// those behind the workers' write the rows that their requests do not count.
+constexpr int kJoinRows = 64;
+
 template <int RF>
 __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
     Args& a = kernel_args();
+    const int d4 = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
+    if ((int)blockIdx.x >= a.workers - 1) {
+        const int b = (int)blockIdx.x - (a.workers - 1), counted = counted_rows(load_uniform(a.query_lengths + b)), each = a.rows - counted;
+        const int64_t rows = (int64_t)a.hq * each;
+        for (int64_t i0 = r0; i0 < rows; i0 += gridDim.y * kJoinRows)
+#pragma unroll 1
+            for (int64_t i = i0; i < min(rows, i0 + kJoinRows); i += 8) {
+                const int head = (int)(i / each), row = counted + (int)(i - (int64_t)head * each);
+                write_row<RF>(a, State{-INFINITY, 0.f, r2o_f4{}}, b, head, row, d4);
+            }
+        return;
+    }
+    const Lane first = lane_of(0);
     int total;
-    find(a, -1, total);
-    const Share share = share_of(a, total);
+    find_request(first, -1, total);
+    const Share share = share_of(total, a.workers);
     const int w = (int)blockIdx.x + 1;
-    if (w >= share.workers) return;
+    if (total == 0 || w >= share.workers) return;
     const int u = share.begin(w);
-    const Entry e = find(a, u, total);
+    const Entry e = find_request(first, u, total);
     if (e.request < 0) return;
-    const Segment s = segment_of(a, e, u);
+    const Segment s = segment_of(e, u);
     if (s.base == u || s.base < share.begin(w - 1) || s.head >= a.hkv) return;  // begun here, or by another than the one before
-    const int count = share.worker(s.base + s.tiles - 1) - (w - 1) + 1;
-    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), d4 = threadIdx.x & 31;
-    if (s.row0 + r >= s.rows) return;
-    State x{-INFINITY, 0.f, r2o_f4{}};
-    join_partial(a, x, split_rows(w - 1, true) + r, d4);
+    const int count = share.worker(s.base + s.tiles - 1) - (w - 1) + 1, here = min(kRows, e.rows - s.row0);
+#pragma unroll 1
+    for (int r = r0; r < min(here, (int)(blockIdx.y + 1) * kJoinRows); r += 8) {
+        State x{-INFINITY, 0.f, r2o_f4{}};
+        join_partial(a, x, split_rows(w - 1, true) + r, d4);
 #pragma unroll 4
-    for (int i = 1; i < count; ++i) join_partial(a, x, split_rows(w - 1 + i, false) + r, d4);
-    const int p = s.row0 + r, row = p / a.group;
-    write_row<RF>(a, x, e.request, s.head * a.group + p - row * a.group, row, d4);
+        for (int i = 1; i < count; ++i) join_partial(a, x, split_rows(w - 1 + i, false) + r, d4);
+        const int p = s.row0 + r, row = p / a.group;
+        write_row<RF>(a, x, e.request, s.head * a.group + p - row * a.group, row, d4);
+    }
 }
 
 // Merged rows: a workgroup a row, whose partial states of the prefix's segment and of its own are shared by 8 groups of 32
@@ -611,49 +1081,35 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
     __shared__ __align__(16) float red[8][128];
     __shared__ float red_ml[8][2];
     Args& a = kernel_args();
+    const Lane first_lane = lane_of(0);
     const int per_request = a.hkv * a.packed;
     const int b = (int)blockIdx.x / per_request, in_request = (int)blockIdx.x - b * per_request, h = in_request / a.packed, p = in_request - h * a.packed;
     const int row = p / a.group, head = h * a.group + p - row * a.group, d4 = threadIdx.x & 31, part = threadIdx.x >> 5;
-    // one pass over the list: its length, and where this row's segments lie
-    int at = 0, before = 0, shared_base = 0, first = 0, members = 0, prefix = -1, own_base = 0;
-    for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
-        const Members x = lane_members(a, g0, before);
-        const int work = lane_prefix_work(a, g0, x), upto = wave_scan(work);
-        const uint64_t mine = __ballot((uint32_t)(b - x.first) < (uint32_t)x.count);
-        if (mine) {
-            const int i = __builtin_ctzll(mine);
-            prefix = g0 + i;
-            shared_base = at + __builtin_amdgcn_readlane(upto - work, i);
-            first = __builtin_amdgcn_readlane(x.first, i);
-            members = __builtin_amdgcn_readlane(x.count, i);
-        }
-        at += last_lane(upto);
-    }
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int work = lane_request_work(a, b0), upto = wave_scan(work);
-        if ((uint32_t)(b - b0) < 64u) own_base = at + __builtin_amdgcn_readlane(upto - work, b - b0);
-        at += last_lane(upto);
-    }
-    const Share share = share_of(a, at);
-    const int shared_tiles = prefix >= 0 ? key_tiles(a.shared, load_uniform(a.shared.lengths + prefix)) : 0;
-    const int own_tiles = key_tiles(a.own, load_uniform(a.own.lengths + b));
-    const int counted = a.query_lengths ? load_uniform(a.query_lengths + b) : a.rows;
+    const Sums sums = sums_of(first_lane, b);
+    const Plan plan = plan_of(a, sums.shared, sums.own, sums.shared_cost, sums.own_cost);
     State s{-INFINITY, 0.f, r2o_f4{}};
-    auto add = [&](int base, int tiles, int r, int64_t whole) {  // the states of one segment, row r of its tile
-        if (tiles == 0 || share.total == 0) return;
-        const int w0 = share.worker(base), count = share.worker(base + tiles - 1) - w0 + 1;
-        if (count == 1) {
-            if (part == 0) join_partial(a, s, whole, d4);
-            return;
+    if (row < sums.of_request.rows) {
+        const Entry& e = sums.of_prefix;
+        if (e.prefix >= 0 && e.n_shared > 0) {
+            const int r = (b - e.first) * a.packed + p, tile = r / kRows, tiles = div_up(e.n_shared, kTile);
+            const int base = e.base + (h * div_up(e.members * a.packed, kRows) + tile) * tiles;
+            const int w0 = plan.shared.worker(base), count = plan.shared.worker(base + tiles - 1) - w0 + 1;
+            if (count == 1) {
+                if (part == 0) join_partial(a, s, whole_prefix_rows(a, e.first, e.members, h) + r, d4);
+            } else {
+                for (int i = part; i < count; i += 8) join_partial(a, s, split_rows(w0 + i, i == 0) + r - tile * kRows, d4);
+            }
         }
-        for (int i = part; i < count; i += 8) join_partial(a, s, split_rows(w0 + i, i == 0) + r, d4);
-    };
-    if (row < counted) {
-        const int r = (b - first) * a.packed + p, tile = r / kRows;
-        if (prefix >= 0)
-            add(shared_base + (h * row_tiles(members * a.packed) + tile) * shared_tiles, shared_tiles, r - tile * kRows,
-                whole_rows(a, true, first, members, b, h) + r);
-        add(own_base + h * own_tiles, own_tiles, p, whole_rows(a, false, 0, 0, b, h) + p);
+        if (sums.of_request.n_own > 0) {
+            const int chunk = p / kWaveRows, tiles = div_up(sums.of_request.n_own, kWaveKeys);
+            const int base = sums.of_request.base + (h * div_up(a.packed, kWaveRows) + chunk) * tiles;
+            const int w0 = plan.own.worker(base), count = plan.own.worker(base + tiles - 1) - w0 + 1;
+            if (count == 1) {
+                if (part == 7) join_partial(a, s, whole_own_rows(a, b, h) + p, d4);
+            } else {
+                for (int i = 7 - part; i < count; i += 8) join_partial(a, s, split_wave_rows(plan.own_first, w0 + i, i == 0) + p - chunk * kWaveRows, d4);
+            }
+        }
     }
     *reinterpret_cast<r2o_f4*>(&red[part][4 * d4]) = s.o;
     if (d4 == 0) {
@@ -706,13 +1162,14 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
         return R2O_EINVAL;
     const int64_t group = p->hq / c.hkv, packed = group * p->rows, all_rows = c.batch * c.hkv * packed;
     if (packed > (1 << 30) || all_rows > (1 << 30)) return R2O_EINVAL;
-    const bool merged = any && packed < kRows;
+    const bool merged = any && packed < kMerged;
     if (p->scratch_floats < 130 * (2 * kRows * p->workers + (merged ? 2 * all_rows : 0))) return R2O_EINVAL;
     // whatever the lengths on the device say
     const int64_t shared = any ? tiles_of(f) : 0, per_request = (packed + kRows - 1) / kRows;
-    const int64_t most = merged ? c.hkv * (((c.batch * packed) / kRows + f.batch) * shared + c.batch * tiles_of(c))
-                                : c.hkv * c.batch * per_request * (shared + tiles_of(c));
-    if (most > 0x7fffffff - R2O_PAGED_MAX_WORKERS) return R2O_EINVAL;
+    const int64_t most = merged ? std::max(c.hkv * (c.batch * packed / kRows + f.batch) * shared,
+                                           c.hkv * c.batch * ((packed + kWaveRows - 1) / kWaveRows) * (kTile / kWaveKeys) * tiles_of(c))
+                                : c.hkv * c.batch * per_request * std::max<int64_t>(1, shared + tiles_of(c));
+    if (most > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS) return R2O_EINVAL;
     PrefixArgs a{};
     a.own = source_of(c);
     a.shared = any ? source_of(f) : a.own;
@@ -741,21 +1198,21 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     a.c2 = p->sm_scale * kLog2e;
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)p->workers);
-    if (c.dtype == 0) hipLaunchKernelGGL(prefix_partial_kernel<0>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(prefix_partial_kernel<1>, grid, dim3(256), 0, st, a);
-    R2O_CHECK_LAUNCH();
+    auto launch = [&](auto partial, auto join_kernel, const dim3& join) {
+        hipLaunchKernelGGL(partial, grid, dim3(64 * kWaves), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return R2O_ELAUNCH;
+        if (join.x == 0) return R2O_OK;
+        hipLaunchKernelGGL(join_kernel, join, dim3(256), 0, st, a);
+        return hipGetLastError() == hipSuccess ? R2O_OK : R2O_ELAUNCH;
+    };
     if (merged) {
         const dim3 join((unsigned)all_rows);
-        if (c.dtype == 0) hipLaunchKernelGGL(prefix_join_merged_kernel<0>, join, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(prefix_join_merged_kernel<1>, join, dim3(256), 0, st, a);
-        R2O_CHECK_LAUNCH();
-    } else if (p->workers > 1) {
-        const dim3 join((unsigned)p->workers - 1, kRows / 8);
-        if (c.dtype == 0) hipLaunchKernelGGL(prefix_join_split_kernel<0>, join, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(prefix_join_split_kernel<1>, join, dim3(256), 0, st, a);
-        R2O_CHECK_LAUNCH();
+        return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0>, join)
+                            : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1>, join);
     }
-    return R2O_OK;
+    const dim3 join((unsigned)(p->workers - 1 + (p->query_lengths ? c.batch : 0)), kRows / kJoinRows);
+    return c.dtype == 0 ? launch(prefix_partial_kernel<0, false>, prefix_join_split_kernel<0>, join)
+                        : launch(prefix_partial_kernel<1, false>, prefix_join_split_kernel<1>, join);
 }
 
 }  // extern "C"

@@ -100,12 +100,12 @@ __device__ __forceinline__ float weighed(float x, float f) { return __builtin_is
 
 // In a tile that some row of the workgroup sees in part, a masked key's probability is 0, but 0 times an infinite
 // or NaN value is NaN: such elements become zero before any product; true if there was one.
-template <int RF>
-__device__ __forceinline__ bool zero_not_finite(r2o_u4 (&x)[4]) {
+template <int RF, int N>
+__device__ __forceinline__ bool zero_not_finite(r2o_u4 (&x)[N]) {
     constexpr uint32_t e = RF == 0 ? 0x7f807f80u : 0x7c007c00u, one = RF == 0 ? 0x00800080u : 0x04000400u;
     uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint32_t bad = ((x[i][k] & e) + one) & 0x80008000u;  // a full exponent carries into the sign's place

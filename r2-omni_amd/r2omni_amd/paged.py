@@ -285,7 +285,7 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedCache, prefix: Paged
     _lib.refuse_gradients(what, query, *(t for c in caches for t in _pools(c)), *(output or ()))
     scale = _scale(sm_scale)
     most = _lib.host().prefix_tiles(batch, hkv, hq, rows, cache.capacity, prefixes, prefix.capacity if prefixes else 0)
-    if most > (1 << 31) - 4097:
+    if most > (1 << 31) - 1 - 8 * 4096:
         raise ValueError("paged prefix attention has more tiles of slots than it can count")
     params = [_params_of(c) for c in caches]
     query = _rows(query)
