@@ -197,11 +197,18 @@ __device__ __forceinline__ Plan plan_of(Args& a, int shared, int own, float shar
     return p;
 }
 
-// What a prefix's and a request's tiles cost, in the time that a compute unit takes for its part of the memory's rate and 16 KB.
-__device__ __forceinline__ float prefix_cost(int work, int rows) { return (float)work * (rows > kRows / 2 ? 3.f : 2.f); }
+// What this lane's prefix and request cost, in the time that a compute unit takes for 16 KB at its part of the memory's rate: a
+// row tile of 256 rows is bound by its products, one of up to 128 by its loads, and a segment's start and end cost a
+// workgroup about seven, a wave among eight about one.
+__device__ __forceinline__ float prefix_cost(const Lane& x, const Members& m) {
+    Args& a = kernel_args();
+    const int rows = m.count * a.packed, keys = div_up(filled(a.shared, x.shared), kTile);
+    const int halves = 2 * (rows / kRows) + div_up(rows % kRows, kRows / 2);
+    return keys ? (float)a.hkv * (2.f * keys * halves + 7.f * div_up(rows, kRows)) : 0.f;
+}
 __device__ __forceinline__ float own_cost(int work) {
     Args& a = kernel_args();
-    return (float)work + (work ? 1.f * a.hkv * div_up(a.packed, kWaveRows) : 0.f);
+    return work ? (float)work + (float)(a.hkv * div_up(a.packed, kWaveRows)) : 0.f;
 }
 
 __device__ __forceinline__ float wave_total(float x) {
@@ -245,7 +252,7 @@ __device__ __forceinline__ Sums sums_of(const Lane& first, int b) {
             s.of_prefix.members = __builtin_amdgcn_readlane(m.count, i);
             s.of_prefix.n_shared = filled(a.shared, __builtin_amdgcn_readlane(x.shared, i));
         }
-        s.shared_cost += wave_total(prefix_cost(work, m.count * a.packed));
+        s.shared_cost += wave_total(prefix_cost(x, m));
         s.shared += last_lane(upto);
     }
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
@@ -405,15 +412,24 @@ __device__ __forceinline__ int page_of(const Side& x, int j) {
     return j < x.n && (uint32_t)id < (uint32_t)x.pages ? id : -1;
 }
 
-// 64 neighbouring pages of a table, one a lane, -1 for one outside the pool.  Scalar loads of a tile's pages, one after the
-// other, took longer than the tile.
+// 64 neighbouring pages of a table, one a lane, -1 for one outside the pool, and a bit for each inside it.  Scalar loads of a
+// tile's pages, one after the other, took longer than the tile.
 struct Window {
     int first, ids;
+    uint64_t ok;
 };
 
 __device__ __forceinline__ Window window_of(SourceArgs& s, const int32_t* table, int first, int lane) {
     const int id = r2o_ldg(table + min(first + lane, s.last_page));
-    return {first, (uint32_t)id < (uint32_t)s.pages ? id : -1};
+    const bool ok = (uint32_t)id < (uint32_t)s.pages;
+    return {first, ok ? id : -1, __ballot(ok)};
+}
+
+// Which of the four groups of 16 slots from j0 (a multiple of 64) on, each within a page, have a page and a filled slot.
+__device__ __forceinline__ int groups_of(const Window& w, int j0, int shift, int n) {
+    const int bits = (int)(w.ok >> ((j0 >> shift) - w.first));
+    const int in_pages = shift == 4 ? bits & 15 : (shift == 5 ? (bits & 1) * 3 | (bits >> 1 & 1) * 12 : (bits & 1) * 15);
+    return n - j0 >= kTile ? in_pages : in_pages & (1 << (max(n - j0, 0) + 15) / 16) - 1;
 }
 
 // Four rows (of 16 from `base` on, the i-th four of them) straight into LDS.
@@ -480,6 +496,10 @@ __device__ __forceinline__ f16v products(const Rows& w, const unsigned char* kl,
     return x;
 }
 
+// The larger of two numbers, by the median of them and infinity: fmaxf makes each operand quiet first, one more instruction for
+// each product.  Of NaN and a number the number; of two NaN, in a row that is NaN anyhow, infinity.
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, INFINITY); }
+
 // Masks of 32 keys from `from` on, of which `groups` (a bit for 16) have a page and which a row sees up to `seen`; and the running
 // maximum raised where it has to be.
 __device__ __forceinline__ void top_of(Rows& w, f16v& x, int from, int seen, int groups, int lane, float c2) {
@@ -488,12 +508,12 @@ __device__ __forceinline__ void top_of(Rows& w, f16v& x, int from, int seen, int
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = (i < 8 ? back0 : back1) >= 8 * (i >> 2) + (i & 3) ? x[i] : -INFINITY;
     }
-    float tmax = fmaxf(x[0], x[1]);
+    float tmax = x[0];
 #pragma unroll
-    for (int i = 2; i < 16; i += 2) tmax = fmaxf(tmax, fmaxf(x[i], x[i + 1]));
+    for (int i = 1; i < 16; ++i) tmax = larger(tmax, x[i]);
     float y, z;
     r2o_row_swap<32>(tmax, y, z);
-    tmax = fmaxf(y, z) * c2;  // -inf stays (c2 > 0)
+    tmax = larger(y, z) * c2;  // -inf stays (c2 > 0)
     if (__any(tmax > w.m + kSlack)) {
         // of the rows that exceed it alone: a row's result does not depend on its neighbours
         const float m_new = tmax > w.m + kSlack ? tmax : w.m;
@@ -602,7 +622,7 @@ __device__ __forceinline__ void store_state(Args& a, const Rows& w, uint32_t to,
     }
 }
 
-constexpr int kKeyTiles = kAhead, kValueTiles = kAhead + 1;
+constexpr unsigned kKeyTiles = kAhead, kValueTiles = kAhead + 1;
 typedef unsigned char Lds[kKeyTiles + kValueTiles][kTileBytes];
 
 __device__ __forceinline__ void lds_barrier() {  // of LDS alone: stores to memory are not waited for
@@ -667,32 +687,32 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
             return window_of(MERGED || it < s.shared ? x.shared : x.own, side.table, slot_of(it) >> side.shift, lane);
         };
         Window window = window_at(begin);
-        int k_at = 0, v_at = kKeyTiles;
-        asm("" : "+s"(k_at), "+s"(v_at));  // or every wave's place in each would be held in a register
-        // This wave's eight rows of K and V; which of the tile's four groups of 16 slots, each within a page, count.
+        unsigned v_at = kKeyTiles;
+        asm("" : "+s"(v_at));  // or every wave's place in each would be held in a register
+        auto keys_of = [&](int it) { return lds[(it - begin) % kKeyTiles]; };
+        // Waves 0 to 3 bring tiles begin, begin + 2, .., waves 4 to 7 the others, 16 rows of K and V a wave: half of the addresses,
+        // and the two waves of a SIMD come out of step, one's products beside the other's exponentials.  Returned for every wave:
+        // which of the tile's four groups of 16 slots count.
         auto stage = [&](int it) {
-            const int j0 = slot_of(it), page0 = j0 >> side.shift;
+            const int j0 = slot_of(it);
             if (!MERGED && it == s.shared && it > begin) {
                 side = side_at(it);
                 window = window_at(it);
-            } else if (page0 - window.first > 63) {
+            } else if ((j0 >> side.shift) - window.first > 63) {
                 window = window_at(it);
             }
-            auto page_at = [&](int j) { return __builtin_amdgcn_readlane(window.ids, (j >> side.shift) - window.first); };
-            int valid = 0;
+            if (((it - begin) & 1) == wave >> 2) {
+                const int j1 = j0 + 16 * (wave & 3), j = j1 & ((1 << side.shift) - 1);
+                const int id = max(__builtin_amdgcn_readlane(window.ids, (j1 >> side.shift) - window.first), 0);
+                const uint16_t* k = side.k + (int64_t)id * side.k_page + (int64_t)j * side.k_slot;
+                const uint16_t* v = side.v + (int64_t)id * side.v_page + (int64_t)j * side.v_slot;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) valid |= (page_at(j0 + 16 * g) >= 0 && j0 + 16 * g < side.n) << g;
-            const int j1 = j0 + 16 * (wave >> 1), i0 = 2 * (wave & 1), j = j1 & ((1 << side.shift) - 1), id = max(page_at(j1), 0);
-            const uint16_t* k = side.k + (int64_t)id * side.k_page + (int64_t)j * side.k_slot;
-            const uint16_t* v = side.v + (int64_t)id * side.v_page + (int64_t)j * side.v_slot;
+                for (int i = 0; i < 4; ++i) stage_four<0>(k, side.k_slot, i, keys_of(it) + (16 * (wave & 3) + 4 * i) * 256, lane);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                stage_four<0>(k, side.k_slot, i0 + i, lds[k_at] + (8 * wave + 4 * i) * 256, lane);
-                stage_four<1>(v, side.v_slot, i0 + i, lds[v_at] + (8 * wave + 4 * i) * 256, lane);
+                for (int i = 0; i < 4; ++i) stage_four<1>(v, side.v_slot, i, lds[v_at] + (16 * (wave & 3) + 4 * i) * 256, lane);
             }
-            k_at = k_at == kKeyTiles - 1 ? 0 : k_at + 1;
             v_at = v_at == kKeyTiles + kValueTiles - 1 ? kKeyTiles : v_at + 1;
-            return valid;
+            return groups_of(window, j0, side.shift, side.n);
         };
         // This wave's eight value rows of a staged tile.  Rows that no row of the workgroup sees may hold anything: zero.  Where some
         // see a row that others do not, 0 times an infinite or NaN value would be NaN: those become zero before any product.
@@ -712,13 +732,13 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
             for (int i = 0; i < 2; ++i) at_lds[64 * i] = x[i];
             lds_barrier();
         };
-        // Tile `it`'s loads have landed for every wave, but for those of `behind` tiles after it.  Behind the barrier no wave reads
-        // the keys of the tile before it, nor the values of the one before that.
-        auto arrive = [&](int behind) {
-            if (behind >= 3) wait_all_but<12>();
-            else if (behind == 2) wait_all_but<8>();
-            else if (behind == 1) wait_all_but<4>();
-            else wait_all_but<0>();
+        // Tile `it`, behind which `behind` more are on their way (at most three), is there for every wave.  Behind the barrier no wave
+        // reads the keys of the tile before it, nor the values of the one before that.
+        auto arrive = [&](int it, int behind) {
+            if (((it - begin) & 1) == wave >> 2) {  // this wave's: but for the tile after next
+                if (behind >= 2) wait_all_but<8>();
+                else wait_all_but<0>();
+            }
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         };
@@ -731,17 +751,16 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
                 valid |= stage(staged) << i;
                 ++staged;
             }
-            arrive(staged - begin - 1);
-            int k_now = 0, v_now = kKeyTiles;
+            arrive(begin, staged - begin - 1);
+            unsigned v_now = kKeyTiles;
             clean(begin, v_now, valid & 15);
             // From tile `it` to the next one: v_last is left for the values that are still to be read.
-            int v_last = 0;
+            unsigned v_last = 0;
             auto next = [&](int it) __attribute__((always_inline)) {
-                k_now = k_now == kKeyTiles - 1 ? 0 : k_now + 1;
                 v_last = v_now;
                 v_now = v_now == kKeyTiles + kValueTiles - 1 ? kKeyTiles : v_now + 1;
                 if (it + 1 < last) {
-                    arrive(staged - it - 2);
+                    arrive(it + 1, staged - it - 2);
                     if (staged < last) {
                         valid |= stage(staged) << 4 * kAhead;
                         ++staged;
@@ -760,7 +779,7 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
                     top_of(w, now, slot_of(it) + 32 * part, last_seen(it), valid >> 2 * part & 3, lane, c2);
                     probabilities<RF>(w, now, pk, c2);
                     next(it);
-                    now = products<RF>(w, lds[k_now], part, lane);
+                    now = products<RF>(w, keys_of(it + 1), part, lane);
                     values<RF>(w, lds[v_last], part, pk, lane);
                 }
             } else {
@@ -768,12 +787,12 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
                 for (int it = begin; it < last; ++it) {
                     r2o_u4 pk[2];
                     top_of(w, even, slot_of(it), last_seen(it), valid & 3, lane, c2);
-                    f16v odd = products<RF>(w, lds[k_now], 1, lane);
+                    f16v odd = products<RF>(w, keys_of(it), 1, lane);
                     probabilities<RF>(w, even, pk, c2);
                     values<RF>(w, lds[v_now], 0, pk, lane);
                     top_of(w, odd, slot_of(it) + 32, last_seen(it), valid >> 2 & 3, lane, c2);
                     next(it);
-                    even = products<RF>(w, lds[k_now], 0, lane);
+                    even = products<RF>(w, keys_of(it + 1), 0, lane);
                     probabilities<RF>(w, odd, pk, c2);
                     values<RF>(w, lds[v_last], 1, pk, lane);
                 }
