@@ -870,14 +870,14 @@ PyObject* paged_rope_extend_call(PyObject* const* args) {
     return status_and(launch_on(args[0], p, device), {q_out});
 }
 
-// Key tiles of a call of the prefix attention, at most: whatever the lengths on the device say.
+// Units of the longest list of a call of the prefix attention, at most: whatever the lengths on the device say.
 bool merged_rows(int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes) { return prefixes && hq / hkv * rows < 128; }
 
 int64_t prefix_tiles(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t capacity, int64_t prefixes, int64_t prefix_capacity) {
     const int64_t packed = hq / hkv * rows, own = div_up(capacity, 64), shared = prefixes ? div_up(prefix_capacity, 64) : 0;
     return merged_rows(hkv, hq, rows, prefixes)
-               ? std::max(hkv * (batch * packed / 256 + prefixes) * shared, hkv * batch * div_up(packed, 32) * 2 * own)
-               : hkv * batch * div_up(packed, 256) * std::max<int64_t>(1, shared + own);
+               ? std::max(hkv * (batch * packed / 256 + prefixes) * (shared + 4), hkv * batch * div_up(packed, 32) * (2 * own + 1))
+               : hkv * batch * div_up(packed, 256) * (1 + shared + own + 4);
 }
 
 // Workgroups that share them: one a compute unit, whose LDS it fills.

@@ -23,6 +23,9 @@ constexpr int kWaves = 8;    // of a workgroup, which fills a compute unit
 constexpr int kRows = 256;   // rows of a workgroup: a wave's 32 each; 128 or fewer: 32 for two waves, which share their keys
 constexpr int kMerged = 128; // packed rows of a request below which all requests of a prefix are one list
 constexpr int kWaveRows = 32, kWaveKeys = 32;  // of a wave that works by itself
+// What a segment's start and end cost beside its tiles, in tiles: of a workgroup about nine microseconds beside 2.3 a tile of 256
+// rows, of one wave among eight five beside four.
+constexpr int kSegment = 4, kWaveSegment = 1;
 constexpr int kAhead = 4;    // tiles in LDS or on their way there, the one in use among them
 
 // One cache's rows, in the kernels' widths (the host has checked that they fit).
@@ -119,17 +122,20 @@ __device__ __forceinline__ int counted_rows(int rows) {
     return min(max(rows, 0), a.rows);
 }
 
-// Tiles of this lane's prefix (merged rows): heads x row tiles x key tiles.
+// A list's unit is a tile, or what a segment costs before its first one: kSegment or kWaveSegment units.
+__device__ __forceinline__ int units(int segments, int tiles, int more) { return tiles ? segments * (tiles + more) : 0; }
+
+// Of this lane's prefix (merged rows): heads x row tiles segments of its key tiles.
 __device__ __forceinline__ int prefix_work(const Lane& x, const Members& m) {
     Args& a = kernel_args();
-    return m.count ? a.hkv * div_up(m.count * a.packed, kRows) * div_up(filled(a.shared, x.shared), kTile) : 0;
+    return m.count ? units(a.hkv * div_up(m.count * a.packed, kRows), div_up(filled(a.shared, x.shared), kTile), kSegment) : 0;
 }
 
-// Tiles of this lane's request's own slots (merged rows), of 32 rows and 32 keys.
+// Of this lane's request's own slots (merged rows), in tiles of 32 rows and 32 keys.
 __device__ __forceinline__ int own_work(const Lane& x, int b0) {
     Args& a = kernel_args();
     const int b = b0 + (threadIdx.x & 63);
-    return b < a.batch ? a.hkv * div_up(a.packed, kWaveRows) * div_up(filled(a.own, x.own), kWaveKeys) : 0;
+    return b < a.batch ? units(a.hkv * div_up(a.packed, kWaveRows), div_up(filled(a.own, x.own), kWaveKeys), kWaveSegment) : 0;
 }
 
 // The prefix of this lane's request, -1 for none, and its length: one step a prefix.
@@ -137,10 +143,12 @@ __device__ __forceinline__ int prefix_of(const Lane& first, int b, int& length) 
     Args& a = kernel_args();
     int of = -1, before = 0;
     length = 0;
+#pragma unroll 1
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
         const Lane x = lane_at(first, g0);
         const Members m = lane_members(x, before);
         const int here = min(64, a.prefixes - g0);
+#pragma unroll 1
         for (int i = 0; i < here; ++i) {
             const bool mine = (uint32_t)(b - __builtin_amdgcn_readlane(m.first, i)) < (uint32_t)__builtin_amdgcn_readlane(m.count, i);
             of = mine ? g0 + i : of;
@@ -150,7 +158,7 @@ __device__ __forceinline__ int prefix_of(const Lane& first, int b, int& length) 
     return of;
 }
 
-// Tiles of this lane's request with its prefix (rows that are not merged).  A row tile without a key has one tile, of none: its
+// Of this lane's request with its prefix (rows that are not merged).  A row tile without a key has one tile, of none: its
 // rows are written there.
 __device__ __forceinline__ int request_work(const Lane& first, const Lane& x, int b0) {
     Args& a = kernel_args();
@@ -158,14 +166,14 @@ __device__ __forceinline__ int request_work(const Lane& first, const Lane& x, in
     int length;
     prefix_of(first, b, length);
     const int tiles = div_up(filled(a.own, x.own), kTile) + div_up(filled(a.shared, length), kTile);
-    return b < a.batch ? a.hkv * div_up(counted_rows(x.rows) * a.group, kRows) * max(tiles, 1) : 0;
+    return b < a.batch ? units(a.hkv * div_up(counted_rows(x.rows) * a.group, kRows), max(tiles, 1), kSegment) : 0;
 }
 
-// A list shared evenly: worker i takes `each` tiles from begin(i) on, the first `more` workers one more.
+// A list shared evenly: worker i takes `each` units from begin(i) on, the first `more` workers one more.
 struct Share {
     int total, workers, each, more;
     __device__ __forceinline__ int begin(int i) const { return i * each + min(i, more); }
-    __device__ __forceinline__ int worker(int at) const {  // the one that takes tile `at`
+    __device__ __forceinline__ int worker(int at) const {  // the one that takes unit `at`
         const int u = min(at, total - 1), wide = more * (each + 1);
         return u < wide ? (int)((uint32_t)u / (uint32_t)(each + 1)) : more + (int)((uint32_t)(u - wide) / (uint32_t)each);
     }
@@ -187,28 +195,14 @@ struct Plan {
     int own_first;
 };
 
-__device__ __forceinline__ Plan plan_of(Args& a, int shared, int own, float shared_cost, float own_cost) {
-    Plan p;
-    int n = __builtin_amdgcn_readfirstlane((int)(a.workers * (shared_cost / (shared_cost + own_cost)) + 0.5f));
-    n = max(min(n, a.workers - (own > 0)), (int)(shared > 0));
-    p.own_first = min(n, a.workers - 1);  // of one workgroup, which does both
-    p.shared = share_of(shared, n);
-    p.own = share_of(own, kWaves * (a.workers - p.own_first));
-    return p;
-}
-
-// What this lane's prefix and request cost, in the time that a compute unit takes for 16 KB at its part of the memory's rate: a
-// row tile of 256 rows is bound by its products, one of up to 128 by its loads, and a segment's start and end cost a
-// workgroup about seven, a wave among eight about one.
+// What this lane's prefix costs, in microseconds of a compute unit: a tile of 256 rows is bound by its products, one of up to
+// 128 by its loads; a request's unit takes 0.6.
+constexpr float kOwnCost = 0.6f;
 __device__ __forceinline__ float prefix_cost(const Lane& x, const Members& m) {
     Args& a = kernel_args();
-    const int rows = m.count * a.packed, keys = div_up(filled(a.shared, x.shared), kTile);
-    const int halves = 2 * (rows / kRows) + div_up(rows % kRows, kRows / 2);
-    return keys ? (float)a.hkv * (2.f * keys * halves + 7.f * div_up(rows, kRows)) : 0.f;
-}
-__device__ __forceinline__ float own_cost(int work) {
-    Args& a = kernel_args();
-    return work ? (float)work + (float)(a.hkv * div_up(a.packed, kWaveRows)) : 0.f;
+    const int rows = m.count * a.packed, keys = div_up(filled(a.shared, x.shared), kTile), left = rows % kRows;
+    const float tile = 2.3f * (rows / kRows) + (left > kRows / 2 ? 2.3f : (left ? 1.5f : 0.f));
+    return keys ? a.hkv * (keys * tile + 9.f * div_up(rows, kRows)) : 0.f;
 }
 
 __device__ __forceinline__ float wave_total(float x) {
@@ -230,7 +224,7 @@ struct Entry {
 // The tiles of the lists, and where request b's parts lie in them (b -1: none).
 struct Sums {
     int shared, own;
-    float shared_cost, own_cost;
+    float shared_cost;
     Entry of_prefix, of_request;
 };
 
@@ -239,6 +233,7 @@ __device__ __forceinline__ Sums sums_of(const Lane& first, int b) {
     Sums s{};
     s.of_prefix.prefix = -1;
     int before = 0;
+#pragma unroll 1
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
         const Lane x = lane_at(first, g0);
         const Members m = lane_members(x, before);
@@ -255,6 +250,7 @@ __device__ __forceinline__ Sums sums_of(const Lane& first, int b) {
         s.shared_cost += wave_total(prefix_cost(x, m));
         s.shared += last_lane(upto);
     }
+#pragma unroll 1
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Lane x = lane_at(first, b0);
         const int work = own_work(x, b0), upto = wave_scan(work);
@@ -263,10 +259,20 @@ __device__ __forceinline__ Sums sums_of(const Lane& first, int b) {
             s.of_request.n_own = filled(a.own, __builtin_amdgcn_readlane(x.own, b - b0));
             s.of_request.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, b - b0));
         }
-        s.own_cost += wave_total(own_cost(work));
         s.own += last_lane(upto);
     }
     return s;
+}
+
+__device__ __forceinline__ Plan plan_of(const Sums& s) {
+    Args& a = kernel_args();
+    Plan p;
+    int n = __builtin_amdgcn_readfirstlane((int)(a.workers * (s.shared_cost / (s.shared_cost + kOwnCost * s.own)) + 0.5f));
+    n = max(min(n, a.workers - (s.own > 0)), (int)(s.shared > 0));
+    p.own_first = min(n, a.workers - 1);  // of one workgroup, which does both
+    p.shared = share_of(s.shared, n);
+    p.own = share_of(s.own, kWaves * (a.workers - p.own_first));
+    return p;
 }
 
 // Merged rows: the prefix that holds tile u of the prefixes' list.
@@ -275,6 +281,7 @@ __device__ __forceinline__ Entry find_prefix(const Lane& first, int u) {
     Entry e{};
     e.request = -2;
     int at = 0, before = 0;
+#pragma unroll 1
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
         const Lane x = lane_at(first, g0);
         const Members m = lane_members(x, before);
@@ -301,6 +308,7 @@ __device__ __forceinline__ Entry find_own(const Lane& first, int u) {
     e.request = -2;
     e.prefix = -1;
     int at = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Lane x = lane_at(first, b0);
         const int work = own_work(x, b0), upto = wave_scan(work), all = last_lane(upto);
@@ -323,6 +331,7 @@ __device__ __forceinline__ Entry find_request(const Lane& first, int u, int& tot
     e.request = -2;
     e.prefix = -1;
     int at = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Lane x = lane_at(first, b0);
         const int work = request_work(first, x, b0), upto = wave_scan(work), all = last_lane(upto);
@@ -346,23 +355,23 @@ __device__ __forceinline__ Entry find_request(const Lane& first, int u, int& tot
 // One row tile of an entry and head, and its key tiles: of a workgroup, `shared` ones of the prefix, then its own; of a
 // wave, own ones.
 struct Segment {
-    int base, tiles;         // in the list
+    int base, tiles;         // the first tile's unit, their number
     int head, row0, shared;  // row0: in the entry's rows
 };
 
-__device__ __forceinline__ Segment segment_at(const Entry& e, int u, int tiles, int row_tiles, int rows) {
+__device__ __forceinline__ Segment segment_at(const Entry& e, int u, int tiles, int more, int row_tiles, int rows) {
     Segment s{};
     s.tiles = max(1, tiles);
-    const int per_head = max(1, row_tiles), at = (int)((uint32_t)(u - e.base) / (uint32_t)s.tiles);
+    const int per_head = max(1, row_tiles), at = (int)((uint32_t)(u - e.base) / (uint32_t)(s.tiles + more));
     s.head = (int)((uint32_t)at / (uint32_t)per_head);
     s.row0 = (at - s.head * per_head) * rows;
-    s.base = e.base + at * s.tiles;
+    s.base = e.base + at * (s.tiles + more) + more;
     return s;
 }
 
 __device__ __forceinline__ Segment segment_of(const Entry& e, int u) {
     const int shared = div_up(e.n_shared, kTile);
-    Segment s = segment_at(e, u, shared + div_up(e.n_own, kTile), div_up(e.rows, kRows), kRows);
+    Segment s = segment_at(e, u, shared + div_up(e.n_own, kTile), kSegment, div_up(e.rows, kRows), kRows);
     s.shared = shared;
     return s;
 }
@@ -644,8 +653,8 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
         const Entry e = MERGED ? find_prefix(first, u) : find_request(first, u, total);
         if (e.request == -2) return;  // lengths that change meanwhile
         const Segment s = segment_of(e, u);
-        const int begin = u - s.base, stop = min(s.tiles, u_end - s.base);
-        if (begin < 0 || stop <= begin || s.head >= a.hkv) return;
+        const int begin = max(0, u - s.base), stop = min(s.tiles, u_end - s.base);
+        if (stop <= begin || s.head >= a.hkv) return;  // nothing but a start that is the next one's, or lengths that change meanwhile
 
         // this lane's row, and the last key of its own that it sees
         int two = __builtin_amdgcn_readfirstlane(e.rows - s.row0 <= kRows / 2);  // waves share the keys of 32 rows, a half of each tile each
@@ -825,7 +834,7 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const La
             for (int i = 0; i < 16; ++i) {
                 const r2o_f4 o = from_lds[64 * i];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w.acc[i >> 2][4 * (i & 3) + k] = weighed(w.acc[i >> 2][4 * (i & 3) + k], f) + weighed(o[k], f2);
+                for (int k = 0; k < 4; ++k) w.acc[i >> 2][4 * (i & 3) + k] = w.acc[i >> 2][4 * (i & 3) + k] * f + o[k] * f2;
             }
             w.l = w.l * f + l2 * f2;
             w.m = mn;
@@ -880,9 +889,9 @@ __device__ __forceinline__ void work_on_own(Lds& lds, const Lane& first, int own
         asm("" : "+v"(lane), "+s"(wave));
         const Entry e = find_own(first, u);
         if (e.request == -2) return;  // lengths that change meanwhile
-        const Segment s = segment_at(e, u, div_up(e.n_own, kWaveKeys), div_up(a.packed, kWaveRows), kWaveRows);
-        const int begin = u - s.base, stop = min(s.tiles, u_end - s.base);
-        if (begin < 0 || stop <= begin || s.head >= a.hkv) return;
+        const Segment s = segment_at(e, u, div_up(e.n_own, kWaveKeys), kWaveSegment, div_up(a.packed, kWaveRows), kWaveRows);
+        const int begin = max(0, u - s.base), stop = min(s.tiles, u_end - s.base);
+        if (stop <= begin || s.head >= a.hkv) return;
         const int p = min(s.row0 + (lane & 31), a.packed - 1), row = p / a.group, head = s.head * a.group + p - row * a.group;
         uint32_t to = kNoRow;
         if (s.row0 + (lane & 31) < a.packed)
@@ -994,7 +1003,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
         int own_first, index, v = 0, v_end = 0;
         {
             const Sums sums = sums_of(first, -1);
-            const Plan plan = plan_of(a, sums.shared, sums.own, sums.shared_cost, sums.own_cost);
+            const Plan plan = plan_of(sums);
             if (sums.shared > 0 && (int)blockIdx.x < plan.shared.workers) {
                 u = plan.shared.begin(blockIdx.x);
                 u_end = plan.shared.begin(blockIdx.x + 1);
@@ -1080,7 +1089,7 @@ __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
     const Entry e = find_request(first, u, total);
     if (e.request < 0) return;
     const Segment s = segment_of(e, u);
-    if (s.base == u || s.base < share.begin(w - 1) || s.head >= a.hkv) return;  // begun here, or by another than the one before
+    if (s.base >= u || s.base < share.begin(w - 1) || s.head >= a.hkv) return;  // begun here, or by another than the one before
     const int count = share.worker(s.base + s.tiles - 1) - (w - 1) + 1, here = min(kRows, e.rows - s.row0);
 #pragma unroll 1
     for (int r = r0; r < min(here, (int)(blockIdx.y + 1) * kJoinRows); r += 8) {
@@ -1105,29 +1114,38 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
     const int b = (int)blockIdx.x / per_request, in_request = (int)blockIdx.x - b * per_request, h = in_request / a.packed, p = in_request - h * a.packed;
     const int row = p / a.group, head = h * a.group + p - row * a.group, d4 = threadIdx.x & 31, part = threadIdx.x >> 5;
     const Sums sums = sums_of(first_lane, b);
-    const Plan plan = plan_of(a, sums.shared, sums.own, sums.shared_cost, sums.own_cost);
+    const Plan plan = plan_of(sums);
     State s{-INFINITY, 0.f, r2o_f4{}};
     if (row < sums.of_request.rows) {
+        // the states of one segment, of `tiles` tiles from unit `base` on: shared by the groups, four loads of each under way
+        auto add = [&](const Share& share, int base, int tiles, uint32_t whole, auto split) {
+            const int w0 = share.worker(base), count = share.worker(base + tiles - 1) - w0 + 1;
+            for (int i0 = part; i0 < count; i0 += 32) {
+                float m2[4], l2[4];
+                r2o_f4 o2[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i = min(i0 + 8 * k, count - 1);
+                    const int64_t at = count == 1 ? whole : split(w0 + i, i == 0);
+                    m2[k] = r2o_ldg(a.partial_ml + 2 * at);
+                    l2[k] = r2o_ldg(a.partial_ml + 2 * at + 1);
+                    o2[k] = r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i0 + 8 * k < count) join_state(s, m2[k], l2[k], o2[k]);
+            }
+        };
         const Entry& e = sums.of_prefix;
         if (e.prefix >= 0 && e.n_shared > 0) {
             const int r = (b - e.first) * a.packed + p, tile = r / kRows, tiles = div_up(e.n_shared, kTile);
-            const int base = e.base + (h * div_up(e.members * a.packed, kRows) + tile) * tiles;
-            const int w0 = plan.shared.worker(base), count = plan.shared.worker(base + tiles - 1) - w0 + 1;
-            if (count == 1) {
-                if (part == 0) join_partial(a, s, whole_prefix_rows(a, e.first, e.members, h) + r, d4);
-            } else {
-                for (int i = part; i < count; i += 8) join_partial(a, s, split_rows(w0 + i, i == 0) + r - tile * kRows, d4);
-            }
+            add(plan.shared, e.base + (h * div_up(e.members * a.packed, kRows) + tile) * (tiles + kSegment) + kSegment, tiles,
+                whole_prefix_rows(a, e.first, e.members, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
         }
         if (sums.of_request.n_own > 0) {
             const int chunk = p / kWaveRows, tiles = div_up(sums.of_request.n_own, kWaveKeys);
-            const int base = sums.of_request.base + (h * div_up(a.packed, kWaveRows) + chunk) * tiles;
-            const int w0 = plan.own.worker(base), count = plan.own.worker(base + tiles - 1) - w0 + 1;
-            if (count == 1) {
-                if (part == 7) join_partial(a, s, whole_own_rows(a, b, h) + p, d4);
-            } else {
-                for (int i = 7 - part; i < count; i += 8) join_partial(a, s, split_wave_rows(plan.own_first, w0 + i, i == 0) + p - chunk * kWaveRows, d4);
-            }
+            add(plan.own, sums.of_request.base + (h * div_up(a.packed, kWaveRows) + chunk) * (tiles + kWaveSegment) + kWaveSegment, tiles,
+                whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(plan.own_first, w, begins) + p - chunk * kWaveRows; });
         }
     }
     *reinterpret_cast<r2o_f4*>(&red[part][4 * d4]) = s.o;
@@ -1185,9 +1203,9 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     if (p->scratch_floats < 130 * (2 * kRows * p->workers + (merged ? 2 * all_rows : 0))) return R2O_EINVAL;
     // whatever the lengths on the device say
     const int64_t shared = any ? tiles_of(f) : 0, per_request = (packed + kRows - 1) / kRows;
-    const int64_t most = merged ? std::max(c.hkv * (c.batch * packed / kRows + f.batch) * shared,
-                                           c.hkv * c.batch * ((packed + kWaveRows - 1) / kWaveRows) * (kTile / kWaveKeys) * tiles_of(c))
-                                : c.hkv * c.batch * per_request * std::max<int64_t>(1, shared + tiles_of(c));
+    const int64_t most = merged ? std::max(c.hkv * (c.batch * packed / kRows + f.batch) * (shared + kSegment),
+                                           c.hkv * c.batch * ((packed + kWaveRows - 1) / kWaveRows) * (kTile / kWaveKeys * tiles_of(c) + kWaveSegment))
+                                : c.hkv * c.batch * per_request * (1 + shared + tiles_of(c) + kSegment);
     if (most > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS) return R2O_EINVAL;
     PrefixArgs a{};
     a.own = source_of(c);
