@@ -884,7 +884,7 @@ int64_t prefix_tiles(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64
 int64_t prefix_workers(int64_t tiles, int64_t cus) { return std::max<int64_t>(1, std::min(cus, tiles)); }
 
 int64_t prefix_scratch(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes, int64_t workers) {
-    return 130 * (512 * workers + (merged_rows(hkv, hq, rows, prefixes) ? 2 * batch * hq * rows : 0));
+    return 130 * (512 * workers + (merged_rows(hkv, hq, rows, prefixes) ? 2 * batch * hq * rows : 0)) + 8 * (1 + std::max(batch, workers));
 }
 
 // paged_prefix_attention(function, query, cache, prefix or None, members, query_lengths, scale): (status, out, lse) or None

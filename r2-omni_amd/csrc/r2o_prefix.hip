@@ -41,6 +41,7 @@ struct PrefixArgs {
     const uint16_t* query;
     uint16_t* out;
     float *lse, *partial_out, *partial_ml;
+    int* notes;  // for the join
     int64_t q_batch, q_head, o_batch, o_head;
     int q_row, o_row, batch, prefixes, hkv, hq, group, rows, packed, workers, merged;  // packed: rows * group
     float c2;  // scale, in log2 units
@@ -138,10 +139,11 @@ __device__ __forceinline__ int own_work(const Lane& x, int b0) {
     return b < a.batch ? units(a.hkv * div_up(a.packed, kWaveRows), div_up(filled(a.own, x.own), kWaveKeys), kWaveSegment) : 0;
 }
 
-// The prefix of this lane's request, -1 for none, and its length: one step a prefix.
-__device__ __forceinline__ int prefix_of(const Lane& first, int b, int& length) {
+// The prefix of this lane's request, -1 for none, its requests and its length: one step a prefix.
+__device__ __forceinline__ int prefix_of(const Lane& first, int b, Members& members, int& length) {
     Args& a = kernel_args();
     int of = -1, before = 0;
+    members = {0, 0};
     length = 0;
 #pragma unroll 1
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
@@ -150,9 +152,12 @@ __device__ __forceinline__ int prefix_of(const Lane& first, int b, int& length) 
         const int here = min(64, a.prefixes - g0);
 #pragma unroll 1
         for (int i = 0; i < here; ++i) {
-            const bool mine = (uint32_t)(b - __builtin_amdgcn_readlane(m.first, i)) < (uint32_t)__builtin_amdgcn_readlane(m.count, i);
+            const int from = __builtin_amdgcn_readlane(m.first, i), count = __builtin_amdgcn_readlane(m.count, i), n = __builtin_amdgcn_readlane(x.shared, i);
+            const bool mine = (uint32_t)(b - from) < (uint32_t)count;
             of = mine ? g0 + i : of;
-            length = mine ? __builtin_amdgcn_readlane(x.shared, i) : length;
+            members.first = mine ? from : members.first;
+            members.count = mine ? count : members.count;
+            length = mine ? n : length;
         }
     }
     return of;
@@ -164,7 +169,8 @@ __device__ __forceinline__ int request_work(const Lane& first, const Lane& x, in
     Args& a = kernel_args();
     const int b = b0 + (threadIdx.x & 63);
     int length;
-    prefix_of(first, b, length);
+    Members members;
+    prefix_of(first, b, members, length);
     const int tiles = div_up(filled(a.own, x.own), kTile) + div_up(filled(a.shared, length), kTile);
     return b < a.batch ? units(a.hkv * div_up(counted_rows(x.rows) * a.group, kRows), max(tiles, 1), kSegment) : 0;
 }
@@ -221,46 +227,25 @@ struct Entry {
     int n_shared, n_own, rows;
 };
 
-// The tiles of the lists, and where request b's parts lie in them (b -1: none).
+// The units of the lists of merged rows.
 struct Sums {
     int shared, own;
     float shared_cost;
-    Entry of_prefix, of_request;
 };
 
-__device__ __forceinline__ Sums sums_of(const Lane& first, int b) {
+__device__ __forceinline__ Sums sums_of(const Lane& first) {
     Args& a = kernel_args();
     Sums s{};
-    s.of_prefix.prefix = -1;
     int before = 0;
 #pragma unroll 1
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
         const Lane x = lane_at(first, g0);
         const Members m = lane_members(x, before);
-        const int work = prefix_work(x, m), upto = wave_scan(work);
-        const uint64_t mine = b < 0 ? 0 : __ballot((uint32_t)(b - m.first) < (uint32_t)m.count);
-        if (mine) {
-            const int i = __builtin_ctzll(mine);
-            s.of_prefix.base = s.shared + __builtin_amdgcn_readlane(upto - work, i);
-            s.of_prefix.prefix = g0 + i;
-            s.of_prefix.first = __builtin_amdgcn_readlane(m.first, i);
-            s.of_prefix.members = __builtin_amdgcn_readlane(m.count, i);
-            s.of_prefix.n_shared = filled(a.shared, __builtin_amdgcn_readlane(x.shared, i));
-        }
+        s.shared += last_lane(wave_scan(prefix_work(x, m)));
         s.shared_cost += wave_total(prefix_cost(x, m));
-        s.shared += last_lane(upto);
     }
 #pragma unroll 1
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const Lane x = lane_at(first, b0);
-        const int work = own_work(x, b0), upto = wave_scan(work);
-        if ((uint32_t)(b - b0) < 64u) {
-            s.of_request.base = s.own + __builtin_amdgcn_readlane(upto - work, b - b0);
-            s.of_request.n_own = filled(a.own, __builtin_amdgcn_readlane(x.own, b - b0));
-            s.of_request.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, b - b0));
-        }
-        s.own += last_lane(upto);
-    }
+    for (int b0 = 0; b0 < a.batch; b0 += 64) s.own += last_lane(wave_scan(own_work(lane_at(first, b0), b0)));
     return s;
 }
 
@@ -273,6 +258,53 @@ __device__ __forceinline__ Plan plan_of(const Sums& s) {
     p.shared = share_of(s.shared, n);
     p.own = share_of(s.own, kWaves * (a.workers - p.own_first));
     return p;
+}
+
+// What the join has to know, left by one wave: it would take longer to find it out again than to read it.  The shares, then of
+// each request the units of its prefix's and its own first tiles and their tiles, its prefix's requests, and its rows that count.
+constexpr int kNote = 8;
+__device__ __forceinline__ void write_notes(const Lane& first, const Plan& plan) {
+    Args& a = kernel_args();
+    const int lane = threadIdx.x & 63;
+    if (lane == 0) {
+        int* to = a.notes;
+        to[0] = plan.shared.total;
+        to[1] = plan.shared.each;
+        to[2] = plan.shared.more;
+        to[3] = plan.own_first;
+        to[4] = plan.own.total;
+        to[5] = plan.own.each;
+        to[6] = plan.own.more;
+    }
+    int own = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const Lane x = lane_at(first, b0);
+        const int b = b0 + lane, work = own_work(x, b0), upto = wave_scan(work);
+        Members members;
+        int length, shared = 0, before = 0;
+        const int of = prefix_of(first, b, members, length);
+#pragma unroll 1
+        for (int g0 = 0; g0 < a.prefixes; g0 += 64) {  // the units before this request's prefix
+            const Lane y = lane_at(first, g0);
+            const Members m = lane_members(y, before);
+            const int units_to = wave_scan(prefix_work(y, m));
+            if (g0 + 64 <= of) shared += last_lane(units_to);
+            const int here = __shfl(units_to, (of - 1) & 63);
+            if (of > g0 && of < g0 + 64) shared += here;
+        }
+        if (b < a.batch) {
+            int* to = a.notes + kNote * (1 + b);
+            to[0] = shared;
+            to[1] = div_up(filled(a.shared, length), kTile);
+            to[2] = members.first;
+            to[3] = members.count;
+            to[4] = own + upto - work;
+            to[5] = div_up(filled(a.own, x.own), kWaveKeys);
+            to[6] = counted_rows(x.rows);
+        }
+        own += last_lane(upto);
+    }
 }
 
 // Merged rows: the prefix that holds tile u of the prefixes' list.
@@ -338,7 +370,8 @@ __device__ __forceinline__ Entry find_request(const Lane& first, int u, int& tot
         if ((uint32_t)(u - at) < (uint32_t)all) {
             const int i = __builtin_ctzll(__ballot(at + upto > u));
             int length;
-            const int of = prefix_of(first, b0 + (threadIdx.x & 63), length);
+            Members members;
+            const int of = prefix_of(first, b0 + (threadIdx.x & 63), members, length);
             e.base = at + __builtin_amdgcn_readlane(upto - work, i);
             e.request = b0 + i;
             e.prefix = __builtin_amdgcn_readlane(of, i);
@@ -1002,13 +1035,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
     if constexpr (MERGED) {
         int own_first, index, v = 0, v_end = 0;
         {
-            const Sums sums = sums_of(first, -1);
+            const Sums sums = sums_of(first);
             const Plan plan = plan_of(sums);
             if (sums.shared > 0 && (int)blockIdx.x < plan.shared.workers) {
                 u = plan.shared.begin(blockIdx.x);
                 u_end = plan.shared.begin(blockIdx.x + 1);
             }
             own_first = plan.own_first;
+            if (blockIdx.x == gridDim.x - 1 && threadIdx.x >= 64 * (kWaves - 1)) write_notes(first, plan);
             index = kWaves * ((int)blockIdx.x - own_first) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
             if (sums.own > 0 && index >= 0 && index < plan.own.workers) {
                 v = plan.own.begin(index);
@@ -1021,9 +1055,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
         int total;
         find_request(first, -1, total);
         const Share share = share_of(total, a.workers);
+        int request = -1, place[4] = {};
         if (total > 0 && (int)blockIdx.x < share.workers) {
             u = share.begin(blockIdx.x);
             u_end = share.begin(blockIdx.x + 1);
+            const Entry e = find_request(first, u, total);
+            const Segment s = segment_of(e, u);
+            // the segment that this workgroup is the second to work on is joined by the note's reader
+            if (e.request >= 0 && s.base < u && s.base >= share.begin((int)blockIdx.x - 1)) {
+                request = e.request;
+                place[0] = s.head;
+                place[1] = s.row0;
+                place[2] = e.rows;
+                place[3] = share.worker(s.base + s.tiles - 1) - (int)blockIdx.x + 2;
+            }
+        }
+        if (threadIdx.x == 0) {
+            int* to = a.notes + kNote * (int)blockIdx.x;
+            to[0] = request;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[1 + i] = place[i];
         }
         work_on_row_tiles<RF, false>(lds, flags, first, u, u_end);
     }
@@ -1062,7 +1113,7 @@ __device__ __forceinline__ void write_row(Args& a, const State& s, int b, int he
 
 // Rows that are not merged.  Workgroups (w, .) join the segment that worker w + 1 is the second to work on, 32 lanes a row;
 // those behind the workers' write the rows that their requests do not count.
-constexpr int kJoinRows = 64;
+constexpr int kJoinRows = 32;
 
 template <int RF>
 __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
@@ -1079,26 +1130,20 @@ __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
             }
         return;
     }
-    const Lane first = lane_of(0);
-    int total;
-    find_request(first, -1, total);
-    const Share share = share_of(total, a.workers);
     const int w = (int)blockIdx.x + 1;
-    if (total == 0 || w >= share.workers) return;
-    const int u = share.begin(w);
-    const Entry e = find_request(first, u, total);
-    if (e.request < 0) return;
-    const Segment s = segment_of(e, u);
-    if (s.base >= u || s.base < share.begin(w - 1) || s.head >= a.hkv) return;  // begun here, or by another than the one before
-    const int count = share.worker(s.base + s.tiles - 1) - (w - 1) + 1, here = min(kRows, e.rows - s.row0);
-#pragma unroll 1
-    for (int r = r0; r < min(here, (int)(blockIdx.y + 1) * kJoinRows); r += 8) {
+    const int* note = a.notes + kNote * w;
+    const int request = load_uniform(note), head = load_uniform(note + 1), row0 = load_uniform(note + 2), rows = load_uniform(note + 3), count = load_uniform(note + 4);
+    if (request < 0) return;
+#pragma unroll
+    for (int k = 0; k < kJoinRows; k += 8) {
+        const int r = r0 + k;
+        if (r >= min(kRows, rows - row0)) break;
         State x{-INFINITY, 0.f, r2o_f4{}};
         join_partial(a, x, split_rows(w - 1, true) + r, d4);
 #pragma unroll 4
         for (int i = 1; i < count; ++i) join_partial(a, x, split_rows(w - 1 + i, false) + r, d4);
-        const int p = s.row0 + r, row = p / a.group;
-        write_row<RF>(a, x, e.request, s.head * a.group + p - row * a.group, row, d4);
+        const int p = row0 + r, row = p / a.group;
+        write_row<RF>(a, x, request, head * a.group + p - row * a.group, row, d4);
     }
 }
 
@@ -1109,14 +1154,15 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
     __shared__ __align__(16) float red[8][128];
     __shared__ float red_ml[8][2];
     Args& a = kernel_args();
-    const Lane first_lane = lane_of(0);
     const int per_request = a.hkv * a.packed;
     const int b = (int)blockIdx.x / per_request, in_request = (int)blockIdx.x - b * per_request, h = in_request / a.packed, p = in_request - h * a.packed;
     const int row = p / a.group, head = h * a.group + p - row * a.group, d4 = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const Sums sums = sums_of(first_lane, b);
-    const Plan plan = plan_of(sums);
+    const int *all = a.notes, *note = a.notes + kNote * (1 + b);
+    const Share shared{load_uniform(all), 0, load_uniform(all + 1), load_uniform(all + 2)}, own{load_uniform(all + 4), 0, load_uniform(all + 5), load_uniform(all + 6)};
+    const int own_first = load_uniform(all + 3), shared_base = load_uniform(note), shared_tiles = load_uniform(note + 1), first = load_uniform(note + 2),
+              members = load_uniform(note + 3), own_base = load_uniform(note + 4), own_tiles = load_uniform(note + 5), counted = load_uniform(note + 6);
     State s{-INFINITY, 0.f, r2o_f4{}};
-    if (row < sums.of_request.rows) {
+    if (row < counted) {
         // the states of one segment, of `tiles` tiles from unit `base` on: shared by the groups, four loads of each under way
         auto add = [&](const Share& share, int base, int tiles, uint32_t whole, auto split) {
             const int w0 = share.worker(base), count = share.worker(base + tiles - 1) - w0 + 1;
@@ -1136,16 +1182,15 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
                     if (i0 + 8 * k < count) join_state(s, m2[k], l2[k], o2[k]);
             }
         };
-        const Entry& e = sums.of_prefix;
-        if (e.prefix >= 0 && e.n_shared > 0) {
-            const int r = (b - e.first) * a.packed + p, tile = r / kRows, tiles = div_up(e.n_shared, kTile);
-            add(plan.shared, e.base + (h * div_up(e.members * a.packed, kRows) + tile) * (tiles + kSegment) + kSegment, tiles,
-                whole_prefix_rows(a, e.first, e.members, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
+        if (shared_tiles > 0) {
+            const int r = (b - first) * a.packed + p, tile = r / kRows;
+            add(shared, shared_base + (h * div_up(members * a.packed, kRows) + tile) * (shared_tiles + kSegment) + kSegment, shared_tiles,
+                whole_prefix_rows(a, first, members, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
         }
-        if (sums.of_request.n_own > 0) {
-            const int chunk = p / kWaveRows, tiles = div_up(sums.of_request.n_own, kWaveKeys);
-            add(plan.own, sums.of_request.base + (h * div_up(a.packed, kWaveRows) + chunk) * (tiles + kWaveSegment) + kWaveSegment, tiles,
-                whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(plan.own_first, w, begins) + p - chunk * kWaveRows; });
+        if (own_tiles > 0) {
+            const int chunk = p / kWaveRows;
+            add(own, own_base + (h * div_up(a.packed, kWaveRows) + chunk) * (own_tiles + kWaveSegment) + kWaveSegment, own_tiles,
+                whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(own_first, w, begins) + p - chunk * kWaveRows; });
         }
     }
     *reinterpret_cast<r2o_f4*>(&red[part][4 * d4]) = s.o;
@@ -1200,7 +1245,8 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     const int64_t group = p->hq / c.hkv, packed = group * p->rows, all_rows = c.batch * c.hkv * packed;
     if (packed > (1 << 30) || all_rows > (1 << 30)) return R2O_EINVAL;
     const bool merged = any && packed < kMerged;
-    if (p->scratch_floats < 130 * (2 * kRows * p->workers + (merged ? 2 * all_rows : 0))) return R2O_EINVAL;
+    const int64_t states = 2 * kRows * p->workers + (merged ? 2 * all_rows : 0);
+    if (p->scratch_floats < 130 * states + kNote * (1 + std::max(c.batch, p->workers))) return R2O_EINVAL;
     // whatever the lengths on the device say
     const int64_t shared = any ? tiles_of(f) : 0, per_request = (packed + kRows - 1) / kRows;
     const int64_t most = merged ? std::max(c.hkv * (c.batch * packed / kRows + f.batch) * (shared + kSegment),
@@ -1216,7 +1262,8 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     a.out = p->out;
     a.lse = p->lse;
     a.partial_out = p->scratch;
-    a.partial_ml = p->scratch + 128 * (p->scratch_floats / 130);
+    a.partial_ml = p->scratch + 128 * states;
+    a.notes = reinterpret_cast<int*>(p->scratch + 130 * states);
     a.q_batch = p->q_strides[0];
     a.q_head = p->q_strides[1];
     a.q_row = (int)p->q_strides[2];

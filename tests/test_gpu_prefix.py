@@ -184,7 +184,7 @@ def test_any_number_of_workers(rows, workers):
     shared, own = _both(dev, (700, 130), (100, 64, 41, 300, 77), 2, 32, BF16, 14)
     q, members = _query(dev, 5, 14, rows, BF16, 14), _ints(dev, 2, 2)
     out, lse = torch.full_like(q, math.nan), torch.full((5, 14, rows), math.nan, device=dev)
-    floats = 130 * (512 * workers + (2 * 5 * 14 * rows if rows == 1 else 0))
+    floats = 130 * (512 * workers + (2 * 5 * 14 * rows if rows == 1 else 0)) + 8 * (1 + max(5, workers))
     scratch = torch.full((floats + 512,), 3.0, device=dev)
     p = _lib.PagedPrefix(cache=paged._params_of(own), prefix=paged._params_of(shared), members=members.data_ptr(), query=q.data_ptr(),
                          out=out.data_ptr(), lse=lse.data_ptr(), q_strides=q.stride()[:3], o_strides=out.stride()[:3], hq=14, rows=rows,
