@@ -7,7 +7,7 @@
 //
 // A row (128 channels of one (request, head, token)) is 16 lanes of 8 channels, one 16-byte load and store; a channel's
 // partner is lane ^ 8, read by DPP.  A wave takes 4 tokens and walks a run of heads: the 64 angles of a token are formed once
-// for all of them, and 4 heads' rows are in flight at a time.
+// for all of them, and four or eight heads' rows are in flight at a time.
 #include <algorithm>
 #include <initializer_list>
 
@@ -28,26 +28,6 @@ struct RotateArgs {
     int hq, hkv, heads, heads_per_wave, hadamard;
 };
 
-// cos and sin of 2 pi turns, |turns| at most 1/2.  The quarter turn that is nearest is taken off (exact), the rest, x in
-// [-pi/4, pi/4], goes through the Taylor polynomials of degree 9 and 8: off by at most x^11 / 11! = 1.8e-9 and x^10 / 10! =
-// 2.5e-8, below half a step of fp32 at the cosine's least value there.
-__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
-    const double quarters = 4.0 * turns, n = __builtin_rint(quarters);
-    const float x = (float)((quarters - n) * 1.5707963267948966), x2 = x * x;
-    float p = __builtin_fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);
-    p = __builtin_fmaf(x2, p, 8.3333333e-3f);
-    p = __builtin_fmaf(x2, p, -0.16666667f);
-    const float sx = __builtin_fmaf(x * x2, p, x);
-    float r = __builtin_fmaf(x2, 2.4801587e-5f, -1.3888889e-3f);
-    r = __builtin_fmaf(x2, r, 4.1666667e-2f);
-    r = __builtin_fmaf(x2, r, -0.5f);
-    const float cx = __builtin_fmaf(x2, r, 1.f);
-    const int q = (int)n & 3;
-    const float a = q & 1 ? sx : cx, b = q & 1 ? cx : sx;
-    c = q == 1 || q == 2 ? -a : a;
-    s = q & 2 ? -b : b;
-}
-
 // The position of a token on an axis.
 __device__ __forceinline__ int64_t position_at(const r2o_rotation& r, int axis, int64_t b, int64_t token) {
     const int64_t at = axis * r.position_strides[0] + b * r.position_strides[1] + token * r.position_strides[2];
@@ -55,8 +35,10 @@ __device__ __forceinline__ int64_t position_at(const r2o_rotation& r, int axis, 
                                  : (int64_t)r2o_ldg(reinterpret_cast<const int32_t*>(r.positions) + at);
 }
 
-// cos and sin of the lane's channels 8 c8 .. 8 c8 + 7, the sine with its channel's sign.  A turn is position * (inv_freq / 2
-// pi) without its whole part, in 64 bits: a position of 2^31 leaves it 2^-24 exact.
+// cos and sin of the lane's channels 8 c8 .. 8 c8 + 7, the sine with its channel's sign.  The angle in half turns, position *
+// (inv_freq / pi), loses its whole part in 64 bits (a position of 2^31 leaves it 2^-24 exact), the rest, at most 1/2, goes to
+// the hardware's sine and cosine, which take turns and are off by at most 1.2e-7 (2^-23; looked at for 2^24 arguments).  Polynomials
+// instead took 15.3 us where this takes 14.1 (4 padded requests of 1037 rows, 16 + 2 heads).
 __device__ __forceinline__ void angles(const r2o_rotation& r, int64_t b, int64_t token, int64_t slot, int c8, float (&c)[8], float (&s)[8]) {
     const int d0 = 8 * (c8 & 7);
     double p0, p1 = 0.0, p2 = 0.0;
@@ -72,10 +54,10 @@ __device__ __forceinline__ void angles(const r2o_rotation& r, int64_t b, int64_t
     for (int i = 0; i < 8; ++i) {
         const double f = r.freq_bytes == 8 ? r2o_ldg(reinterpret_cast<const double*>(r.inv_freq) + d0 + i)
                                            : (double)r2o_ldg(reinterpret_cast<const float*>(r.inv_freq) + d0 + i);
-        const double p = m1 >> i & 1 ? p1 : (m2 >> i & 1 ? p2 : p0), t = p * (f * 0.15915494309189535);
-        cos_sin(t - __builtin_rint(t), c[i], s[i]);
-        c[i] *= r.scaling;
-        s[i] *= c8 < 8 ? -r.scaling : r.scaling;
+        const double p = m1 >> i & 1 ? p1 : (m2 >> i & 1 ? p2 : p0), halves = p * (f * 0.3183098861837907), n = __builtin_rint(halves);
+        const float x = 0.5f * (float)(halves - n), sign = __builtin_amdgcn_fract(0.5 * n) != 0.0 ? -r.scaling : r.scaling;
+        c[i] = __builtin_amdgcn_cosf(x) * sign;
+        s[i] = __builtin_amdgcn_sinf(x) * (c8 < 8 ? -sign : sign);
     }
 }
 
@@ -101,11 +83,27 @@ __device__ __forceinline__ void rotate_row(float (&x)[8], const float (&cs)[8], 
     for (int i = 0; i < 8; ++i) x[i] = y[i];
 }
 
-constexpr int kHeadsInFlight = 4;
+// Rows of a call past what the caches hold (STREAM) are read once and written into pages past them, eight heads' at a time:
+// into pages, 187 us so for 32641 rows of 32 + 2 x 8 heads with norms become 141, with four heads at a time 152; the query rows
+// written so too, 164.
+template <bool STREAM>
+constexpr int kHeadsInFlight = STREAM ? 8 : 4;
+
+template <bool STREAM>
+__device__ __forceinline__ r2o_u4 load_row(const uint16_t* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load((const R2O_GLOBAL r2o_u4*)p);
+    return r2o_load8<true>(p);
+}
+
+template <bool STREAM>
+__device__ __forceinline__ void store_slot(uint16_t* p, const r2o_u4& w) {
+    if constexpr (STREAM) __builtin_nontemporal_store(w, (R2O_GLOBAL r2o_u4*)p);
+    else r2o_store8<true>(p, w);
+}
 
 // grid (ceil(items / 16), ceil(heads / heads_per_wave)), block 256.  Lanes past the last item work on it again and store
 // nothing: the exchanges need every lane of the wave.
-template <int DT, bool NORM, bool PAGED>
+template <int DT, bool NORM, bool PAGED, bool STREAM>
 __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
     const int lane = threadIdx.x & 63, c8 = lane & 15;
     const uint32_t item = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
@@ -130,31 +128,36 @@ __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
             }
         }
     }
+    auto in_head = [&](const int64_t (&st)[3]) { return b * st[0] + token * st[2] + 8 * c8; };
+    const int64_t qo0 = in_head(a.qo_strides), ko0 = PAGED ? 0 : in_head(a.ko_strides);
+    const int h_end = min(a.heads, (int)(blockIdx.y + 1) * a.heads_per_wave);
+    if (PAGED && !__any(live && counts)) {  // of a padded request: zeros
+        for (int h = blockIdx.y * a.heads_per_wave; h < min(h_end, a.hq); ++h)
+            if (live) r2o_store8<true>(a.q_out + qo0 + h * a.qo_strides[1], r2o_u4{});
+        return;
+    }
     float cs[8], sn[8], wq[8], wk[8];
     angles(a.rotation, b, token, slot, c8, cs, sn);
     if constexpr (NORM) {
         r2o_unpack8<DT>(r2o_load8<true>(a.rotation.q_weight + 8 * c8), wq);
         r2o_unpack8<DT>(r2o_load8<true>(a.rotation.k_weight + 8 * c8), wk);
     }
-    auto in_head = [&](const int64_t (&st)[3]) { return b * st[0] + token * st[2] + 8 * c8; };
     const int64_t q0 = in_head(a.q_strides), k0 = in_head(a.k_strides), v0 = PAGED ? in_head(a.v_strides) : 0;
-    const int64_t qo0 = in_head(a.qo_strides), ko0 = PAGED ? 0 : in_head(a.ko_strides);
-    const int h_end = min(a.heads, (int)(blockIdx.y + 1) * a.heads_per_wave);
-    for (int h0 = blockIdx.y * a.heads_per_wave; h0 < h_end; h0 += kHeadsInFlight) {
-        r2o_u4 raw[kHeadsInFlight];
+    for (int h0 = blockIdx.y * a.heads_per_wave; h0 < h_end; h0 += kHeadsInFlight<STREAM>) {
+        r2o_u4 raw[kHeadsInFlight<STREAM>];
 #pragma unroll
-        for (int u = 0; u < kHeadsInFlight; ++u) {  // h is wave-uniform
+        for (int u = 0; u < kHeadsInFlight<STREAM>; ++u) {  // h is wave-uniform
             const int h = min(h0 + u, h_end - 1);
-            if (h < a.hq) raw[u] = r2o_load8<true>(a.q + q0 + h * a.q_strides[1]);
-            else if (!PAGED || h < a.hq + a.hkv) raw[u] = r2o_load8<true>(a.k + k0 + (h - a.hq) * a.k_strides[1]);
-            else raw[u] = r2o_load8<true>(a.v + v0 + (h - a.hq - a.hkv) * a.v_strides[1]);
+            if (h < a.hq) raw[u] = load_row<STREAM>(a.q + q0 + h * a.q_strides[1]);
+            else if (!PAGED || h < a.hq + a.hkv) raw[u] = load_row<STREAM>(a.k + k0 + (h - a.hq) * a.k_strides[1]);
+            else raw[u] = load_row<STREAM>(a.v + v0 + (h - a.hq - a.hkv) * a.v_strides[1]);
         }
 #pragma unroll
-        for (int u = 0; u < kHeadsInFlight; ++u) {
+        for (int u = 0; u < kHeadsInFlight<STREAM>; ++u) {
             const int h = h0 + u;
             if (h >= h_end) break;
             if (PAGED && h >= a.hq + a.hkv) {
-                if (key_at >= 0) r2o_store8<true>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
+                if (key_at >= 0) store_slot<STREAM>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
                 continue;
             }
             float x[8];
@@ -168,7 +171,7 @@ __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
             } else if constexpr (PAGED) {
                 const int64_t kv = h - a.hq;
                 if (key_at >= 0) {
-                    r2o_store8<true>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
+                    store_slot<STREAM>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
                     if (a.cache.weight_pages && c8 == 0)
                         a.cache.weight_pages[weight_at + kv * a.cache.weight_strides[1]] =
                             a.weights ? r2o_ldg(a.weights + b * a.weights_strides[0] + kv * a.weights_strides[1] + token) : 0.f;
@@ -194,9 +197,27 @@ bool rotation_ok(const r2o_rotation& r, bool slots) {
     return (r.position_bytes == 4 || r.position_bytes == 8) && r2o_aligned(r.positions, r.position_bytes);
 }
 
-// Heads of a wave: all of them share its angles, but a call of few tokens is spread over the chip first.  kFullWaves waves are
-// 8 for each SIMD.
-constexpr int64_t kFullWaves = 8192;
+// Heads of a wave: all of them share its angles, but a call of few tokens is spread over the chip first.  With kFullWaves waves, 4
+// for each SIMD, 4096 rows of 36 heads into their pages take 16.4 us; 19.5 with twice as many, which form the angles twice as often.
+constexpr int64_t kFullWaves = 4096;
+
+// Bytes of rows from which on they pass the caches by: 267 MB (32641 rows of 32 heads) take 89 us so and 114 through the caches; 63
+// MB (6153 rows of 40 heads) 30.0 and 28.8, 45 MB into pages 22.7 and 19.4: those still lie there.
+constexpr int64_t kStreamed = (int64_t)1 << 27;
+
+template <bool PAGED, bool STREAM>
+int launch_kernel(const RotateArgs& a, int64_t dtype, dim3 grid, hipStream_t st) {
+    const bool norm = a.rotation.q_weight != nullptr;
+    if (dtype == 0) {
+        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<0, true, PAGED, STREAM>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rotate_by_position_kernel<0, false, PAGED, STREAM>), grid, dim3(256), 0, st, a);
+    } else {
+        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<1, true, PAGED, STREAM>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rotate_by_position_kernel<1, false, PAGED, STREAM>), grid, dim3(256), 0, st, a);
+    }
+    R2O_CHECK_LAUNCH();
+    return R2O_OK;
+}
 
 template <bool PAGED>
 int launch(RotateArgs& a, int64_t dtype, int64_t batch, int64_t tokens, int64_t heads, hipStream_t st) {
@@ -210,16 +231,7 @@ int launch(RotateArgs& a, int64_t dtype, int64_t batch, int64_t tokens, int64_t 
     per = std::max(per, (heads + 65534) / 65535);  // the grid's second dimension
     a.heads_per_wave = (int)per;
     const dim3 grid((unsigned)((items + 15) / 16), (unsigned)((heads + per - 1) / per));
-    const bool norm = a.rotation.q_weight != nullptr;
-    if (dtype == 0) {
-        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<0, true, PAGED>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((rotate_by_position_kernel<0, false, PAGED>), grid, dim3(256), 0, st, a);
-    } else {
-        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<1, true, PAGED>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((rotate_by_position_kernel<1, false, PAGED>), grid, dim3(256), 0, st, a);
-    }
-    R2O_CHECK_LAUNCH();
-    return R2O_OK;
+    return heads * items > kStreamed / 256 ? launch_kernel<PAGED, true>(a, dtype, grid, st) : launch_kernel<PAGED, false>(a, dtype, grid, st);
 }
 
 }  // namespace
