@@ -24,6 +24,7 @@
 #include <cstring>
 #include <vector>
 
+#include "r2o_place.hpp"
 #include "r2o_sspa.h"
 
 namespace {
@@ -870,21 +871,19 @@ PyObject* paged_rope_extend_call(PyObject* const* args) {
     return status_and(launch_on(args[0], p, device), {q_out});
 }
 
-// Units of the longest list of a call of the prefix attention, at most: whatever the lengths on the device say.
-bool merged_rows(int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes) { return prefixes && hq / hkv * rows < 128; }
+// Workgroups that share a call's list, one a compute unit, whose LDS it fills, and the call's scratch; none where its units are
+// more than the kernels count.
+struct PrefixPlan {
+    int64_t workers, scratch;
+};
 
-int64_t prefix_tiles(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t capacity, int64_t prefixes, int64_t prefix_capacity) {
-    const int64_t packed = hq / hkv * rows, own = div_up(capacity, 64), shared = prefixes ? div_up(prefix_capacity, 64) : 0;
-    return merged_rows(hkv, hq, rows, prefixes)
-               ? std::max(hkv * (batch * packed / 256 + prefixes) * (shared + 4), hkv * batch * div_up(packed, 32) * (2 * own + 1))
-               : hkv * batch * div_up(packed, 256) * (1 + shared + own + 4);
-}
-
-// Workgroups that share them: one a compute unit, whose LDS it fills.
-int64_t prefix_workers(int64_t tiles, int64_t cus) { return std::max<int64_t>(1, std::min(cus, tiles)); }
-
-int64_t prefix_scratch(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t prefixes, int64_t workers) {
-    return 130 * (512 * workers + (merged_rows(hkv, hq, rows, prefixes) ? 2 * batch * hq * rows : 0)) + 8 * (1 + std::max(batch, workers));
+PrefixPlan prefix_plan(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t slots, int64_t prefixes, int64_t shared, bool some_count, int64_t cus) {
+    const int64_t packed = hq / hkv * rows, all_rows = batch * hq * rows;
+    const bool merged = r2o_prefix_merged(prefixes > 0, packed, all_rows, shared, some_count);
+    const int64_t units = r2o_prefix_units(merged, batch, hkv, packed, slots, prefixes, shared);
+    if (units > 0x7fffffff - 8 * R2O_PAGED_MAX_WORKERS) return {0, 0};
+    const int64_t workers = std::max<int64_t>(1, std::min(cus, units));
+    return {workers, r2o_prefix_scratch(workers, r2o_prefix_room(prefixes > 0, packed, all_rows), all_rows, batch)};
 }
 
 // paged_prefix_attention(function, query, cache, prefix or None, members, query_lengths, scale): (status, out, lse) or None
@@ -912,12 +911,13 @@ PyObject* paged_prefix_attention_call(PyObject* const* args) {
         !mask_args(Py_None, kZero, args[6], window, sinks, p.sm_scale) || !lengths_arg(args[4], f.batch, device, p.members) ||
         !lengths_arg(args[5], c.batch, device, p.query_lengths))
         Py_RETURN_NONE;
-    const int64_t tiles = prefix_tiles(c.batch, c.hkv, p.hq, p.rows, c.max_pages * c.page_size, f.batch, f.max_pages * f.page_size);
-    if (tiles > 0x7fffffff - 8 * R2O_PAGED_MAX_WORKERS) Py_RETURN_NONE;
+    const PrefixPlan plan = prefix_plan(c.batch, c.hkv, p.hq, p.rows, c.max_pages * c.page_size, f.batch, f.max_pages * f.page_size,
+                                        p.query_lengths != nullptr, compute_units((int)device));
+    if (!plan.workers) Py_RETURN_NONE;
     at::Tensor out = at::empty_like(*q);
     if (!row_strides(out, axes, p.o_strides, true) || p.o_strides[2] > R2O_MAX_ROW_STRIDE) Py_RETURN_NONE;
-    p.workers = prefix_workers(tiles, compute_units((int)device));
-    p.scratch_floats = prefix_scratch(c.batch, c.hkv, p.hq, p.rows, f.batch, p.workers);
+    p.workers = plan.workers;
+    p.scratch_floats = plan.scratch;
     const auto f32 = at::TensorOptions().device(q->device()).dtype(at::kFloat);
     at::Tensor lse = at::empty(q->sizes().slice(0, axes), f32), scratch = at::empty({p.scratch_floats}, f32);
     p.query = static_cast<const uint16_t*>(q->data_ptr());
@@ -955,22 +955,11 @@ PyObject* paged_workers_rule(PyObject*, PyObject* args) {
     return PyLong_FromLongLong(paged_workers(x[0], x[1], x[2], x[3]));
 }
 
-PyObject* prefix_tiles_rule(PyObject*, PyObject* args) {
-    long long x[7];
-    if (!PyArg_ParseTuple(args, "LLLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5, x + 6)) return nullptr;
-    return PyLong_FromLongLong(prefix_tiles(x[0], x[1], x[2], x[3], x[4], x[5], x[6]));
-}
-
-PyObject* prefix_workers_rule(PyObject*, PyObject* args) {
-    long long x[2];
-    if (!PyArg_ParseTuple(args, "LL", x, x + 1)) return nullptr;
-    return PyLong_FromLongLong(prefix_workers(x[0], x[1]));
-}
-
-PyObject* prefix_scratch_rule(PyObject*, PyObject* args) {
-    long long x[6];
-    if (!PyArg_ParseTuple(args, "LLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5)) return nullptr;
-    return PyLong_FromLongLong(prefix_scratch(x[0], x[1], x[2], x[3], x[4], x[5]));
+PyObject* prefix_plan_rule(PyObject*, PyObject* args) {
+    long long x[9];
+    if (!PyArg_ParseTuple(args, "LLLLLLLLL", x, x + 1, x + 2, x + 3, x + 4, x + 5, x + 6, x + 7, x + 8)) return nullptr;
+    const PrefixPlan plan = prefix_plan(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7] != 0, x[8]);
+    return Py_BuildValue("LL", (long long)plan.workers, (long long)plan.scratch);
 }
 
 #define FAST(call, n) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<call, n>)), METH_FASTCALL, nullptr
@@ -988,9 +977,7 @@ PyMethodDef kMethods[] = {
     {"position_rope", FAST(position_rope_call, 6)},
     {"paged_rope_extend", FAST(paged_rope_extend_call, 9)},
     {"paged_prefix_attention", FAST(paged_prefix_attention_call, 7)},
-    {"prefix_tiles", prefix_tiles_rule, METH_VARARGS, nullptr},
-    {"prefix_workers", prefix_workers_rule, METH_VARARGS, nullptr},
-    {"prefix_scratch", prefix_scratch_rule, METH_VARARGS, nullptr},
+    {"prefix_plan", prefix_plan_rule, METH_VARARGS, nullptr},
     {"attention_splits", attention_splits_rule, METH_VARARGS, nullptr},
     {"weight_splits", weight_splits_rule, METH_VARARGS, nullptr},
     {"paged_workers", paged_workers_rule, METH_VARARGS, nullptr},

@@ -13,6 +13,7 @@
 
 #include "r2o_cache_check.hpp"
 #include "r2o_common.hpp"
+#include "r2o_place.hpp"
 #include "r2o_tiles.hpp"
 
 namespace {
@@ -21,11 +22,8 @@ using namespace r2o_tiles;
 
 constexpr int kWaves = 8;    // of a workgroup, which fills a compute unit
 constexpr int kRows = 256;   // rows of a workgroup: a wave's 32 each; 128 or fewer: 32 for two waves, which share their keys
-constexpr int kMerged = 128; // packed rows of a request below which all requests of a prefix are one list
 constexpr int kWaveRows = 32, kWaveKeys = 32;  // of a wave that works by itself
-// What a segment's start and end cost beside its tiles, in tiles: of a workgroup about nine microseconds beside 2.3 a tile of 256
-// rows, of one wave among eight five beside four.
-constexpr int kSegment = 4, kWaveSegment = 1;
+constexpr int kSegment = kR2oSegment, kWaveSegment = kR2oWaveSegment;
 constexpr int kAhead = 4;    // tiles in LDS or on their way there, the one in use among them
 
 // One cache's rows, in the kernels' widths (the host has checked that they fit).
@@ -70,6 +68,12 @@ __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
     return x;
+}
+
+// A number that all lanes share, in a scalar register: compared where it is asked, not held as a mask of lanes.
+__device__ __forceinline__ int opaque(int x) {
+    asm("" : "+v"(x));
+    return __builtin_amdgcn_readfirstlane(x);
 }
 
 __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
@@ -118,6 +122,18 @@ __device__ __forceinline__ Members lane_members(const Lane& x, int& before) {
 }
 
 __device__ __forceinline__ int div_up(int x, int by) { return (x + by - 1) / by; }
+
+// The rows that count of the requests before b, one query head's: where query_lengths say so, summed up in LDS.
+__device__ __forceinline__ int rows_before(const int* sums, int b) {
+    Args& a = kernel_args();
+    return a.query_lengths ? sums[b] : b * a.rows;
+}
+
+// Rows of a lane's prefix, of all query heads of a KV head.
+__device__ __forceinline__ int member_rows(const int* sums, const Members& m) {
+    return (rows_before(sums, m.first + m.count) - rows_before(sums, m.first)) * kernel_args().group;
+}
+
 __device__ __forceinline__ int counted_rows(int rows) {
     Args& a = kernel_args();
     return min(max(rows, 0), a.rows);
@@ -127,16 +143,16 @@ __device__ __forceinline__ int counted_rows(int rows) {
 __device__ __forceinline__ int units(int segments, int tiles, int more) { return tiles ? segments * (tiles + more) : 0; }
 
 // Of this lane's prefix (merged rows): heads x row tiles segments of its key tiles.
-__device__ __forceinline__ int prefix_work(const Lane& x, const Members& m) {
+__device__ __forceinline__ int prefix_work(const Lane& x, int rows) {
     Args& a = kernel_args();
-    return m.count ? units(a.hkv * div_up(m.count * a.packed, kRows), div_up(filled(a.shared, x.shared), kTile), kSegment) : 0;
+    return units(a.hkv * div_up(rows, kRows), div_up(filled(a.shared, x.shared), kTile), kSegment);
 }
 
 // Of this lane's request's own slots (merged rows), in tiles of 32 rows and 32 keys.
 __device__ __forceinline__ int own_work(const Lane& x, int b0) {
     Args& a = kernel_args();
     const int b = b0 + (threadIdx.x & 63);
-    return b < a.batch ? units(a.hkv * div_up(a.packed, kWaveRows), div_up(filled(a.own, x.own), kWaveKeys), kWaveSegment) : 0;
+    return b < a.batch ? units(a.hkv * div_up(counted_rows(x.rows) * a.group, kWaveRows), div_up(filled(a.own, x.own), kWaveKeys), kWaveSegment) : 0;
 }
 
 // The prefix of this lane's request, -1 for none, its requests and its length: one step a prefix.
@@ -204,9 +220,9 @@ struct Plan {
 // What this lane's prefix costs, in microseconds of a compute unit: a tile of 256 rows is bound by its products, one of up to
 // 128 by its loads; a request's unit takes 0.6.
 constexpr float kOwnCost = 0.6f;
-__device__ __forceinline__ float prefix_cost(const Lane& x, const Members& m) {
+__device__ __forceinline__ float prefix_cost(const Lane& x, int rows) {
     Args& a = kernel_args();
-    const int rows = m.count * a.packed, keys = div_up(filled(a.shared, x.shared), kTile), left = rows % kRows;
+    const int keys = div_up(filled(a.shared, x.shared), kTile), left = rows % kRows;
     const float tile = 2.3f * (rows / kRows) + (left > kRows / 2 ? 2.3f : (left ? 1.5f : 0.f));
     return keys ? a.hkv * (keys * tile + 9.f * div_up(rows, kRows)) : 0.f;
 }
@@ -223,8 +239,8 @@ __device__ __forceinline__ float wave_total(float x) {
 struct Entry {
     int base;             // tiles before it
     int prefix, request;  // request -1: all of a prefix's; -2: no entry
-    int first, members;   // of the prefix
-    int n_shared, n_own, rows;
+    int first, members;   // of the prefix: its requests
+    int n_shared, n_own, rows, before;  // before: rows of the requests before the prefix's, as many as `rows` are of its own
 };
 
 // The units of the lists of merged rows.
@@ -233,16 +249,16 @@ struct Sums {
     float shared_cost;
 };
 
-__device__ __forceinline__ Sums sums_of(const Lane& first) {
+__device__ __forceinline__ Sums sums_of(const Lane& first, const int* sums) {
     Args& a = kernel_args();
     Sums s{};
     int before = 0;
 #pragma unroll 1
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
         const Lane x = lane_at(first, g0);
-        const Members m = lane_members(x, before);
-        s.shared += last_lane(wave_scan(prefix_work(x, m)));
-        s.shared_cost += wave_total(prefix_cost(x, m));
+        const int rows = member_rows(sums, lane_members(x, before));
+        s.shared += last_lane(wave_scan(prefix_work(x, rows)));
+        s.shared_cost += wave_total(prefix_cost(x, rows));
     }
 #pragma unroll 1
     for (int b0 = 0; b0 < a.batch; b0 += 64) s.own += last_lane(wave_scan(own_work(lane_at(first, b0), b0)));
@@ -261,9 +277,10 @@ __device__ __forceinline__ Plan plan_of(const Sums& s) {
 }
 
 // What the join has to know, left by one wave: it would take longer to find it out again than to read it.  The shares, then of
-// each request the units of its prefix's and its own first tiles and their tiles, its prefix's requests, and its rows that count.
+// each request the units before its prefix and its own slots and their tiles, the rows before its prefix's requests', theirs, its own
+// that count, and those before it.
 constexpr int kNote = 8;
-__device__ __forceinline__ void write_notes(const Lane& first, const Plan& plan) {
+__device__ __forceinline__ void write_notes(const Lane& first, const int* sums, const Plan& plan) {
     Args& a = kernel_args();
     const int lane = threadIdx.x & 63;
     if (lane == 0) {
@@ -288,7 +305,7 @@ __device__ __forceinline__ void write_notes(const Lane& first, const Plan& plan)
         for (int g0 = 0; g0 < a.prefixes; g0 += 64) {  // the units before this request's prefix
             const Lane y = lane_at(first, g0);
             const Members m = lane_members(y, before);
-            const int units_to = wave_scan(prefix_work(y, m));
+            const int units_to = wave_scan(prefix_work(y, member_rows(sums, m)));
             if (g0 + 64 <= of) shared += last_lane(units_to);
             const int here = __shfl(units_to, (of - 1) & 63);
             if (of > g0 && of < g0 + 64) shared += here;
@@ -297,18 +314,19 @@ __device__ __forceinline__ void write_notes(const Lane& first, const Plan& plan)
             int* to = a.notes + kNote * (1 + b);
             to[0] = shared;
             to[1] = div_up(filled(a.shared, length), kTile);
-            to[2] = members.first;
-            to[3] = members.count;
+            to[2] = rows_before(sums, members.first) * a.group;
+            to[3] = member_rows(sums, members);
             to[4] = own + upto - work;
             to[5] = div_up(filled(a.own, x.own), kWaveKeys);
             to[6] = counted_rows(x.rows);
+            to[7] = rows_before(sums, b) * a.group;
         }
         own += last_lane(upto);
     }
 }
 
 // Merged rows: the prefix that holds tile u of the prefixes' list.
-__device__ __forceinline__ Entry find_prefix(const Lane& first, int u) {
+__device__ __forceinline__ Entry find_prefix(const Lane& first, const int* sums, int u) {
     Args& a = kernel_args();
     Entry e{};
     e.request = -2;
@@ -317,7 +335,7 @@ __device__ __forceinline__ Entry find_prefix(const Lane& first, int u) {
     for (int g0 = 0; g0 < a.prefixes; g0 += 64) {
         const Lane x = lane_at(first, g0);
         const Members m = lane_members(x, before);
-        const int work = prefix_work(x, m), upto = wave_scan(work), all = last_lane(upto);
+        const int rows = member_rows(sums, m), work = prefix_work(x, rows), upto = wave_scan(work), all = last_lane(upto);
         if ((uint32_t)(u - at) < (uint32_t)all) {
             const int i = __builtin_ctzll(__ballot(at + upto > u));
             e.base = at + __builtin_amdgcn_readlane(upto - work, i);
@@ -326,7 +344,8 @@ __device__ __forceinline__ Entry find_prefix(const Lane& first, int u) {
             e.first = __builtin_amdgcn_readlane(m.first, i);
             e.members = __builtin_amdgcn_readlane(m.count, i);
             e.n_shared = filled(a.shared, __builtin_amdgcn_readlane(x.shared, i));
-            e.rows = e.members * a.packed;
+            e.rows = __builtin_amdgcn_readlane(rows, i);
+            e.before = __builtin_amdgcn_readfirstlane(rows_before(sums, e.first)) * a.group;
         }
         at += all;
     }
@@ -416,8 +435,8 @@ __device__ __forceinline__ uint32_t split_rows(int worker, bool begins) { return
 __device__ __forceinline__ uint32_t split_wave_rows(int own_first, int wave, bool begins) {  // wave: of all that take requests
     return 2u * kRows * own_first + (2u * wave + begins) * kWaveRows;
 }
-__device__ __forceinline__ uint32_t whole_prefix_rows(Args& a, int first, int members, int head) {
-    return 2u * kRows * a.workers + ((uint32_t)first * a.hkv + (uint32_t)head * members) * a.packed;
+__device__ __forceinline__ uint32_t whole_prefix_rows(Args& a, int before, int rows, int head) {
+    return 2u * kRows * a.workers + (uint32_t)before * a.hkv + (uint32_t)head * rows;
 }
 __device__ __forceinline__ uint32_t whole_own_rows(Args& a, int b, int head) {
     return 2u * kRows * a.workers + ((uint32_t)(a.batch + b) * a.hkv + head) * a.packed;
@@ -677,36 +696,47 @@ __device__ __forceinline__ void lds_barrier() {  // of LDS alone: stores to memo
 // rows a product), O^T += V^T P^T; three tiles ahead go into LDS while one is computed on.  A tile is two halves of 32 keys: the
 // products of the half that follows run beside the exponentials of the one before it.
 template <int RF, bool MERGED>
-__device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const Lane& first, int u, int u_end) {
+__device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const int* sums, const Lane& first, int u, int u_end) {
     while (u < u_end) {
         Args& a = kernel_args();
         int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), worker = blockIdx.x;
         asm("" : "+v"(lane), "+s"(wave), "+s"(worker));  // or what depends on them alone would be held from one segment to the next
         int total;
-        const Entry e = MERGED ? find_prefix(first, u) : find_request(first, u, total);
+        const Entry e = MERGED ? find_prefix(first, sums, u) : find_request(first, u, total);
         if (e.request == -2) return;  // lengths that change meanwhile
         const Segment s = segment_of(e, u);
         const int begin = max(0, u - s.base), stop = min(s.tiles, u_end - s.base);
         if (stop <= begin || s.head >= a.hkv) return;  // nothing but a start that is the next one's, or lengths that change meanwhile
 
         // this lane's row, and the last key of its own that it sees
-        int two = __builtin_amdgcn_readfirstlane(e.rows - s.row0 <= kRows / 2);  // waves share the keys of 32 rows, a half of each tile each
+        const int two = opaque(e.rows - s.row0 <= kRows / 2);  // waves share the keys of 32 rows, a half of each tile each
         const int part = two ? wave >> 2 : 0, in_tile = 32 * (two ? wave & 3 : wave) + (lane & 31);
         const int at = min(s.row0 + in_tile, e.rows - 1), group = a.group;
-        const int rank = MERGED ? at / a.packed : 0, p = at - rank * a.packed, row = p / group, head = s.head * group + p - row * group;
-        const int b = MERGED ? e.first + rank : e.request;
-        int busy = __builtin_amdgcn_readfirstlane(s.row0 + in_tile - (lane & 31) < e.rows);  // of this wave
-        asm("" : "+s"(two), "+s"(busy));  // compared where they are asked, not held as masks
+        int row = at / group, b = e.request;
+        const int head = s.head * group + at - row * group;
+        if constexpr (MERGED) {  // the request that row `row` of the prefix's is of, and which of its rows that is
+            if (a.query_lengths) {
+                row += e.before / group;
+                b = e.first;
+                for (int step = 512; step; step >>= 1)
+                    if (b + step < e.first + e.members && sums[b + step] <= row) b += step;
+                row -= sums[b];
+            } else {
+                b = e.first + row / a.rows;
+                row -= (b - e.first) * a.rows;
+            }
+        }
+        const int busy = opaque(s.row0 + in_tile - (lane & 31) < e.rows);  // this wave
         uint32_t to = kNoRow;
         if (s.row0 + in_tile < e.rows && part == 0) {
             if (begin > 0 || stop < s.tiles) to = split_rows(worker, begin == 0) + in_tile;
-            else if (MERGED) to = whole_prefix_rows(a, e.first, e.members, s.head) + s.row0 + in_tile;
+            else if (MERGED) to = whole_prefix_rows(a, e.before, e.rows, s.head) + s.row0 + in_tile;
             else to = kResult;
         }
         Rows w;
         start_rows(w, a.query + (int64_t)b * a.q_batch + (int64_t)head * a.q_head + (int64_t)row * a.q_row + 8 * (lane >> 5));
         int counted = a.rows;
-        if (a.query_lengths) counted = counted_rows(r2o_ldg(a.query_lengths + b));
+        if (!MERGED && a.query_lengths) counted = counted_rows(r2o_ldg(a.query_lengths + b));
         const int see_own = min(e.n_own - counted + row, e.n_own - 1);
         // the least and the most that a row of the workgroup sees of them; no row of a prefix's segment has any
         const int base_row = e.n_own - __builtin_amdgcn_readfirstlane(counted);
@@ -922,17 +952,17 @@ __device__ __forceinline__ void work_on_own(Lds& lds, const Lane& first, int own
         asm("" : "+v"(lane), "+s"(wave));
         const Entry e = find_own(first, u);
         if (e.request == -2) return;  // lengths that change meanwhile
-        const Segment s = segment_at(e, u, div_up(e.n_own, kWaveKeys), kWaveSegment, div_up(a.packed, kWaveRows), kWaveRows);
+        const Segment s = segment_at(e, u, div_up(e.n_own, kWaveKeys), kWaveSegment, div_up(e.rows * a.group, kWaveRows), kWaveRows);
         const int begin = max(0, u - s.base), stop = min(s.tiles, u_end - s.base);
         if (stop <= begin || s.head >= a.hkv) return;
-        const int p = min(s.row0 + (lane & 31), a.packed - 1), row = p / a.group, head = s.head * a.group + p - row * a.group;
+        const int end = e.rows * a.group, p = min(s.row0 + (lane & 31), end - 1), row = p / a.group, head = s.head * a.group + p - row * a.group;
         uint32_t to = kNoRow;
-        if (s.row0 + (lane & 31) < a.packed)
+        if (s.row0 + (lane & 31) < end)
             to = (begin > 0 || stop < s.tiles ? split_wave_rows(own_first, index, begin == 0) : whole_own_rows(a, e.request, s.head) + s.row0) + (lane & 31);
         Rows w;
         start_rows(w, a.query + (int64_t)e.request * a.q_batch + (int64_t)head * a.q_head + (int64_t)row * a.q_row + 8 * (lane >> 5));
         const int off = e.n_own - e.rows, seen = min(off + row, e.n_own - 1);
-        const int least = min(off + s.row0 / a.group, e.n_own - 1), most = min(off + min(s.row0 + kWaveRows - 1, a.packed - 1) / a.group, e.n_own - 1);
+        const int least = min(off + s.row0 / a.group, e.n_own - 1), most = min(off + min(s.row0 + kWaveRows - 1, end - 1) / a.group, e.n_own - 1);
         const int last = min(stop, most >= 0 ? most / kWaveKeys + 1 : 0);  // tiles behind it are seen by no row
         const float c2 = a.c2;
         const Side side = side_of(a.own, e.request, s.head, e.n_own);
@@ -1028,28 +1058,40 @@ __device__ __forceinline__ void work_on_own(Lds& lds, const Lane& first, int own
 template <int RF, bool MERGED>
 __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixArgs) {
     __shared__ __align__(1024) Lds lds;
-    __shared__ int flags[kWaves];
+    __shared__ int flags[kWaves], sums_lds[R2O_PAGED_MAX_BATCH + 1];
     Args& a = kernel_args();
     const Lane first = lane_of(0);
     int u = 0, u_end = 0;
     if constexpr (MERGED) {
         int own_first, index, v = 0, v_end = 0;
+        if (a.query_lengths) {
+            if (threadIdx.x < 64) {
+                int before = 0;
+#pragma unroll 1
+                for (int b0 = 0; b0 <= a.batch; b0 += 64) {
+                    const int b = b0 + (int)threadIdx.x, rows = b < a.batch ? counted_rows(lane_at(first, b0).rows) : 0, upto = wave_scan(rows);
+                    if (b <= a.batch) sums_lds[b] = before + upto - rows;
+                    before += last_lane(upto);
+                }
+            }
+            __syncthreads();
+        }
         {
-            const Sums sums = sums_of(first);
+            const Sums sums = sums_of(first, sums_lds);
             const Plan plan = plan_of(sums);
             if (sums.shared > 0 && (int)blockIdx.x < plan.shared.workers) {
                 u = plan.shared.begin(blockIdx.x);
                 u_end = plan.shared.begin(blockIdx.x + 1);
             }
             own_first = plan.own_first;
-            if (blockIdx.x == gridDim.x - 1 && threadIdx.x >= 64 * (kWaves - 1)) write_notes(first, plan);
+            if (blockIdx.x == gridDim.x - 1 && threadIdx.x >= 64 * (kWaves - 1)) write_notes(first, sums_lds, plan);
             index = kWaves * ((int)blockIdx.x - own_first) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
             if (sums.own > 0 && index >= 0 && index < plan.own.workers) {
                 v = plan.own.begin(index);
                 v_end = plan.own.begin(index + 1);
             }
         }
-        work_on_row_tiles<RF, true>(lds, flags, first, u, u_end);
+        work_on_row_tiles<RF, true>(lds, flags, sums_lds, first, u, u_end);
         work_on_own<RF>(lds, first, own_first, index, v, v_end);
     } else {
         int total;
@@ -1076,7 +1118,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
 #pragma unroll
             for (int i = 0; i < 4; ++i) to[1 + i] = place[i];
         }
-        work_on_row_tiles<RF, false>(lds, flags, first, u, u_end);
+        work_on_row_tiles<RF, false>(lds, flags, sums_lds, first, u, u_end);
     }
 }
 
@@ -1147,31 +1189,37 @@ __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
     }
 }
 
-// Merged rows: a workgroup a row, whose partial states of the prefix's segment and of its own are shared by 8 groups of 32
-// lanes.
-template <int RF>
+// Rows of a call from which on 32 lanes join a row: fewer have the states of many workgroups each.  Eight times 32 lanes and 32, of
+// 1792 rows: 27 and 28 us, 33 and 36 (a whole call); 2048: 23.8 and 23.3; 3584: 44 and 42, 36 and 34; 16384: 62 and 38.
+constexpr int64_t kJoinAlone = 2048;
+
+// Merged rows: PARTS groups of 32 lanes (8, or 1) share a row's partial states of the prefix's segment and of its own.
+template <int RF, int PARTS>
 __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
-    __shared__ __align__(16) float red[8][128];
-    __shared__ float red_ml[8][2];
+    __shared__ __align__(16) float red[PARTS][128];
+    __shared__ float red_ml[PARTS][2];
     Args& a = kernel_args();
-    const int per_request = a.hkv * a.packed;
-    const int b = (int)blockIdx.x / per_request, in_request = (int)blockIdx.x - b * per_request, h = in_request / a.packed, p = in_request - h * a.packed;
-    const int row = p / a.group, head = h * a.group + p - row * a.group, d4 = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int d4 = threadIdx.x & 31, group = threadIdx.x >> 5, part = PARTS == 1 ? 0 : group;
+    const int per_request = a.hkv * a.packed, at_row = PARTS == 1 ? 8 * (int)blockIdx.x + group : (int)blockIdx.x;
+    if (PARTS == 1 && at_row >= a.batch * per_request) return;
+    const int b = at_row / per_request, in_request = at_row - b * per_request, h = in_request / a.packed, p = in_request - h * a.packed;
+    const int row = p / a.group, head = h * a.group + p - row * a.group;
     const int *all = a.notes, *note = a.notes + kNote * (1 + b);
+    auto load = [](const int* from) { return PARTS == 1 ? r2o_ldg(from) : load_uniform(from); };
     const Share shared{load_uniform(all), 0, load_uniform(all + 1), load_uniform(all + 2)}, own{load_uniform(all + 4), 0, load_uniform(all + 5), load_uniform(all + 6)};
-    const int own_first = load_uniform(all + 3), shared_base = load_uniform(note), shared_tiles = load_uniform(note + 1), first = load_uniform(note + 2),
-              members = load_uniform(note + 3), own_base = load_uniform(note + 4), own_tiles = load_uniform(note + 5), counted = load_uniform(note + 6);
+    const int own_first = load_uniform(all + 3), shared_base = load(note), shared_tiles = load(note + 1), before = load(note + 2), rows = load(note + 3),
+              own_base = load(note + 4), own_tiles = load(note + 5), counted = load(note + 6), place = load(note + 7);
     State s{-INFINITY, 0.f, r2o_f4{}};
     if (row < counted) {
         // the states of one segment, of `tiles` tiles from unit `base` on: shared by the groups, four loads of each under way
         auto add = [&](const Share& share, int base, int tiles, uint32_t whole, auto split) {
             const int w0 = share.worker(base), count = share.worker(base + tiles - 1) - w0 + 1;
-            for (int i0 = part; i0 < count; i0 += 32) {
+            for (int i0 = part; i0 < count; i0 += 4 * PARTS) {
                 float m2[4], l2[4];
                 r2o_f4 o2[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int i = min(i0 + 8 * k, count - 1);
+                    const int i = min(i0 + PARTS * k, count - 1);
                     const int64_t at = count == 1 ? whole : split(w0 + i, i == 0);
                     m2[k] = r2o_ldg(a.partial_ml + 2 * at);
                     l2[k] = r2o_ldg(a.partial_ml + 2 * at + 1);
@@ -1179,29 +1227,31 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (i0 + 8 * k < count) join_state(s, m2[k], l2[k], o2[k]);
+                    if (i0 + PARTS * k < count) join_state(s, m2[k], l2[k], o2[k]);
             }
         };
         if (shared_tiles > 0) {
-            const int r = (b - first) * a.packed + p, tile = r / kRows;
-            add(shared, shared_base + (h * div_up(members * a.packed, kRows) + tile) * (shared_tiles + kSegment) + kSegment, shared_tiles,
-                whole_prefix_rows(a, first, members, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
+            const int r = place - before + p, tile = r / kRows;
+            add(shared, shared_base + (h * div_up(rows, kRows) + tile) * (shared_tiles + kSegment) + kSegment, shared_tiles,
+                whole_prefix_rows(a, before, rows, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
         }
         if (own_tiles > 0) {
             const int chunk = p / kWaveRows;
-            add(own, own_base + (h * div_up(a.packed, kWaveRows) + chunk) * (own_tiles + kWaveSegment) + kWaveSegment, own_tiles,
+            add(own, own_base + (h * div_up(counted * a.group, kWaveRows) + chunk) * (own_tiles + kWaveSegment) + kWaveSegment, own_tiles,
                 whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(own_first, w, begins) + p - chunk * kWaveRows; });
         }
     }
-    *reinterpret_cast<r2o_f4*>(&red[part][4 * d4]) = s.o;
-    if (d4 == 0) {
-        red_ml[part][0] = s.m;
-        red_ml[part][1] = s.l;
+    if constexpr (PARTS > 1) {
+        *reinterpret_cast<r2o_f4*>(&red[part][4 * d4]) = s.o;
+        if (d4 == 0) {
+            red_ml[part][0] = s.m;
+            red_ml[part][1] = s.l;
+        }
+        __syncthreads();
+        if (part) return;
+    #pragma unroll
+        for (int i = 1; i < PARTS; ++i) join_state(s, red_ml[i][0], red_ml[i][1], *reinterpret_cast<const r2o_f4*>(&red[i][4 * d4]));
     }
-    __syncthreads();
-    if (part) return;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) join_state(s, red_ml[i][0], red_ml[i][1], *reinterpret_cast<const r2o_f4*>(&red[i][4 * d4]));
     write_row<RF>(a, s, b, head, row, d4);
 }
 
@@ -1225,8 +1275,6 @@ Source source_of(const r2o_paged_cache& c) {
     return s;
 }
 
-int64_t tiles_of(const r2o_paged_cache& c) { return (c.max_pages * c.page_size + kTile - 1) / kTile; }
-
 }  // namespace
 
 extern "C" {
@@ -1236,23 +1284,22 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     const r2o_paged_cache &c = p->cache, &f = p->prefix;
     const bool any = f.batch != 0;  // of the prefixes; without one their fields are not looked at
     if (any && (!r2o_paged_cache_ok(f) || f.weight_pages || f.hkv != c.hkv || f.dtype != c.dtype || (f.batch > 1 && !p->members))) return R2O_EINVAL;
-    if (p->hq < c.hkv || p->hq % c.hkv || p->rows < 1 || p->rows > (1 << 29) || !r2o_aligned(p->query, 16) || !r2o_aligned(p->out, 16) ||
+    if (p->hq < c.hkv || p->hq > (1 << 30) || p->hq % c.hkv || p->rows < 1 || p->rows > (1 << 29) || !r2o_aligned(p->query, 16) || !r2o_aligned(p->out, 16) ||
         !r2o_aligned(p->lse, 4) || !r2o_strides_ok(p->q_strides, 3, INT64_MAX) || !r2o_strides_ok(p->o_strides, 3, INT64_MAX) ||
         p->q_strides[2] > R2O_MAX_ROW_STRIDE || p->o_strides[2] > R2O_MAX_ROW_STRIDE || reinterpret_cast<uintptr_t>(p->members) % 4 ||
         reinterpret_cast<uintptr_t>(p->query_lengths) % 4 || !(p->sm_scale > 0.f) || !(p->sm_scale < INFINITY) || p->workers < 1 ||
         p->workers > R2O_PAGED_MAX_WORKERS || !r2o_aligned(p->scratch, 16))
         return R2O_EINVAL;
-    const int64_t group = p->hq / c.hkv, packed = group * p->rows, all_rows = c.batch * c.hkv * packed;
-    if (packed > (1 << 30) || all_rows > (1 << 30)) return R2O_EINVAL;
-    const bool merged = any && packed < kMerged;
-    const int64_t states = 2 * kRows * p->workers + (merged ? 2 * all_rows : 0);
-    if (p->scratch_floats < 130 * states + kNote * (1 + std::max(c.batch, p->workers))) return R2O_EINVAL;
-    // whatever the lengths on the device say
-    const int64_t shared = any ? tiles_of(f) : 0, per_request = (packed + kRows - 1) / kRows;
-    const int64_t most = merged ? std::max(c.hkv * (c.batch * packed / kRows + f.batch) * (shared + kSegment),
-                                           c.hkv * c.batch * ((packed + kWaveRows - 1) / kWaveRows) * (kTile / kWaveKeys * tiles_of(c) + kWaveSegment))
-                                : c.hkv * c.batch * per_request * (1 + shared + tiles_of(c) + kSegment);
-    if (most > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS) return R2O_EINVAL;
+    const int64_t group = p->hq / c.hkv, packed = group * p->rows;
+    if (packed > (1 << 30)) return R2O_EINVAL;
+    const int64_t all_rows = c.batch * c.hkv * packed;
+    if (all_rows > (1 << 30)) return R2O_EINVAL;
+    const int64_t shared = any ? f.max_pages * f.page_size : 0;
+    const bool room = r2o_prefix_room(any, packed, all_rows), merged = r2o_prefix_merged(any, packed, all_rows, shared, p->query_lengths);
+    if (p->scratch_floats < r2o_prefix_scratch(p->workers, room, all_rows, c.batch)) return R2O_EINVAL;
+    const int64_t states = r2o_prefix_states(p->workers, room, all_rows);
+    if (r2o_prefix_units(merged, c.batch, c.hkv, packed, c.max_pages * c.page_size, f.batch, shared) > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS)
+        return R2O_EINVAL;
     PrefixArgs a{};
     a.own = source_of(c);
     a.shared = any ? source_of(f) : a.own;
@@ -1290,9 +1337,14 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
         return hipGetLastError() == hipSuccess ? R2O_OK : R2O_ELAUNCH;
     };
     if (merged) {
+        if (all_rows >= kJoinAlone) {
+            const dim3 join((unsigned)((all_rows + 7) / 8));
+            return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0, 1>, join)
+                                : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1, 1>, join);
+        }
         const dim3 join((unsigned)all_rows);
-        return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0>, join)
-                            : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1>, join);
+        return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0, 8>, join)
+                            : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1, 8>, join);
     }
     const dim3 join((unsigned)(p->workers - 1 + (p->query_lengths ? c.batch : 0)), kRows / kJoinRows);
     return c.dtype == 0 ? launch(prefix_partial_kernel<0, false>, prefix_join_split_kernel<0>, join)

@@ -284,10 +284,11 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedCache, prefix: Paged
     query_lengths = _lengths(query_lengths, batch, dev, "query_lengths")
     _lib.refuse_gradients(what, query, *(t for c in caches for t in _pools(c)), *(output or ()))
     scale = _scale(sm_scale)
-    most = _lib.host().prefix_tiles(batch, hkv, hq, rows, cache.capacity, prefixes, prefix.capacity if prefixes else 0)
-    if most > (1 << 31) - 1 - 8 * 4096:
-        raise ValueError("paged prefix attention has more tiles of slots than it can count")
     params = [_params_of(c) for c in caches]
+    workers, floats = _lib.host().prefix_plan(batch, hkv, hq, rows, cache.capacity, prefixes, prefix.capacity if prefixes else 0,
+                                              query_lengths is not None, _lib.num_cus(dev))
+    if not workers:
+        raise ValueError("paged prefix attention has more tiles of slots than it can count")
     query = _rows(query)
     if output is None:
         out = _like(query)
@@ -302,10 +303,8 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedCache, prefix: Paged
                          rows=rows, sm_scale=scale)
     if prefixes:
         p.prefix = params[1]
-    p.workers = _lib.host().prefix_workers(most, _lib.num_cus(dev))
-    p.scratch_floats = _lib.host().prefix_scratch(batch, hkv, hq, rows, prefixes, p.workers)
-    scratch = torch.empty(p.scratch_floats, dtype=torch.float32, device=dev)
-    p.scratch = scratch.data_ptr()
+    scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+    p.workers, p.scratch_floats, p.scratch = workers, floats, scratch.data_ptr()
     _lib.launch("r2o_paged_prefix_attention", p, dev)
     return (out[:, :, 0], lse[..., 0]) if token else (out, lse)
 

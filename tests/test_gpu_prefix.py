@@ -72,6 +72,23 @@ def test_padded_batches(rows):
     assert not out[1].any() and (lse[1] == -math.inf).all() and not out[4].any()
 
 
+# the counted rows of a prefix's requests stand side by side: none, one, all, runs without any, more requests than a wave
+@pytest.mark.parametrize("hq,hkv", [(14, 2), (4, 4), (28, 1)])
+@pytest.mark.parametrize("rows", [1, 2, 7, 18])
+def test_ragged_batches_of_some_prefixes(rows, hq, hkv):
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(rows)
+    batch = 150
+    counts = torch.randint(-1, rows + 2, (batch,), generator=gen)
+    counts[20:40] = 0
+    counts[64:70] = rows
+    lengths = torch.randint(0, 60, (batch,), generator=gen).tolist()
+    shared, own = _both(dev, (200, 2100, 0, 77), lengths, hkv, 16, BF16, rows)
+    q = _query(dev, batch, hq, rows, BF16, 27)
+    for members in ((30, 8, 2, 100), (150, 0, 0, 0), (0, 19, 3, 41)):
+        check(q, own, shared, _ints(dev, *members), _ints(dev, *counts.tolist()))
+
+
 @pytest.mark.parametrize("rows", [1, 3, 40])
 def test_empty_prefixes_and_requests(rows):
     """A prefix or request without slots; lengths below 0, below the rows and past the table."""
@@ -174,17 +191,17 @@ def test_scales(scale, rows):
 
 
 @pytest.mark.parametrize("workers", [1, 2, 3, 7, 50, 512, 4096])
-@pytest.mark.parametrize("rows", [1, 40])
-def test_any_number_of_workers(rows, workers):
+@pytest.mark.parametrize("rows,prefix", [(1, 700), (40, 700), (40, 2100), (80, 700)])
+def test_any_number_of_workers(rows, prefix, workers):
     """Each within the 64-bit bound: the joins add partial results of other cuts.  Rows of the scratch that a call has no
     right to stay as they were."""
     from r2omni_amd import _lib, paged
 
     dev = _cuda()
-    shared, own = _both(dev, (700, 130), (100, 64, 41, 300, 77), 2, 32, BF16, 14)
+    shared, own = _both(dev, (prefix, 130), (100, 64, 41, 300, 77), 2, 32, BF16, 14)
     q, members = _query(dev, 5, 14, rows, BF16, 14), _ints(dev, 2, 2)
     out, lse = torch.full_like(q, math.nan), torch.full((5, 14, rows), math.nan, device=dev)
-    floats = 130 * (512 * workers + (2 * 5 * 14 * rows if rows == 1 else 0)) + 8 * (1 + max(5, workers))
+    floats = 130 * (512 * workers + (2 * 5 * 14 * rows if 7 * rows < 512 else 0)) + 8 * (1 + max(5, workers))
     scratch = torch.full((floats + 512,), 3.0, device=dev)
     p = _lib.PagedPrefix(cache=paged._params_of(own), prefix=paged._params_of(shared), members=members.data_ptr(), query=q.data_ptr(),
                          out=out.data_ptr(), lse=lse.data_ptr(), q_strides=q.stride()[:3], o_strides=out.stride()[:3], hq=14, rows=rows,
