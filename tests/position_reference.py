@@ -1,8 +1,8 @@
 """Rotation by positions in 64 bits, and how far a kernel's results may be from it.
 
-Bounds count roundings, with u = 2^-24, a half step of fp32 relative to 1.  Cosine and sine are off by at most 4 u: half of one
-for each of the polynomial's cut-off term (2.5e-8), its last addition and the argument's rounding, and the argument's own
-part, position * 2^-52 turns; `scaling` adds another u.  A product of two fp32 values and a fused sum add 2 u.  So a rotated
+Bounds count roundings, with u = 2^-24, a half step of fp32 relative to 1.  Cosine and sine are off by at most 4 u: two for the
+hardware's functions (2^-23 measured), one for the rounding of their argument, at most a half as half turns (pi 2^-26), and the
+argument's own part, position * 2^-52 turns; `scaling` adds another u.  A product of two fp32 values and a fused sum add 2 u.  So a rotated
 channel is off by at most 8 u scaling (|x| + |x'|).  Norms: the sum of squares is off by 12 u of itself (8 in a lane, 4 across),
 half of which enters the root; that, the division, the root and two products make 10 u, taken as 16.  FWHT-128: seven sums of
 growing terms and one product, 8 u of sum |y| / sqrt(128), beside the mean-square growth of what is there, at most sum of the
