@@ -83,11 +83,12 @@ __device__ __forceinline__ void rotate_row(float (&x)[8], const float (&cs)[8], 
     for (int i = 0; i < 8; ++i) x[i] = y[i];
 }
 
-// Rows of a call past what the caches hold (STREAM) are read once and written into pages past them, eight heads' at a time:
-// into pages, 187 us so for 32641 rows of 32 + 2 x 8 heads with norms become 141, with four heads at a time 152; the query rows
-// written so too, 164.
+// Rows of a call past what the caches hold (STREAM) are read and written past them, 16 heads' at a time.  32641 rows of 32 heads take
+// 101 us so (5.28 TB/s, as a copy's) and 113 through the caches, four at a time; into pages, 32 + 2 x 8 heads with norms, 153 and
+// 189.  With 8 heads at a time 107 and 163, 12: 105 and 154, 24: 104 and 156; with loads alone past the caches 107 and 162, stores
+// alone 105 and 157.
 template <bool STREAM>
-constexpr int kHeadsInFlight = STREAM ? 8 : 4;
+constexpr int kHeadsInFlight = STREAM ? 16 : 4;
 
 template <bool STREAM>
 __device__ __forceinline__ r2o_u4 load_row(const uint16_t* p) {
@@ -96,7 +97,7 @@ __device__ __forceinline__ r2o_u4 load_row(const uint16_t* p) {
 }
 
 template <bool STREAM>
-__device__ __forceinline__ void store_slot(uint16_t* p, const r2o_u4& w) {
+__device__ __forceinline__ void store_row(uint16_t* p, const r2o_u4& w) {
     if constexpr (STREAM) __builtin_nontemporal_store(w, (R2O_GLOBAL r2o_u4*)p);
     else r2o_store8<true>(p, w);
 }
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
             const int h = h0 + u;
             if (h >= h_end) break;
             if (PAGED && h >= a.hq + a.hkv) {
-                if (key_at >= 0) store_slot<STREAM>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
+                if (key_at >= 0) store_row<STREAM>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
                 continue;
             }
             float x[8];
@@ -167,17 +168,17 @@ __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
             r2o_u4 y = r2o_pack8<DT>(x);
             if (h < a.hq) {
                 if (PAGED && !counts) y = r2o_u4{};
-                if (live) r2o_store8<true>(a.q_out + qo0 + h * a.qo_strides[1], y);
+                if (live) store_row<STREAM>(a.q_out + qo0 + h * a.qo_strides[1], y);
             } else if constexpr (PAGED) {
                 const int64_t kv = h - a.hq;
                 if (key_at >= 0) {
-                    store_slot<STREAM>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
+                    store_row<STREAM>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
                     if (a.cache.weight_pages && c8 == 0)
                         a.cache.weight_pages[weight_at + kv * a.cache.weight_strides[1]] =
                             a.weights ? r2o_ldg(a.weights + b * a.weights_strides[0] + kv * a.weights_strides[1] + token) : 0.f;
                 }
             } else if (live) {
-                r2o_store8<true>(a.k_out + ko0 + (h - a.hq) * a.ko_strides[1], y);
+                store_row<STREAM>(a.k_out + ko0 + (h - a.hq) * a.ko_strides[1], y);
             }
         }
     }
@@ -201,9 +202,10 @@ bool rotation_ok(const r2o_rotation& r, bool slots) {
 // for each SIMD, 4096 rows of 36 heads into their pages take 16.4 us; 19.5 with twice as many, which form the angles twice as often.
 constexpr int64_t kFullWaves = 4096;
 
-// Bytes of rows from which on they pass the caches by: 267 MB (32641 rows of 32 heads) take 89 us so and 114 through the caches; 63
-// MB (6153 rows of 40 heads) 30.0 and 28.8, 45 MB into pages 22.7 and 19.4: those still lie there.
-constexpr int64_t kStreamed = (int64_t)1 << 27;
+// Bytes of rows from which on they pass the caches by.  Rows that lie in memory: 16 MB take 13.3 us so and 11.6 through the caches, 33
+// MB 18.2 and 19.0, 66 MB 27.4 and 31.6, 197 MB 76 and 85, into pages with norms 49 MB 24.7 and 27.6, 98 MB 44 and 46, 148 MB 61 and
+// 73.  Rows that the caches still hold, 45 MB into pages: 22.7 and 19.4, 63 MB: 30.0 and 28.8.
+constexpr int64_t kStreamed = (int64_t)1 << 26;
 
 template <bool PAGED, bool STREAM>
 int launch_kernel(const RotateArgs& a, int64_t dtype, dim3 grid, hipStream_t st) {

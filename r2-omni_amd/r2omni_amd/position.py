@@ -7,7 +7,7 @@
 
 ``rope.qwen_qk_mrope`` and ``rope.qwen3_qk_norm_rope`` take cos and sin tables that the model has rounded, for parity with
 the reference's decode step; here the angles are formed in 64 bits from the positions (a position of 2^31 leaves a turn
-exact to 2^-24), there is no table to make, and every row is rounded once.  No counterpart in the reference, whose rotary
+exact to 2^-23), there is no table to make, and every row is rounded once.  No counterpart in the reference, whose rotary
 tables are the model's (qwen_sspa_attention.py:1228-1247).
 """
 from __future__ import annotations
