@@ -1189,19 +1189,24 @@ __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
     }
 }
 
-// Rows of a call from which on 32 lanes join a row: fewer have the states of many workgroups each.  Eight times 32 lanes and 32, of
-// 1792 rows: 27 and 28 us, 33 and 36 (a whole call); 2048: 23.8 and 23.3; 3584: 44 and 42, 36 and 34; 16384: 62 and 38.
-constexpr int64_t kJoinAlone = 2048;
+// Rows of a call from which on 128 lanes join a row, and 32: fewer rows have the states of more workgroups each.  A whole call of 32
+// rows takes 16.3 us by 256 lanes a row and 17.3 by 128; 672: 41.7, 41.6 and by 32 49.3; 1792: 57.6, 57.7, 58.6; 3584: 35.3, 33.5,
+// 33.3; 7168: 49.8, 44.1, 41.7; 16128: 85.0, 72.7, 63.3.
+constexpr int64_t kJoinBy128 = 512, kJoinBy32 = 4096;
 
-// Merged rows: PARTS groups of 32 lanes (8, or 1) share a row's partial states of the prefix's segment and of its own.
+// Merged rows: PARTS groups of 32 lanes share a row's partial states of the prefix's segment and of its own.
 template <int RF, int PARTS>
 __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
-    __shared__ __align__(16) float red[PARTS][128];
-    __shared__ float red_ml[PARTS][2];
+    constexpr int kRowsHere = 8 / PARTS;
+    __shared__ __align__(16) float red[8][128];
+    __shared__ float red_ml[8][2];
     Args& a = kernel_args();
-    const int d4 = threadIdx.x & 31, group = threadIdx.x >> 5, part = PARTS == 1 ? 0 : group;
-    const int per_request = a.hkv * a.packed, at_row = PARTS == 1 ? 8 * (int)blockIdx.x + group : (int)blockIdx.x;
-    if (PARTS == 1 && at_row >= a.batch * per_request) return;
+    const int d4 = threadIdx.x & 31, group = threadIdx.x >> 5, part = group % PARTS;
+    const int per_request = a.hkv * a.packed, all_rows = a.batch * per_request;
+    int at_row = kRowsHere * (int)blockIdx.x + group / PARTS;
+    if (PARTS > 1) at_row = __builtin_amdgcn_readfirstlane(at_row);  // of both groups of a wave
+    const bool live = at_row < all_rows;
+    at_row = min(at_row, all_rows - 1);
     const int b = at_row / per_request, in_request = at_row - b * per_request, h = in_request / a.packed, p = in_request - h * a.packed;
     const int row = p / a.group, head = h * a.group + p - row * a.group;
     const int *all = a.notes, *note = a.notes + kNote * (1 + b);
@@ -1210,7 +1215,7 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
     const int own_first = load_uniform(all + 3), shared_base = load(note), shared_tiles = load(note + 1), before = load(note + 2), rows = load(note + 3),
               own_base = load(note + 4), own_tiles = load(note + 5), counted = load(note + 6), place = load(note + 7);
     State s{-INFINITY, 0.f, r2o_f4{}};
-    if (row < counted) {
+    if (live && row < counted) {
         // the states of one segment, of `tiles` tiles from unit `base` on: shared by the groups, four loads of each under way
         auto add = [&](const Share& share, int base, int tiles, uint32_t whole, auto split) {
             const int w0 = share.worker(base), count = share.worker(base + tiles - 1) - w0 + 1;
@@ -1242,17 +1247,17 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
         }
     }
     if constexpr (PARTS > 1) {
-        *reinterpret_cast<r2o_f4*>(&red[part][4 * d4]) = s.o;
+        *reinterpret_cast<r2o_f4*>(&red[group][4 * d4]) = s.o;
         if (d4 == 0) {
-            red_ml[part][0] = s.m;
-            red_ml[part][1] = s.l;
+            red_ml[group][0] = s.m;
+            red_ml[group][1] = s.l;
         }
         __syncthreads();
         if (part) return;
-    #pragma unroll
-        for (int i = 1; i < PARTS; ++i) join_state(s, red_ml[i][0], red_ml[i][1], *reinterpret_cast<const r2o_f4*>(&red[i][4 * d4]));
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) join_state(s, red_ml[group + i][0], red_ml[group + i][1], *reinterpret_cast<const r2o_f4*>(&red[group + i][4 * d4]));
     }
-    write_row<RF>(a, s, b, head, row, d4);
+    if (live) write_row<RF>(a, s, b, head, row, d4);
 }
 
 // ------------------------------------------------------------------------------------ host checks
@@ -1337,14 +1342,15 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
         return hipGetLastError() == hipSuccess ? R2O_OK : R2O_ELAUNCH;
     };
     if (merged) {
-        if (all_rows >= kJoinAlone) {
-            const dim3 join((unsigned)((all_rows + 7) / 8));
-            return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0, 1>, join)
-                                : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1, 1>, join);
-        }
-        const dim3 join((unsigned)all_rows);
-        return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0, 8>, join)
-                            : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1, 8>, join);
+        auto join = [&](auto parts) {
+            constexpr int kParts = decltype(parts)::value;
+            const dim3 blocks((unsigned)((all_rows * kParts + 7) / 8));
+            return c.dtype == 0 ? launch(prefix_partial_kernel<0, true>, prefix_join_merged_kernel<0, kParts>, blocks)
+                                : launch(prefix_partial_kernel<1, true>, prefix_join_merged_kernel<1, kParts>, blocks);
+        };
+        if (all_rows < kJoinBy128) return join(std::integral_constant<int, 8>());
+        if (all_rows < kJoinBy32) return join(std::integral_constant<int, 4>());
+        return join(std::integral_constant<int, 1>());
     }
     const dim3 join((unsigned)(p->workers - 1 + (p->query_lengths ? c.batch : 0)), kRows / kJoinRows);
     return c.dtype == 0 ? launch(prefix_partial_kernel<0, false>, prefix_join_split_kernel<0>, join)
