@@ -906,7 +906,8 @@ PyObject* paged_prefix_attention_call(PyObject* const* args) {
     p.hq = q->size(1);
     p.rows = axes == 3 ? q->size(2) : 1;
     int64_t window, sinks;
-    if (p.hq < 1 || p.hq % c.hkv || p.rows < 1 || p.hq * p.rows > (1 << 30) || c.batch * p.hq * p.rows > (1 << 30) ||
+    if (p.hq < 1 || p.hq % c.hkv || p.rows < 1 || p.hq > (1 << 30) || p.rows > (1 << 30) ||
+        p.hq * p.rows > (1 << 30) || c.batch * p.hq * p.rows > (1 << 30) ||
         !row_strides(*q, axes, p.q_strides) || p.q_strides[2] > R2O_MAX_ROW_STRIDE ||
         !mask_args(Py_None, kZero, args[6], window, sinks, p.sm_scale) || !lengths_arg(args[4], f.batch, device, p.members) ||
         !lengths_arg(args[5], c.batch, device, p.query_lengths))

@@ -49,7 +49,7 @@ struct PrefixArgs {
     float *lse, *partial_out, *partial_ml;
     int* notes;  // for the join
     int64_t q_batch, q_head, o_batch, o_head;
-    int q_row, o_row, batch, prefixes, hkv, hq, group, rows, packed, workers, merged;  // packed: rows * group
+    int q_row, o_row, batch, prefixes, hkv, hq, group, rows, packed, workers;  // packed: rows * group
     float c2;  // scale, in log2 units
 };
 
@@ -276,7 +276,7 @@ __device__ __forceinline__ Sums sums_of(const Lane& first, const int* sums) {
 __device__ __forceinline__ Plan plan_of(const Sums& s) {
     Args& a = kernel_args();
     Plan p;
-    int n = __builtin_amdgcn_readfirstlane((int)(a.workers * (s.shared_cost / (s.shared_cost + kOwnCost * s.own)) + 0.5f));
+    int n = s.shared > 0 ? __builtin_amdgcn_readfirstlane((int)(a.workers * (s.shared_cost / (s.shared_cost + kOwnCost * s.own)) + 0.5f)) : 0;
     n = max(min(n, a.workers - (s.own > 0)), (int)(s.shared > 0));
     p.own_first = min(n, a.workers - 1);  // of one workgroup, which does both
     p.shared = share_of(s.shared, n);
@@ -1243,12 +1243,12 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
                     if (i0 + PARTS * k < count) join_state(s, m2[k], l2[k], o2[k]);
             }
         };
-        if (shared_tiles > 0) {
+        if (shared_tiles > 0 && shared.total > 0) {  // a list without units: lengths that changed meanwhile
             const int r = place - before + p, tile = r / kRows;
             add(shared, shared_base + (h * div_up(rows, kRows) + tile) * (shared_tiles + kSegment) + kSegment, shared_tiles,
                 whole_prefix_rows(a, before, rows, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
         }
-        if (own_tiles > 0) {
+        if (own_tiles > 0 && own.total > 0) {
             const int chunk = p / kWaveRows;
             add(own, own_base + (h * div_up(counted * a.group, kWaveRows) + chunk) * (own_tiles + kWaveSegment) + kWaveSegment, own_tiles,
                 whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(own_first, w, begins) + p - chunk * kWaveRows; });
@@ -1338,7 +1338,6 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     a.rows = (int)p->rows;
     a.packed = (int)packed;
     a.workers = (int)p->workers;
-    a.merged = merged;
     a.c2 = p->sm_scale * kLog2e;
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)p->workers);
