@@ -879,11 +879,11 @@ struct PrefixPlan {
 
 PrefixPlan prefix_plan(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t slots, int64_t prefixes, int64_t shared, bool some_count, int64_t cus) {
     const int64_t packed = hq / hkv * rows, all_rows = batch * hq * rows;
-    const bool merged = r2o_prefix_merged(prefixes > 0, packed, all_rows, shared, some_count);
+    const bool merged = r2o_prefix_merged(batch, prefixes, packed, all_rows, slots, shared, some_count);
     const int64_t units = r2o_prefix_units(merged, batch, hkv, packed, slots, prefixes, shared);
     if (units > 0x7fffffff - 8 * R2O_PAGED_MAX_WORKERS) return {0, 0};
     const int64_t workers = std::max<int64_t>(1, std::min(cus, units));
-    return {workers, r2o_prefix_scratch(workers, r2o_prefix_room(prefixes > 0, packed, all_rows), all_rows, batch)};
+    return {workers, r2o_prefix_scratch(workers, r2o_prefix_room(packed, all_rows), all_rows, batch)};
 }
 
 // paged_prefix_attention(function, query, cache, prefix or None, members, query_lengths, scale): (status, out, lse) or None

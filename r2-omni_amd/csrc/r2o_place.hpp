@@ -44,17 +44,34 @@ constexpr int64_t r2o_place_blocks(int64_t tiles, int64_t splits, int64_t batche
 
 // Whether the prefix attention may make one list of the rows of all requests of a prefix, and so needs room for their states.
 // packed: a request's rows of a KV head; all_rows: the call's.
-constexpr bool r2o_prefix_room(bool prefixes, int64_t packed, int64_t all_rows) {
-    return prefixes && packed < 512 && (packed < 128 || all_rows <= 1 << 18);
+constexpr bool r2o_prefix_room(int64_t packed, int64_t all_rows) { return packed < 512 && (packed < 128 || all_rows <= 1 << 18); }
+
+// A key tile of a row list, in microseconds of a compute unit: 256 rows are bound by their products, up to 128 by the loads.
+constexpr double r2o_prefix_tile_cost(int64_t rows) {
+    const int64_t left = rows % 256;
+    return 2.3 * (double)(rows / 256) + (left > 128 ? 2.3 : left > 0 ? 1.5 : 0.0);
 }
 
-// Whether it does.  Row tiles have 256 rows: a list wastes them once a prefix and not once a request, but leaves each row's state
-// to a join, which takes as long as some hundred slots of a prefix.  Measured, in us apart and in one list, heads 28 over 4, 16
-// requests of one prefix of 32641 slots: 168 rows a request 274 and 220, 252: 307 and 313, 280: 563 and 343, 448: 566 and 533, 511: 593 and
-// 607; query_lengths that count five eighths of them: 270 and 132, 275 and 193, 303 and 219, 443 and 327, 414 and 376; eights of
-// requests over 700 slots, heads 16 over 2, 288 rows: 45 and 53, 320: 44 and 58.
-constexpr bool r2o_prefix_merged(bool prefixes, int64_t packed, int64_t all_rows, int64_t slots, bool some_count) {
-    return r2o_prefix_room(prefixes, packed, all_rows) && (packed < 128 || (slots >= 2048 && (some_count || 4 * ((packed + 255) / 256 * 256 - packed) >= packed)));
+// Whether it does: one list wastes row tiles once a prefix and not once a request, but the requests' own slots then go through
+// single waves, 32 rows and keys at a time, and each row's state through a join.  What either costs, a request and head, by the
+// slots that the tables hold, for the lengths are on the device; with counts, as if they were a quarter to all of the rows.
+// Measured, in us apart and in one list, heads 28 over 4, 16 requests over 32000 slots and up to 2000 own: 7 rows a request and KV head
+// 170 and 39, 84: 195 and 139, 280: 565 and 387, 448: 566 and 594 (with counts 476 and 388); over 8000 and up to 8000 own 7: 93 and 59,
+// 56: 105 and 110, 126: 116 and 191, 280: 279 and 401; heads 16 over 2, eights of requests over 1000 and up to 1000 own 32: 41 and 35,
+// 64: 44 and 47, 192: 61 and 92.
+constexpr bool r2o_prefix_merged(int64_t batch, int64_t prefixes, int64_t packed, int64_t all_rows, int64_t slots, int64_t shared, bool some_count) {
+    if (!r2o_prefix_room(packed, all_rows)) return false;
+    const int64_t members = prefixes ? std::max<int64_t>(1, batch / prefixes) : 1, rows = some_count ? (5 * packed + 7) / 8 : packed, parts = some_count ? 4 : 1;
+    const double keys = prefixes ? (double)shared / 64 : 0.0, own = (double)slots / 64;
+    double tile = 0.0, chunks = 0.0;
+    for (int64_t i = 1; i <= parts; ++i) {
+        const int64_t r = (i * packed + parts - 1) / parts;
+        tile += r2o_prefix_tile_cost(r) / (double)parts;
+        chunks += (double)((r + 31) / 32) / (double)parts;
+    }
+    const double apart = (keys + own) * tile + 9.0 * (double)((rows + 255) / 256);
+    const double together = keys * r2o_prefix_tile_cost(rows * members) / (double)members + chunks * 2.0 * own * 0.6 + 0.25 * (double)rows;
+    return together < apart;
 }
 
 // What a segment's start and end cost beside its tiles, in tiles: of a workgroup about nine microseconds beside 2.3 a tile of 256

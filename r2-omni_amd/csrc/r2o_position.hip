@@ -36,7 +36,7 @@ __device__ __forceinline__ int64_t position_at(const r2o_rotation& r, int axis, 
 }
 
 // cos and sin of the lane's channels 8 c8 .. 8 c8 + 7, the sine with its channel's sign.  The angle in half turns, position *
-// (inv_freq / pi), loses its whole part in 64 bits (a position of 2^31 leaves it 2^-24 exact), the rest, at most 1/2, goes to
+// (inv_freq / pi), loses its whole part in 64 bits (a position of 2^31 leaves 2^-22 of one), the rest, at most 1/2, goes to
 // the hardware's sine and cosine, which take turns and are off by at most 1.2e-7 (2^-23; looked at for 2^24 arguments).  Polynomials
 // instead took 15.3 us where this takes 14.1 (4 padded requests of 1037 rows, 16 + 2 heads).
 __device__ __forceinline__ void angles(const r2o_rotation& r, int64_t b, int64_t token, int64_t slot, int c8, float (&c)[8], float (&s)[8]) {

@@ -1161,40 +1161,71 @@ __device__ __forceinline__ void write_row(Args& a, const State& s, int b, int he
     if (d4 == 0) a.lse[((int64_t)b * a.hq + head) * a.rows + row] = live ? (s.m + __builtin_amdgcn_logf(s.l)) * kLn2 : -INFINITY;
 }
 
-// Rows that are not merged.  Workgroups (w, .) join the segment that worker w + 1 is the second to work on, 32 lanes a row;
-// those behind the workers' write the rows that their requests do not count.
-constexpr int kJoinRows = 32;
+// Rows that are not merged.  Workgroups (w, .) join the segment that worker w + 1 is the second to work on, eight rows each; those
+// behind the workers' write the rows that their requests do not count.  A row's states are added by 32 lanes where they are few;
+// where they are more the eight groups of 32 lanes share them, for all eight rows at a time: one request of 126 rows over 32000 slots,
+// 64 states a row, takes 42 us so and 72 by 32 lanes a row.
+constexpr int kJoinRows = 8, kFewStates = 4;
 
 template <int RF>
 __global__ __launch_bounds__(256) void prefix_join_split_kernel(PrefixArgs) {
+    __shared__ __align__(16) float red[8][kJoinRows][128];
+    __shared__ float red_ml[8][kJoinRows][2];
     Args& a = kernel_args();
-    const int d4 = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
+    const int d4 = threadIdx.x & 31, part = threadIdx.x >> 5, r0 = blockIdx.y * kJoinRows;
     if ((int)blockIdx.x >= a.workers - 1) {
         const int b = (int)blockIdx.x - (a.workers - 1), counted = counted_rows(load_uniform(a.query_lengths + b)), each = a.rows - counted;
         const int64_t rows = (int64_t)a.hq * each;
-        for (int64_t i0 = r0; i0 < rows; i0 += gridDim.y * kJoinRows)
-#pragma unroll 1
-            for (int64_t i = i0; i < min(rows, i0 + kJoinRows); i += 8) {
-                const int head = (int)(i / each), row = counted + (int)(i - (int64_t)head * each);
-                write_row<RF>(a, State{-INFINITY, 0.f, r2o_f4{}}, b, head, row, d4);
-            }
+        for (int64_t i = r0 + part; i < rows; i += gridDim.y * kJoinRows) {
+            const int head = (int)(i / each), row = counted + (int)(i - (int64_t)head * each);
+            write_row<RF>(a, State{-INFINITY, 0.f, r2o_f4{}}, b, head, row, d4);
+        }
         return;
     }
     const int w = (int)blockIdx.x + 1;
     const int* note = a.notes + kNote * w;
     const int request = load_uniform(note), head = load_uniform(note + 1), row0 = load_uniform(note + 2), rows = load_uniform(note + 3), count = load_uniform(note + 4);
-    if (request < 0) return;
-#pragma unroll
-    for (int k = 0; k < kJoinRows; k += 8) {
-        const int r = r0 + k;
-        if (r >= min(kRows, rows - row0)) break;
-        State x{-INFINITY, 0.f, r2o_f4{}};
-        join_partial(a, x, split_rows(w - 1, true) + r, d4);
+    const int here = min(kJoinRows, min(kRows, rows - row0) - r0);
+    if (request < 0 || here <= 0) return;
+    auto states_at = [&](int i) { return (i == 0 ? split_rows(w - 1, true) : split_rows(w - 1 + i, false)) + r0; };
+    State x{-INFINITY, 0.f, r2o_f4{}};
+    if (count <= kFewStates) {
+        if (part >= here) return;
 #pragma unroll 4
-        for (int i = 1; i < count; ++i) join_partial(a, x, split_rows(w - 1 + i, false) + r, d4);
-        const int p = row0 + r, row = p / a.group;
-        write_row<RF>(a, x, request, head * a.group + p - row * a.group, row, d4);
+        for (int i = 0; i < count; ++i) join_partial(a, x, states_at(i) + part, d4);
+    } else {
+        State s[kJoinRows];
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k) s[k] = x;
+        for (int i = part; i < count; i += 8) {
+            const uint32_t at0 = states_at(i);
+            float m2[kJoinRows], l2[kJoinRows];
+            r2o_f4 o2[kJoinRows];
+#pragma unroll
+            for (int k = 0; k < kJoinRows; ++k) {
+                const int64_t at = at0 + min(k, here - 1);
+                m2[k] = r2o_ldg(a.partial_ml + 2 * at);
+                l2[k] = r2o_ldg(a.partial_ml + 2 * at + 1);
+                o2[k] = r2o_ldg(reinterpret_cast<const r2o_f4*>(a.partial_out + at * 128) + d4);
+            }
+#pragma unroll
+            for (int k = 0; k < kJoinRows; ++k) join_state(s[k], m2[k], l2[k], o2[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k) {
+            *reinterpret_cast<r2o_f4*>(&red[part][k][4 * d4]) = s[k].o;
+            if (d4 == 0) {
+                red_ml[part][k][0] = s[k].m;
+                red_ml[part][k][1] = s[k].l;
+            }
+        }
+        __syncthreads();
+        if (part >= here) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) join_state(x, red_ml[i][part][0], red_ml[i][part][1], *reinterpret_cast<const r2o_f4*>(&red[i][part][4 * d4]));
     }
+    const int p = row0 + r0 + part, row = p / a.group;
+    write_row<RF>(a, x, request, head * a.group + p - row * a.group, row, d4);
 }
 
 // Rows of a call from which on 128 lanes join a row, and 32: fewer rows have the states of more workgroups each.  A whole call of 32
@@ -1308,10 +1339,11 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     const int64_t all_rows = c.batch * c.hkv * packed;
     if (all_rows > (1 << 30)) return R2O_EINVAL;
     const int64_t shared = any ? f.max_pages * f.page_size : 0;
-    const bool room = r2o_prefix_room(any, packed, all_rows), merged = r2o_prefix_merged(any, packed, all_rows, shared, p->query_lengths);
+    const int64_t slots = c.max_pages * c.page_size;
+    const bool room = r2o_prefix_room(packed, all_rows), merged = r2o_prefix_merged(c.batch, f.batch, packed, all_rows, slots, shared, p->query_lengths);
     if (p->scratch_floats < r2o_prefix_scratch(p->workers, room, all_rows, c.batch)) return R2O_EINVAL;
     const int64_t states = r2o_prefix_states(p->workers, room, all_rows);
-    if (r2o_prefix_units(merged, c.batch, c.hkv, packed, c.max_pages * c.page_size, f.batch, shared) > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS)
+    if (r2o_prefix_units(merged, c.batch, c.hkv, packed, slots, f.batch, shared) > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS)
         return R2O_EINVAL;
     PrefixArgs a{};
     a.own = source_of(c);

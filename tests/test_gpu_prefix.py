@@ -74,7 +74,7 @@ def test_padded_batches(rows):
 
 # the counted rows of a prefix's requests stand side by side: none, one, all, runs without any, more requests than a wave
 @pytest.mark.parametrize("hq,hkv", [(14, 2), (4, 4), (28, 1)])
-@pytest.mark.parametrize("rows", [1, 2, 7, 18])
+@pytest.mark.parametrize("rows", [1, 2, 7, 14, 18])
 def test_ragged_batches_of_some_prefixes(rows, hq, hkv):
     dev = _cuda()
     gen = torch.Generator().manual_seed(rows)
@@ -83,7 +83,7 @@ def test_ragged_batches_of_some_prefixes(rows, hq, hkv):
     counts[20:40] = 0
     counts[64:70] = rows
     lengths = torch.randint(0, 60, (batch,), generator=gen).tolist()
-    shared, own = _both(dev, (200, 2100, 0, 77), lengths, hkv, 16, BF16, rows)
+    shared, own = _both(dev, (200, 8000, 0, 77), lengths, hkv, 16, BF16, rows)
     q = _query(dev, batch, hq, rows, BF16, 27)
     for members in ((30, 8, 2, 100), (150, 0, 0, 0), (0, 19, 3, 41)):
         check(q, own, shared, _ints(dev, *members), _ints(dev, *counts.tolist()))
@@ -125,6 +125,16 @@ def test_without_a_prefix(rows):
     own = _cache(dev, (1000, 64, 41, 300), 2, 64, FP16, rows)
     check(_query(dev, 4, 14, rows, FP16, 8), own)
     check(_query(dev, 4, 14, rows, FP16, 8), own, query_lengths=_ints(dev, 1, 0, rows, rows))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 18, 37, 130])
+def test_one_long_request(rows):
+    """Its slots are shared by all workgroups: each row has the states of many."""
+    dev = _cuda()
+    own = _cache(dev, (20_001,), 2, 32, BF16, rows)
+    q = _query(dev, 1, 14, rows, BF16, 28)
+    check(q, own)
+    check(q, own, query_lengths=_ints(dev, max(1, rows - 9)))
 
 
 @pytest.mark.parametrize("rows", [1, 70])
@@ -191,7 +201,7 @@ def test_scales(scale, rows):
 
 
 @pytest.mark.parametrize("workers", [1, 2, 3, 7, 50, 512, 4096])
-@pytest.mark.parametrize("rows,prefix", [(1, 700), (40, 700), (40, 2100), (80, 700)])
+@pytest.mark.parametrize("rows,prefix", [(1, 700), (40, 700), (40, 20000), (80, 700)])
 def test_any_number_of_workers(rows, prefix, workers):
     """Each within the 64-bit bound: the joins add partial results of other cuts.  Rows of the scratch that a call has no
     right to stay as they were."""

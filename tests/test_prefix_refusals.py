@@ -120,7 +120,7 @@ def test_the_plan_of_a_call(batch, hkv, hq, rows, slots, prefixes, shared, count
     plan = _lib.host().prefix_plan(batch, hkv, hq, rows, slots, prefixes, shared, counted, 256)
     assert 1 <= plan[0] <= 256
     packed, total = hq // hkv * rows, batch * hq * rows
-    room = prefixes and (packed < 128 or (packed < 512 and total <= 1 << 18))
+    room = packed < 128 or (packed < 512 and total <= 1 << 18)
     assert plan[1] == 130 * (512 * plan[0] + (2 * total if room else 0)) + 8 * (1 + max(batch, plan[0]))
     bad = _attention(cache=_plain(batch=batch, hkv=hkv, max_pages=slots // 16 or 1, table_stride=slots // 16 or 1),
                      prefix=_plain(batch=prefixes, hkv=hkv, max_pages=max(1, shared // 16), table_stride=max(1, shared // 16)), members=0x16000, hq=hq,
