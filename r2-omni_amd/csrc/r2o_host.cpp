@@ -808,6 +808,11 @@ bool heads_arg(const at::Tensor* t, int64_t device, int64_t* strides) {
            row_code(*t) >= 0 && !needs_grad(*t) && row_strides(*t, 3, strides) && strides[2] <= R2O_MAX_ROW_STRIDE;
 }
 
+// What empty_like gives, without its look at strides where they are not kept anyhow: rows in order, or views of a fused projection.
+at::Tensor result_like(const at::Tensor& t) {
+    return t.is_contiguous() || !t.is_non_overlapping_and_dense() ? at::empty(t.sizes(), t.options()) : at::empty_like(t);
+}
+
 // position_rope(function, query, key, positions, rotary, hadamard): (status, query, key) or None
 PyObject* position_rope_call(PyObject* const* args) {
     r2o_position_rope_params p{};
@@ -826,7 +831,7 @@ PyObject* position_rope_call(PyObject* const* args) {
     if (!rotary.read(args[4], (int)p.dtype, device) || !rotary.place(args[3], p.batch, p.tokens, device) || p.batch * p.tokens > 0x7fffffff)
         Py_RETURN_NONE;
     p.rotation = rotary.r;
-    at::Tensor q_out = at::empty_like(*q), k_out = at::empty_like(*k);
+    at::Tensor q_out = result_like(*q), k_out = result_like(*k);
     if (!row_strides(q_out, 3, p.qo_strides, true) || !row_strides(k_out, 3, p.ko_strides, true)) Py_RETURN_NONE;
     p.query = static_cast<const uint16_t*>(q->data_ptr());
     p.key = static_cast<const uint16_t*>(k->data_ptr());
@@ -862,7 +867,7 @@ PyObject* paged_rope_extend_call(PyObject* const* args) {
     Rotary rotary;
     if (!rotary.read(args[5], (int)c.dtype, device) || (args[6] != Py_None && !rotary.place(args[6], c.batch, p.rows, device))) Py_RETURN_NONE;
     p.rotation = rotary.r;
-    at::Tensor q_out = at::empty_like(*q);
+    at::Tensor q_out = result_like(*q);
     if (!row_strides(q_out, 3, p.qo_strides, true)) Py_RETURN_NONE;
     p.query = static_cast<const uint16_t*>(q->data_ptr());
     p.key = static_cast<const uint16_t*>(k->data_ptr());
@@ -915,7 +920,7 @@ PyObject* paged_prefix_attention_call(PyObject* const* args) {
     const PrefixPlan plan = prefix_plan(c.batch, c.hkv, p.hq, p.rows, c.max_pages * c.page_size, f.batch, f.max_pages * f.page_size,
                                         p.query_lengths != nullptr, compute_units((int)device));
     if (!plan.workers) Py_RETURN_NONE;
-    at::Tensor out = at::empty_like(*q);
+    at::Tensor out = result_like(*q);
     if (!row_strides(out, axes, p.o_strides, true) || p.o_strides[2] > R2O_MAX_ROW_STRIDE) Py_RETURN_NONE;
     p.workers = plan.workers;
     p.scratch_floats = plan.scratch;
