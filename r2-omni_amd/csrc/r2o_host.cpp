@@ -884,7 +884,7 @@ struct PrefixPlan {
 
 PrefixPlan prefix_plan(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int64_t slots, int64_t prefixes, int64_t shared, bool some_count, int64_t cus) {
     const int64_t packed = hq / hkv * rows, all_rows = batch * hq * rows;
-    const bool merged = r2o_prefix_merged(batch, prefixes, packed, all_rows, slots, shared, some_count);
+    const bool merged = r2o_prefix_merged(batch, prefixes, packed, all_rows, shared, some_count);
     const int64_t units = r2o_prefix_units(merged, batch, hkv, packed, slots, prefixes, shared);
     if (units > 0x7fffffff - 8 * R2O_PAGED_MAX_WORKERS) return {0, 0};
     const int64_t workers = std::max<int64_t>(1, std::min(cus, units));

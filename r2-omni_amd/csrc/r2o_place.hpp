@@ -52,26 +52,21 @@ constexpr double r2o_prefix_tile_cost(int64_t rows) {
     return 2.3 * (double)(rows / 256) + (left > 128 ? 2.3 : left > 0 ? 1.5 : 0.0);
 }
 
-// Whether it does: one list wastes row tiles once a prefix and not once a request, but the requests' own slots then go through
-// single waves, 32 rows and keys at a time, and each row's state through a join.  What either costs, a request and head, by the
-// slots that the tables hold, for the lengths are on the device; with counts, as if they were a quarter to all of the rows.
-// Measured, in us apart and in one list, heads 28 over 4, 16 requests over 32000 slots and up to 2000 own: 7 rows a request and KV head
-// 170 and 39, 84: 195 and 139, 280: 565 and 387, 448: 566 and 594 (with counts 476 and 388); over 8000 and up to 8000 own 7: 93 and 59,
-// 56: 105 and 110, 126: 116 and 191, 280: 279 and 401; heads 16 over 2, eights of requests over 1000 and up to 1000 own 32: 41 and 35,
-// 64: 44 and 47, 192: 61 and 92.
-constexpr bool r2o_prefix_merged(int64_t batch, int64_t prefixes, int64_t packed, int64_t all_rows, int64_t slots, int64_t shared, bool some_count) {
+// Whether it does: one list of a prefix's rows wastes row tiles once a prefix and not once a request, but leaves each row's state to a
+// join.  Priced, in microseconds of a compute unit a request and head, by the prefixes' slots that the tables hold, for the lengths are
+// on the device; with counts, as if they were a quarter to all of the rows.  Measured, in us apart and in one list, heads 28 over 4, 16
+// requests over 32000 slots and 2000 own: 7 rows a request and KV head 171 and 39, 84: 193 and 134, 280: 589 and 370, 448: 592 and 554;
+// over 8000 and 8000 own 7: 95 and 58, 56: 103 and 84, 280: 288 and 237; 64 requests over 2100 and 2000 own 84: 102 and 95, 126: 107 and
+// 124, 280: 244 and 261.  Without a prefix one list wins by its join: one request of 126 rows over 32000 slots 42 and 33, 16 over 8000 71
+// and 69; but for 25 to 32 rows, which single waves take: 16 over 500 17 and 20.
+constexpr bool r2o_prefix_merged(int64_t batch, int64_t prefixes, int64_t packed, int64_t all_rows, int64_t shared, bool some_count) {
     if (!r2o_prefix_room(packed, all_rows)) return false;
-    const int64_t members = prefixes ? std::max<int64_t>(1, batch / prefixes) : 1, rows = some_count ? (5 * packed + 7) / 8 : packed, parts = some_count ? 4 : 1;
-    const double keys = prefixes ? (double)shared / 64 : 0.0, own = (double)slots / 64;
-    double tile = 0.0, chunks = 0.0;
-    for (int64_t i = 1; i <= parts; ++i) {
-        const int64_t r = (i * packed + parts - 1) / parts;
-        tile += r2o_prefix_tile_cost(r) / (double)parts;
-        chunks += (double)((r + 31) / 32) / (double)parts;
-    }
-    const double apart = (keys + own) * tile + 9.0 * (double)((rows + 255) / 256);
-    const double together = keys * r2o_prefix_tile_cost(rows * members) / (double)members + chunks * 2.0 * own * 0.6 + 0.25 * (double)rows;
-    return together < apart;
+    if (!prefixes) return packed <= 24 || packed > 32;
+    if (packed <= 32) return true;
+    const int64_t members = std::max<int64_t>(1, batch / prefixes), rows = some_count ? (5 * packed + 7) / 8 : packed, parts = some_count ? 4 : 1;
+    double tile = 0.0;
+    for (int64_t i = 1; i <= parts; ++i) tile += r2o_prefix_tile_cost((i * packed + parts - 1) / parts) / (double)parts;
+    return (double)shared / 64 * (tile - r2o_prefix_tile_cost(rows * members) / (double)members) > 0.2 * (double)rows;
 }
 
 // What a segment's start and end cost beside its tiles, in tiles: of a workgroup about nine microseconds beside 2.3 a tile of 256

@@ -7,8 +7,7 @@
 // tiles of 256: a wave's 32 rows are one operand of its products, eight waves share a key tile in LDS, and the prefix's rows are
 // read once for all of them.  The (row tile, key tile) pairs of a call are one list too, shared evenly over the workgroups,
 // whatever the lengths; where a row tile's keys fall to several, or to a prefix and a request of its own, each leaves (maximum,
-// sum, products) in scratch for the join.  Beside them, where rows are merged, the requests' own slots: few rows each, no row in
-// common, so single waves take them.
+// sum, products) in scratch for the join.  Beside them, where rows are merged, the requests' own slots, which no two share.
 //
 // What bounds it: a tile of 256 rows and 64 keys takes 2.3 to 2.7 us (790 to 930 TFLOP/s; a large library product of these types
 // reaches 1220), 2.06 without its loads: exponentials beside products.  One of up to 128 rows takes 1.55, the rows' bytes at 5.3
@@ -90,9 +89,12 @@ __device__ __forceinline__ int filled(SourceArgs& s, int length) { return min(ma
 
 // ------------------------------------------------------------------------------------- the work
 // Where rows are merged there are two lists: the prefixes' (with the rows of all their requests), whose row tiles workgroups
-// take as a whole, and the requests' own slots, of few rows each, which waves take by themselves: a workgroup's eight have
-// eight requests' latencies under way at a time.  Otherwise there is one list, of the requests, a prefix's slots before the own
-// ones.  The wave goes through prefixes and requests 64 at a time, one a lane; what the first 64 hold is loaded at once and kept.
+// take as a whole, and the requests' own slots.  Those go to single waves, 32 rows and 32 keys at a time, where that costs less: a
+// workgroup's eight have eight requests' latencies under way; or to workgroups in row tiles too.  Otherwise there is one list, of the
+// requests, a prefix's slots before the own ones.  The wave goes through prefixes and requests 64 at a time, one a lane; what the
+// first 64 hold is loaded at once and kept.
+enum List { kPrefixes, kOwn, kRequests };  // whose row tiles a workgroup works on
+
 struct Lane {
     int members, shared, own, rows;  // as the tensors have them: a prefix's, a request's
 };
@@ -163,6 +165,13 @@ __device__ __forceinline__ int own_work(const Lane& x, int b0) {
     return b < a.batch ? units(a.hkv * div_up(counted_rows(x.rows) * a.group, kWaveRows), div_up(filled(a.own, x.own), kWaveKeys), kWaveSegment) : 0;
 }
 
+// The same in row tiles and key tiles of workgroups.
+__device__ __forceinline__ int own_row_work(const Lane& x, int b0) {
+    Args& a = kernel_args();
+    const int b = b0 + (threadIdx.x & 63);
+    return b < a.batch ? units(a.hkv * div_up(counted_rows(x.rows) * a.group, kRows), div_up(filled(a.own, x.own), kTile), kSegment) : 0;
+}
+
 // The prefix of this lane's request, -1 for none, its requests and its length: one step a prefix.
 __device__ __forceinline__ int prefix_of(const Lane& first, int b, Members& members, int& length) {
     Args& a = kernel_args();
@@ -221,19 +230,22 @@ __device__ __forceinline__ Share share_of(int total, int workers) {
 // Both lists of merged rows.  Workgroups 0 .. n - 1 take the prefixes', those from `own_first` on the requests', their number by
 // what the lists cost.
 struct Plan {
-    Share shared, own;  // own: waves
-    int own_first;
+    Share shared, own;  // own: waves, or workgroups
+    int own_first, by_tiles;
 };
 
-// What this lane's prefix costs, in microseconds of a compute unit: a tile of 256 rows is bound by its products, one of up to
-// 128 by its loads; a request's unit takes 0.6.
+// What a list's entry costs, in microseconds of a compute unit: a tile of 256 rows is bound by its products, one of up to 128 by its
+// loads; a unit of one wave among eight takes 0.6.  A request's own slots go to waves or to workgroups by these costs: 16 requests of
+// 126 rows and 8000 own slots, heads 28 over 4, take 173 us by waves and 71 by workgroups; of 28 rows 59 by either, of 7: 50 and 56.
 constexpr float kOwnCost = 0.6f;
-__device__ __forceinline__ float prefix_cost(const Lane& x, int rows) {
+__device__ __forceinline__ float tiles_cost(int rows, int keys) {
     Args& a = kernel_args();
-    const int keys = div_up(filled(a.shared, x.shared), kTile), left = rows % kRows;
+    const int left = rows % kRows;
     const float tile = 2.3f * (rows / kRows) + (left > kRows / 2 ? 2.3f : (left ? 1.5f : 0.f));
     return keys ? a.hkv * (keys * tile + 9.f * div_up(rows, kRows)) : 0.f;
 }
+
+__device__ __forceinline__ float prefix_cost(const Lane& x, int rows) { return tiles_cost(rows, div_up(filled(kernel_args().shared, x.shared), kTile)); }
 
 __device__ __forceinline__ float wave_total(float x) {
     x += r2o_lane_xor<1>(x);
@@ -253,8 +265,8 @@ struct Entry {
 
 // The units of the lists of merged rows.
 struct Sums {
-    int shared, own;
-    float shared_cost;
+    int shared, own, own_tiles;  // own_tiles: as row tiles; 0 where waves have all rows of a request
+    float shared_cost, tiles_cost;
 };
 
 __device__ __forceinline__ Sums sums_of(const Lane& first, const int* sums) {
@@ -269,18 +281,29 @@ __device__ __forceinline__ Sums sums_of(const Lane& first, const int* sums) {
         s.shared_cost += wave_total(prefix_cost(x, rows));
     }
 #pragma unroll 1
-    for (int b0 = 0; b0 < a.batch; b0 += 64) s.own += last_lane(wave_scan(own_work(lane_at(first, b0), b0)));
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const Lane x = lane_at(first, b0);
+        s.own += last_lane(wave_scan(own_work(x, b0)));
+        if (a.packed > kWaveRows) {
+            const int work = own_row_work(x, b0);
+            s.own_tiles += last_lane(wave_scan(work));
+            s.tiles_cost += wave_total(work ? tiles_cost(counted_rows(x.rows) * a.group, div_up(filled(a.own, x.own), kTile)) : 0.f);
+        }
+    }
     return s;
 }
 
 __device__ __forceinline__ Plan plan_of(const Sums& s) {
     Args& a = kernel_args();
     Plan p;
-    int n = s.shared > 0 ? __builtin_amdgcn_readfirstlane((int)(a.workers * (s.shared_cost / (s.shared_cost + kOwnCost * s.own)) + 0.5f)) : 0;
+    const float waves = kOwnCost * s.own;
+    p.by_tiles = __builtin_amdgcn_readfirstlane(s.own_tiles > 0 && s.tiles_cost < 1.25f * waves);  // waves' last ones end unevenly
+    const float own = p.by_tiles ? s.tiles_cost : waves;
+    int n = s.shared > 0 ? __builtin_amdgcn_readfirstlane((int)(a.workers * (s.shared_cost / (s.shared_cost + own)) + 0.5f)) : 0;
     n = max(min(n, a.workers - (s.own > 0)), (int)(s.shared > 0));
     p.own_first = min(n, a.workers - 1);  // of one workgroup, which does both
     p.shared = share_of(s.shared, n);
-    p.own = share_of(s.own, kWaves * (a.workers - p.own_first));
+    p.own = p.by_tiles ? share_of(s.own_tiles, a.workers - p.own_first) : share_of(s.own, kWaves * (a.workers - p.own_first));
     return p;
 }
 
@@ -300,12 +323,13 @@ __device__ __forceinline__ void write_notes(const Lane& first, const int* sums, 
         to[4] = plan.own.total;
         to[5] = plan.own.each;
         to[6] = plan.own.more;
+        to[7] = plan.by_tiles;
     }
     int own = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Lane x = lane_at(first, b0);
-        const int b = b0 + lane, work = own_work(x, b0), upto = wave_scan(work);
+        const int b = b0 + lane, work = plan.by_tiles ? own_row_work(x, b0) : own_work(x, b0), upto = wave_scan(work);
         Members members;
         int length, shared = 0, before = 0;
         const int of = prefix_of(first, b, members, length);
@@ -325,7 +349,7 @@ __device__ __forceinline__ void write_notes(const Lane& first, const int* sums, 
             to[2] = rows_before(sums, members.first) * a.group;
             to[3] = member_rows(sums, members);
             to[4] = own + upto - work;
-            to[5] = div_up(filled(a.own, x.own), kWaveKeys);
+            to[5] = div_up(filled(a.own, x.own), plan.by_tiles ? kTile : kWaveKeys);
             to[6] = counted_rows(x.rows);
             to[7] = rows_before(sums, b) * a.group;
         }
@@ -360,7 +384,8 @@ __device__ __forceinline__ Entry find_prefix(const Lane& first, const int* sums,
     return e;
 }
 
-// Merged rows: the request that holds tile u of the requests' list.
+// Merged rows: the request that holds unit u of the requests' list, of waves or of workgroups (rows: of all query heads of a KV head).
+template <bool TILES>
 __device__ __forceinline__ Entry find_own(const Lane& first, int u) {
     Args& a = kernel_args();
     Entry e{};
@@ -370,13 +395,13 @@ __device__ __forceinline__ Entry find_own(const Lane& first, int u) {
 #pragma unroll 1
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const Lane x = lane_at(first, b0);
-        const int work = own_work(x, b0), upto = wave_scan(work), all = last_lane(upto);
+        const int work = TILES ? own_row_work(x, b0) : own_work(x, b0), upto = wave_scan(work), all = last_lane(upto);
         if ((uint32_t)(u - at) < (uint32_t)all) {
             const int i = __builtin_ctzll(__ballot(at + upto > u));
             e.base = at + __builtin_amdgcn_readlane(upto - work, i);
             e.request = b0 + i;
             e.n_own = filled(a.own, __builtin_amdgcn_readlane(x.own, i));
-            e.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, i));
+            e.rows = counted_rows(__builtin_amdgcn_readlane(x.rows, i)) * (TILES ? a.group : 1);
         }
         at += all;
     }
@@ -703,14 +728,14 @@ __device__ __forceinline__ void lds_barrier() {  // of LDS alone: stores to memo
 // A workgroup's part of a list of row tiles, its own slots behind a prefix's where rows are not merged.  S^T = K Q^T (32 keys x 32
 // rows a product), O^T += V^T P^T; three tiles ahead go into LDS while one is computed on.  A tile is two halves of 32 keys: the
 // products of the half that follows run beside the exponentials of the one before it.
-template <int RF, bool MERGED>
+template <int RF, List LIST>
 __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const int* sums, const Lane& first, int u, int u_end) {
     while (u < u_end) {
         Args& a = kernel_args();
         int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), worker = blockIdx.x;
         asm("" : "+v"(lane), "+s"(wave), "+s"(worker));  // or what depends on them alone would be held from one segment to the next
         int total;
-        const Entry e = MERGED ? find_prefix(first, sums, u) : find_request(first, u, total);
+        const Entry e = LIST == kPrefixes ? find_prefix(first, sums, u) : LIST == kOwn ? find_own<true>(first, u) : find_request(first, u, total);
         if (e.request == -2) return;  // lengths that change meanwhile
         const Segment s = segment_of(e, u);
         const int begin = max(0, u - s.base), stop = min(s.tiles, u_end - s.base);
@@ -722,7 +747,7 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const in
         const int at = min(s.row0 + in_tile, e.rows - 1), group = a.group;
         int row = at / group, b = e.request;
         const int head = s.head * group + at - row * group;
-        if constexpr (MERGED) {  // the request that row `row` of the prefix's is of, and which of its rows that is
+        if constexpr (LIST == kPrefixes) {  // the request that row `row` of the prefix's is of, and which of its rows that is
             if (a.query_lengths) {
                 row += e.before / group;
                 b = e.first;
@@ -738,33 +763,35 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const in
         uint32_t to = kNoRow;
         if (s.row0 + in_tile < e.rows && part == 0) {
             if (begin > 0 || stop < s.tiles) to = split_rows(worker, begin == 0) + in_tile;
-            else if (MERGED) to = whole_prefix_rows(a, e.before, e.rows, s.head) + s.row0 + in_tile;
+            else if (LIST == kPrefixes) to = whole_prefix_rows(a, e.before, e.rows, s.head) + s.row0 + in_tile;
+            else if (LIST == kOwn) to = whole_own_rows(a, e.request, s.head) + s.row0 + in_tile;
             else to = kResult;
         }
         Rows w;
         start_rows(w, a.query + (int64_t)b * a.q_batch + (int64_t)head * a.q_head + (int64_t)row * a.q_row + 8 * (lane >> 5));
         int counted = a.rows;
-        if (!MERGED && a.query_lengths) counted = counted_rows(r2o_ldg(a.query_lengths + b));
+        if (LIST != kPrefixes && a.query_lengths) counted = counted_rows(r2o_ldg(a.query_lengths + b));
         const int see_own = min(e.n_own - counted + row, e.n_own - 1);
         // the least and the most that a row of the workgroup sees of them; no row of a prefix's segment has any
         const int base_row = e.n_own - __builtin_amdgcn_readfirstlane(counted);
-        const int least = MERGED ? 0 : min(base_row + s.row0 / group, e.n_own - 1);
-        const int most = MERGED ? -1 : min(base_row + min(s.row0 + kRows - 1, e.rows - 1) / group, e.n_own - 1);
+        const int least = LIST == kPrefixes ? 0 : min(base_row + s.row0 / group, e.n_own - 1);
+        const int most = LIST == kPrefixes ? -1 : min(base_row + min(s.row0 + kRows - 1, e.rows - 1) / group, e.n_own - 1);
         const int last = min(stop, s.shared + (most >= 0 ? most / kTile + 1 : 0));  // tiles behind it are seen by no row
         const float c2 = a.c2;
         bool bad = false;
 
+        auto of_prefix = [&](int it) { return LIST == kPrefixes || (LIST == kRequests && it < s.shared); };
         auto side_at = [&](int it) {
             Args& x = kernel_args();
-            return MERGED || it < s.shared ? side_of(x.shared, e.prefix, s.head, e.n_shared) : side_of(x.own, e.request, s.head, e.n_own);
+            return of_prefix(it) ? side_of(x.shared, e.prefix, s.head, e.n_shared) : side_of(x.own, e.request, s.head, e.n_own);
         };
-        auto slot_of = [&](int it) { return (MERGED || it < s.shared ? it : it - s.shared) * kTile; };
-        auto last_seen = [&](int it) { return MERGED || it < s.shared ? e.n_shared - 1 : see_own; };
+        auto slot_of = [&](int it) { return (LIST != kRequests || it < s.shared ? it : it - s.shared) * kTile; };
+        auto last_seen = [&](int it) { return of_prefix(it) ? e.n_shared - 1 : see_own; };
         // The side and the pages of the next tile to be staged, and its buffers.
         Side side = side_at(begin);
         auto window_at = [&](int it) {
             Args& x = kernel_args();
-            return window_of(MERGED || it < s.shared ? x.shared : x.own, side.table, slot_of(it) >> side.shift, lane);
+            return window_of(of_prefix(it) ? x.shared : x.own, side.table, slot_of(it) >> side.shift, lane);
         };
         Window window = window_at(begin);
         unsigned v_at = kKeyTiles;
@@ -775,7 +802,7 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const in
         // which of the tile's four groups of 16 slots count.
         auto stage = [&](int it) {
             const int j0 = slot_of(it);
-            if (!MERGED && it == s.shared && it > begin) {
+            if (LIST == kRequests && it == s.shared && it > begin) {
                 side = side_at(it);
                 window = window_at(it);
             } else if ((j0 >> side.shift) - window.first > 63) {
@@ -797,8 +824,8 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const in
         // This wave's eight value rows of a staged tile.  Rows that no row of the workgroup sees may hold anything: zero.  Where some
         // see a row that others do not, 0 times an infinite or NaN value would be NaN: those become zero before any product.
         auto clean = [&](int it, int v_buffer, int valid) {
-            const int n = MERGED || it < s.shared ? e.n_shared : e.n_own, j0 = slot_of(it);
-            const bool some = !MERGED && it >= s.shared && j0 + kTile - 1 > least && least < n - 1;
+            const int n = of_prefix(it) ? e.n_shared : e.n_own, j0 = slot_of(it);
+            const bool some = !of_prefix(it) && j0 + kTile - 1 > least && least < n - 1;
             if (valid == 15 && j0 + kTile <= n && !some) return;  // the same for all waves
             r2o_u4* at_lds = reinterpret_cast<r2o_u4*>(lds[v_buffer] + 8 * wave * 256) + lane;
             r2o_u4 x[2];
@@ -920,13 +947,13 @@ __device__ __forceinline__ void work_on_row_tiles(Lds& lds, int* flags, const in
                 f16v extra = f16v{};
 #pragma unroll 1
                 for (int from = begin, to_tile; from < last; from = to_tile) {  // the prefix's, then its own
-                    to_tile = MERGED || from >= s.shared ? last : min(last, s.shared);
+                    to_tile = LIST != kRequests || from >= s.shared ? last : min(last, s.shared);
                     add_not_finite<RF>(extra, db, side_at(from), slot_of(from), slot_of(from) + (to_tile - from) * kTile, last_seen(from), counts, lane);
                 }
                 take_not_finite(w.acc[db], extra);
             }
         }
-        if (!MERGED && to == kResult) {
+        if (LIST == kRequests && to == kResult) {
             Args& x = kernel_args();
             const bool live = counts && !(w.l == 0.f);  // no key seen; NaN logits leave m, and a NaN sum
             const float inv = live ? 1.f / w.l : 0.f;
@@ -958,7 +985,7 @@ __device__ __forceinline__ void work_on_own(Lds& lds, const Lane& first, int own
         Args& a = kernel_args();
         int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         asm("" : "+v"(lane), "+s"(wave));
-        const Entry e = find_own(first, u);
+        const Entry e = find_own<false>(first, u);
         if (e.request == -2) return;  // lengths that change meanwhile
         const Segment s = segment_at(e, u, div_up(e.n_own, kWaveKeys), kWaveSegment, div_up(e.rows * a.group, kWaveRows), kWaveRows);
         const int begin = max(0, u - s.base), stop = min(s.tiles, u_end - s.base);
@@ -1071,7 +1098,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
     const Lane first = lane_of(0);
     int u = 0, u_end = 0;
     if constexpr (MERGED) {
-        int own_first, index, v = 0, v_end = 0;
+        int own_first, by_tiles, index, v = 0, v_end = 0;
         if (a.query_lengths) {
             if (threadIdx.x < 64) {
                 int before = 0;
@@ -1093,14 +1120,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
             }
             own_first = plan.own_first;
             if (blockIdx.x == gridDim.x - 1 && threadIdx.x >= 64 * (kWaves - 1)) write_notes(first, sums_lds, plan);
-            index = kWaves * ((int)blockIdx.x - own_first) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            by_tiles = plan.by_tiles;
+            index = (int)blockIdx.x - own_first;
+            if (!by_tiles) index = kWaves * index + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
             if (sums.own > 0 && index >= 0 && index < plan.own.workers) {
                 v = plan.own.begin(index);
                 v_end = plan.own.begin(index + 1);
             }
         }
-        work_on_row_tiles<RF, true>(lds, flags, sums_lds, first, u, u_end);
-        work_on_own<RF>(lds, first, own_first, index, v, v_end);
+        work_on_row_tiles<RF, kPrefixes>(lds, flags, sums_lds, first, u, u_end);
+        if (by_tiles) work_on_row_tiles<RF, kOwn>(lds, flags, sums_lds, first, v, v_end);
+        else work_on_own<RF>(lds, first, own_first, index, v, v_end);
     } else {
         int total;
         find_request(first, -1, total);
@@ -1126,7 +1156,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixAr
 #pragma unroll
             for (int i = 0; i < 4; ++i) to[1 + i] = place[i];
         }
-        work_on_row_tiles<RF, false>(lds, flags, sums_lds, first, u, u_end);
+        work_on_row_tiles<RF, kRequests>(lds, flags, sums_lds, first, u, u_end);
     }
 }
 
@@ -1252,7 +1282,7 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
     auto load = [](const int* from) { return PARTS == 1 ? r2o_ldg(from) : load_uniform(from); };
     const Share shared{load_uniform(all), 0, load_uniform(all + 1), load_uniform(all + 2)}, own{load_uniform(all + 4), 0, load_uniform(all + 5), load_uniform(all + 6)};
     const int own_first = load_uniform(all + 3), shared_base = load(note), shared_tiles = load(note + 1), before = load(note + 2), rows = load(note + 3),
-              own_base = load(note + 4), own_tiles = load(note + 5), counted = load(note + 6), place = load(note + 7);
+              own_base = load(note + 4), own_tiles = load(note + 5), counted = load(note + 6), place = load(note + 7), by_tiles = load_uniform(all + 7);
     State s{-INFINITY, 0.f, r2o_f4{}};
     if (live && row < counted) {
         // the states of one segment, of `tiles` tiles from unit `base` on: shared by the groups, four loads of each under way
@@ -1280,9 +1310,15 @@ __global__ __launch_bounds__(256) void prefix_join_merged_kernel(PrefixArgs) {
                 whole_prefix_rows(a, before, rows, h) + r, [&](int w, bool begins) { return split_rows(w, begins) + r - tile * kRows; });
         }
         if (own_tiles > 0 && own.total > 0) {
-            const int chunk = p / kWaveRows;
-            add(own, own_base + (h * div_up(counted * a.group, kWaveRows) + chunk) * (own_tiles + kWaveSegment) + kWaveSegment, own_tiles,
-                whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(own_first, w, begins) + p - chunk * kWaveRows; });
+            if (by_tiles) {
+                const int tile = p / kRows;
+                add(own, own_base + (h * div_up(counted * a.group, kRows) + tile) * (own_tiles + kSegment) + kSegment, own_tiles,
+                    whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_rows(own_first + w, begins) + p - tile * kRows; });
+            } else {
+                const int chunk = p / kWaveRows;
+                add(own, own_base + (h * div_up(counted * a.group, kWaveRows) + chunk) * (own_tiles + kWaveSegment) + kWaveSegment, own_tiles,
+                    whole_own_rows(a, b, h) + p, [&](int w, bool begins) { return split_wave_rows(own_first, w, begins) + p - chunk * kWaveRows; });
+            }
         }
     }
     if constexpr (PARTS > 1) {
@@ -1340,7 +1376,7 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     if (all_rows > (1 << 30)) return R2O_EINVAL;
     const int64_t shared = any ? f.max_pages * f.page_size : 0;
     const int64_t slots = c.max_pages * c.page_size;
-    const bool room = r2o_prefix_room(packed, all_rows), merged = r2o_prefix_merged(c.batch, f.batch, packed, all_rows, slots, shared, p->query_lengths);
+    const bool room = r2o_prefix_room(packed, all_rows), merged = r2o_prefix_merged(c.batch, f.batch, packed, all_rows, shared, p->query_lengths);
     if (p->scratch_floats < r2o_prefix_scratch(p->workers, room, all_rows, c.batch)) return R2O_EINVAL;
     const int64_t states = r2o_prefix_states(p->workers, room, all_rows);
     if (r2o_prefix_units(merged, c.batch, c.hkv, packed, slots, f.batch, shared) > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS)
