@@ -137,6 +137,19 @@ def test_one_long_request(rows):
     check(q, own, query_lengths=_ints(dev, max(1, rows - 9)))
 
 
+@pytest.mark.parametrize("rows", [9, 18, 30, 60])
+@pytest.mark.parametrize("lengths", [(900, 2500, 61, 130, 1777), (64, 70, 100, 90, 65)])
+def test_rows_and_own_slots_in_tiles(rows, lengths):
+    """A prefix's rows in one list and the requests' own slots in row tiles, or single waves where they are few."""
+    dev = _cuda()
+    shared, own = _both(dev, (7000, 6500), lengths, 2, 32, FP16, rows)
+    q = _query(dev, 5, 14, rows, FP16, 29)
+    check(q, own, shared, _ints(dev, 3, 1))
+    check(q, own, shared, _ints(dev, 1, 4), _ints(dev, rows, rows // 2, 0, 1, rows))
+    own.lengths[1] = 3  # fewer slots than rows
+    check(q, own, shared, _ints(dev, 2, 2))
+
+
 @pytest.mark.parametrize("rows", [1, 70])
 def test_a_token_without_its_axis_and_pools_of_one_tensor(rows):
     """[B, Hq, 128]; prefix and own slots in pages of one pool, K and V views of it; pages of different sizes."""
@@ -226,14 +239,14 @@ def test_any_number_of_workers(rows, prefix, workers):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-@pytest.mark.parametrize("rows", [1, 6, 40])
-def test_infinite_and_nan_values(rows, dtype):
+@pytest.mark.parametrize("rows,prefix", [(1, 200), (6, 200), (40, 200), (40, 6000)])
+def test_infinite_and_nan_values(rows, prefix, dtype):
     """What a row sees of a channel's infinities and NaN is its result there, whatever their weights; what it does not see is
     not."""
     import r2omni_amd as ro
 
     dev = _cuda()
-    shared, own = _both(dev, (200, 70), (100, 64, 41, 50), 2, 16, dtype, 15)
+    shared, own = _both(dev, (prefix, 70), (100, 64, 41, 50), 2, 16, dtype, 15)
     q, members = _query(dev, 4, 8, rows, dtype, 15, gain=4.0), _ints(dev, 2, 1)
 
     def put(cache, row, slot, channel, x):
@@ -259,13 +272,13 @@ def test_infinite_and_nan_values(rows, dtype):
     assert torch.equal(out[~odd], clean[~odd])
 
 
-@pytest.mark.parametrize("rows", [1, 40])
-def test_nan_and_infinite_keys(rows):
+@pytest.mark.parametrize("rows,prefix", [(1, 200), (40, 200), (40, 6000)])
+def test_nan_and_infinite_keys(rows, prefix):
     """A NaN logit makes its row NaN; one of -inf weighs nothing."""
     import r2omni_amd as ro
 
     dev = _cuda()
-    shared, own = _both(dev, (200,), (100, 64), 2, 16, BF16, 16)
+    shared, own = _both(dev, (prefix,), (100, 64), 2, 16, BF16, 16)
     q = _query(dev, 2, 8, rows, BF16, 16)
     q[..., 0] = 1.0
     clean, clean_lse = check(q, own, shared)
