@@ -808,9 +808,17 @@ bool heads_arg(const at::Tensor* t, int64_t device, int64_t* strides) {
            row_code(*t) >= 0 && !needs_grad(*t) && row_strides(*t, 3, strides) && strides[2] <= R2O_MAX_ROW_STRIDE;
 }
 
-// What empty_like gives, without its look at strides where they are not kept anyhow: rows in order, or views of a fused projection.
+// A result whose axes lie in memory in the operand's order, as empty_like gives it: of a fused projection's heads [B, S, H, 128], so
+// that what follows joins the heads without a copy (of 32641 rows of 28 heads: 153 us, more than their rotation).  Where the axes stand
+// in order anyhow, as of one token's heads, without its look at them (0.3 us).
 at::Tensor result_like(const at::Tensor& t) {
-    return t.is_contiguous() || !t.is_non_overlapping_and_dense() ? at::empty(t.sizes(), t.options()) : at::empty_like(t);
+    int64_t before = INT64_MAX;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        if (t.size(i) < 2) continue;
+        if (t.stride(i) >= before || t.stride(i) < 1) return at::empty_like(t);
+        before = t.stride(i);
+    }
+    return at::empty(t.sizes(), t.options());
 }
 
 // position_rope(function, query, key, positions, rotary, hadamard): (status, query, key) or None
