@@ -606,6 +606,8 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream);
 
 /* -------------------------------------------------------- rotation by positions ---- */
 
+#define R2O_POSITION_MAX_TOKENS ((1 << 28) - 16) /* of all requests of a call: a launch's 2^32 - 1 lanes, 256 for 16 tokens */
+
 /* Channel pair (i, i + 64) of a row turns by the angle position * inv_freq[i] of its axis: axis 1 or 2 where bit i of pairs_1
  * or pairs_2 is set (both never are), axis 0 elsewhere.  Angles are formed in 64 bits; cosine and sine are
  * multiplied by `scaling`.  With q_weight and k_weight (both or neither, [128], the rows' type) a row is first divided by
@@ -630,7 +632,7 @@ typedef struct r2o_position_rope_params {
     uint16_t* query_out;
     uint16_t* key_out;
     int64_t q_strides[3], k_strides[3], qo_strides[3], ko_strides[3];
-    int64_t batch, hq, hkv, tokens, dtype, hadamard;
+    int64_t batch, hq, hkv, tokens, dtype, hadamard; /* batch * tokens at most R2O_POSITION_MAX_TOKENS */
 } r2o_position_rope_params;
 int r2o_position_rope(const r2o_position_rope_params* p, void* stream);
 
@@ -647,7 +649,7 @@ typedef struct r2o_paged_rope_extend_params {
     const float* weights;     /* fp32 [batch, hkv, rows], element strides (batch, head), or NULL */
     const int32_t* counts;
     int64_t q_strides[3], k_strides[3], v_strides[3], qo_strides[3], weights_strides[2];
-    int64_t hq, rows;
+    int64_t hq, rows;         /* batch * rows at most R2O_POSITION_MAX_TOKENS */
 } r2o_paged_rope_extend_params;
 int r2o_paged_rope_extend(const r2o_paged_rope_extend_params* p, void* stream);
 

@@ -836,7 +836,7 @@ PyObject* position_rope_call(PyObject* const* args) {
     p.tokens = q->size(2);
     p.hadamard = args[5] == Py_True;
     Rotary rotary;
-    if (!rotary.read(args[4], (int)p.dtype, device) || !rotary.place(args[3], p.batch, p.tokens, device) || p.batch * p.tokens > 0x7fffffff)
+    if (!rotary.read(args[4], (int)p.dtype, device) || !rotary.place(args[3], p.batch, p.tokens, device) || p.batch * p.tokens > R2O_POSITION_MAX_TOKENS)
         Py_RETURN_NONE;
     p.rotation = rotary.r;
     at::Tensor q_out = result_like(*q), k_out = result_like(*k);
@@ -862,7 +862,7 @@ PyObject* paged_rope_extend_call(PyObject* const* args) {
         Py_RETURN_NONE;
     p.hq = q->size(1);
     p.rows = q->size(2);
-    if (p.rows > c.max_pages * c.page_size || c.batch * p.rows > 0x7fffffff || !lengths_arg(args[7], c.batch, device, p.counts)) Py_RETURN_NONE;
+    if (p.rows > c.max_pages * c.page_size || c.batch * p.rows > R2O_POSITION_MAX_TOKENS || !lengths_arg(args[7], c.batch, device, p.counts)) Py_RETURN_NONE;
     if (args[8] != Py_None) {
         const at::Tensor* w = exact_tensor(args[8]);
         if (!w || !c.weight_pages || needs_grad(*w) || !on_device(*w, device) || w->scalar_type() != at::kFloat || w->dim() != 3 ||

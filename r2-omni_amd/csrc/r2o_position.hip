@@ -223,8 +223,8 @@ int launch_kernel(const RotateArgs& a, int64_t dtype, dim3 grid, hipStream_t st)
 
 template <bool PAGED>
 int launch(RotateArgs& a, int64_t dtype, int64_t batch, int64_t tokens, int64_t heads, hipStream_t st) {
+    if (heads > 0x7fffffff / 2 || tokens > R2O_POSITION_MAX_TOKENS || batch > R2O_POSITION_MAX_TOKENS / tokens) return R2O_EINVAL;
     const int64_t items = batch * tokens;
-    if (heads > 0x7fffffff / 2 || tokens > 0x7fffffff || batch > 0x7fffffff || items > 0x7fffffff) return R2O_EINVAL;
     a.items = (uint32_t)items;
     a.tokens = (uint32_t)tokens;
     a.heads = (int)heads;

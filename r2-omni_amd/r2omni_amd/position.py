@@ -24,6 +24,7 @@ from .prompt import _check_like, _lengths, _like, _rows, _strides
 _PAIRS = 64
 _POSITION_BYTES = {torch.int32: 4, torch.int64: 8}
 _FREQ_BYTES = {torch.float32: 4, torch.float64: 8}
+_MOST_TOKENS = (1 << 28) - 16  # of all requests: what one launch has lanes for
 
 
 @dataclass(frozen=True, eq=False)
@@ -105,15 +106,16 @@ def _check_heads(query: torch.Tensor, key: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} requires equal batch sizes and token counts, and positive head and token counts")
     if query.device != key.device or query.dtype != key.dtype:
         raise ValueError("Q/K device and dtype must match")
-    if query.shape[0] * query.shape[2] >= 1 << 31:
-        raise ValueError(f"{what} takes less than 2^31 tokens")
+    if query.shape[0] * query.shape[2] > _MOST_TOKENS:
+        raise ValueError(f"{what} takes at most 2^28 - 16 tokens over all requests")
     _lib.dtype_code(query.dtype)
 
 
 def qk_position_rope(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, rotary: PositionRotary, *,
                      apply_hadamard: bool = False, output: tuple[torch.Tensor, torch.Tensor] | None = None):
     """Query [B, Hq, S, 128] and key [B, Hkv, S, 128] (bf16 or fp16) rotated by ``positions`` (int32 or int64 [axes, B, S], or
-    [B, S] for one axis) as ``rotary`` says, in one launch; returns (query, key).
+    [B, S] for one axis) as ``rotary`` says, in one launch (of at most 2^28 - 16 tokens over all requests); returns (query,
+    key).
 
     With ``apply_hadamard``, followed by the orthonormal FWHT-128 of both, as the packed cache's keys are.  Strided views
     are read in place where the channels are unit-strided and rows 16-byte aligned (copied otherwise): those of a fused
