@@ -598,8 +598,9 @@ typedef struct r2o_paged_prefix_params {
     int64_t hq, rows;         /* batch * hq * rows at most 2^30 */
     float sm_scale;           /* positive and finite */
     float* scratch;           /* 16-byte aligned */
-    int64_t scratch_floats;   /* at least 130 (512 workers + r) + 8 (1 + the larger of batch and workers), r = 2 batch hq rows where
-                                 hq / hkv * rows is below 128, or below 512 and batch hq rows at most 2^18, else 0 */
+    int64_t scratch_floats;   /* at least 130 (512 workers + r) + 8 (1 + the larger of batch and workers), r = 2 batch hq rows where the
+                                 rows of a prefix's requests are one list, which they are at most where hq / hkv * rows is below
+                                 128, or below 512 and batch hq rows at most 2^18; else 0 */
     int64_t workers;          /* workgroups that share the slots */
 } r2o_paged_prefix_params;
 int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream);

@@ -896,7 +896,7 @@ PrefixPlan prefix_plan(int64_t batch, int64_t hkv, int64_t hq, int64_t rows, int
     const int64_t units = r2o_prefix_units(merged, batch, hkv, packed, slots, prefixes, shared);
     if (units > 0x7fffffff - 8 * R2O_PAGED_MAX_WORKERS) return {0, 0};
     const int64_t workers = std::max<int64_t>(1, std::min(cus, units));
-    return {workers, r2o_prefix_scratch(workers, r2o_prefix_room(packed, all_rows), all_rows, batch)};
+    return {workers, r2o_prefix_scratch(workers, merged, all_rows, batch)};
 }
 
 // paged_prefix_attention(function, query, cache, prefix or None, members, query_lengths, scale): (status, out, lse) or None

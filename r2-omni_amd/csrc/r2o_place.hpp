@@ -42,7 +42,7 @@ constexpr int64_t r2o_place_blocks(int64_t tiles, int64_t splits, int64_t batche
     return (batches * tiles * splits + dies - 1) / dies * dies * heads;
 }
 
-// Whether the prefix attention may make one list of the rows of all requests of a prefix, and so needs room for their states.
+// Whether the prefix attention may make one list of the rows of all requests of a prefix, whose states need room.
 // packed: a request's rows of a KV head; all_rows: the call's.
 constexpr bool r2o_prefix_room(int64_t packed, int64_t all_rows) { return packed < 512 && (packed < 128 || all_rows <= 1 << 18); }
 
@@ -81,9 +81,9 @@ constexpr int64_t r2o_prefix_units(bool merged, int64_t batch, int64_t hkv, int6
                   : hkv * batch * ((packed + 255) / 256) * (1 + keys + own + kR2oSegment);
 }
 
-// Scratch of such a call, in floats: states of 130, two tiles of 256 rows a workgroup and two of each row, then eight words for each
-// request or workgroup and for all.
-constexpr int64_t r2o_prefix_states(int64_t workers, bool room, int64_t all_rows) { return 512 * workers + (room ? 2 * all_rows : 0); }
-constexpr int64_t r2o_prefix_scratch(int64_t workers, bool room, int64_t all_rows, int64_t batch) {
-    return 130 * r2o_prefix_states(workers, room, all_rows) + 8 * (1 + std::max(batch, workers));
+// Scratch of such a call, in floats: states of 130, two tiles of 256 rows a workgroup and, merged, two of each row, then eight words
+// for each request or workgroup and for all.
+constexpr int64_t r2o_prefix_states(int64_t workers, bool merged, int64_t all_rows) { return 512 * workers + (merged ? 2 * all_rows : 0); }
+constexpr int64_t r2o_prefix_scratch(int64_t workers, bool merged, int64_t all_rows, int64_t batch) {
+    return 130 * r2o_prefix_states(workers, merged, all_rows) + 8 * (1 + std::max(batch, workers));
 }

@@ -1378,9 +1378,9 @@ int r2o_paged_prefix_attention(const r2o_paged_prefix_params* p, void* stream) {
     if (all_rows > (1 << 30)) return R2O_EINVAL;
     const int64_t shared = any ? f.max_pages * f.page_size : 0;
     const int64_t slots = c.max_pages * c.page_size;
-    const bool room = r2o_prefix_room(packed, all_rows), merged = r2o_prefix_merged(c.batch, f.batch, packed, all_rows, shared, p->query_lengths);
-    if (p->scratch_floats < r2o_prefix_scratch(p->workers, room, all_rows, c.batch)) return R2O_EINVAL;
-    const int64_t states = r2o_prefix_states(p->workers, room, all_rows);
+    const bool merged = r2o_prefix_merged(c.batch, f.batch, packed, all_rows, shared, p->query_lengths);
+    if (p->scratch_floats < r2o_prefix_scratch(p->workers, merged, all_rows, c.batch)) return R2O_EINVAL;
+    const int64_t states = r2o_prefix_states(p->workers, merged, all_rows);
     if (r2o_prefix_units(merged, c.batch, c.hkv, packed, slots, f.batch, shared) > 0x7fffffff - kWaves * R2O_PAGED_MAX_WORKERS)
         return R2O_EINVAL;
     PrefixArgs a{};
