@@ -7,7 +7,7 @@
 //
 // A row (128 channels of one (request, head, token)) is 16 lanes of 8 channels, one 16-byte load and store; a channel's
 // partner is lane ^ 8, read by DPP.  A wave takes 4 tokens and walks a run of heads: the 64 angles of a token are formed once
-// for all of them, and four or eight heads' rows are in flight at a time.
+// for all of them, and the rows of four heads, in large calls of sixteen, are in flight at a time.
 #include <algorithm>
 #include <initializer_list>
 
@@ -83,28 +83,39 @@ __device__ __forceinline__ void rotate_row(float (&x)[8], const float (&cs)[8], 
     for (int i = 0; i < 8; ++i) x[i] = y[i];
 }
 
-// Rows of a call past what the caches hold (STREAM) are read and written past them, 16 heads' at a time.  32641 rows of 32 heads take
+// Rows of a call past what the caches hold (not kThroughCaches) are read and written past them, 16 heads' at a time.  32641 rows of 32 heads take
 // 101 us so (5.28 TB/s, as a copy's) and 113 through the caches, four at a time; into pages, 32 + 2 x 8 heads with norms, 153 and
 // 189.  With 8 heads at a time 107 and 163, 12: 105 and 154, 24: 104 and 156; with loads alone past the caches 107 and 162, stores
 // alone 105 and 157.
-template <bool STREAM>
-constexpr int kHeadsInFlight = STREAM ? 16 : 4;
+// A round of fewer heads loads its last one's rows again in place of the missing ones', without a branch: but not where more than a
+// third of a wave's loads would be such (kPastShortRounds), for past the caches they are read again.  100003 rows of 4 heads take 42 us
+// so and 62 with them, 32641 of 18 60 and 68, of 20 into pages 66 and 72, 100003 of 24, where a quarter would be, 230 and 227; 32641
+// of 48 with norms, where none is, 156 and 153.
+enum Caches { kThroughCaches, kPastCaches, kPastShortRounds };
 
-template <bool STREAM>
+template <Caches CACHES>
+constexpr int kHeadsInFlight = CACHES ? 16 : 4;
+
+constexpr bool short_rounds(int64_t heads) {  // of a wave
+    const int64_t each = kHeadsInFlight<kPastCaches>, loads = (heads + each - 1) / each * each;
+    return 3 * (loads - heads) > loads;
+}
+
+template <Caches CACHES>
 __device__ __forceinline__ r2o_u4 load_row(const uint16_t* p) {
-    if constexpr (STREAM) return __builtin_nontemporal_load((const R2O_GLOBAL r2o_u4*)p);
+    if constexpr (CACHES != kThroughCaches) return __builtin_nontemporal_load((const R2O_GLOBAL r2o_u4*)p);
     return r2o_load8<true>(p);
 }
 
-template <bool STREAM>
+template <Caches CACHES>
 __device__ __forceinline__ void store_row(uint16_t* p, const r2o_u4& w) {
-    if constexpr (STREAM) __builtin_nontemporal_store(w, (R2O_GLOBAL r2o_u4*)p);
+    if constexpr (CACHES != kThroughCaches) __builtin_nontemporal_store(w, (R2O_GLOBAL r2o_u4*)p);
     else r2o_store8<true>(p, w);
 }
 
 // grid (ceil(items / 16), ceil(heads / heads_per_wave)), block 256.  Lanes past the last item work on it again and store
 // nothing: the exchanges need every lane of the wave.
-template <int DT, bool NORM, bool PAGED, bool STREAM>
+template <int DT, bool NORM, bool PAGED, Caches CACHES>
 __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
     const int lane = threadIdx.x & 63, c8 = lane & 15;
     const uint32_t item = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
@@ -144,21 +155,22 @@ __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
         r2o_unpack8<DT>(r2o_load8<true>(a.rotation.k_weight + 8 * c8), wk);
     }
     const int64_t q0 = in_head(a.q_strides), k0 = in_head(a.k_strides), v0 = PAGED ? in_head(a.v_strides) : 0;
-    for (int h0 = blockIdx.y * a.heads_per_wave; h0 < h_end; h0 += kHeadsInFlight<STREAM>) {
-        r2o_u4 raw[kHeadsInFlight<STREAM>];
+    for (int h0 = blockIdx.y * a.heads_per_wave; h0 < h_end; h0 += kHeadsInFlight<CACHES>) {
+        r2o_u4 raw[kHeadsInFlight<CACHES>];
 #pragma unroll
-        for (int u = 0; u < kHeadsInFlight<STREAM>; ++u) {  // h is wave-uniform
+        for (int u = 0; u < kHeadsInFlight<CACHES>; ++u) {  // h is wave-uniform
+            if (CACHES == kPastShortRounds && u && h0 + u >= h_end) break;
             const int h = min(h0 + u, h_end - 1);
-            if (h < a.hq) raw[u] = load_row<STREAM>(a.q + q0 + h * a.q_strides[1]);
-            else if (!PAGED || h < a.hq + a.hkv) raw[u] = load_row<STREAM>(a.k + k0 + (h - a.hq) * a.k_strides[1]);
-            else raw[u] = load_row<STREAM>(a.v + v0 + (h - a.hq - a.hkv) * a.v_strides[1]);
+            if (h < a.hq) raw[u] = load_row<CACHES>(a.q + q0 + h * a.q_strides[1]);
+            else if (!PAGED || h < a.hq + a.hkv) raw[u] = load_row<CACHES>(a.k + k0 + (h - a.hq) * a.k_strides[1]);
+            else raw[u] = load_row<CACHES>(a.v + v0 + (h - a.hq - a.hkv) * a.v_strides[1]);
         }
 #pragma unroll
-        for (int u = 0; u < kHeadsInFlight<STREAM>; ++u) {
+        for (int u = 0; u < kHeadsInFlight<CACHES>; ++u) {
             const int h = h0 + u;
             if (h >= h_end) break;
             if (PAGED && h >= a.hq + a.hkv) {
-                if (key_at >= 0) store_row<STREAM>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
+                if (key_at >= 0) store_row<CACHES>(a.cache.value_pages + value_at + (h - a.hq - a.hkv) * a.cache.value_strides[1], raw[u]);
                 continue;
             }
             float x[8];
@@ -168,17 +180,17 @@ __global__ __launch_bounds__(256) void rotate_by_position_kernel(RotateArgs a) {
             r2o_u4 y = r2o_pack8<DT>(x);
             if (h < a.hq) {
                 if (PAGED && !counts) y = r2o_u4{};
-                if (live) store_row<STREAM>(a.q_out + qo0 + h * a.qo_strides[1], y);
+                if (live) store_row<CACHES>(a.q_out + qo0 + h * a.qo_strides[1], y);
             } else if constexpr (PAGED) {
                 const int64_t kv = h - a.hq;
                 if (key_at >= 0) {
-                    store_row<STREAM>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
+                    store_row<CACHES>(a.cache.key_pages + key_at + kv * a.cache.key_strides[1], y);
                     if (a.cache.weight_pages && c8 == 0)
                         a.cache.weight_pages[weight_at + kv * a.cache.weight_strides[1]] =
                             a.weights ? r2o_ldg(a.weights + b * a.weights_strides[0] + kv * a.weights_strides[1] + token) : 0.f;
                 }
             } else if (live) {
-                store_row<STREAM>(a.k_out + ko0 + (h - a.hq) * a.ko_strides[1], y);
+                store_row<CACHES>(a.k_out + ko0 + (h - a.hq) * a.ko_strides[1], y);
             }
         }
     }
@@ -207,15 +219,15 @@ constexpr int64_t kFullWaves = 4096;
 // 73.  Rows that the caches still hold, 45 MB into pages: 22.7 and 19.4, 63 MB: 30.0 and 28.8.
 constexpr int64_t kStreamed = (int64_t)1 << 26;
 
-template <bool PAGED, bool STREAM>
+template <bool PAGED, Caches CACHES>
 int launch_kernel(const RotateArgs& a, int64_t dtype, dim3 grid, hipStream_t st) {
     const bool norm = a.rotation.q_weight != nullptr;
     if (dtype == 0) {
-        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<0, true, PAGED, STREAM>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((rotate_by_position_kernel<0, false, PAGED, STREAM>), grid, dim3(256), 0, st, a);
+        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<0, true, PAGED, CACHES>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rotate_by_position_kernel<0, false, PAGED, CACHES>), grid, dim3(256), 0, st, a);
     } else {
-        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<1, true, PAGED, STREAM>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((rotate_by_position_kernel<1, false, PAGED, STREAM>), grid, dim3(256), 0, st, a);
+        if (norm) hipLaunchKernelGGL((rotate_by_position_kernel<1, true, PAGED, CACHES>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rotate_by_position_kernel<1, false, PAGED, CACHES>), grid, dim3(256), 0, st, a);
     }
     R2O_CHECK_LAUNCH();
     return R2O_OK;
@@ -233,7 +245,8 @@ int launch(RotateArgs& a, int64_t dtype, int64_t batch, int64_t tokens, int64_t 
     per = std::max(per, (heads + 65534) / 65535);  // the grid's second dimension
     a.heads_per_wave = (int)per;
     const dim3 grid((unsigned)((items + 15) / 16), (unsigned)((heads + per - 1) / per));
-    return heads * items > kStreamed / 256 ? launch_kernel<PAGED, true>(a, dtype, grid, st) : launch_kernel<PAGED, false>(a, dtype, grid, st);
+    if (heads * items <= kStreamed / 256) return launch_kernel<PAGED, kThroughCaches>(a, dtype, grid, st);
+    return short_rounds(per) ? launch_kernel<PAGED, kPastShortRounds>(a, dtype, grid, st) : launch_kernel<PAGED, kPastCaches>(a, dtype, grid, st);
 }
 
 }  // namespace
