@@ -638,7 +638,8 @@ typedef struct r2o_position_rope_params {
 int r2o_position_rope(const r2o_position_rope_params* p, void* stream);
 
 /* r2o_paged_extend of rotated keys, and their queries rotated: row i of request b (i < counts[b], all `rows` without counts) is
- * its slot lengths[b] - counts[b] + i.  positions NULL: a row's slot is its position on every axis.  Query rows behind a
+ * its slot lengths[b] - counts[b] + i.  positions NULL: a row's slot is its position on every axis, also where
+ * r2o_paged_prefix_attention has a prefix before it, whose length they then leave out.  Query rows behind a
  * request's count are 0 in query_out. */
 typedef struct r2o_paged_rope_extend_params {
     r2o_paged_cache cache;

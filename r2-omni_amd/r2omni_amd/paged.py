@@ -244,8 +244,9 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedCache, prefix: Paged
     none; without it all share the one prefix there is.  Counts past the batch's end are cut off.  Row i of a request with q
     query rows (S, or ``query_lengths[b]``) and n = ``cache.lengths[b]`` slots, the new ones among them, sees all of its
     prefix and its own slots j <= n - q + i.  A row that sees nothing, or lies behind its request's rows, is 0 with lse
-    -inf; infinite and NaN values count as in ``prompt_attention``.  Without a prefix it is causal attention of a chunk over
-    its paged cache.  Caches that keep weights are refused: ``dataclasses.replace(cache, weight_pages=None)``.  ``output``:
+    -inf; infinite and NaN values count as in ``prompt_attention``.  Own rows' positions are the caller's: they go on behind the
+    prefix, where ``paged_rope_extend`` without ``positions`` counts from 0.  Without a prefix it is causal attention of a chunk
+    over its paged cache.  Caches that keep weights are refused: ``dataclasses.replace(cache, weight_pages=None)``.  ``output``:
     the two result tensors, the first with unit-strided channels and 16-byte aligned rows, neither overlapping an input."""
     if output is None:
         made = _lib.host().paged_prefix_attention(_lib.entry("r2o_paged_prefix_attention"), query, cache, prefix, members,

@@ -156,10 +156,12 @@ def paged_rope_extend(cache: PagedCache, query: torch.Tensor, key: torch.Tensor,
     """``paged_extend`` of key and value [B, Hkv, S, 128], the keys rotated as ``rotary`` says on the way, and query [B, Hq,
     S, 128] rotated; returns the rotated query.
 
-    Positions as in ``qk_position_rope``; without them a row's position is its slot, on every axis.  ``cache.lengths``,
-    ``counts`` and ``weights`` as in ``paged_extend``.  Query rows behind a request's count are 0 in the result.  ``output``:
-    the result tensor; it may be the query, rotated in place.  For the next step ``paged_attention`` (without ``append``) and
-    ``paged_prefix_attention`` take the result with the same cache."""
+    Positions as in ``qk_position_rope``; without them a row's position is its slot in ``cache``, on every axis, which is right
+    where the cache holds all of a request's tokens.  Behind a shared prefix it is not: the rows' positions go on where the
+    prefix ends (its length + the slot, for text), and have to be given.  ``cache.lengths``, ``counts`` and ``weights`` as in
+    ``paged_extend``.  Query rows behind a request's count are 0 in the result.  ``output``: the result tensor; it may be the
+    query, rotated in place.  ``paged_attention`` (without ``append``) and, with such positions, ``paged_prefix_attention``
+    take the result with the same cache."""
     if output is None:
         made = _lib.host().paged_rope_extend(_lib.entry("r2o_paged_rope_extend"), cache, query, key, value, rotary, positions, counts, weights)
         if made is not None:
