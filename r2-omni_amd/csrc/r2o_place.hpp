@@ -46,7 +46,9 @@ constexpr int64_t r2o_place_blocks(int64_t tiles, int64_t splits, int64_t batche
 // packed: a request's rows of a KV head; all_rows: the call's.
 constexpr bool r2o_prefix_room(int64_t packed, int64_t all_rows) { return packed < 512 && (packed < 128 || all_rows <= 1 << 18); }
 
-// A key tile of a row list, in microseconds of a compute unit: 256 rows are bound by their products, up to 128 by the loads.
+// A key tile of a row list, in microseconds of a compute unit: 256 rows are bound by their products, up to 128 by the loads.  Measured
+// where the keys come from memory (1 GB of them): 28 and 63 rows 1.4, 112 and 126 1.6, 133 2.05, 168 2.2, 224 2.4, 252 2.5; where they lie
+// in the 256 MB behind the L2s 1.1, 1.2, 1.8, 1.85, 1.95 and 2.05 (63, 112, 133, 168, 224 and 252).
 constexpr double r2o_prefix_tile_cost(int64_t rows) {
     const int64_t left = rows % 256;
     return 2.3 * (double)(rows / 256) + (left > 128 ? 2.3 : left > 0 ? 1.5 : 0.0);
@@ -55,10 +57,12 @@ constexpr double r2o_prefix_tile_cost(int64_t rows) {
 // Whether it does: one list of a prefix's rows wastes row tiles once a prefix and not once a request, but leaves each row's state to a
 // join.  Priced, in microseconds of a compute unit a request and head, by the prefixes' slots that the tables hold, for the lengths are
 // on the device; with counts, as if they were a quarter to all of the rows.  Measured, in us apart and in one list, heads 28 over 4, 16
-// requests over 32000 slots and 2000 own: 7 rows a request and KV head 171 and 39, 84: 193 and 134, 280: 589 and 370, 448: 592 and 554;
-// over 8000 and 8000 own 7: 95 and 58, 56: 103 and 84, 280: 288 and 237; 64 requests over 2100 and 2000 own 84: 102 and 95, 126: 107 and
-// 124, 280: 244 and 261.  Without a prefix one list wins by its join: one request of 126 rows over 32000 slots 42 and 33, 16 over 8000 71
-// and 69; but for 25 to 32 rows, which single waves take: 16 over 500 17 and 20.
+// requests over 32000 slots and 2000 own: 7 rows a request and KV head 173 and 41, 84: 191 and 134, 280: 572 and 340, 448: 572 and 524;
+// over 8000 and 8000 own 7: 91 and 58, 56: 101 and 81, 280: 281 and 223; 64 requests over 2100 and 2000 own 84: 101 and 91, 126: 107 and
+// 115, 280: 236 and 246.  Without a prefix one list wins by its join: one request of 126 rows over 32000 slots 42 and 32, 16 over 8000 71
+// and 64; but for 25 to 32 rows, which single waves take: 28 rows 33 and 37, and 55 and 59.
+// Requests a prefix are taken to be alike, and the table's rows to be used: 16 requests of 84 rows that all share one of 16 table rows
+// are kept apart and take 199 us, one of two 135.
 constexpr bool r2o_prefix_merged(int64_t batch, int64_t prefixes, int64_t packed, int64_t all_rows, int64_t shared, bool some_count) {
     if (!r2o_prefix_room(packed, all_rows)) return false;
     if (!prefixes) return packed <= 24 || packed > 32;

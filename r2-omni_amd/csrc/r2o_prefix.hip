@@ -10,10 +10,11 @@
 // sum, products) in scratch for the join.  Beside them, where rows are merged, the requests' own slots, which no two share.
 //
 // What bounds it: a tile of 256 rows and 64 keys takes 2.3 to 2.7 us (790 to 930 TFLOP/s; a large library product of these types
-// reaches 1220), 2.06 without its loads: exponentials beside products.  One of up to 128 rows takes 1.55, the rows' bytes at 5.3
-// TB/s.  A call has 22 to 27 us beside its tiles: lengths and shares 2, a first tile's pages and rows 12, a state's way out 4, the join 6
-// to 10.  64 requests over 65409 slots, heads 32 over 8: 113 us; 24 over 32641, 28 over 4: 43; 16 questions of 13 to 58 rows over
-// 16257: 166 (800 TFLOP/s).  With 128 rows a workgroup and two of them a compute unit 229, 73 and 345.
+// reaches 1220), 2.06 without its loads: exponentials beside products.  One of 129 to 224 rows takes 2.05 to 2.4 (1.8 to 1.95 where its
+// keys lie in the 256 MB behind the L2s), one of up to 128 1.6, the rows' bytes at 5.3 TB/s.  A call has 22 to 27 us beside its
+// tiles: lengths and shares 2, the first tile's pages and rows 5.5, a state's way out 4, the join's launch and way 6 to 13, and the
+// uneven end.  64 requests over 65409 slots, heads 32 over 8: 113 us (105 to 118 box to box); 24 over 32641, 28 over 4: 43; 16 questions of 13
+// to 58 rows over 16257: 165 to 174 (760 to 800 TFLOP/s).  With 128 rows a workgroup and two of them a compute unit 229, 73 and 345.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -1086,7 +1087,8 @@ __device__ __forceinline__ void work_on_own(Lds& lds, const Lane& first, int own
 }
 
 // The probabilities are rounded to the rows' 16 bits for the product with V, whose two operands are of one type; their sum
-// takes them unrounded.
+// takes them unrounded.  Results differ from those of 32-bit probabilities by 1.5e-4 to 3.6e-4 of their size in bf16 and 4e-5 in fp16,
+// where both are 1.6e-3 and 2.1e-4 off 64 bits by their own rounding.
 template <int RF, bool MERGED>
 __global__ __launch_bounds__(64 * kWaves, 2) void prefix_partial_kernel(PrefixArgs) {
     __shared__ __align__(1024) Lds lds;

@@ -18,7 +18,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum is raised only when a tile exceeds it by more than this (log2 units): p stays below 2^8
 // and most tiles skip the rescaling of 64 accumulators.  Maximum, sum and accumulators refer to one value, so
-// the quotient is exact.
+// the quotient does not depend on it but by the rounding of p to 16 bits: that of a key which outweighs all others is 1,
+// without an error, where the value is its own, and up to 2^8, half a step off, where it is not.  Attention over a prefix,
+// bf16, 128 conversations: 1.680e-3 off 64 bits with the slack, 1.670e-3 without, as with p of 32 bits (1.669e-3), but
+// 170 us become 183 (questions) and 43 become 47 (24 requests).
 constexpr float kSlack = 8.f;
 
 template <int RF>

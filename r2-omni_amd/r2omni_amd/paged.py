@@ -246,8 +246,9 @@ def paged_prefix_attention(query: torch.Tensor, cache: PagedCache, prefix: Paged
     prefix and its own slots j <= n - q + i.  A row that sees nothing, or lies behind its request's rows, is 0 with lse
     -inf; infinite and NaN values count as in ``prompt_attention``.  Own rows' positions are the caller's: they go on behind the
     prefix, where ``paged_rope_extend`` without ``positions`` counts from 0.  Without a prefix it is causal attention of a chunk
-    over its paged cache.  Caches that keep weights are refused: ``dataclasses.replace(cache, weight_pages=None)``.  ``output``:
-    the two result tensors, the first with unit-strided channels and 16-byte aligned rows, neither overlapping an input."""
+    over its paged cache.  Caches that keep weights are refused, for none are accumulated (``paged_evict`` would not know what
+    was attended here): ``dataclasses.replace(cache, weight_pages=None)``.  ``output``: the two result tensors, the first with
+    unit-strided channels and 16-byte aligned rows, neither overlapping an input."""
     if output is None:
         made = _lib.host().paged_prefix_attention(_lib.entry("r2o_paged_prefix_attention"), query, cache, prefix, members,
                                                   query_lengths, sm_scale)
