@@ -13,7 +13,7 @@
 // reaches 1220), 2.06 without its loads: exponentials beside products.  One of 129 to 224 rows takes 2.05 to 2.4 (1.8 to 1.95 where its
 // keys lie in the 256 MB behind the L2s), one of up to 128 1.6, the rows' bytes at 5.3 TB/s.  A call has 22 to 27 us beside its
 // tiles: lengths and shares 2, the first tile's pages and rows 5.5, a state's way out 4, the join's launch and way 6 to 13, and the
-// uneven end.  64 requests over 65409 slots, heads 32 over 8: 113 us (105 to 118 box to box); 24 over 32641, 28 over 4: 43; 16 questions of 13
+// uneven end.  64 requests over 65409 slots, heads 32 over 8: 113 us (105 to 118 card to card); 24 over 32641, 28 over 4: 43; 16 questions of 13
 // to 58 rows over 16257: 165 to 174 (760 to 800 TFLOP/s).  With 128 rows a workgroup and two of them a compute unit 229, 73 and 345.
 #include <algorithm>
 #include <initializer_list>

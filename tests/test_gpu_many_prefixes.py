@@ -53,3 +53,29 @@ def test_a_prefix_each_takes_about_what_one_for_sixteen_does(rows):
         q, members = _query(dev, 1024, 16, rows, BF16, rows), _ints(dev, *[1024 // prefixes] * prefixes)
         times.append(_time(dev, lambda: ro.paged_prefix_attention(q, own, shared, members=members)))
     assert times[1] < 4 * times[0], times
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_captured_call_follows_many_prefixes(rows):
+    import r2omni_amd as ro
+
+    dev, prefixes, batch = _cuda(), 130, 200
+    gen = torch.Generator().manual_seed(rows)
+    shared, own = _both(dev, (33,) * prefixes, (40,) * batch, 1, 16, BF16, rows)
+    q, members = _query(dev, batch, 2, rows, BF16, rows), _ints(dev, *[1] * prefixes)
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ro.paged_prefix_attention(q, own, shared, members=members)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = ro.paged_prefix_attention(q, own, shared, members=members)
+    for _ in range(5):
+        members.copy_(torch.randint(-1, 5, (prefixes,), generator=gen))
+        shared.lengths.copy_(torch.randint(0, 34, (prefixes,), generator=gen))
+        own.lengths.copy_(torch.randint(0, 41, (batch,), generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = check(q, own, shared, members)
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
